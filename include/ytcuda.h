@@ -453,6 +453,75 @@ int ytcuda_latent_attn_fwd(int dtype, const void* q, const void* uk_bf16, const 
                            void* out, int batch, int len, int64_t pos0, int heads, int dim, int rot, int vdim, int rank,
                            const float* freq, float scale, void* stream);
 
+/* ---------------------------------------------------------------- a cache in pages
+ * Keys and values of many sequences of any lengths, for all layers, in pages of a pool (YTensor has no counterpart: one
+ * contiguous cache, example/qwen3/src/qwen3.cpp:70-126). A slot is one sequence: position p lies in row p % page of page
+ * table[slot][p / page]; the first held[slot] entries of its row of the table count, lens[slot] positions are written, and
+ * refs[page] is the number of slots that hold a page (0: free). All of it lives on the device and every call below is a few
+ * kernels without a host round trip, so that a captured graph serves any lengths. Calls on one cache are ordered by the
+ * caller (one stream, or events), as writes of one tensor are.
+ * What only the device can see to be wrong is never followed to memory: the call sets a bit of *status and leaves out what
+ * it concerns. YTC_PAGES_FULL: a reserve or compact found too few free pages (or entries of the table) and changed
+ * nothing. YTC_PAGES_INVALID: an index outside its range, a position without a page, or a tree that is none.
+ * YTC_PAGES_SHARED: rows would have gone to a page that other slots hold too (reserve comes first). */
+#define YTC_PAGES_FULL 1
+#define YTC_PAGES_INVALID 2
+#define YTC_PAGES_SHARED 4
+typedef struct {
+  void* k; /* [layers, pages, kv_heads, page, dim], strides in elements, unit stride along dim */
+  void* v;
+  int64_t k_strides[4]; /* layer, page, head, position */
+  int64_t v_strides[4];
+  int32_t* table;   /* [slots, max_pages] */
+  int32_t* lens;    /* [slots] */
+  int32_t* held;    /* [slots] */
+  int32_t* refs;    /* [pages] */
+  int32_t* status;  /* [1] */
+  int32_t* scratch; /* ytcuda_pages_scratch() bytes, zero before the first call, the cache's own */
+  int layers, pages, page, kv_heads, dim, slots, max_pages;
+  int dtype; /* YTC_F32, YTC_BF16 or YTC_F16 */
+} ytcuda_pages;
+uint64_t ytcuda_pages_scratch(const ytcuda_pages* cache);
+
+/* Room for counts[slot] more positions behind lens[slot] (0: the slot is left as it is): free pages are handed out, the lowest
+ * numbers first, in the order of the slots; where position lens[slot] falls inside a page that other slots hold too, the slot
+ * gets a copy of its rows (its first new page). All slots get theirs or none. */
+int ytcuda_pages_reserve(const ytcuda_pages* cache, const int32_t* counts, void* stream);
+
+/* Row starts[s] + i of k and v [rows, kv_heads, dim] (i < starts[s + 1] - starts[s], starts [slots + 1] on the device, not
+ * decreasing) goes to position lens[s] + i of slot s in one layer. Strides {row, head}. lens stays. */
+int ytcuda_pages_append(const ytcuda_pages* cache, int layer, const void* k, const int64_t* k_strides, const void* v,
+                        const int64_t* v_strides, const int32_t* starts, int rows, void* stream);
+
+/* Attention of new rows in one layer. Rows starts[s] .. starts[s + 1] - 1 of q and o [rows, heads, dim] belong to slot s, row
+ * starts[s] + i to node i at position lens[s] + i. A node sees the lens[s] positions in front of all nodes, itself, and its
+ * ancestors: parents[starts[s] + i] is a smaller node of the same slot or -1 (NULL: node i - 1, a chain; with parents a slot
+ * has at most 1024 nodes). heads is a multiple of kv_heads, query head h reads key head h / (heads / kv_heads). With k and v
+ * [rows, kv_heads, dim] the nodes' keys and values are stored first, as by ytcuda_pages_append (both NULL: they are in the
+ * pages already). scale 0: 1 / sqrt(dim). Scores, softmax and sums in fp32; results rounded to nearest even. Rows behind
+ * starts[slots] are left as they were. Strides {row, head}; dim <= 256. workspace: ytcuda_pages_attend_workspace() bytes
+ * that no other call uses until this one has run. */
+uint64_t ytcuda_pages_attend_workspace(const ytcuda_pages* cache, int rows, int heads);
+int ytcuda_pages_attend(const ytcuda_pages* cache, int layer, const void* q, const int64_t* q_strides, const void* k,
+                        const int64_t* k_strides, const void* v, const int64_t* v_strides, void* o, const int64_t* o_strides,
+                        const int32_t* starts, const int32_t* parents, int rows, int heads, float scale, void* workspace,
+                        uint64_t workspace_bytes, void* stream);
+
+/* Of the rows behind position base[s] (NULL: lens[s]) the first kept[s] of accepted[s][0 .. depth - 1] stay, in every layer:
+ * row base + accepted[s][j] moves to base + j, and lens[s] = base + kept[s]. accepted [slots, depth] is strictly increasing
+ * along a row (NULL: the rows stay where they are). The pages behind stay with the slot. */
+int ytcuda_pages_keep(const ytcuda_pages* cache, const int32_t* kept, const int32_t* accepted, int depth, const int32_t* base,
+                      void* stream);
+
+/* All slots at once: slot s becomes a copy of slot source[s] as it was before the call (its own number: unchanged; -1: emptied),
+ * holding the same pages up to its length. With `gone` instead (source NULL) the slots with gone[s] != 0 are emptied. */
+int ytcuda_pages_fork(const ytcuda_pages* cache, const int32_t* source, const int32_t* gone, void* stream);
+
+/* The pages in use, in the order of their numbers, become pages 0, 1, .. of another cache with the same slots, layers, heads,
+ * type and table, and its table, lens, held and refs those of this one. The other cache's status says YTC_PAGES_FULL where
+ * its pool is too small: nothing is written then. */
+int ytcuda_pages_compact(const ytcuda_pages* cache, const ytcuda_pages* into, void* stream);
+
 /* ---------------------------------------------------------------- handles of the models below */
 void ytcuda_lm_destroy(void* handle);
 /* Starts every sequence anew. */

@@ -1,0 +1,642 @@
+// A cache in pages: handing out pages, storing rows, forking, keeping accepted rows, compacting the pool.
+//
+// All of it is copying and counting. The counting (which pages are free, who holds one) is whole numbers of a few KB and runs
+// in one CTA or one per slot, so that its results do not depend on any order; the copying runs on the whole GPU, a warp for a
+// piece of at most 4 KB with eight 16-byte loads of a lane in flight before the first store. A call that counts and copies is
+// two kernels, the second launched while the first one runs (programmatic dependent launch).
+#include "pages.cuh"
+
+namespace ytk {
+
+constexpr int PG_WARPS = 8;      // warps per CTA of the copying kernels
+constexpr int PG_UNROLL = 8;     // pieces of a row that a lane has in flight
+constexpr int PG_COUNT = 1024;   // threads of the counting kernels
+
+template <int BYTES>
+struct PgWord;
+template <>
+struct PgWord<16> {
+  using type = uint4;
+};
+template <>
+struct PgWord<4> {
+  using type = uint32_t;
+};
+template <>
+struct PgWord<2> {
+  using type = uint16_t;
+};
+
+__device__ __forceinline__ void pg_flag(const PgCache& c, int bit) { atomicOr(c.status, bit); }
+
+// Sum of the values of the threads in front, and of all (PG_COUNT threads).
+__device__ __forceinline__ int pg_scan(int v, int* sums, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();  // (`sums` may still be read from the call before)
+  if (lane == 31) sums[warp] = x;
+  __syncthreads();
+  int w = sums[lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += y;
+  }
+  *total = __shfl_sync(0xffffffffu, w, 31);
+  const int before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+  return x - v + (warp ? before : 0);
+}
+
+// The warp copies `rows` rows of `words` words each.
+template <typename W>
+__device__ __forceinline__ void pg_copy_rows(char* dst, int64_t dst_row, const char* src, int64_t src_row, int rows, int words) {
+  const int lane = threadIdx.x & 31;
+  const int n = rows * words;
+  const bool whole = dst_row == words * static_cast<int64_t>(sizeof(W)) && src_row == dst_row;
+  for (int i0 = lane; i0 < n; i0 += 32 * PG_UNROLL) {
+    W w[PG_UNROLL];
+#pragma unroll
+    for (int u = 0; u < PG_UNROLL; ++u) {
+      const int i = i0 + 32 * u;
+      if (i < n) {
+        const int r = whole ? 0 : i / words;
+        w[u] = *reinterpret_cast<const W*>(src + r * src_row + (i - r * words) * static_cast<int64_t>(sizeof(W)));
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < PG_UNROLL; ++u) {
+      const int i = i0 + 32 * u;
+      if (i < n) {
+        const int r = whole ? 0 : i / words;
+        *reinterpret_cast<W*>(dst + r * dst_row + (i - r * words) * static_cast<int64_t>(sizeof(W))) = w[u];
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- append
+// A warp stores the keys or the values of one new row. The row's slot: the last one that starts at or before it.
+template <int BYTES>
+__global__ void __launch_bounds__(PG_WARPS * 32) pages_append_kernel(const PgCache c, const PgRows k, const PgRows v, const int32_t* starts,
+                                                                     int rows, int layer, int row_words) {
+  using W = typename PgWord<BYTES>::type;
+  const int lane = threadIdx.x & 31;
+  const int64_t warps = static_cast<int64_t>(gridDim.x) * PG_WARPS;
+  const int last = min(rows, starts[c.slots]);
+  for (int64_t item = static_cast<int64_t>(blockIdx.x) * PG_WARPS + (threadIdx.x >> 5); item < 2ll * rows; item += warps) {
+    const int row = static_cast<int>(item >> 1);
+    if (row >= last || row < starts[0]) continue;
+    int lo = 0, hi = c.slots;  // starts[lo] <= row < starts[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      (starts[mid] <= row ? lo : hi) = mid;
+    }
+    const int64_t at = static_cast<int64_t>(c.lens[lo]) + (row - starts[lo]);
+    const int pg = pg_page_of(c, lo, at);
+    if (pg < 0 || c.refs[pg] != 1) {
+      if (lane == 0) pg_flag(c, pg < 0 ? YTC_PAGES_INVALID : YTC_PAGES_SHARED);
+      continue;
+    }
+    const PgPool pool = item & 1 ? c.v : c.k;
+    const PgRows src = item & 1 ? v : k;
+    pg_copy_rows<W>(pool.p + layer * pool.layer + pg * pool.page + (at % c.page) * pool.row, pool.head, src.p + row * src.row, src.head,
+                    c.heads, row_words);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- reserve
+// One CTA: what each slot wants, the free pages in ascending order, and who gets which. Reading refs once at 16 bytes a lane is
+// what it costs: 64k pages are 256 KB, which one SM reads in about 4 us.
+__global__ void __launch_bounds__(PG_COUNT) pages_reserve_kernel(const PgCache c, const int32_t* counts) {
+  dependent_trigger();
+  __shared__ int sums[32];
+  __shared__ int bad, n_copies;
+  const PgScratch at = pg_scratch(c.slots, c.max_pages, c.pages);
+  int32_t* const base = c.scratch + at.base;
+  int32_t* const mark = c.scratch + at.mark;
+  int32_t* const ids = c.scratch + at.ids;
+  const int t = threadIdx.x;
+  if (t == 0) bad = n_copies = 0;
+  __syncthreads();
+  int want_all = 0;
+  for (int s0 = 0; s0 < c.slots; s0 += PG_COUNT) {
+    const int s = s0 + t;
+    int want = 0;
+    if (s < c.slots) {
+      const int len = c.lens[s], held = c.held[s], count = counts[s];
+      mark[s] = -1;
+      if (count) {
+        const int64_t need = (static_cast<int64_t>(len) + count + c.page - 1) / c.page;
+        const int first = len / c.page;
+        bool ok = count > 0 && len >= 0 && held >= 0 && held <= c.max_pages;
+        int copy = -1;
+        if (ok && len % c.page) {
+          const int pg = pg_page_of(c, s, len);
+          ok = pg >= 0;
+          if (ok && c.refs[pg] > 1) copy = pg;
+        }
+        ok = ok && first <= held;  // (the positions that are written have their pages)
+        if (!ok) {
+          pg_flag(c, YTC_PAGES_INVALID);
+          mark[s] = -2;
+        } else if (need > c.max_pages) {
+          bad = 1;
+        } else {
+          mark[s] = copy;
+          want = (need > held ? static_cast<int>(need) - held : 0) + (copy >= 0);
+        }
+      }
+    }
+    int total;
+    const int before = pg_scan(want, sums, &total);
+    if (s < c.slots) base[s] = want_all + before;
+    want_all += total;
+  }
+  if (t == 0) base[c.slots] = want_all;
+  // the first want_all free pages
+  int found = 0;
+  const bool wide = reinterpret_cast<uintptr_t>(c.refs) % 16 == 0;
+  for (int p0 = 0; p0 < c.pages && found < want_all; p0 += 8 * PG_COUNT) {
+    const int p = p0 + 8 * t;
+    int32_t r[8];
+    if (wide && p + 8 <= c.pages) {
+      *reinterpret_cast<int4*>(r) = *reinterpret_cast<const int4*>(c.refs + p);
+      *reinterpret_cast<int4*>(r + 4) = *reinterpret_cast<const int4*>(c.refs + p + 4);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) r[u] = p + u < c.pages ? c.refs[p + u] : 1;
+    }
+    int n = 0;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) n += r[u] == 0;
+    int total;
+    int k = found + pg_scan(n, sums, &total);
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (r[u] == 0) {
+        if (k < want_all) ids[k] = p + u;
+        ++k;
+      }
+    found += total;
+  }
+  __syncthreads();
+  const bool full = bad || found < want_all;
+  if (full) {
+    if (t == 0) {
+      pg_flag(c, YTC_PAGES_FULL);
+      c.scratch[at.copies] = 0;
+    }
+    return;
+  }
+  for (int r = t; r < want_all; r += PG_COUNT) {
+    int lo = 0, hi = c.slots;  // base[lo] <= r < base[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      (base[mid] <= r ? lo : hi) = mid;
+    }
+    const int k = r - base[lo], old = mark[lo], len = c.lens[lo], id = ids[r];
+    const bool copy = old >= 0;
+    const int i = copy && k == 0 ? len / c.page : c.held[lo] + k - copy;
+    c.table[static_cast<int64_t>(lo) * c.max_pages + i] = id;
+    c.refs[id] = 1;
+    if (copy && k == 0) {
+      const int n = atomicAdd(&n_copies, 1);
+      c.scratch[at.src + n] = old;
+      c.scratch[at.dst + n] = id;
+      c.scratch[at.rows + n] = len % c.page;
+      atomicSub(c.refs + old, 1);
+    }
+  }
+  __syncthreads();
+  for (int s = t; s < c.slots; s += PG_COUNT)
+    if (counts[s] > 0 && mark[s] != -2) {
+      const int need = static_cast<int>((static_cast<int64_t>(c.lens[s]) + counts[s] + c.page - 1) / c.page);
+      if (need > c.held[s]) c.held[s] = need;
+    }
+  if (t == 0) c.scratch[at.copies] = n_copies;
+}
+
+// A warp copies the rows of one head, layer and pool of a page.
+template <int BYTES>
+__global__ void __launch_bounds__(PG_WARPS * 32) pages_copy_kernel(const PgCache c, int row_words) {
+  using W = typename PgWord<BYTES>::type;
+  const PgScratch at = pg_scratch(c.slots, c.max_pages, c.pages);
+  dependent_wait();
+  const int64_t per_copy = 2ll * c.layers * c.heads;
+  const int64_t items = c.scratch[at.copies] * per_copy, warps = static_cast<int64_t>(gridDim.x) * PG_WARPS;
+  for (int64_t item = static_cast<int64_t>(blockIdx.x) * PG_WARPS + (threadIdx.x >> 5); item < items; item += warps) {
+    const int n = static_cast<int>(item / per_copy);
+    int rest = static_cast<int>(item - n * per_copy);
+    const PgPool& pool = rest & 1 ? c.v : c.k;
+    rest >>= 1;
+    char* const p = pool.p + rest / c.heads * pool.layer + rest % c.heads * pool.head;
+    pg_copy_rows<W>(p + c.scratch[at.dst + n] * pool.page, pool.row, p + c.scratch[at.src + n] * pool.page, pool.row,
+                    c.scratch[at.rows + n], row_words);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- keep
+// Whether the accepted rows of a slot can move (the same answer in every lane of the warp).
+__device__ __forceinline__ int pg_keep_bad(const PgCache& c, int s, int64_t base, int n, const int32_t* accepted, int depth) {
+  const int lane = threadIdx.x & 31;
+  int bad = n < 0 || base < 0 || (accepted && n > depth) ? YTC_PAGES_INVALID : 0;
+  if (base + n > static_cast<int64_t>(c.held[s]) * c.page) bad = YTC_PAGES_INVALID;
+  if (!bad && accepted)
+    for (int j = lane; j < n; j += 32) {
+      const int a = accepted[static_cast<int64_t>(s) * depth + j];
+      const int b = j ? accepted[static_cast<int64_t>(s) * depth + j - 1] : -1;
+      const int to = pg_page_of(c, s, base + j);
+      if (a <= b || to < 0 || pg_page_of(c, s, base + a) < 0) bad |= YTC_PAGES_INVALID;
+      else if (a != j && c.refs[to] != 1) bad |= YTC_PAGES_SHARED;
+    }
+  return __reduce_or_sync(0xffffffffu, bad);
+}
+
+// A warp moves the accepted rows of one slot, layer, head and pool. Rows only move down and in ascending order, so a batch that
+// has been read before it is written never hides a row of a later batch. The CTA that finishes last writes the lengths: every
+// other one has read them by then.
+template <int BYTES>
+__global__ void __launch_bounds__(PG_WARPS * 32) pages_keep_kernel(const PgCache c, const int32_t* kept, const int32_t* accepted,
+                                                                   int depth, const int32_t* base, int row_words) {
+  using W = typename PgWord<BYTES>::type;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int per_slot = 2 * c.layers * c.heads;
+  const int64_t items = accepted ? static_cast<int64_t>(c.slots) * per_slot : 0, warps = static_cast<int64_t>(gridDim.x) * PG_WARPS;
+  for (int64_t item = static_cast<int64_t>(blockIdx.x) * PG_WARPS + warp; item < items; item += warps) {
+    const int s = static_cast<int>(item / per_slot);
+    int rest = static_cast<int>(item - static_cast<int64_t>(s) * per_slot);
+    const PgPool& pool = rest & 1 ? c.v : c.k;
+    rest >>= 1;
+    const int n = kept[s];
+    const int64_t b = base ? base[s] : c.lens[s];
+    if (n <= 0 || pg_keep_bad(c, s, b, n, accepted, depth)) continue;
+    char* const p = pool.p + rest / c.heads * pool.layer + rest % c.heads * pool.head;
+    const int batch = max(1, 32 * PG_UNROLL / row_words);  // rows that fit the lanes' registers (row_words <= 128 * PG_UNROLL)
+    for (int j0 = 0; j0 < n; j0 += batch) {
+      const int m = min(batch, n - j0) * row_words;
+      for (int w0 = 0; w0 < m; w0 += 32 * PG_UNROLL) {  // (more than one round only where one row takes it)
+        W w[PG_UNROLL];
+        char* to[PG_UNROLL];
+#pragma unroll
+        for (int u = 0; u < PG_UNROLL; ++u) {
+          const int i = w0 + lane + 32 * u;
+          to[u] = nullptr;
+          if (i < m) {
+            const int r = i / row_words, j = j0 + r;
+            const int a = accepted[static_cast<int64_t>(s) * depth + j];
+            if (a != j) {
+              const int64_t x = b + a, y = b + j, off = (i - r * row_words) * static_cast<int64_t>(sizeof(W));
+              w[u] = *reinterpret_cast<const W*>(p + pg_page_of(c, s, x) * pool.page + x % c.page * pool.row + off);
+              to[u] = p + pg_page_of(c, s, y) * pool.page + y % c.page * pool.row + off;
+            }
+          }
+        }
+        __syncwarp();
+#pragma unroll
+        for (int u = 0; u < PG_UNROLL; ++u)
+          if (to[u]) *reinterpret_cast<W*>(to[u]) = w[u];
+        __syncwarp();
+      }
+    }
+  }
+  __shared__ int last;
+  int32_t* const ticket = c.scratch + pg_scratch(c.slots, c.max_pages, c.pages).ticket;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __threadfence();
+    last = atomicAdd(ticket, 1) == static_cast<int>(gridDim.x) - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  if (threadIdx.x == 0) *ticket = 0;
+  for (int s = warp; s < c.slots; s += PG_WARPS) {
+    const int n = kept[s];
+    const int64_t b = base ? base[s] : c.lens[s];
+    const int bad = pg_keep_bad(c, s, b, n, accepted, depth);
+    if (lane == 0) {
+      if (bad) pg_flag(c, bad);
+      else c.lens[s] = static_cast<int>(b + n);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- fork
+// A CTA per slot: the new row of the table goes to the scratch (another slot may still have to read the old one), the counts
+// are whole numbers and may be changed in any order.
+__global__ void __launch_bounds__(256) pages_fork_kernel(const PgCache c, const int32_t* source, const int32_t* gone) {
+  dependent_trigger();
+  const PgScratch at = pg_scratch(c.slots, c.max_pages, c.pages);
+  const int s = blockIdx.x, t = threadIdx.x;
+  const int from = source ? source[s] : gone[s] ? -1 : s;
+  int len = 0, held = -1;  // (-1: the slot stays as it is)
+  const int old = c.held[s];
+  if (from != s) {
+    bool ok = from >= -1 && from < c.slots && old >= 0 && old <= c.max_pages;
+    held = 0;
+    if (ok && from >= 0) {
+      len = c.lens[from];
+      held = len / c.page + (len % c.page != 0);
+      ok = len >= 0 && held <= c.held[from] && held <= c.max_pages;
+    }
+    if (!ok) {
+      if (t == 0) pg_flag(c, YTC_PAGES_INVALID);
+      held = -1;
+    }
+  }
+  if (t == 0) {
+    c.scratch[at.held + s] = held;
+    c.scratch[at.lens + s] = len;
+  }
+  if (held < 0) return;
+  const int32_t* mine = c.table + static_cast<int64_t>(s) * c.max_pages;
+  for (int i = t; i < old; i += 256) {
+    const int pg = mine[i];
+    if (pg >= 0 && pg < c.pages) atomicSub(c.refs + pg, 1);
+    else pg_flag(c, YTC_PAGES_INVALID);
+  }
+  if (!held) return;
+  const int32_t* theirs = c.table + static_cast<int64_t>(from) * c.max_pages;
+  for (int i = t; i < held; i += 256) {
+    const int pg = theirs[i];
+    c.scratch[at.table + static_cast<int64_t>(s) * c.max_pages + i] = pg;
+    if (pg >= 0 && pg < c.pages) atomicAdd(c.refs + pg, 1);
+    else pg_flag(c, YTC_PAGES_INVALID);
+  }
+}
+__global__ void __launch_bounds__(256) pages_fork_store_kernel(const PgCache c) {
+  const PgScratch at = pg_scratch(c.slots, c.max_pages, c.pages);
+  const int s = blockIdx.x, t = threadIdx.x;
+  dependent_wait();
+  const int held = c.scratch[at.held + s];
+  if (held < 0) return;
+  const int64_t row = static_cast<int64_t>(s) * c.max_pages;
+  for (int i = t; i < held; i += 256) c.table[row + i] = c.scratch[at.table + row + i];
+  if (t == 0) {
+    c.held[s] = held;
+    c.lens[s] = c.scratch[at.lens + s];
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- compact
+// One CTA: the new numbers of the pages in use, and what the other cache says of its slots.
+__global__ void __launch_bounds__(PG_COUNT) pages_number_kernel(const PgCache c, const PgCache to) {
+  dependent_trigger();
+  __shared__ int sums[32];
+  const PgScratch at = pg_scratch(c.slots, c.max_pages, c.pages);
+  int32_t* const ids = c.scratch + at.ids;
+  int32_t* const number = c.scratch + at.number;
+  const int t = threadIdx.x;
+  const bool wide = reinterpret_cast<uintptr_t>(c.refs) % 16 == 0;
+  int found = 0;
+  for (int p0 = 0; p0 < c.pages; p0 += 8 * PG_COUNT) {
+    const int p = p0 + 8 * t;
+    int32_t r[8];
+    if (wide && p + 8 <= c.pages) {
+      *reinterpret_cast<int4*>(r) = *reinterpret_cast<const int4*>(c.refs + p);
+      *reinterpret_cast<int4*>(r + 4) = *reinterpret_cast<const int4*>(c.refs + p + 4);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) r[u] = p + u < c.pages ? c.refs[p + u] : 0;
+    }
+    int n = 0;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) n += r[u] > 0;
+    int total;
+    int k = found + pg_scan(n, sums, &total);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      if (p + u < c.pages) number[p + u] = r[u] > 0 ? k : -1;
+      if (r[u] > 0) ids[k++] = p + u;
+    }
+    found += total;
+  }
+  __syncthreads();
+  const bool full = found > to.pages;
+  if (t == 0) {
+    c.scratch[at.copies] = full ? -1 : found;
+    if (full) pg_flag(to, YTC_PAGES_FULL);
+  }
+  if (full) return;
+  for (int p = t; p < to.pages; p += PG_COUNT) to.refs[p] = p < found ? c.refs[ids[p]] : 0;
+  for (int s = t; s < c.slots; s += PG_COUNT) {
+    to.lens[s] = c.lens[s];
+    to.held[s] = c.held[s];
+  }
+}
+// A warp copies a piece of up to 4 KB of what one page holds of a layer (of a head, where the heads do not lie one behind another).
+template <int BYTES>
+__global__ void __launch_bounds__(PG_WARPS * 32) pages_compact_kernel(const PgCache c, const PgCache to, int row_words, int merged) {
+  using W = typename PgWord<BYTES>::type;
+  const PgScratch at = pg_scratch(c.slots, c.max_pages, c.pages);
+  dependent_wait();
+  const int pages = c.scratch[at.copies];
+  if (pages < 0) return;
+  const int64_t entries = static_cast<int64_t>(c.slots) * c.max_pages, threads = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < entries; i += threads) {
+    if (i % c.max_pages >= c.held[i / c.max_pages]) continue;
+    const int old = c.table[i];
+    const int now = old >= 0 && old < c.pages ? c.scratch[at.number + old] : -1;
+    to.table[i] = now;
+    if (now < 0) pg_flag(to, YTC_PAGES_INVALID);
+  }
+  const int blocks = merged ? 1 : c.heads, words = (merged ? c.heads : 1) * c.page * row_words;
+  const int rows_a_piece = merged ? 1 : max(1, 32 * PG_UNROLL / row_words);
+  const int pieces = merged ? (words + 32 * PG_UNROLL - 1) / (32 * PG_UNROLL) : (c.page + rows_a_piece - 1) / rows_a_piece;
+  const int64_t per_page = static_cast<int64_t>(pieces) * blocks * 2 * c.layers;
+  const int64_t items = pages * per_page, warps = static_cast<int64_t>(gridDim.x) * PG_WARPS;
+  for (int64_t item = static_cast<int64_t>(blockIdx.x) * PG_WARPS + (threadIdx.x >> 5); item < items; item += warps) {
+    const int now = static_cast<int>(item / per_page);
+    int rest = static_cast<int>(item - now * per_page);
+    const int piece = rest % pieces;
+    rest /= pieces;
+    const int head = rest % blocks;
+    rest /= blocks;
+    const PgPool &x = rest & 1 ? c.v : c.k, &y = rest & 1 ? to.v : to.k;
+    const int layer = rest >> 1;
+    const char* src = x.p + layer * x.layer + c.scratch[at.ids + now] * x.page + head * x.head;
+    char* dst = y.p + layer * y.layer + now * y.page + head * y.head;
+    if (merged) {
+      const int first = piece * 32 * PG_UNROLL, n = min(32 * PG_UNROLL, words - first);
+      pg_copy_rows<W>(dst + first * static_cast<int64_t>(BYTES), n * static_cast<int64_t>(BYTES), src + first * static_cast<int64_t>(BYTES),
+                      n * static_cast<int64_t>(BYTES), 1, n);
+    } else {
+      const int r = piece * rows_a_piece;
+      pg_copy_rows<W>(dst + r * y.row, y.row, src + r * x.row, x.row, min(rows_a_piece, c.page - r), row_words);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- host
+int pg_take(const char* who, const ytcuda_pages* c, PgCache* out) {
+  YTC_REQUIRE(c != nullptr, "%s: no cache", who);
+  YTC_REQUIRE(c->dtype == YTC_F32 || c->dtype == YTC_BF16 || c->dtype == YTC_F16, "%s: dtype %d is not fp32, bf16 or fp16", who, c->dtype);
+  YTC_REQUIRE(c->layers >= 1 && c->pages >= 0 && c->page >= 1 && c->kv_heads >= 1 && c->dim >= 1 && c->slots >= 0 && c->max_pages >= 0,
+              "%s: bad extents (layers %d, pages %d of %d positions, heads %d, dim %d, slots %d of %d pages)", who, c->layers, c->pages,
+              c->page, c->kv_heads, c->dim, c->slots, c->max_pages);
+  YTC_REQUIRE(c->page <= 65536 && c->kv_heads <= 65536 && c->dim <= 65536 && c->layers <= 65536 &&
+                  static_cast<int64_t>(c->slots) * c->max_pages < (1ll << 31) &&
+                  static_cast<int64_t>(c->page) * c->kv_heads * c->dim < (1ll << 31),
+              "%s: extents above the limits (pages of 65536 positions and 2^31 elements a layer, tables of 2^31 entries)", who);
+  YTC_REQUIRE(c->slots == 0 || c->pages == 0 || (c->k && c->v && c->lens && c->held && c->refs && c->status && c->scratch &&
+                                                (c->table || c->max_pages == 0)),
+              "%s: null tensor in the cache", who);
+  const int size = dtype_size(c->dtype);
+  YTC_REQUIRE((reinterpret_cast<uint64_t>(c->k) | reinterpret_cast<uint64_t>(c->v)) % size == 0, "%s: misaligned pool", who);
+  auto pool = [&](void* p, const int64_t* s) {
+    return PgPool{static_cast<char*>(p), s[0] * size, s[1] * size, s[2] * size, s[3] * size};
+  };
+  for (int i = 0; i < 4; ++i) YTC_REQUIRE(c->k_strides[i] >= 0 && c->v_strides[i] >= 0, "%s: negative stride in a pool", who);
+  *out = PgCache{pool(c->k, c->k_strides), pool(c->v, c->v_strides), c->table, c->lens, c->held, c->refs, c->status, c->scratch,
+                 c->layers, c->pages, c->page, c->kv_heads, c->dim, c->slots, c->max_pages};
+  return YTC_OK;
+}
+
+int pg_rows(const char* who, const char* what, const void* p, const int64_t* strides, int size, PgRows* out) {
+  YTC_REQUIRE(p && strides, "%s: null %s", who, what);
+  YTC_REQUIRE(reinterpret_cast<uint64_t>(p) % size == 0, "%s: misaligned %s", who, what);
+  *out = PgRows{const_cast<char*>(static_cast<const char*>(p)), strides[0] * size, strides[1] * size};
+  return YTC_OK;
+}
+
+static unsigned copy_grid(int64_t items) {
+  const int64_t blocks = (items + PG_WARPS - 1) / PG_WARPS, most = 8ll * sm_count();
+  return static_cast<unsigned>(blocks < 1 ? 1 : blocks < most ? blocks : most);
+}
+
+}  // namespace ytk
+
+using namespace ytk;
+
+// One launch for each width in which rows can be copied.
+#define PG_BY_WIDTH(width, launch)    \
+  do {                                \
+    if ((width) == 16) {              \
+      constexpr int B = 16;           \
+      launch;                         \
+    } else if ((width) == 4) {        \
+      constexpr int B = 4;            \
+      launch;                         \
+    } else {                          \
+      constexpr int B = 2;            \
+      launch;                         \
+    }                                 \
+  } while (0)
+
+extern "C" {
+
+uint64_t ytcuda_pages_scratch(const ytcuda_pages* cache) {
+  if (!cache || cache->slots < 0 || cache->max_pages < 0 || cache->pages < 0) return 0;
+  return 4ull * static_cast<uint64_t>(pg_scratch(cache->slots, cache->max_pages, cache->pages).words);
+}
+
+int ytcuda_pages_append(const ytcuda_pages* cache, int layer, const void* k, const int64_t* k_strides, const void* v,
+                        const int64_t* v_strides, const int32_t* starts, int rows, void* stream) {
+  const char* who = "ytcuda_pages_append";
+  PgCache c;
+  if (const int rc = pg_take(who, cache, &c)) return rc;
+  YTC_REQUIRE(layer >= 0 && layer < c.layers, "%s: layer %d of %d", who, layer, c.layers);
+  YTC_REQUIRE(rows >= 0, "%s: negative number of rows", who);
+  if (rows == 0 || c.slots == 0) return YTC_OK;
+  YTC_REQUIRE(starts != nullptr, "%s: null starts", who);
+  YTC_REQUIRE(c.pages > 0, "%s: a pool without pages", who);
+  const int size = dtype_size(cache->dtype);
+  PgRows kr, vr;
+  if (const int rc = pg_rows(who, "k", k, k_strides, size, &kr)) return rc;
+  if (const int rc = pg_rows(who, "v", v, v_strides, size, &vr)) return rc;
+  const int width = pg_width(pg_bits(c.k) | pg_bits(c.v) | pg_bits(kr) | pg_bits(vr) | static_cast<uint64_t>(c.dim * size));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  PG_BY_WIDTH(width, (pages_append_kernel<B><<<copy_grid(2ll * rows), PG_WARPS * 32, 0, st>>>(c, kr, vr, starts, rows, layer, c.dim * size / B)));
+  count_launch();
+  YTC_CUDA(cudaGetLastError());
+  return YTC_OK;
+}
+
+int ytcuda_pages_reserve(const ytcuda_pages* cache, const int32_t* counts, void* stream) {
+  const char* who = "ytcuda_pages_reserve";
+  PgCache c;
+  if (const int rc = pg_take(who, cache, &c)) return rc;
+  if (c.slots == 0) return YTC_OK;
+  YTC_REQUIRE(counts != nullptr, "%s: null counts", who);
+  YTC_REQUIRE(c.pages > 0, "%s: a pool without pages", who);
+  const int size = dtype_size(cache->dtype);
+  const int width = pg_width(pg_bits(c.k) | pg_bits(c.v) | static_cast<uint64_t>(c.dim * size));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  pages_reserve_kernel<<<1, PG_COUNT, 0, st>>>(c, counts);
+  count_launch();
+  YTC_CUDA(cudaGetLastError());
+  const unsigned grid = copy_grid(2ll * c.slots * c.layers * c.heads);
+  PG_BY_WIDTH(width, YTC_CUDA(pg_launch_behind(pages_copy_kernel<B>, dim3(grid), dim3(PG_WARPS * 32), 0, st, c, c.dim * size / B)));
+  count_launch();
+  return YTC_OK;
+}
+
+int ytcuda_pages_keep(const ytcuda_pages* cache, const int32_t* kept, const int32_t* accepted, int depth, const int32_t* base,
+                      void* stream) {
+  const char* who = "ytcuda_pages_keep";
+  PgCache c;
+  if (const int rc = pg_take(who, cache, &c)) return rc;
+  YTC_REQUIRE(depth >= 0, "%s: negative depth", who);
+  if (c.slots == 0) return YTC_OK;
+  YTC_REQUIRE(kept != nullptr, "%s: null kept", who);
+  YTC_REQUIRE(c.pages > 0, "%s: a pool without pages", who);
+  if (depth == 0) accepted = nullptr;
+  const int size = dtype_size(cache->dtype);
+  const int width = pg_width(pg_bits(c.k) | pg_bits(c.v) | static_cast<uint64_t>(c.dim * size));
+  const unsigned grid = accepted ? copy_grid(2ll * c.slots * c.layers * c.heads) : 1u;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  PG_BY_WIDTH(width, (pages_keep_kernel<B><<<grid, PG_WARPS * 32, 0, st>>>(c, kept, accepted, depth, base, c.dim * size / B)));
+  count_launch();
+  YTC_CUDA(cudaGetLastError());
+  return YTC_OK;
+}
+
+int ytcuda_pages_fork(const ytcuda_pages* cache, const int32_t* source, const int32_t* gone, void* stream) {
+  const char* who = "ytcuda_pages_fork";
+  PgCache c;
+  if (const int rc = pg_take(who, cache, &c)) return rc;
+  if (c.slots == 0) return YTC_OK;
+  YTC_REQUIRE((source != nullptr) != (gone != nullptr), "%s: source or gone, one of them", who);
+  YTC_REQUIRE(c.pages > 0, "%s: a pool without pages", who);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  pages_fork_kernel<<<c.slots, 256, 0, st>>>(c, source, gone);
+  count_launch();
+  YTC_CUDA(cudaGetLastError());
+  YTC_CUDA(pg_launch_behind(pages_fork_store_kernel, dim3(c.slots), dim3(256), 0, st, c));
+  count_launch();
+  return YTC_OK;
+}
+
+int ytcuda_pages_compact(const ytcuda_pages* cache, const ytcuda_pages* into, void* stream) {
+  const char* who = "ytcuda_pages_compact";
+  PgCache c, to;
+  if (const int rc = pg_take(who, cache, &c)) return rc;
+  if (const int rc = pg_take(who, into, &to)) return rc;
+  YTC_REQUIRE(cache->dtype == into->dtype && c.layers == to.layers && c.page == to.page && c.heads == to.heads && c.dim == to.dim &&
+                  c.slots == to.slots && c.max_pages == to.max_pages,
+              "%s: the caches differ in type, layers, page, heads, dim, slots or table", who);
+  if (c.slots == 0) return YTC_OK;
+  YTC_REQUIRE(c.pages > 0 && to.pages > 0, "%s: a pool without pages", who);
+  YTC_REQUIRE(c.k.p != to.k.p && c.k.p != to.v.p && c.v.p != to.v.p && c.v.p != to.k.p && c.table != to.table && c.lens != to.lens &&
+                  c.held != to.held && c.refs != to.refs,
+              "%s: the caches share memory", who);
+  const int size = dtype_size(cache->dtype);
+  const int width = pg_width(pg_bits(c.k) | pg_bits(c.v) | pg_bits(to.k) | pg_bits(to.v) | static_cast<uint64_t>(c.dim * size));
+  int merged = 1;
+  for (const PgPool* p : {&c.k, &c.v, &to.k, &to.v})
+    merged = merged && p->row == c.dim * size && (p->head == c.page * p->row || c.heads == 1);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  pages_number_kernel<<<1, PG_COUNT, 0, st>>>(c, to);
+  count_launch();
+  YTC_CUDA(cudaGetLastError());
+  const unsigned grid = copy_grid(1ll << 30);
+  PG_BY_WIDTH(width, YTC_CUDA(pg_launch_behind(pages_compact_kernel<B>, dim3(grid), dim3(PG_WARPS * 32), 0, st, c, to, c.dim * size / B, merged)));
+  count_launch();
+  return YTC_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,83 @@
+// What the kernels over a cache in pages share (pages.cu, paged_attn.cu): the cache as kernels get it, and the host's checks.
+#pragma once
+#include "ytc_common.cuh"
+
+namespace ytk {
+
+// Rows of new tokens [rows, heads, dim] in memory; strides in bytes.
+struct PgRows {
+  char* p;
+  int64_t row, head;
+};
+
+// One pool of pages; strides in bytes.
+struct PgPool {
+  char* p;
+  int64_t layer, page, head, row;
+};
+
+struct PgCache {
+  PgPool k, v;
+  int32_t *table, *lens, *held, *refs, *status, *scratch;
+  int layers, pages, page, heads, dim, slots, max_pages;
+};
+
+// Places in the scratch of a cache (int32 words).
+struct PgScratch {
+  int64_t ticket, copies, base, mark, src, dst, rows, held, lens, table, ids, number, words;
+};
+__host__ __device__ __forceinline__ PgScratch pg_scratch(int64_t slots, int64_t max_pages, int64_t pages) {
+  PgScratch s;
+  int64_t at = 0;
+  auto take = [&](int64_t n) {
+    const int64_t here = at;
+    at += (n + 3) / 4 * 4;
+    return here;
+  };
+  s.ticket = take(1);
+  s.copies = take(1);
+  s.base = take(slots + 1);
+  s.mark = take(slots);
+  s.src = take(slots);
+  s.dst = take(slots);
+  s.rows = take(slots);
+  s.held = take(slots);
+  s.lens = take(slots);
+  s.table = take(slots * max_pages);
+  s.ids = take(pages);
+  s.number = take(pages);
+  s.words = at;
+  return s;
+}
+
+// Checks a cache that a caller hands in and turns its strides into bytes.
+int pg_take(const char* who, const ytcuda_pages* c, PgCache* out);
+// The rows of new tokens of a call, checked; `heads` of `dim` elements of `size` bytes.
+int pg_rows(const char* who, const char* what, const void* p, const int64_t* strides, int size, PgRows* out);
+// The widest of 16, 4 and 2 bytes in which rows of dim elements of these places can be copied.
+inline int pg_width(uint64_t all_bits_or) { return all_bits_or % 16 == 0 ? 16 : all_bits_or % 4 == 0 ? 4 : 2; }
+inline uint64_t pg_bits(const PgPool& p) {
+  return reinterpret_cast<uint64_t>(p.p) | static_cast<uint64_t>(p.layer | p.page | p.head | p.row);
+}
+inline uint64_t pg_bits(const PgRows& r) { return reinterpret_cast<uint64_t>(r.p) | static_cast<uint64_t>(r.row | r.head); }
+
+#ifdef __CUDACC__
+// Row of position `at` of a slot in one pool (layer and head added by the caller), nullptr where the slot holds no page there.
+__device__ __forceinline__ int pg_page_of(const PgCache& c, int slot, int64_t at) {
+  const int64_t i = at / c.page;
+  if (at < 0 || i >= c.held[slot] || i >= c.max_pages) return -1;
+  const int pg = c.table[static_cast<int64_t>(slot) * c.max_pages + i];
+  return pg >= 0 && pg < c.pages ? pg : -1;
+}
+// A launch behind another of the same call, whose set-up may overlap it: the kernel calls dependent_wait() first of all.
+template <typename... KArgs, typename... Args>
+cudaError_t pg_launch_behind(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args&&... args) {
+  const bool was = overlap_scope();
+  overlap_scope() = true;
+  const cudaError_t e = launch_overlapped(kernel, grid, block, smem, st, static_cast<Args&&>(args)...);
+  overlap_scope() = was;
+  return e;
+}
+#endif
+
+}  // namespace ytk

@@ -1,0 +1,197 @@
+"""Keys and values of many sequences in pages: the cache of a program that serves requests of different lengths, drafts
+tokens ahead, or searches with beams.
+
+A pool holds the keys and values of all layers, [layers, pages, kv_heads, page, dim]. A slot is one sequence: position p lies
+in row p % page of the page that table[slot, p // page] names; the slot holds the first held[slot] entries of its row of the
+table, and lens[slot] positions are written. refs[page] counts the slots that hold a page: a fork shares pages instead of
+copying them, and `reserve` copies the one page that would be written while others hold it too. YTensor has one contiguous
+cache per model (reference example/qwen3/src/qwen3.cpp:70-126) and no counterpart.
+
+Everything lives on the device and no call waits for it, so that a step can be captured in a CUDA graph and replayed at any
+lengths. A step that drafts tokens:
+
+    cache.reserve(counts)                                    # once, for all layers
+    for layer ...: o = cache.attend(layer, q, starts, k, v, parents=parents)
+    cache.keep(kept, accepted)                               # once, for all layers
+
+What only the device can see to be wrong (no free page, an index out of its range, a write into a shared page) is left out
+and noted in `status`; `check()` reads it. Calls on one cache follow one another (one stream, or events between streams).
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _lib
+from ._lib import check, lib
+from .api import _dt, _i64, _require_cuda, _stream
+
+FULL, INVALID, SHARED = 1, 2, 4  # bits of `status`
+_TEXT = {FULL: "too few free pages: nothing was reserved or compacted",
+         INVALID: "an index out of its range, a position without a page, or a tree that is none",
+         SHARED: "rows for a page that other slots hold too (reserve comes first)"}
+
+
+class _Pages(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_strides", C.c_int64 * 4), ("v_strides", C.c_int64 * 4),
+                *((n, C.c_void_p) for n in ("table", "lens", "held", "refs", "status", "scratch")),
+                *((n, C.c_int) for n in ("layers", "pages", "page", "kv_heads", "dim", "slots", "max_pages", "dtype"))]
+
+
+def _bad(text: str):
+    return _lib.YtCudaInvalidArgument(_lib.INVALID_ARG, text)
+
+
+class PagedCache:
+    def __init__(self, layers: int, pages: int, page: int, kv_heads: int, dim: int, slots: int, max_pages: int,
+                 dtype: torch.dtype = torch.bfloat16, device="cuda"):
+        """An empty cache: `pages` pages of `page` positions, `slots` sequences of at most max_pages pages each."""
+        shape = (layers, pages, kv_heads, page, dim)
+        self._set(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device),
+                  *(torch.zeros(s, dtype=torch.int32, device=device) for s in ((slots, max_pages), slots, slots, pages)))
+
+    @classmethod
+    def over(cls, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, held: torch.Tensor,
+             refs: torch.Tensor) -> "PagedCache":
+        """A cache over tensors that are there already. k and v may have any strides (a pool laid out
+        [layers, pages, page, kv_heads, dim] is handed in transposed) but a unit stride along dim."""
+        self = cls.__new__(cls)
+        self._set(k, v, table, lens, held, refs)
+        return self
+
+    def _set(self, k, v, table, lens, held, refs):
+        if k.dim() != 5 or k.shape != v.shape or k.dtype != v.dtype:
+            raise _bad("paged cache: k and v are [layers, pages, kv_heads, page, dim] of one shape and type")
+        for t in (k, v):
+            if t.shape[-1] > 1 and t.stride(-1) != 1:
+                raise _bad("paged cache: k and v need a unit stride along dim")
+        slots = lens.numel()
+        for name, t, shape in (("table", table, (slots, table.shape[-1] if table.dim() else 0)), ("lens", lens, (slots,)),
+                               ("held", held, (slots,)), ("refs", refs, (k.shape[1],))):
+            if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+                raise _bad(f"paged cache: {name} is a contiguous int32 tensor {list(shape)}")
+        if len({t.device for t in (k, v, table, lens, held, refs)}) != 1:
+            raise _bad("paged cache: tensors on different devices")
+        _require_cuda(k)
+        self.k, self.v, self.table, self.lens, self.held, self.refs = k, v, table, lens, held, refs
+        self.layers, self.pages, self.kv_heads, self.page, self.dim = k.shape
+        self.slots, self.max_pages, self.dtype, self.device = slots, table.shape[1], k.dtype, k.device
+        self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
+        c = _Pages(k.data_ptr(), v.data_ptr(), tuple(k.stride()[:4]), tuple(v.stride()[:4]), table.data_ptr(), lens.data_ptr(),
+                   held.data_ptr(), refs.data_ptr(), self.status.data_ptr(), None, self.layers, self.pages, self.page,
+                   self.kv_heads, self.dim, self.slots, self.max_pages, _dt(k))
+        self._scratch = torch.zeros(max(4, lib().ytcuda_pages_scratch(C.addressof(c)) // 4), dtype=torch.int32, device=k.device)
+        c.scratch = self._scratch.data_ptr()
+        self._c, self._at = c, C.addressof(c)
+
+    # ------------------------------------------------------------------ checks of arguments
+    def _here(self):
+        if self.device.index != torch._C._cuda_getDevice():
+            raise _bad(f"paged cache: it lies on {self.device}, which is not the current device")
+
+    def _slots_arg(self, t, name: str, shape=None) -> int:
+        shape = (self.slots,) if shape is None else shape
+        if t.dtype is not torch.int32 or t.shape != shape or t.device != self.device or not t.is_contiguous():
+            raise _bad(f"paged cache: {name} is a contiguous int32 tensor {list(shape)} on {self.device}")
+        return t.data_ptr()
+
+    def _rows_arg(self, t, name: str, rows: int, heads: int) -> tuple:
+        if t.dtype is not self.dtype or t.shape != (rows, heads, self.dim) or t.device != self.device:
+            raise _bad(f"paged cache: {name} is {self.dtype} [{rows}, {heads}, {self.dim}] on {self.device}, "
+                       f"got {t.dtype} {list(t.shape)} on {t.device}")
+        st = t.stride()
+        if st[2] != 1 and self.dim > 1:
+            raise _bad(f"paged cache: {name} needs a unit stride along dim")
+        return t.data_ptr(), _i64(st[:2])
+
+    def _layer(self, layer: int) -> int:
+        if not 0 <= layer < self.layers:
+            raise _bad(f"paged cache: layer {layer} of {self.layers}")
+        return layer
+
+    # ------------------------------------------------------------------ pages
+    def reserve(self, counts: torch.Tensor) -> None:
+        """Room for counts[slot] more positions behind lens[slot] (int32 [slots]; 0: the slot stays as it is). Free pages are
+        handed out in ascending order, slot by slot; where the next position falls inside a page that other slots hold too,
+        the slot first gets a copy of its rows. All slots get their pages or, with FULL in `status`, none."""
+        self._here()
+        check(lib().ytcuda_pages_reserve(self._at, self._slots_arg(counts, "counts"), _stream()))
+
+    def fork(self, source: torch.Tensor) -> None:
+        """All slots at once: slot s becomes a copy of slot source[s] as it was before (int32 [slots]; its own number: it stays
+        as it is, -1: it is emptied). The copy holds the same pages up to its length; nothing is moved."""
+        self._here()
+        check(lib().ytcuda_pages_fork(self._at, self._slots_arg(source, "source"), None, _stream()))
+
+    def free(self, gone: torch.Tensor) -> None:
+        """Empties the slots with gone[slot] != 0 (int32 [slots]); pages that nobody else holds are free again."""
+        self._here()
+        check(lib().ytcuda_pages_fork(self._at, None, self._slots_arg(gone, "gone"), _stream()))
+
+    def keep(self, kept: torch.Tensor, accepted: torch.Tensor | None = None, *, base: torch.Tensor | None = None) -> None:
+        """Of the rows behind position base[slot] (int32 [slots], default lens) the first kept[slot] of accepted [slots, depth]
+        stay, in every layer: row base + accepted[slot, j] moves to base + j, and lens becomes base + kept. Numbers of
+        accepted rows ascend along a row; without `accepted` the first kept[slot] rows stay where they are. The pages behind
+        stay with the slot, for the next drafted rows."""
+        self._here()
+        depth = accepted.shape[-1] if accepted is not None and accepted.dim() else 0
+        check(lib().ytcuda_pages_keep(self._at, self._slots_arg(kept, "kept"),
+                                      None if accepted is None else self._slots_arg(accepted, "accepted", (self.slots, depth)),
+                                      depth, None if base is None else self._slots_arg(base, "base"), _stream()))
+
+    def compact(self, into: "PagedCache") -> None:
+        """The pages in use, in ascending order, become pages 0, 1, .. of another (smaller, larger, differently laid out) cache of
+        the same slots, and its table, lens, held and refs those of this one. FULL in its `status`: its pool is too small,
+        nothing was written."""
+        self._here()
+        if into.device != self.device:
+            raise _bad("paged cache: compact into a cache on another device")
+        check(lib().ytcuda_pages_compact(self._at, into._at, _stream()))
+
+    # ------------------------------------------------------------------ one layer
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor) -> None:
+        """Stores rows of new tokens: row starts[s] + i of k and v [rows, kv_heads, dim] goes to position lens[s] + i of slot s
+        (starts int32 [slots + 1]). lens stays until `keep`, so that every layer of a step writes the same places."""
+        self._here()
+        rows = k.shape[0] if k.dim() else 0
+        check(lib().ytcuda_pages_append(self._at, self._layer(layer), *self._rows_arg(k, "k", rows, self.kv_heads),
+                                        *self._rows_arg(v, "v", rows, self.kv_heads),
+                                        self._slots_arg(starts, "starts", (self.slots + 1,)), rows, _stream()))
+
+    def attend(self, layer: int, q: torch.Tensor, starts: torch.Tensor, k: torch.Tensor | None = None,
+               v: torch.Tensor | None = None, *, parents: torch.Tensor | None = None, scale: float = 0.0,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+        """Attention of new rows: q [rows, heads, dim], rows starts[s] .. starts[s + 1] - 1 are the nodes of slot s, node i at
+        position lens[s] + i. A node sees the lens[s] positions of its sequence, itself and its ancestors: parents (int32
+        [rows]) names for each row a smaller node of its slot, or -1 where it follows the sequence itself; at most 1024 nodes
+        a slot. Without parents the nodes are a chain (the next token, or a piece of a prompt), of any length. heads is a
+        multiple of kv_heads; dim is at most 256. k and v [rows, kv_heads, dim] are stored behind the sequences as by
+        `append`, in the same launch; without them they are in the pages already. scale 0: 1 / sqrt(dim).
+
+        Scores, softmax and sums are fp32, results are rounded to nearest even. Rows behind starts[slots] are not written."""
+        self._here()
+        if q.dim() != 3 or q.shape[1] % self.kv_heads:
+            raise _bad(f"paged cache: q is [rows, heads, dim] with heads a multiple of {self.kv_heads}, got {list(q.shape)}")
+        rows, heads = q.shape[0], q.shape[1]
+        if (k is None) != (v is None):
+            raise _bad("paged cache: k and v come together")
+        if out is None:
+            out = torch.empty((rows, heads, self.dim), dtype=self.dtype, device=self.device)
+        new = (None,) * 4 if k is None else (*self._rows_arg(k, "k", rows, self.kv_heads), *self._rows_arg(v, "v", rows, self.kv_heads))
+        size = lib().ytcuda_pages_attend_workspace(self._at, rows, heads)
+        # (its own for every call: two streams, or two captured graphs, never share it)
+        space = torch.empty(size, dtype=torch.uint8, device=self.device)
+        check(lib().ytcuda_pages_attend(self._at, self._layer(layer), *self._rows_arg(q, "q", rows, heads), *new,
+                                        *self._rows_arg(out, "out", rows, heads),
+                                        self._slots_arg(starts, "starts", (self.slots + 1,)),
+                                        None if parents is None else self._slots_arg(parents, "parents", (rows,)), rows, heads,
+                                        scale, space.data_ptr(), size, _stream()))
+        return out
+
+    def check(self) -> None:
+        """Raises what the device has noted since the last check (waits for the current stream)."""
+        bits = int(self.status.item())
+        if bits:
+            self.status.zero_()
+            raise _lib.YtCudaError(_lib.INVALID_ARG, "paged cache: " + "; ".join(t for b, t in _TEXT.items() if bits & b))

@@ -10,6 +10,8 @@
 // with the running maximum; 2 to the power of s log2(e) throughout. A cut's pieces join as m = max m_i, O = sum 2^(m_i - m) O_i.
 #include <math_constants.h>
 
+#include <type_traits>
+
 #include "pages.cuh"
 
 namespace ytk {
@@ -360,6 +362,626 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_ffma_kernel(const PaPar
   }
 }
 
+// ---------------------------------------------------------------------------------------------- matrix-instruction forms
+// 16-bit types with dims of whole 16-byte words: rows of a tile in the M of mma m16n8k16, keys in its N (S = Q K^T) and then in
+// its K (O += P V). Keys and values stay as they lie in the pages: cp.async brings rows of 2 DP bytes into a ring, 16-byte words
+// at (word ^ row % 8), so that ldmatrix reads eight rows without bank conflicts; what a row of the table does not reach is zero.
+// The softmax reference of a row is its running maximum, moved only when it grows by more than 2^8 (P then stays below 2^8, and
+// a row of O is hardly ever rescaled); P is rounded to the cache's type as the operand of a matrix instruction has to be, its sum
+// l is of the unrounded numbers in fp32.
+constexpr float PA_SLACK = 8.f;
+
+__device__ __forceinline__ void pa_copy16(uint32_t dst, const char* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void pa_copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void pa_copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void pa_ldmatrix(uint32_t at, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void pa_ldmatrix_t(uint32_t at, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void pa_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (sizeof(T) == 2 && !std::is_same<T, __half>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float pa_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pa_pack(float lo, float hi) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __half>::value) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ bool pa_finite2(uint32_t x) {  // both halves
+  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+  return (x & e) != e && ((x >> 16) & e) != e;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pa_finite_part(uint32_t x) {  // zero for a half that is none
+  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+  return ((x & e) != e ? x & 0xffffu : 0u) | (((x >> 16) & e) != e ? x & 0xffff0000u : 0u);
+}
+
+// Where the row of position `at` of a slot and head lies; nullptr where there is none. `pg`: its page, looked up before (-1: none).
+struct PaRow {
+  const char *k, *v;
+};
+__device__ __forceinline__ int pa_lookup(const PaParams& p, int slot, const PaSlot& s, int64_t at) {
+  return at < s.len + static_cast<int64_t>(p.fresh ? 0 : s.nodes) ? pg_page_of(p.c, slot, at) : -1;
+}
+__device__ __forceinline__ PaRow pa_row(const PaParams& p, const PaSlot& s, int head, int64_t at, int pg) {
+  PaRow r{nullptr, nullptr};
+  if (pg >= 0) {
+    const int row = static_cast<int>(at % p.c.page);
+    r.k = p.c.k.p + pg * p.c.k.page + head * p.c.k.head + row * p.c.k.row;
+    r.v = p.c.v.p + pg * p.c.v.page + head * p.c.v.head + row * p.c.v.row;
+  } else if (p.fresh && at >= s.len && at < s.len + static_cast<int64_t>(s.nodes)) {
+    const int64_t row = s.start + (at - s.len);
+    r.k = p.k.p + row * p.k.row + head * p.k.head;
+    r.v = p.v.p + row * p.v.row + head * p.v.head;
+  }
+  return r;
+}
+
+// What one warp holds of 16 rows: thread (g = lane / 4, t = lane % 4) has rows g and g + 8.
+template <typename T, int DP>
+struct PaWarp {
+  float o[DP / 8][4], m[2], l[2];
+  uint32_t q[DP <= 128 ? DP / 16 : 1][4];
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+    m[0] = m[1] = -CUDART_INF_F;
+    l[0] = l[1] = 0.f;
+  }
+
+  // S = Q K^T for NK keys from shared row `key0` on, P, and O += P V. kt, vt: a ring slot's keys and values; q_at: Q in shared
+  // memory where it is too wide for registers. seen(row half, key of the step): for steps that hide something.
+  template <int NK, bool HIDES, typename Seen>
+  __device__ __forceinline__ void step(uint32_t kt, uint32_t vt, int key0, float scale, uint32_t q_at, Seen seen, float* spare) {
+    const int lane = threadIdx.x & 31;
+    float s[NK / 8][4];
+#pragma unroll
+    for (int n = 0; n < NK / 8; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[n][j] = 0.f;
+    const int krow = (lane & 7) + ((lane >> 4) << 3), kword = (lane >> 3) & 1;
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) {
+      uint32_t a[4];
+      if constexpr (DP <= 128) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) a[j] = q[d][j];
+      } else {
+        const int r = lane & 15, w = 2 * d + (lane >> 4);
+        pa_ldmatrix(q_at + r * (DP * 2) + ((w ^ (r & 7)) << 4), a);
+      }
+#pragma unroll
+      for (int n = 0; n < NK / 16; ++n) {
+        const int r = key0 + 16 * n + krow, w = 2 * d + kword;
+        uint32_t b[4];
+        pa_ldmatrix(kt + r * (DP * 2) + ((w ^ (r & 7)) << 4), b);
+        pa_mma<T>(s[2 * n], a, b[0], b[1]);
+        pa_mma<T>(s[2 * n + 1], a, b[2], b[3]);
+      }
+    }
+    float top[2] = {-CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+    for (int n = 0; n < NK / 8; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[n][j] *= scale;
+        if (HIDES && !seen(j >> 1, 8 * n + 2 * (lane & 3) + (j & 1))) s[n][j] = -CUDART_INF_F;
+        top[j >> 1] = fmaxf(top[j >> 1], s[n][j]);
+      }
+    float shrink[2];
+    bool moves = false;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+      const bool up = top[h] > m[h] + PA_SLACK || (m[h] == -CUDART_INF_F && top[h] > m[h]);
+      shrink[h] = up ? pa_exp2(m[h] - top[h]) : 1.f;
+      if (up) m[h] = top[h];
+      moves = moves || up;
+    }
+    if (__any_sync(0xffffffffu, moves)) {
+#pragma unroll
+      for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[i][j] *= shrink[j >> 1];
+      l[0] *= shrink[0];
+      l[1] *= shrink[1];
+    }
+    const float ref[2] = {m[0] == -CUDART_INF_F ? 0.f : m[0], m[1] == -CUDART_INF_F ? 0.f : m[1]};
+#pragma unroll
+    for (int n = 0; n < NK / 8; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[n][j] = pa_exp2(s[n][j] - ref[j >> 1]);
+        l[j >> 1] += s[n][j];
+      }
+    // A hidden row of V that is not finite would spoil every row (0 x infinity): such numbers are left out of the product and
+    // added behind it, to the rows that see them.
+    bool fine = true;
+    if (HIDES) {
+      for (int i = lane; i < NK * DP / 8; i += 32) {
+        uint4 x;
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(vt + key0 * (DP * 2) + i * 16));
+        fine = fine && pa_finite2<T>(x.x) && pa_finite2<T>(x.y) && pa_finite2<T>(x.z) && pa_finite2<T>(x.w);
+      }
+      fine = __all_sync(0xffffffffu, fine);
+    }
+    const int vrow = (lane & 7) + (((lane >> 3) & 1) << 3), vword = lane >> 4;
+#pragma unroll
+    for (int n = 0; n < NK / 16; ++n) {
+      const uint32_t a[4] = {pa_pack<T>(s[2 * n][0], s[2 * n][1]), pa_pack<T>(s[2 * n][2], s[2 * n][3]),
+                             pa_pack<T>(s[2 * n + 1][0], s[2 * n + 1][1]), pa_pack<T>(s[2 * n + 1][2], s[2 * n + 1][3])};
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) {
+        const int r = key0 + 16 * n + vrow, w = 2 * d + vword;
+        uint32_t b[4];
+        pa_ldmatrix_t(vt + r * (DP * 2) + ((w ^ (r & 7)) << 4), b);
+        if (HIDES && !fine) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) b[j] = pa_finite_part<T>(b[j]);
+        }
+        pa_mma<T>(o[2 * d], a, b[0], b[1]);
+        pa_mma<T>(o[2 * d + 1], a, b[2], b[3]);
+      }
+    }
+    if (HIDES && !fine) add_infinite<NK>(s, vt, key0, spare);
+  }
+
+  // O += P V for the numbers of V that are not finite and weights that are not zero. spare: 16 x 8 floats of the warp's own.
+  template <int NK>
+  __device__ __forceinline__ void add_infinite(const float (&s)[NK / 8][4], uint32_t vt, int key0, float* spare) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll 1
+    for (int n = 0; n < NK / 8; ++n) {
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float x = 0.f;
+#pragma unroll
+        for (int i = 0; i < NK / 8; ++i)
+          if (i == n) x = s[i][j];
+        spare[(g + 8 * (j >> 1)) * 8 + 2 * t + (j & 1)] = x;
+      }
+      __syncwarp();
+#pragma unroll 1
+      for (int kk = 0; kk < 8; ++kk) {
+        const float w0 = spare[g * 8 + kk], w1 = spare[(g + 8) * 8 + kk];
+        const int r = key0 + 8 * n + kk;
+#pragma unroll
+        for (int d = 0; d < DP / 8; ++d) {
+          uint32_t x;
+          asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x) : "r"(vt + r * (DP * 2) + ((d ^ (r & 7)) << 4) + 4 * t));
+          if (pa_finite2<T>(x)) continue;
+          const uint32_t odd = x ^ pa_finite_part<T>(x);  // (the finite half is zero)
+          T lo, hi;
+          const uint16_t bits_lo = static_cast<uint16_t>(odd), bits_hi = static_cast<uint16_t>(odd >> 16);
+          memcpy(&lo, &bits_lo, 2);
+          memcpy(&hi, &bits_hi, 2);
+          const float y0 = pa_load(&lo), y1 = pa_load(&hi);
+          if (w0 != 0.f) {
+            o[d][0] = fmaf(w0, y0, o[d][0]);
+            o[d][1] = fmaf(w0, y1, o[d][1]);
+          }
+          if (w1 != 0.f) {
+            o[d][2] = fmaf(w1, y0, o[d][2]);
+            o[d][3] = fmaf(w1, y1, o[d][3]);
+          }
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void finish_sums() {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+    }
+  }
+};
+
+// Two neighbouring elements of a query row as one word (zero past the ends).
+__device__ __forceinline__ uint32_t pa_q2(const PaParams& p, const PaSlot& s, int head, int row, int rows_all, int d) {
+  if (row >= rows_all || d >= p.c.dim) return 0u;
+  const int node = row / p.groups, g = row - node * p.groups;
+  return *reinterpret_cast<const uint32_t*>(p.q.p + (s.start + static_cast<int64_t>(node)) * p.q.row + (head * p.groups + g) * p.q.head + 2 * d);
+}
+
+// Rows of new keys and values that a tile holds in shared memory go to their pages. `first` .. `first + n`: positions, `row0`: the
+// shared row of the first; for `nt` threads of which this is number t.
+template <int DP>
+__device__ __forceinline__ void pa_store_new(const PaParams& p, const PaSlot& s, int slot, int head, int64_t first, int n, uint32_t kt,
+                                             uint32_t vt, int row0, int t, int nt) {
+  const int words = p.c.dim / 8;
+  for (int i = t; i < n * words; i += nt) {
+    const int r = i / words, w = i - r * words;
+    const int64_t at = first + r;
+    if (at < s.len || at >= s.len + static_cast<int64_t>(s.nodes)) continue;
+    const int pg = pg_page_of(p.c, slot, at);
+    if (pg < 0 || p.c.refs[pg] != 1) {
+      atomicOr(p.c.status, pg < 0 ? YTC_PAGES_INVALID : YTC_PAGES_SHARED);
+      continue;
+    }
+    const int row = static_cast<int>(at % p.c.page);
+    const uint32_t off = (row0 + r) * (DP * 2) + ((w ^ ((row0 + r) & 7)) << 4);
+    uint4 x;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(kt + off));
+    *reinterpret_cast<uint4*>(p.c.k.p + pg * p.c.k.page + head * p.c.k.head + row * p.c.k.row + w * 16) = x;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(vt + off));
+    *reinterpret_cast<uint4*>(p.c.v.p + pg * p.c.v.page + head * p.c.v.head + row * p.c.v.row + w * 16) = x;
+  }
+}
+
+// Up to 16 rows: every warp has its own keys (16 of each tile of 64), its own ring, and no barrier until the unit ends, where the
+// four warps' sums are joined. What bounds it is the copy of keys and values: 512 bytes a key and head at dim 128.
+template <typename T, int DP>
+struct PaNarrow {
+  static constexpr int RT = 16, BN = 64, WARPS = 4, STAGES = DP == 64 ? 6 : 3, SLOT = 16 * DP * 2;  // bytes of 16 keys
+  uint4 ring[WARPS][STAGES][2][SLOT / 16];
+  uint4 q[DP > 128 ? 16 * DP * 2 / 16 : 1];
+  float spare[WARPS][16 * 8];
+  float m[WARPS][16], l[WARPS][16];
+  uint32_t seen[RT][PA_TREE / 32];
+  int16_t up[PA_TREE];
+  int64_t from, to, before;
+  int slot;
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) paged_attn_narrow_kernel(const PaParams p) {
+  using S = PaNarrow<T, DP>;
+  constexpr int RT = S::RT, BN = S::BN, ST = S::STAGES, WORDS = DP / 8, PER = 32 / WORDS;  // rows of a copy instruction
+  extern __shared__ __align__(128) unsigned char raw[];
+  S& sm = *reinterpret_cast<S*>(raw);
+  dependent_trigger();
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, g = lane >> 2, c4 = lane & 3;
+  const PgCache& c = p.c;
+  if (warp == 0) {
+    bool bad = false;
+    const PaPlace at = pa_place(p, RT, BN, blockIdx.x, gridDim.x, &bad);
+    if (__any_sync(0xffffffffu, bad) && lane == 0 && blockIdx.x == 0) atomicOr(c.status, YTC_PAGES_INVALID);
+    if (lane == 0) {
+      sm.from = at.at;
+      sm.to = at.total * (blockIdx.x + 1) / gridDim.x;
+      sm.before = at.before;
+      sm.slot = at.slot;
+    }
+  }
+  __syncthreads();
+  int64_t pos = sm.from;
+  const int64_t end = sm.to;
+  int slot = sm.slot;
+  int64_t off = pos - sm.before;
+  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(sm.ring[warp]));
+  const int word = lane % WORDS, words = c.dim / 8;
+  while (pos < end) {
+    bool bad = false;
+    const PaSlot s = pa_slot(p, slot, &bad);
+    const int64_t work = pa_work(p, s, RT, BN);
+    if (off >= work) {
+      off -= work;
+      ++slot;
+      continue;
+    }
+    const int tiles = pa_key_tiles(s, BN), row_tiles = pa_row_tiles(p, s, RT);
+    const int unit = static_cast<int>(off / tiles), t0 = static_cast<int>(off - static_cast<int64_t>(unit) * tiles);
+    const int t1 = static_cast<int>(end - pos < tiles - t0 ? t0 + (end - pos) : tiles);
+    const int head = unit / row_tiles, rtile = unit - head * row_tiles;
+    const int row0 = rtile * RT, rows_all = s.nodes * p.groups, rows = min(RT, rows_all - row0);
+    const int64_t mine = 16 * warp;
+    // (a lane looks up the page of key lane % 16 of a step, one step before the copies need it)
+    const auto lookup = [&](int tile) { return tile < t1 ? pa_lookup(p, slot, s, static_cast<int64_t>(tile) * BN + mine + (lane & 15)) : -1; };
+    const auto fetch = [&](int tile, int pg) {
+      if (tile < t1) {
+        const PaRow r = pa_row(p, s, head, static_cast<int64_t>(tile) * BN + mine + (lane & 15), pg);
+        const uint32_t kt = ring + (tile - t0) % ST * (2 * S::SLOT);
+        const unsigned long long kp = reinterpret_cast<unsigned long long>(r.k), vp = reinterpret_cast<unsigned long long>(r.v);
+#pragma unroll
+        for (int i = 0; i < 16 / PER; ++i) {
+          const int row = i * PER + lane / WORDS;
+          const unsigned long long a = __shfl_sync(0xffffffffu, kp, row), b = __shfl_sync(0xffffffffu, vp, row);
+          const bool there = a != 0 && word < words;
+          const uint32_t to = kt + row * (DP * 2) + ((word ^ (row & 7)) << 4);
+          pa_copy16(to, there ? reinterpret_cast<const char*>(a) + word * 16 : c.k.p, there);
+          pa_copy16(to + S::SLOT, there ? reinterpret_cast<const char*>(b) + word * 16 : c.v.p, there);
+        }
+      }
+      pa_copy_commit();
+    };
+    __syncthreads();  // (the unit before is done with the shared memory)
+    int pg = lookup(t0);
+#pragma unroll
+    for (int i = 0; i < ST - 1; ++i) {
+      const int next = lookup(t0 + i + 1);
+      fetch(t0 + i, pg);
+      pg = next;
+    }
+    PaWarp<T, DP> w;
+    w.clear();
+    uint32_t q_at = 0;
+    if constexpr (DP <= 128) {
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w.q[d][j] = pa_q2(p, s, head, row0 + g + 8 * (j & 1), rows_all, 16 * d + 2 * c4 + 8 * (j >> 1));
+    } else {
+      q_at = static_cast<uint32_t>(__cvta_generic_to_shared(sm.q));
+      for (int i = t; i < 16 * DP / 2; i += PA_THREADS) {
+        const int r = i / (DP / 2), d = i % (DP / 2) * 2;
+        reinterpret_cast<uint32_t*>(sm.q)[r * (DP / 2) + (((d / 8) ^ (r & 7)) * 4) + d % 8 / 2] = pa_q2(p, s, head, row0 + r, rows_all, d);
+      }
+      __syncthreads();
+    }
+    const int node0 = row0 / p.groups;
+    const int node[2] = {(row0 + min(g, rows - 1)) / p.groups, (row0 + min(g + 8, rows - 1)) / p.groups};
+    if (p.parents && t1 * static_cast<int64_t>(BN) > s.len) pa_ancestors(p, s, node0, min(RT, s.nodes - node0), sm.seen, sm.up);
+    for (int tile = t0; tile < t1; ++tile) {
+      const int next = lookup(tile + ST);
+      fetch(tile + ST - 1, pg);  // (into the slot that the step before has read)
+      pg = next;
+      pa_copy_wait<ST - 1>();
+      __syncwarp();
+      const uint32_t kt = ring + (tile - t0) % ST * (2 * S::SLOT), vt = kt + S::SLOT;
+      const int64_t first = static_cast<int64_t>(tile) * BN + mine;
+      if (first + 16 <= s.len) {
+        w.template step<16, false>(kt, vt, 0, p.scale, q_at, [](int, int) { return true; }, nullptr);
+      } else if (first < s.len + static_cast<int64_t>(s.nodes)) {
+        const int before = static_cast<int>(s.len - first);
+        w.template step<16, true>(
+            kt, vt, 0, p.scale, q_at,
+            [&](int h, int key) {
+              const int n = key - before;
+              if (n < 0) return true;
+              if (n >= s.nodes) return false;
+              return p.parents ? ((sm.seen[node[h] - node0][n >> 5] >> (n & 31)) & 1) != 0 : n <= node[h];
+            },
+            sm.spare[warp]);
+        if (p.fresh && rtile == 0) pa_store_new<DP>(p, s, slot, head, first, 16, kt, vt, 0, lane, 32);
+      }
+      __syncwarp();
+    }
+    pa_copy_wait<0>();
+    w.finish_sums();
+    // the warps' sums: O of each in its own ring
+    __syncwarp();
+    float* mine_o = reinterpret_cast<float*>(sm.ring[warp]);
+#pragma unroll
+    for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) *reinterpret_cast<float2*>(mine_o + (g + 8 * h) * DP + 8 * d + 2 * c4) = make_float2(w.o[d][2 * h], w.o[d][2 * h + 1]);
+    if (c4 == 0) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        sm.m[warp][g + 8 * h] = w.m[h];
+        sm.l[warp][g + 8 * h] = w.l[h];
+      }
+    }
+    __syncthreads();
+    const bool whole = t0 == 0 && t1 == tiles;
+    float* piece = p.work + (2 * static_cast<int64_t>(blockIdx.x) + (t0 == 0)) * pa_piece(RT, DP);
+    for (int i = t; i < rows * (DP / 4); i += PA_THREADS) {
+      const int r = i / (DP / 4), d = i % (DP / 4) * 4;
+      float m = -CUDART_INF_F;
+#pragma unroll
+      for (int k = 0; k < S::WARPS; ++k) m = fmaxf(m, sm.m[k][r]);
+      float l = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < S::WARPS; ++k) {
+        const float mk = sm.m[k][r], f = mk == -CUDART_INF_F ? 0.f : pa_exp2(mk - m);
+        const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sm.ring[k]) + r * DP + d);
+        l = fmaf(f, sm.l[k][r], l);
+        o.x = fmaf(f, x.x, o.x);
+        o.y = fmaf(f, x.y, o.y);
+        o.z = fmaf(f, x.z, o.z);
+        o.w = fmaf(f, x.w, o.w);
+      }
+      if (whole) {
+        if (d >= c.dim) continue;
+        const int nd = (row0 + r) / p.groups, gg = (row0 + r) % p.groups;
+        const float f = 1.f / l;
+        *reinterpret_cast<uint2*>(p.o.p + (s.start + static_cast<int64_t>(nd)) * p.o.row + (head * p.groups + gg) * p.o.head + 2 * d) =
+            make_uint2(pa_pack<T>(o.x * f, o.y * f), pa_pack<T>(o.z * f, o.w * f));
+      } else {
+        *reinterpret_cast<float4*>(piece + r * DP + d) = o;
+        if (d == 0) {
+          piece[RT * DP + r] = m;
+          piece[RT * DP + RT + r] = l;
+        }
+      }
+    }
+    pos += t1 - t0;
+    off += t1 - t0;
+  }
+}
+
+// Up to 64 rows of a tile: a warp for 16 of them (warps without rows only copy), all over the same tiles of 64 keys.
+template <typename T, int DP>
+struct PaWide {
+  static constexpr int RT = 64, BN = 64, STAGES = 3, SLOT = BN * DP * 2;
+  uint4 ring[STAGES][2][SLOT / 16];
+  uint4 q[DP > 128 ? RT * DP * 2 / 16 : 1];
+  const char* row[2][2][BN];  // (where the next tile's rows lie)
+  float spare[4][16 * 8];
+  uint32_t seen[RT][PA_TREE / 32];
+  int16_t up[PA_TREE];
+  int64_t from, to, before;
+  int slot;
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) paged_attn_wide_kernel(const PaParams p) {
+  using S = PaWide<T, DP>;
+  constexpr int RT = S::RT, BN = S::BN, ST = S::STAGES, WORDS = DP / 8, PER = PA_THREADS / WORDS;
+  extern __shared__ __align__(128) unsigned char raw[];
+  S& sm = *reinterpret_cast<S*>(raw);
+  dependent_trigger();
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, g = lane >> 2, c4 = lane & 3;
+  const PgCache& c = p.c;
+  if (warp == 0) {
+    bool bad = false;
+    const PaPlace at = pa_place(p, RT, BN, blockIdx.x, gridDim.x, &bad);
+    if (__any_sync(0xffffffffu, bad) && lane == 0 && blockIdx.x == 0) atomicOr(c.status, YTC_PAGES_INVALID);
+    if (lane == 0) {
+      sm.from = at.at;
+      sm.to = at.total * (blockIdx.x + 1) / gridDim.x;
+      sm.before = at.before;
+      sm.slot = at.slot;
+    }
+  }
+  __syncthreads();
+  int64_t pos = sm.from;
+  const int64_t end = sm.to;
+  int slot = sm.slot;
+  int64_t off = pos - sm.before;
+  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(sm.ring));
+  const int word = t % WORDS, words = c.dim / 8;
+  while (pos < end) {
+    bool bad = false;
+    const PaSlot s = pa_slot(p, slot, &bad);
+    const int64_t work = pa_work(p, s, RT, BN);
+    if (off >= work) {
+      off -= work;
+      ++slot;
+      continue;
+    }
+    const int tiles = pa_key_tiles(s, BN), row_tiles = pa_row_tiles(p, s, RT);
+    const int unit = static_cast<int>(off / tiles), t0 = static_cast<int>(off - static_cast<int64_t>(unit) * tiles);
+    const int t1 = static_cast<int>(end - pos < tiles - t0 ? t0 + (end - pos) : tiles);
+    const int head = unit / row_tiles, rtile = unit - head * row_tiles;
+    const int row0 = rtile * RT, rows_all = s.nodes * p.groups, rows = min(RT, rows_all - row0);
+    const int node_last = (row0 + rows - 1) / p.groups;
+    // Thread t < 64 finds row t of a tile, one tile before the copies of it.
+    const auto find = [&](int tile) {
+      if (t < BN && tile < t1) {
+        const int64_t at = static_cast<int64_t>(tile) * BN + t;
+        const PaRow r = pa_row(p, s, head, at, pa_lookup(p, slot, s, at));
+        sm.row[tile & 1][0][t] = r.k;
+        sm.row[tile & 1][1][t] = r.v;
+      }
+    };
+    const auto fetch = [&](int tile) {
+      if (tile < t1) {
+        const uint32_t kt = ring + (tile - t0) % ST * (2 * S::SLOT);
+#pragma unroll
+        for (int i = 0; i < BN / PER; ++i) {
+          const int row = i * PER + t / WORDS;
+          const char *a = sm.row[tile & 1][0][row], *b = sm.row[tile & 1][1][row];
+          const bool there = a != nullptr && word < words;
+          const uint32_t to = kt + row * (DP * 2) + ((word ^ (row & 7)) << 4);
+          pa_copy16(to, there ? a + word * 16 : c.k.p, there);
+          pa_copy16(to + S::SLOT, there ? b + word * 16 : c.v.p, there);
+        }
+      }
+      pa_copy_commit();
+    };
+    __syncthreads();
+    find(t0);
+    find(t0 + 1);
+    __syncthreads();
+    fetch(t0);
+    fetch(t0 + 1);
+    __syncthreads();
+    find(t0 + 2);
+    PaWarp<T, DP> w;
+    w.clear();
+    const int wrow = row0 + 16 * warp;
+    uint32_t q_at = 0;
+    if constexpr (DP <= 128) {
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w.q[d][j] = pa_q2(p, s, head, wrow + g + 8 * (j & 1), rows_all, 16 * d + 2 * c4 + 8 * (j >> 1));
+    } else {
+      q_at = static_cast<uint32_t>(__cvta_generic_to_shared(sm.q)) + warp * 16 * (DP * 2);
+      for (int i = t; i < RT * DP / 2; i += PA_THREADS) {
+        const int r = i / (DP / 2), d = i % (DP / 2) * 2;
+        reinterpret_cast<uint32_t*>(sm.q)[r * (DP / 2) + (((d / 8) ^ (r & 7)) * 4) + d % 8 / 2] = pa_q2(p, s, head, row0 + r, rows_all, d);
+      }
+    }
+    const int node0 = row0 / p.groups;
+    const int node[2] = {min(wrow + g, rows_all - 1) / p.groups, min(wrow + g + 8, rows_all - 1) / p.groups};
+    if (p.parents && t1 * static_cast<int64_t>(BN) > s.len) pa_ancestors(p, s, node0, node_last - node0 + 1, sm.seen, sm.up);
+    for (int tile = t0; tile < t1; ++tile) {
+      pa_copy_wait<ST - 2>();
+      __syncthreads();  // the tile is there, the one before has been read, and where the next rows lie has been written
+      fetch(tile + ST - 1);
+      const uint32_t kt = ring + (tile - t0) % ST * (2 * S::SLOT), vt = kt + S::SLOT;
+      const int64_t first = static_cast<int64_t>(tile) * BN;
+      if (16 * warp < rows) {
+        if (first + BN <= s.len) {
+          w.template step<BN, false>(kt, vt, 0, p.scale, q_at, [](int, int) { return true; }, nullptr);
+        } else if (first <= s.len + static_cast<int64_t>(node_last)) {
+          const int before = static_cast<int>(s.len - first);
+          w.template step<BN, true>(
+              kt, vt, 0, p.scale, q_at,
+              [&](int h, int key) {
+                const int n = key - before;
+                if (n < 0) return true;
+                if (n > node_last) return false;
+                return p.parents ? ((sm.seen[node[h] - node0][n >> 5] >> (n & 31)) & 1) != 0 : n <= node[h];
+              },
+              sm.spare[warp]);
+        }
+      }
+      if (p.fresh && rtile == 0 && first + BN > s.len) pa_store_new<DP>(p, s, slot, head, first, BN, kt, vt, 0, t, PA_THREADS);
+      find(tile + ST);
+    }
+    pa_copy_wait<0>();
+    w.finish_sums();
+    const bool whole = t0 == 0 && t1 == tiles;
+    float* piece = p.work + (2 * static_cast<int64_t>(blockIdx.x) + (t0 == 0)) * pa_piece(RT, DP);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = 16 * warp + g + 8 * h;
+      if (r >= rows) continue;
+      if (whole) {
+        char* out = p.o.p + (s.start + static_cast<int64_t>(node[h])) * p.o.row + (head * p.groups + (row0 + r) % p.groups) * p.o.head;
+        const float f = 1.f / w.l[h];
+#pragma unroll
+        for (int d = 0; d < DP / 8; ++d)
+          if (8 * d < c.dim) *reinterpret_cast<uint32_t*>(out + 16 * d + 4 * c4) = pa_pack<T>(w.o[d][2 * h] * f, w.o[d][2 * h + 1] * f);
+      } else {
+#pragma unroll
+        for (int d = 0; d < DP / 8; ++d) *reinterpret_cast<float2*>(piece + r * DP + 8 * d + 2 * c4) = make_float2(w.o[d][2 * h], w.o[d][2 * h + 1]);
+        if (c4 == 0) {
+          piece[RT * DP + r] = w.m[h];
+          piece[RT * DP + RT + r] = w.l[h];
+        }
+      }
+    }
+    pos += t1 - t0;
+    off += t1 - t0;
+  }
+}
+
 // ---------------------------------------------------------------------------------------------- joining
 // CTA (x, y): the unit that cut number x + 1 runs through, if it is the first one inside it; rows y, y + gridDim.y, ...; the
 // pieces are shared by the warps, and their sums by way of shared memory joined in the order of the warps.
@@ -467,21 +1089,47 @@ static void pa_ffma(PaForm* f) {
   f->kernel = reinterpret_cast<const void*>(paged_attn_ffma_kernel<T, DP, RPT>);
   f->ctas = sm_count() * (f->smem <= 110 * 1024 ? 2 : 1);
 }
+template <typename T, int DP>
+static void pa_mma_form(PaForm* f, int rows) {
+  f->dp = DP;
+  f->ctas = sm_count() * (DP == 256 ? 1 : 2);
+  if (rows <= 16) {
+    f->rt = PaNarrow<T, DP>::RT;
+    f->bn = PaNarrow<T, DP>::BN;
+    f->smem = static_cast<int>(sizeof(PaNarrow<T, DP>));
+    f->kernel = reinterpret_cast<const void*>(paged_attn_narrow_kernel<T, DP>);
+  } else {
+    f->rt = PaWide<T, DP>::RT;
+    f->bn = PaWide<T, DP>::BN;
+    f->smem = static_cast<int>(sizeof(PaWide<T, DP>));
+    f->kernel = reinterpret_cast<const void*>(paged_attn_wide_kernel<T, DP>);
+  }
+}
 template <typename T>
-static PaForm pa_form(int dim, int rows) {
+static PaForm pa_form(int dim, int rows, bool words) {
   PaForm f{};
+  if constexpr (sizeof(T) == 2) {
+    if (words) {
+      dim <= 64 ? pa_mma_form<T, 64>(&f, rows) : dim <= 128 ? pa_mma_form<T, 128>(&f, rows) : pa_mma_form<T, 256>(&f, rows);
+      return f;
+    }
+  }
   if (dim <= 64) rows <= 8 ? pa_ffma<T, 64, 1>(&f) : rows <= 16 ? pa_ffma<T, 64, 2>(&f) : pa_ffma<T, 64, 4>(&f);
   else if (dim <= 128) rows <= 8 ? pa_ffma<T, 128, 1>(&f) : rows <= 16 ? pa_ffma<T, 128, 2>(&f) : pa_ffma<T, 128, 4>(&f);
   else rows <= 8 ? pa_ffma<T, 256, 1>(&f) : rows <= 16 ? pa_ffma<T, 256, 2>(&f) : pa_ffma<T, 256, 4>(&f);
   return f;
 }
-// The form of a call: `rows` rows over `slots` slots. Tiles of as many rows as a slot with an even share of them has.
-static PaForm pa_choose(const ytcuda_pages* c, int rows, int heads) {
+// The form of a call: `rows` rows over `slots` slots. Tiles of as many rows as a slot with an even share of them has. `words`: all
+// rows are whole 16-byte words on their boundaries.
+static PaForm pa_choose(const ytcuda_pages* c, int rows, int heads, bool words) {
   const int share = c->slots ? (rows + c->slots - 1) / c->slots : 1;
   const int64_t tile = static_cast<int64_t>(share) * (heads / c->kv_heads);
   const int r = static_cast<int>(tile < 4096 ? tile : 4096);
-  return c->dtype == YTC_F32 ? pa_form<float>(c->dim, r) : c->dtype == YTC_BF16 ? pa_form<__nv_bfloat16>(c->dim, r) : pa_form<__half>(c->dim, r);
+  return c->dtype == YTC_F32    ? pa_form<float>(c->dim, r, words)
+         : c->dtype == YTC_BF16 ? pa_form<__nv_bfloat16>(c->dim, r, words)
+                                : pa_form<__half>(c->dim, r, words);
 }
+static uint64_t pa_space(const PaForm& f) { return 4ull * 2 * static_cast<uint64_t>(f.ctas) * static_cast<uint64_t>(pa_piece(f.rt, f.dp)); }
 
 template <typename T>
 static cudaError_t pa_join(const PaForm& f, const PaParams& p, cudaStream_t st) {
@@ -499,8 +1147,8 @@ extern "C" {
 
 uint64_t ytcuda_pages_attend_workspace(const ytcuda_pages* cache, int rows, int heads) {
   if (!cache || rows <= 0 || heads <= 0 || cache->kv_heads <= 0 || cache->slots <= 0 || cache->dim <= 0) return 0;
-  const PaForm f = pa_choose(cache, rows, heads);
-  return 4ull * 2 * static_cast<uint64_t>(f.ctas) * static_cast<uint64_t>(pa_piece(f.rt, f.dp));
+  const uint64_t a = pa_space(pa_choose(cache, rows, heads, false)), b = pa_space(pa_choose(cache, rows, heads, true));
+  return a > b ? a : b;
 }
 
 int ytcuda_pages_attend(const ytcuda_pages* cache, int layer, const void* q, const int64_t* q_strides, const void* k,
@@ -529,7 +1177,9 @@ int ytcuda_pages_attend(const ytcuda_pages* cache, int layer, const void* q, con
     if (const int rc = pg_rows(who, "k", k, k_strides, size, &p.k)) return rc;
     if (const int rc = pg_rows(who, "v", v, v_strides, size, &p.v)) return rc;
   }
-  const PaForm f = pa_choose(cache, rows, heads);
+  const bool words = pg_width(pg_bits(p.c.k) | pg_bits(p.c.v) | pg_bits(p.q) | pg_bits(p.o) | pg_bits(p.k) | pg_bits(p.v) |
+                              static_cast<uint64_t>(p.c.dim * size)) == 16;
+  const PaForm f = pa_choose(cache, rows, heads, words);
   YTC_REQUIRE(workspace && workspace_bytes >= ytcuda_pages_attend_workspace(cache, rows, heads) && reinterpret_cast<uint64_t>(workspace) % 16 == 0,
               "%s: a workspace of %llu bytes on a 16-byte boundary is needed", who,
               static_cast<unsigned long long>(ytcuda_pages_attend_workspace(cache, rows, heads)));

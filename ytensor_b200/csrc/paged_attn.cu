@@ -23,11 +23,13 @@ constexpr float PA_LOG2E = 1.4426950408889634f;
 struct PaParams {
   PgCache c;  // (the pools at the layer)
   PgRows q, k, v, o;
+  PgDiv by_group;  // division by the query heads of a key head
   const int32_t *starts, *parents;
-  int rows, heads, groups;
-  int fresh;  // k and v hold the new rows: they are read from there, and stored
+  int rows, groups;
+  int fresh;    // k and v hold the new rows: they are read from there, and stored
   float scale;  // times log2(e)
-  float* work;
+  float* work;  // pieces of cut units
+  int4* cuts;   // two words for each CTA: the unit that starts in its share and goes on behind it
 };
 
 // What a slot brings: its rows in the call, its nodes, its length.
@@ -36,63 +38,144 @@ struct PaSlot {
 };
 __device__ __forceinline__ PaSlot pa_slot(const PaParams& p, int s, bool* bad) {
   PaSlot r{p.starts[s], p.starts[s + 1], p.c.lens[s]};
-  const int end = r.nodes;
+  const int end = r.nodes, held = p.c.held[s];
   r.nodes = end - r.start;
   const bool ok = r.start >= 0 && end >= r.start && end <= p.rows && r.len >= 0 && !(p.parents && r.nodes > PA_TREE) &&
-                  r.len + static_cast<int64_t>(p.fresh ? 0 : r.nodes) <= static_cast<int64_t>(p.c.held[s]) * p.c.page &&
-                  p.c.held[s] <= p.c.max_pages;
+                  r.len <= 0x7ffffff0 - r.nodes && held <= p.c.max_pages &&
+                  r.len + static_cast<int64_t>(p.fresh ? 0 : r.nodes) <= static_cast<int64_t>(held) * p.c.page;
   if (!ok) {
     *bad = *bad || r.nodes != 0;
     r.nodes = 0;
   }
   return r;
 }
-__device__ __forceinline__ int pa_key_tiles(const PaSlot& s, int bn) { return static_cast<int>((static_cast<int64_t>(s.len) + s.nodes + bn - 1) / bn); }
-__device__ __forceinline__ int pa_row_tiles(const PaParams& p, const PaSlot& s, int rt) {
-  return static_cast<int>((static_cast<int64_t>(s.nodes) * p.groups + rt - 1) / rt);
+// Key tiles and row tiles of a slot; the units of a slot are its heads' row tiles, the row tiles of a head next to one another (they
+// read the same keys at about the same time). All numbers stay below 2^31: the host sees to that.
+template <int BN>
+__device__ __forceinline__ uint32_t pa_key_tiles(const PaSlot& s) {
+  return (static_cast<uint32_t>(s.len) + static_cast<uint32_t>(s.nodes) + BN - 1) / BN;
 }
-__device__ __forceinline__ int64_t pa_work(const PaParams& p, const PaSlot& s, int rt, int bn) {
-  return s.nodes ? static_cast<int64_t>(pa_key_tiles(s, bn)) * pa_row_tiles(p, s, rt) * p.c.heads : 0;
+template <int RT>
+__device__ __forceinline__ uint32_t pa_row_tiles(const PaParams& p, const PaSlot& s) {
+  return (static_cast<uint32_t>(s.nodes) * static_cast<uint32_t>(p.groups) + RT - 1) / RT;
+}
+template <int RT, int BN>
+__device__ __forceinline__ uint32_t pa_work(const PaParams& p, const PaSlot& s) {
+  return s.nodes ? pa_key_tiles<BN>(s) * pa_row_tiles<RT>(p, s) * p.c.heads : 0u;
 }
 
-// All key tiles of the call, and the slot that tile total * part / parts falls into with the tiles in front of it. For one warp.
-struct PaPlace {
-  int64_t total, at, before;
+// The share of a CTA: tiles from .. to of all, the first of them tile `off` of slot `slot`. Shares differ by at most one tile, the
+// longer ones first: share i begins at i * each + min(i, more).
+struct PaShare {
+  uint32_t from, to, off, each, more;
   int slot;
 };
-__device__ __forceinline__ PaPlace pa_place(const PaParams& p, int rt, int bn, int64_t part, int64_t parts, bool* bad) {
-  const int lane = threadIdx.x & 31;
-  PaPlace r{0, 0, 0, p.c.slots};
-  for (int s0 = 0; s0 < p.c.slots; s0 += 32) {
-    int64_t w = s0 + lane < p.c.slots ? pa_work(p, pa_slot(p, s0 + lane, bad), rt, bn) : 0;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
-    r.total += w;
-  }
-  r.at = r.total * part / parts;
-  int64_t before = 0;
-  for (int s0 = 0; s0 < p.c.slots; s0 += 32) {
-    const int64_t w = s0 + lane < p.c.slots ? pa_work(p, pa_slot(p, s0 + lane, bad), rt, bn) : 0;
-    int64_t x = w;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
+__device__ __forceinline__ uint32_t pa_share_of(const PaShare& s, uint32_t tile) {
+  const uint32_t longer = s.more * (s.each + 1);
+  return tile < longer ? tile / (s.each + 1) : s.more + (tile - longer) / s.each;
+}
+// All threads of the CTA call it; one warp works it out.
+template <int RT, int BN>
+__device__ __forceinline__ void pa_share(const PaParams& p, PaShare* out) {
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    bool bad = false;
+    uint32_t total = 0, w = 0;
+    for (int s0 = 0; s0 < p.c.slots; s0 += 32) {
+      w = s0 + lane < p.c.slots ? pa_work<RT, BN>(p, pa_slot(p, s0 + lane, &bad)) : 0;
+      total += __reduce_add_sync(0xffffffffu, w);
     }
-    const unsigned hit = __ballot_sync(0xffffffffu, before + x > r.at);
-    if (hit) {
-      const int l = __ffs(hit) - 1;
-      r.slot = s0 + l;
-      r.before = before + __shfl_sync(0xffffffffu, x - w, l);
-      return r;
+    if (blockIdx.x == 0 && __any_sync(0xffffffffu, bad) && lane == 0) atomicOr(p.c.status, YTC_PAGES_INVALID);
+    PaShare r;
+    r.each = total / gridDim.x;
+    r.more = total - r.each * gridDim.x;
+    r.from = blockIdx.x * r.each + min(blockIdx.x, r.more);
+    r.to = r.from + r.each + (blockIdx.x < r.more);
+    r.off = 0;
+    r.slot = p.c.slots;
+    uint32_t before = 0;
+    for (int s0 = 0; s0 < p.c.slots; s0 += 32) {
+      if (p.c.slots > 32) w = s0 + lane < p.c.slots ? pa_work<RT, BN>(p, pa_slot(p, s0 + lane, &bad)) : 0;
+      uint32_t x = w;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, before + x > r.from);
+      if (hit) {
+        const int l = __ffs(hit) - 1;
+        r.slot = s0 + l;
+        r.off = r.from - before - __shfl_sync(0xffffffffu, x - w, l);
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, x, 31);
     }
-    before += __shfl_sync(0xffffffffu, x, 31);
+    if (lane == 0) *out = r;
   }
+  __syncthreads();
+}
+
+// A piece of work: tiles t0 .. t1 of a unit that has `tiles`.
+struct PaPart {
+  PaSlot s;
+  uint32_t tiles, t0, t1;
+  int slot, head, rtile, row0, rows, rows_all;
+};
+// The next piece at tile `pos` of all (tile `off` of slot `slot`, both moved past slots without rows).
+template <int RT, int BN>
+__device__ __forceinline__ PaPart pa_part(const PaParams& p, uint32_t pos, uint32_t end, int* slot, uint32_t* off) {
+  PaPart r;
+  bool bad = false;
+  while (true) {
+    r.s = pa_slot(p, *slot, &bad);
+    const uint32_t work = pa_work<RT, BN>(p, r.s);
+    if (*off < work) break;
+    *off -= work;
+    ++*slot;
+  }
+  r.slot = *slot;
+  r.tiles = pa_key_tiles<BN>(r.s);
+  const uint32_t row_tiles = pa_row_tiles<RT>(p, r.s), unit = *off / r.tiles;
+  r.t0 = *off - unit * r.tiles;
+  r.t1 = min(r.tiles, r.t0 + (end - pos));
+  r.head = static_cast<int>(unit / row_tiles);
+  r.rtile = static_cast<int>(unit - r.head * row_tiles);
+  r.row0 = r.rtile * RT;
+  r.rows_all = r.s.nodes * p.groups;
+  r.rows = min(RT, r.rows_all - r.row0);
   return r;
 }
 
-// Floats of the workspace that one CTA has: two pieces (its first and its last unit may be cut) of O [rt][dp], m [rt], l [rt].
+// Floats of a piece in the workspace: O [rt][dp], m [rt], l [rt]. A CTA has two: its first and its last unit may be cut.
 __host__ __device__ __forceinline__ int64_t pa_piece(int rt, int dp) { return static_cast<int64_t>(rt) * (dp + 2); }
+template <int RT, int DP>
+__device__ __forceinline__ float* pa_piece_of(const PaParams& p, const PaPart& w) {
+  return p.work + (2 * static_cast<int64_t>(blockIdx.x) + (w.t0 == 0)) * pa_piece(RT, DP);
+}
+// What joining has to know of the unit that starts in this CTA's share and goes on: kept by one thread, stored at the end.
+struct PaCut {
+  int4 a{0, 0, 0, 0}, b{0, 0, 0, 0};  // rows (0: no such unit), first row, head, start of the slot's rows; last share
+  __device__ __forceinline__ void note(const PaShare& sh, const PaPart& w, uint32_t pos) {
+    if (w.t0 == 0 && w.t1 < w.tiles) {
+      a = make_int4(w.rows, w.row0, w.head, w.s.start);
+      b.x = static_cast<int>(pa_share_of(sh, pos + w.tiles - 1));
+    }
+  }
+  __device__ __forceinline__ void store(const PaParams& p) const {
+    p.cuts[2 * blockIdx.x] = a;
+    p.cuts[2 * blockIdx.x + 1] = b;
+  }
+};
+// Where the result of a row goes.
+__device__ __forceinline__ char* pa_out(const PaParams& p, int start, int head, int row) {
+  const int node = static_cast<int>(p.by_group.of(row)), g = row - node * p.groups;
+  return p.o.p + (start + static_cast<int64_t>(node)) * p.o.row + static_cast<int64_t>(head * p.groups + g) * p.o.head;
+}
+__device__ __forceinline__ const char* pa_query(const PaParams& p, const PaPart& w, int row) {
+  const int node = static_cast<int>(p.by_group.of(row)), g = row - node * p.groups;
+  return p.q.p + (w.s.start + static_cast<int64_t>(node)) * p.q.row + static_cast<int64_t>(w.head * p.groups + g) * p.q.head;
+}
 
 // Element loads and stores in the cache's type; 16-bit results round to nearest even.
 __device__ __forceinline__ float pa_load(const float* p) { return *p; }
@@ -104,7 +187,7 @@ __device__ __forceinline__ void pa_store(__half* p, float v) { *p = __float2half
 
 // Ancestors of the nodes of a row tile: bit j of seen[i - first] says that node j is node i or one of its ancestors. `up` takes
 // the slot's parents. All threads of the CTA; a parent that is none counts as -1.
-__device__ __forceinline__ void pa_ancestors(const PaParams& p, const PaSlot& s, int first, int count, uint32_t (*seen)[PA_TREE / 32], int16_t* up) {
+__device__ __forceinline__ void pa_ancestors(const PaParams& p, const PaSlot& s, int first, int count, uint32_t (*seen)[PA_TREE / 32 + 1], int16_t* up) {
   const int t = threadIdx.x, nt = blockDim.x;
   for (int i = t; i < s.nodes; i += nt) {
     int a = p.parents[s.start + i];
@@ -122,28 +205,101 @@ __device__ __forceinline__ void pa_ancestors(const PaParams& p, const PaSlot& s,
   __syncthreads();
 }
 
+// Which of 64 keys a node sees, the first of them being node n0 of its slot (negative: in front of the nodes). line: its ancestors
+// (nullptr: a chain).
+__device__ __forceinline__ uint64_t pa_sees(const uint32_t* line, int words, int node, int n0) {
+  const int upto = line ? -n0 : node + 1 - n0;  // keys that are seen whatever the tree
+  const uint64_t low = upto >= 64 ? ~0ull : upto > 0 ? (1ull << upto) - 1 : 0ull;
+  if (!line || upto >= 64) return low;
+  const int first = n0 > 0 ? n0 >> 5 : 0, shift = n0 > 0 ? n0 & 31 : 0;
+  uint32_t w[3];
+#pragma unroll
+  for (int i = 0; i < 3; ++i) w[i] = first + i < words ? line[first + i] : 0u;
+  const uint64_t bits = static_cast<uint64_t>(__funnelshift_r(w[0], w[1], shift)) | static_cast<uint64_t>(__funnelshift_r(w[1], w[2], shift)) << 32;
+  return low | (n0 < 0 ? bits << -n0 : bits);
+}
+
+// Where the rows of a position of a slot and head lie; nullptr where there are none. `pg`: its page, looked up before (-1: none).
+struct PaRow {
+  const char *k, *v;
+};
+__device__ __forceinline__ int pa_lookup(const PaParams& p, const PaPart& w, uint32_t at) {
+  return at < static_cast<uint32_t>(w.s.len) + (p.fresh ? 0u : static_cast<uint32_t>(w.s.nodes)) ? pg_page_of(p.c, w.slot, at) : -1;
+}
+__device__ __forceinline__ PaRow pa_row(const PaParams& p, const PaPart& w, uint32_t at, int pg) {
+  PaRow r{nullptr, nullptr};
+  const uint32_t len = w.s.len;
+  if (pg >= 0) {
+    const int row = pg_row_of(p.c, at);
+    r.k = p.c.k.p + pg * p.c.k.page + w.head * p.c.k.head + row * p.c.k.row;
+    r.v = p.c.v.p + pg * p.c.v.page + w.head * p.c.v.head + row * p.c.v.row;
+  } else if (p.fresh && at >= len && at - len < static_cast<uint32_t>(w.s.nodes)) {
+    const int64_t row = w.s.start + static_cast<int64_t>(at - len);
+    r.k = p.k.p + row * p.k.row + w.head * p.k.head;
+    r.v = p.v.p + row * p.v.row + w.head * p.v.head;
+  }
+  return r;
+}
+// The place in the pages that node n's keys and values go to; a node without one is noted.
+__device__ __forceinline__ bool pa_place(const PaParams& p, const PaPart& w, int n, char** k, char** v) {
+  const int64_t at = static_cast<int64_t>(w.s.len) + n;
+  const int pg = pg_page_of(p.c, w.slot, at);
+  if (pg < 0 || p.c.refs[pg] != 1) {
+    atomicOr(p.c.status, pg < 0 ? YTC_PAGES_INVALID : YTC_PAGES_SHARED);
+    return false;
+  }
+  const int row = pg_row_of(p.c, at);
+  *k = p.c.k.p + pg * p.c.k.page + w.head * p.c.k.head + row * p.c.k.row;
+  *v = p.c.v.p + pg * p.c.v.page + w.head * p.c.v.head + row * p.c.v.row;
+  return true;
+}
+// New rows of nodes n0 .. n1 of a slot and head go to their pages, in `words` pieces of type W each, by `nt` threads of which
+// this is number t.
+template <typename W>
+__device__ __forceinline__ void pa_store_new(const PaParams& p, const PaPart& w, int n0, int n1, int words, int t, int nt) {
+#pragma unroll 1
+  for (int i = t; i < (n1 - n0) * words; i += nt) {
+    const int n = n0 + i / words, x = i % words;
+    char *k, *v;
+    if (!pa_place(p, w, n, &k, &v)) continue;
+    const int64_t row = w.s.start + static_cast<int64_t>(n);
+    reinterpret_cast<W*>(k)[x] = reinterpret_cast<const W*>(p.k.p + row * p.k.row + w.head * p.k.head)[x];
+    reinterpret_cast<W*>(v)[x] = reinterpret_cast<const W*>(p.v.p + row * p.v.row + w.head * p.v.head)[x];
+  }
+}
+
+__device__ __forceinline__ void pa_copy16(uint32_t dst, const char* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void pa_copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void pa_copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ float pa_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // ---------------------------------------------------------------------------------------------- FFMA form
 // fp32, and 16-bit rows that no matrix instruction takes (dims that are not a multiple of 8, odd alignments). 8 x 16 threads:
-// thread (a, b) holds rows a + 8 i (RPT of them) with keys b + 16 j of S and with columns 4 b + 64 j of O.
-template <int DP>
-constexpr int PA_BN_F = DP == 256 ? 32 : 64;
-
+// thread (a, b) holds rows a + 8 i (RPT of them) with keys b + 16 j of S and with columns 4 b + 64 j of O. Two tiles of keys and
+// values as fp32 in shared memory, the next one on its way while one is worked on (WORDS: by cp.async; else element by element).
 template <typename T, int DP, int RPT>
-struct PaSmemF {
-  static constexpr int RT = 8 * RPT, BN = PA_BN_F<DP>;
-  float q[RT][DP + 4], k[BN][DP + 4], v[BN][DP], s[RT][BN + 4];
-  const T *kp[BN], *vp[BN];
-  T *ks[BN], *vs[BN];
-  uint32_t seen[RT][PA_TREE / 32];
+struct PaFfma {
+  static constexpr int RT = 8 * RPT, BN = DP == 64 ? 64 : 32;
+  float q[RT][DP + 4], k[2][BN][DP + 4], v[2][BN][DP], s[RT][BN + 4];
+  const T* row[2][2][BN];
+  uint32_t seen[RT][PA_TREE / 32 + 1];
   int16_t up[PA_TREE];
-  int64_t from, to, before;
-  int slot;
+  PaShare share;
 };
 
 // O += S V of one tile. HIDDEN: weights of zero take nothing along (a hidden position may hold an infinity or NaN).
 template <int DP, int RPT, int BN, bool HIDDEN>
 __device__ __forceinline__ void pa_ffma_values(const float (*s)[BN + 4], const float (*v)[DP], int a, int b, float (*o)[DP / 16]) {
-#pragma unroll 2
+#pragma unroll(HIDDEN ? 1 : 2)
   for (int kk = 0; kk < BN; kk += 4) {
     float4 e[RPT];
 #pragma unroll
@@ -166,120 +322,85 @@ __device__ __forceinline__ void pa_ffma_values(const float (*s)[BN + 4], const f
   }
 }
 
-template <typename T, int DP, int RPT>
+template <typename T, int DP, int RPT, bool WORDS>
 __global__ void __launch_bounds__(PA_THREADS) paged_attn_ffma_kernel(const PaParams p) {
-  using S = PaSmemF<T, DP, RPT>;
+  using S = PaFfma<T, DP, RPT>;
+  static_assert(!WORDS || std::is_same<T, float>::value, "words are copied as they are");
   constexpr int RT = S::RT, BN = S::BN, KPT = BN / 16, CJ = DP / 64;
-  extern __shared__ __align__(16) unsigned char raw[];
+  extern __shared__ __align__(128) unsigned char raw[];
   S& sm = *reinterpret_cast<S*>(raw);
   dependent_trigger();
   const int t = threadIdx.x, a = t >> 4, b = t & 15;
   const PgCache& c = p.c;
-  if (t < 32) {
-    bool bad = false;
-    const PaPlace at = pa_place(p, RT, BN, blockIdx.x, gridDim.x, &bad);
-    if (__any_sync(0xffffffffu, bad) && t == 0 && blockIdx.x == 0) atomicOr(c.status, YTC_PAGES_INVALID);
-    if (t == 0) {
-      sm.from = at.at;
-      sm.to = at.total * (blockIdx.x + 1) / gridDim.x;
-      sm.before = at.before;
-      sm.slot = at.slot;
-    }
-  }
-  __syncthreads();
-  int64_t pos = sm.from;
-  const int64_t end = sm.to;
-  int slot = sm.slot;
-  int64_t off = pos - sm.before;
+  pa_share<RT, BN>(p, &sm.share);
+  PaCut cut;
+  uint32_t pos = sm.share.from, off = sm.share.off;
+  const uint32_t end = sm.share.to;
+  int slot = sm.share.slot;
   while (pos < end) {
-    bool bad = false;
-    const PaSlot s = pa_slot(p, slot, &bad);
-    const int64_t work = pa_work(p, s, RT, BN);
-    if (off >= work) {  // (slots without rows too)
-      off -= work;
-      ++slot;
-      continue;
-    }
-    const int tiles = pa_key_tiles(s, BN), row_tiles = pa_row_tiles(p, s, RT);
-    const int unit = static_cast<int>(off / tiles), t0 = static_cast<int>(off - static_cast<int64_t>(unit) * tiles);
-    const int t1 = static_cast<int>(end - pos < tiles - t0 ? t0 + (end - pos) : tiles);
-    const int head = unit / row_tiles, rtile = unit - head * row_tiles;
-    const int row0 = rtile * RT, rows = min(RT, s.nodes * p.groups - row0);
-    const int keys = s.len + s.nodes;
-    const int node0 = row0 / p.groups;
+    const PaPart w = pa_part<RT, BN>(p, pos, end, &slot, &off);
+    const int nodes = w.s.nodes, words = (nodes + 31) / 32;
+    const int node0 = static_cast<int>(p.by_group.of(w.row0)), node1 = static_cast<int>(p.by_group.of(w.row0 + w.rows - 1));
+    const auto find = [&](uint32_t tile) {  // where the tile's rows lie
+      if (t < BN && tile < w.t1) {
+        const uint32_t at = tile * BN + t;
+        const PaRow r = pa_row(p, w, at, pa_lookup(p, w, at));
+        sm.row[tile & 1][0][t] = reinterpret_cast<const T*>(r.k);
+        sm.row[tile & 1][1][t] = reinterpret_cast<const T*>(r.v);
+      }
+    };
+    const auto fetch = [&](uint32_t tile) {
+      if (tile >= w.t1) return;
+      const int x = tile & 1;
+      if constexpr (WORDS) {
+#pragma unroll 4
+        for (int i = t; i < BN * DP / 4; i += PA_THREADS) {
+          const int r = i / (DP / 4), d = i % (DP / 4) * 4;
+          const T *kp = sm.row[x][0][r], *vp = sm.row[x][1][r];
+          const bool there = kp != nullptr && d < c.dim;
+          pa_copy16(static_cast<uint32_t>(__cvta_generic_to_shared(&sm.k[x][r][d])), there ? reinterpret_cast<const char*>(kp + d) : c.k.p, there);
+          pa_copy16(static_cast<uint32_t>(__cvta_generic_to_shared(&sm.v[x][r][d])), there ? reinterpret_cast<const char*>(vp + d) : c.v.p, there);
+        }
+        pa_copy_commit();
+      } else {
+#pragma unroll 4
+        for (int i = t; i < BN * DP; i += PA_THREADS) {
+          const int r = i / DP, d = i % DP;
+          const T *kp = sm.row[x][0][r], *vp = sm.row[x][1][r];
+          const bool there = kp != nullptr && d < c.dim;
+          sm.k[x][r][d] = there ? pa_load(kp + d) : 0.f;
+          sm.v[x][r][d] = there ? pa_load(vp + d) : 0.f;
+        }
+      }
+    };
+    __syncthreads();  // (the part before is done with the shared memory)
+    find(w.t0);
+    find(w.t0 + 1);
     __syncthreads();
+    fetch(w.t0);
     for (int i = t; i < RT * DP; i += PA_THREADS) {
       const int r = i / DP, d = i % DP;
-      float x = 0.f;
-      if (r < rows && d < c.dim) {
-        const int node = (row0 + r) / p.groups, g = (row0 + r) % p.groups;
-        x = pa_load(reinterpret_cast<const T*>(p.q.p + (s.start + node) * p.q.row + (head * p.groups + g) * p.q.head) + d);
-      }
-      sm.q[r][d] = x * p.scale;
+      sm.q[r][d] = r < w.rows && d < c.dim ? pa_load(reinterpret_cast<const T*>(pa_query(p, w, w.row0 + r)) + d) * p.scale : 0.f;
     }
-    if (p.parents && t1 * static_cast<int64_t>(BN) > s.len) pa_ancestors(p, s, node0, min(RT, s.nodes - node0), sm.seen, sm.up);
+    if (p.parents && static_cast<uint64_t>(w.t1) * BN > static_cast<uint32_t>(w.s.len)) pa_ancestors(p, w.s, node0, node1 - node0 + 1, sm.seen, sm.up);
     float m[RPT], l[RPT], o[RPT][4 * CJ];
     int node[RPT];
 #pragma unroll
     for (int i = 0; i < RPT; ++i) {
       m[i] = -CUDART_INF_F;
       l[i] = 0.f;
-      node[i] = (row0 + min(a + 8 * i, rows - 1)) / p.groups;
+      node[i] = static_cast<int>(p.by_group.of(w.row0 + min(a + 8 * i, w.rows - 1)));
 #pragma unroll
       for (int j = 0; j < 4 * CJ; ++j) o[i][j] = 0.f;
     }
-    for (int tile = t0; tile < t1; ++tile) {
-      const int k0 = tile * BN;
+#pragma unroll 1
+    for (uint32_t tile = w.t0; tile < w.t1; ++tile) {
+      if constexpr (WORDS) pa_copy_wait<0>();
       __syncthreads();
-      if (t < BN) {  // where the tile's rows are, and where they go
-        const int at = k0 + t, j = at - s.len;
-        const T *kp = nullptr, *vp = nullptr;
-        T *ks = nullptr, *vs = nullptr;
-        if (at < keys) {
-          const int pg = j < 0 || !p.fresh || rtile == 0 ? pg_page_of(c, slot, at) : -1;
-          const int64_t row = at % c.page;
-          char* kc = c.k.p + pg * c.k.page + head * c.k.head + row * c.k.row;
-          char* vc = c.v.p + pg * c.v.page + head * c.v.head + row * c.v.row;
-          if (j >= 0 && p.fresh) {
-            kp = reinterpret_cast<const T*>(p.k.p + (s.start + j) * p.k.row + head * p.k.head);
-            vp = reinterpret_cast<const T*>(p.v.p + (s.start + j) * p.v.row + head * p.v.head);
-            if (rtile == 0) {
-              if (pg >= 0 && c.refs[pg] == 1) {
-                ks = reinterpret_cast<T*>(kc);
-                vs = reinterpret_cast<T*>(vc);
-              } else {
-                atomicOr(c.status, pg < 0 ? YTC_PAGES_INVALID : YTC_PAGES_SHARED);
-              }
-            }
-          } else if (pg >= 0) {
-            kp = reinterpret_cast<const T*>(kc);
-            vp = reinterpret_cast<const T*>(vc);
-          } else {
-            atomicOr(c.status, YTC_PAGES_INVALID);
-          }
-        }
-        sm.kp[t] = kp;
-        sm.vp[t] = vp;
-        sm.ks[t] = ks;
-        sm.vs[t] = vs;
-      }
-      __syncthreads();
-      for (int i = t; i < BN * DP; i += PA_THREADS) {
-        const int r = i / DP, d = i % DP;
-        float x = 0.f, y = 0.f;
-        if (d < c.dim && sm.kp[r]) {
-          const T xk = sm.kp[r][d], xv = sm.vp[r][d];
-          x = pa_load(&xk);
-          y = pa_load(&xv);
-          if (sm.ks[r]) {
-            sm.ks[r][d] = xk;
-            sm.vs[r][d] = xv;
-          }
-        }
-        sm.k[r][d] = x;
-        sm.v[r][d] = y;
-      }
-      __syncthreads();
+      fetch(tile + 1);
+      find(tile + 2);
+      const int cur = tile & 1, n0 = static_cast<int>(tile * BN) - w.s.len;  // the node at the tile's first key
+      if (n0 > node1) continue;                                              // (no row of the tile sees any of it)
       float x[RPT][KPT];
 #pragma unroll
       for (int i = 0; i < RPT; ++i)
@@ -289,7 +410,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_ffma_kernel(const PaPar
       for (int d = 0; d < DP; d += 4) {
         float4 kk[KPT];
 #pragma unroll
-        for (int j = 0; j < KPT; ++j) kk[j] = *reinterpret_cast<const float4*>(&sm.k[b + 16 * j][d]);
+        for (int j = 0; j < KPT; ++j) kk[j] = *reinterpret_cast<const float4*>(&sm.k[cur][b + 16 * j][d]);
 #pragma unroll
         for (int i = 0; i < RPT; ++i) {
           const float4 qq = *reinterpret_cast<const float4*>(&sm.q[a + 8 * i][d]);
@@ -298,22 +419,23 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_ffma_kernel(const PaPar
             x[i][j] = fmaf(qq.x, kk[j].x, fmaf(qq.y, kk[j].y, fmaf(qq.z, kk[j].z, fmaf(qq.w, kk[j].w, x[i][j]))));
         }
       }
-      const bool masked = k0 + BN > s.len;
+      const bool masked = n0 + BN > 0;
+      if (masked) {
+#pragma unroll
+        for (int i = 0; i < RPT; ++i) {
+          const uint64_t sees = pa_sees(p.parents ? sm.seen[node[i] - node0] : nullptr, words, node[i], n0);
+#pragma unroll
+          for (int j = 0; j < KPT; ++j)
+            if (!((sees >> (b + 16 * j)) & 1)) x[i][j] = -CUDART_INF_F;
+        }
+      }
 #pragma unroll
       for (int i = 0; i < RPT; ++i) {
         float top = m[i];
 #pragma unroll
-        for (int j = 0; j < KPT; ++j) {
-          if (masked) {
-            const int n = k0 + b + 16 * j - s.len;
-            bool seen = n < 0;
-            if (!seen && n < s.nodes) seen = p.parents ? (sm.seen[node[i] - node0][n >> 5] >> (n & 31)) & 1 : n <= node[i];
-            if (!seen) x[i][j] = -CUDART_INF_F;
-          }
-          top = fmaxf(top, x[i][j]);
-        }
+        for (int j = 0; j < KPT; ++j) top = fmaxf(top, x[i][j]);
 #pragma unroll
-        for (int w = 8; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+        for (int k = 8; k; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
         const float ref = top == -CUDART_INF_F ? 0.f : top, shrink = exp2f(m[i] - ref);
         float sum = 0.f;
 #pragma unroll
@@ -328,21 +450,26 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_ffma_kernel(const PaPar
         for (int j = 0; j < 4 * CJ; ++j) o[i][j] *= shrink;
       }
       __syncwarp();  // (a row of S is written and read by one half of a warp)
-      if (masked) pa_ffma_values<DP, RPT, BN, true>(sm.s, sm.v, a, b, o);
-      else pa_ffma_values<DP, RPT, BN, false>(sm.s, sm.v, a, b, o);
+      if (masked) pa_ffma_values<DP, RPT, BN, true>(sm.s, sm.v[cur], a, b, o);
+      else pa_ffma_values<DP, RPT, BN, false>(sm.s, sm.v[cur], a, b, o);
+      __syncwarp();
     }
-    const bool whole = t0 == 0 && t1 == tiles;
-    float* piece = p.work + (2 * static_cast<int64_t>(blockIdx.x) + (t0 == 0)) * pa_piece(RT, DP);
+    if constexpr (WORDS) pa_copy_wait<0>();
+    if (p.fresh && w.rtile == 0) {
+      const int64_t n0 = static_cast<int64_t>(w.t0) * BN - w.s.len, n1 = static_cast<int64_t>(w.t1) * BN - w.s.len;
+      if (n1 > 0) pa_store_new<T>(p, w, n0 < 0 ? 0 : static_cast<int>(n0), static_cast<int>(n1 < nodes ? n1 : nodes), c.dim, t, PA_THREADS);
+    }
+    const bool whole = w.t0 == 0 && w.t1 == w.tiles;
+    float* piece = pa_piece_of<RT, DP>(p, w);
 #pragma unroll
     for (int i = 0; i < RPT; ++i) {
       const int r = a + 8 * i;
       float sum = l[i];
 #pragma unroll
-      for (int w = 8; w; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-      if (r >= rows) continue;
+      for (int k = 8; k; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+      if (r >= w.rows) continue;
       if (whole) {
-        const int g = (row0 + r) % p.groups;
-        T* out = reinterpret_cast<T*>(p.o.p + (s.start + node[i]) * p.o.row + (head * p.groups + g) * p.o.head);
+        T* out = reinterpret_cast<T*>(pa_out(p, w.s.start, w.head, w.row0 + r));
 #pragma unroll
         for (int j = 0; j < 4 * CJ; ++j) {
           const int d = 4 * b + 64 * (j / 4) + j % 4;
@@ -357,9 +484,11 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_ffma_kernel(const PaPar
         }
       }
     }
-    pos += t1 - t0;
-    off += t1 - t0;
+    cut.note(sm.share, w, pos);
+    pos += w.t1 - w.t0;
+    off += w.t1 - w.t0;
   }
+  if (t == 0) cut.store(p);
 }
 
 // ---------------------------------------------------------------------------------------------- matrix-instruction forms
@@ -371,14 +500,6 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_ffma_kernel(const PaPar
 // l is of the unrounded numbers in fp32.
 constexpr float PA_SLACK = 8.f;
 
-__device__ __forceinline__ void pa_copy16(uint32_t dst, const char* src, bool there) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void pa_copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void pa_copy_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 __device__ __forceinline__ void pa_ldmatrix(uint32_t at, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
@@ -387,7 +508,7 @@ __device__ __forceinline__ void pa_ldmatrix_t(uint32_t at, uint32_t (&r)[4]) {
 }
 template <typename T>
 __device__ __forceinline__ void pa_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (sizeof(T) == 2 && !std::is_same<T, __half>::value)
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -395,11 +516,6 @@ __device__ __forceinline__ void pa_mma(float (&d)[4], const uint32_t (&a)[4], ui
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ float pa_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 template <typename T>
 __device__ __forceinline__ uint32_t pa_pack(float lo, float hi) {
@@ -409,36 +525,9 @@ __device__ __forceinline__ uint32_t pa_pack(float lo, float hi) {
   return r;
 }
 template <typename T>
-__device__ __forceinline__ bool pa_finite2(uint32_t x) {  // both halves
-  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
-  return (x & e) != e && ((x >> 16) & e) != e;
-}
-
-template <typename T>
-__device__ __forceinline__ uint32_t pa_finite_part(uint32_t x) {  // zero for a half that is none
+__device__ __forceinline__ uint32_t pa_finite_part(uint32_t x) {  // zero for a half that is an infinity or NaN
   constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
   return ((x & e) != e ? x & 0xffffu : 0u) | (((x >> 16) & e) != e ? x & 0xffff0000u : 0u);
-}
-
-// Where the row of position `at` of a slot and head lies; nullptr where there is none. `pg`: its page, looked up before (-1: none).
-struct PaRow {
-  const char *k, *v;
-};
-__device__ __forceinline__ int pa_lookup(const PaParams& p, int slot, const PaSlot& s, int64_t at) {
-  return at < s.len + static_cast<int64_t>(p.fresh ? 0 : s.nodes) ? pg_page_of(p.c, slot, at) : -1;
-}
-__device__ __forceinline__ PaRow pa_row(const PaParams& p, const PaSlot& s, int head, int64_t at, int pg) {
-  PaRow r{nullptr, nullptr};
-  if (pg >= 0) {
-    const int row = static_cast<int>(at % p.c.page);
-    r.k = p.c.k.p + pg * p.c.k.page + head * p.c.k.head + row * p.c.k.row;
-    r.v = p.c.v.p + pg * p.c.v.page + head * p.c.v.head + row * p.c.v.row;
-  } else if (p.fresh && at >= s.len && at < s.len + static_cast<int64_t>(s.nodes)) {
-    const int64_t row = s.start + (at - s.len);
-    r.k = p.k.p + row * p.k.row + head * p.k.head;
-    r.v = p.v.p + row * p.v.row + head * p.v.head;
-  }
-  return r;
 }
 
 // What one warp holds of 16 rows: thread (g = lane / 4, t = lane % 4) has rows g and g + 8.
@@ -456,10 +545,10 @@ struct PaWarp {
     l[0] = l[1] = 0.f;
   }
 
-  // S = Q K^T for NK keys from shared row `key0` on, P, and O += P V. kt, vt: a ring slot's keys and values; q_at: Q in shared
-  // memory where it is too wide for registers. seen(row half, key of the step): for steps that hide something.
-  template <int NK, bool HIDES, typename Seen>
-  __device__ __forceinline__ void step(uint32_t kt, uint32_t vt, int key0, float scale, uint32_t q_at, Seen seen, float* spare) {
+  // S = Q K^T for the NK keys at kt, P, and O += P V with the values at vt. q_at: Q in shared memory where it is too wide for
+  // registers. hides (the same for the warp): row half h sees the keys of bits sees[h] only.
+  template <int NK>
+  __device__ __forceinline__ void step(uint32_t kt, uint32_t vt, float scale, uint32_t q_at, bool hides, const uint64_t (&sees)[2], float* spare) {
     const int lane = threadIdx.x & 31;
     float s[NK / 8][4];
 #pragma unroll
@@ -479,31 +568,50 @@ struct PaWarp {
       }
 #pragma unroll
       for (int n = 0; n < NK / 16; ++n) {
-        const int r = key0 + 16 * n + krow, w = 2 * d + kword;
+        const int r = 16 * n + krow, w = 2 * d + kword;
         uint32_t b[4];
         pa_ldmatrix(kt + r * (DP * 2) + ((w ^ (r & 7)) << 4), b);
         pa_mma<T>(s[2 * n], a, b[0], b[1]);
         pa_mma<T>(s[2 * n + 1], a, b[2], b[3]);
       }
     }
-    float top[2] = {-CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
     for (int n = 0; n < NK / 8; ++n)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s[n][j] *= scale;
-        if (HIDES && !seen(j >> 1, 8 * n + 2 * (lane & 3) + (j & 1))) s[n][j] = -CUDART_INF_F;
-        top[j >> 1] = fmaxf(top[j >> 1], s[n][j]);
+      for (int j = 0; j < 4; ++j) s[n][j] *= scale;
+    bool fine = true;
+    if (hides) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint64_t mine = sees[h] >> (2 * (lane & 3));
+#pragma unroll
+        for (int n = 0; n < NK / 8; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            if (!((mine >> (8 * n + j)) & 1)) s[n][2 * h + j] = -CUDART_INF_F;
       }
+      // A hidden row of V that is not finite would spoil every row (0 x infinity): such numbers are left out of the product
+      // and added behind it, to the rows that see them.
+#pragma unroll 1
+      for (int i = lane; i < NK * DP / 8; i += 32) {
+        uint4 x;
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(vt + i * 16));
+        fine = fine && pa_finite_part<T>(x.x) == x.x && pa_finite_part<T>(x.y) == x.y && pa_finite_part<T>(x.z) == x.z && pa_finite_part<T>(x.w) == x.w;
+      }
+      fine = __all_sync(0xffffffffu, fine);
+    }
     float shrink[2];
     bool moves = false;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-      const bool up = top[h] > m[h] + PA_SLACK || (m[h] == -CUDART_INF_F && top[h] > m[h]);
-      shrink[h] = up ? pa_exp2(m[h] - top[h]) : 1.f;
-      if (up) m[h] = top[h];
+      float top = -CUDART_INF_F;
+#pragma unroll
+      for (int n = 0; n < NK / 8; ++n) top = fmaxf(top, fmaxf(s[n][2 * h], s[n][2 * h + 1]));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const bool up = top > m[h] + PA_SLACK || (m[h] == -CUDART_INF_F && top > m[h]);
+      shrink[h] = up ? pa_exp2(m[h] - top) : 1.f;
+      if (up) m[h] = top;
       moves = moves || up;
     }
     if (__any_sync(0xffffffffu, moves)) {
@@ -522,17 +630,6 @@ struct PaWarp {
         s[n][j] = pa_exp2(s[n][j] - ref[j >> 1]);
         l[j >> 1] += s[n][j];
       }
-    // A hidden row of V that is not finite would spoil every row (0 x infinity): such numbers are left out of the product and
-    // added behind it, to the rows that see them.
-    bool fine = true;
-    if (HIDES) {
-      for (int i = lane; i < NK * DP / 8; i += 32) {
-        uint4 x;
-        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(vt + key0 * (DP * 2) + i * 16));
-        fine = fine && pa_finite2<T>(x.x) && pa_finite2<T>(x.y) && pa_finite2<T>(x.z) && pa_finite2<T>(x.w);
-      }
-      fine = __all_sync(0xffffffffu, fine);
-    }
     const int vrow = (lane & 7) + (((lane >> 3) & 1) << 3), vword = lane >> 4;
 #pragma unroll
     for (int n = 0; n < NK / 16; ++n) {
@@ -540,10 +637,10 @@ struct PaWarp {
                              pa_pack<T>(s[2 * n + 1][0], s[2 * n + 1][1]), pa_pack<T>(s[2 * n + 1][2], s[2 * n + 1][3])};
 #pragma unroll
       for (int d = 0; d < DP / 16; ++d) {
-        const int r = key0 + 16 * n + vrow, w = 2 * d + vword;
+        const int r = 16 * n + vrow, w = 2 * d + vword;
         uint32_t b[4];
         pa_ldmatrix_t(vt + r * (DP * 2) + ((w ^ (r & 7)) << 4), b);
-        if (HIDES && !fine) {
+        if (!fine) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) b[j] = pa_finite_part<T>(b[j]);
         }
@@ -551,12 +648,12 @@ struct PaWarp {
         pa_mma<T>(o[2 * d + 1], a, b[2], b[3]);
       }
     }
-    if (HIDES && !fine) add_infinite<NK>(s, vt, key0, spare);
+    if (!fine) add_infinite<NK>(s, vt, spare);
   }
 
   // O += P V for the numbers of V that are not finite and weights that are not zero. spare: 16 x 8 floats of the warp's own.
   template <int NK>
-  __device__ __forceinline__ void add_infinite(const float (&s)[NK / 8][4], uint32_t vt, int key0, float* spare) {
+  __device__ __forceinline__ void add_infinite(const float (&s)[NK / 8][4], uint32_t vt, float* spare) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll 1
     for (int n = 0; n < NK / 8; ++n) {
@@ -573,14 +670,14 @@ struct PaWarp {
 #pragma unroll 1
       for (int kk = 0; kk < 8; ++kk) {
         const float w0 = spare[g * 8 + kk], w1 = spare[(g + 8) * 8 + kk];
-        const int r = key0 + 8 * n + kk;
+        const int r = 8 * n + kk;
 #pragma unroll
         for (int d = 0; d < DP / 8; ++d) {
           uint32_t x;
           asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x) : "r"(vt + r * (DP * 2) + ((d ^ (r & 7)) << 4) + 4 * t));
-          if (pa_finite2<T>(x)) continue;
-          const uint32_t odd = x ^ pa_finite_part<T>(x);  // (the finite half is zero)
-          T lo, hi;
+          const uint32_t odd = x ^ pa_finite_part<T>(x);
+          if (odd == 0) continue;
+          T lo, hi;  // (the half that is finite, if one is, counts as zero)
           const uint16_t bits_lo = static_cast<uint16_t>(odd), bits_hi = static_cast<uint16_t>(odd >> 16);
           memcpy(&lo, &bits_lo, 2);
           memcpy(&hi, &bits_hi, 2);
@@ -598,6 +695,29 @@ struct PaWarp {
     }
   }
 
+  // Q of rows row .. row + 15 of the part (zero past the ends).
+  __device__ __forceinline__ void load_q(const PaParams& p, const PaPart& w, int row) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = row + (lane >> 2) + 8 * h, d0 = 2 * (lane & 3);
+      const uint32_t* at = reinterpret_cast<const uint32_t*>(pa_query(p, w, min(r, w.rows_all - 1)) + 2 * d0);
+#pragma unroll
+      for (int d = 0; d < (DP <= 128 ? DP / 16 : 1); ++d) {
+        q[d][h] = r < w.rows_all && 16 * d + d0 < p.c.dim ? at[8 * d] : 0u;
+        q[d][2 + h] = r < w.rows_all && 16 * d + 8 + d0 < p.c.dim ? at[8 * d + 4] : 0u;
+      }
+    }
+  }
+  // The same into shared memory, `rows` rows by all threads of the CTA.
+  static __device__ __forceinline__ void stage_q(const PaParams& p, const PaPart& w, uint4* to, int rows) {
+    for (int i = threadIdx.x; i < rows * (DP / 8); i += PA_THREADS) {
+      const int r = i / (DP / 8), x = i % (DP / 8);
+      const bool there = w.row0 + r < w.rows_all && 8 * x < p.c.dim;
+      to[r * (DP / 8) + (x ^ (r & 7))] = there ? reinterpret_cast<const uint4*>(pa_query(p, w, w.row0 + r))[x] : make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
+
   __device__ __forceinline__ void finish_sums() {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -607,39 +727,7 @@ struct PaWarp {
   }
 };
 
-// Two neighbouring elements of a query row as one word (zero past the ends).
-__device__ __forceinline__ uint32_t pa_q2(const PaParams& p, const PaSlot& s, int head, int row, int rows_all, int d) {
-  if (row >= rows_all || d >= p.c.dim) return 0u;
-  const int node = row / p.groups, g = row - node * p.groups;
-  return *reinterpret_cast<const uint32_t*>(p.q.p + (s.start + static_cast<int64_t>(node)) * p.q.row + (head * p.groups + g) * p.q.head + 2 * d);
-}
-
-// Rows of new keys and values that a tile holds in shared memory go to their pages. `first` .. `first + n`: positions, `row0`: the
-// shared row of the first; for `nt` threads of which this is number t.
-template <int DP>
-__device__ __forceinline__ void pa_store_new(const PaParams& p, const PaSlot& s, int slot, int head, int64_t first, int n, uint32_t kt,
-                                             uint32_t vt, int row0, int t, int nt) {
-  const int words = p.c.dim / 8;
-  for (int i = t; i < n * words; i += nt) {
-    const int r = i / words, w = i - r * words;
-    const int64_t at = first + r;
-    if (at < s.len || at >= s.len + static_cast<int64_t>(s.nodes)) continue;
-    const int pg = pg_page_of(p.c, slot, at);
-    if (pg < 0 || p.c.refs[pg] != 1) {
-      atomicOr(p.c.status, pg < 0 ? YTC_PAGES_INVALID : YTC_PAGES_SHARED);
-      continue;
-    }
-    const int row = static_cast<int>(at % p.c.page);
-    const uint32_t off = (row0 + r) * (DP * 2) + ((w ^ ((row0 + r) & 7)) << 4);
-    uint4 x;
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(kt + off));
-    *reinterpret_cast<uint4*>(p.c.k.p + pg * p.c.k.page + head * p.c.k.head + row * p.c.k.row + w * 16) = x;
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(vt + off));
-    *reinterpret_cast<uint4*>(p.c.v.p + pg * p.c.v.page + head * p.c.v.head + row * p.c.v.row + w * 16) = x;
-  }
-}
-
-// Up to 16 rows: every warp has its own keys (16 of each tile of 64), its own ring, and no barrier until the unit ends, where the
+// Up to 16 rows: every warp has its own keys (16 of each tile of 64), its own ring, and no barrier until the part ends, where the
 // four warps' sums are joined. What bounds it is the copy of keys and values: 512 bytes a key and head at dim 128.
 template <typename T, int DP>
 struct PaNarrow {
@@ -648,10 +736,9 @@ struct PaNarrow {
   uint4 q[DP > 128 ? 16 * DP * 2 / 16 : 1];
   float spare[WARPS][16 * 8];
   float m[WARPS][16], l[WARPS][16];
-  uint32_t seen[RT][PA_TREE / 32];
+  uint32_t seen[RT][PA_TREE / 32 + 1];
   int16_t up[PA_TREE];
-  int64_t from, to, before;
-  int slot;
+  PaShare share;
 };
 
 template <typename T, int DP>
@@ -663,45 +750,23 @@ __global__ void __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) paged_attn_narr
   dependent_trigger();
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, g = lane >> 2, c4 = lane & 3;
   const PgCache& c = p.c;
-  if (warp == 0) {
-    bool bad = false;
-    const PaPlace at = pa_place(p, RT, BN, blockIdx.x, gridDim.x, &bad);
-    if (__any_sync(0xffffffffu, bad) && lane == 0 && blockIdx.x == 0) atomicOr(c.status, YTC_PAGES_INVALID);
-    if (lane == 0) {
-      sm.from = at.at;
-      sm.to = at.total * (blockIdx.x + 1) / gridDim.x;
-      sm.before = at.before;
-      sm.slot = at.slot;
-    }
-  }
-  __syncthreads();
-  int64_t pos = sm.from;
-  const int64_t end = sm.to;
-  int slot = sm.slot;
-  int64_t off = pos - sm.before;
+  pa_share<RT, BN>(p, &sm.share);
+  PaCut cut;
+  uint32_t pos = sm.share.from, off = sm.share.off;
+  const uint32_t end = sm.share.to;
+  int slot = sm.share.slot;
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(sm.ring[warp]));
   const int word = lane % WORDS, words = c.dim / 8;
   while (pos < end) {
-    bool bad = false;
-    const PaSlot s = pa_slot(p, slot, &bad);
-    const int64_t work = pa_work(p, s, RT, BN);
-    if (off >= work) {
-      off -= work;
-      ++slot;
-      continue;
-    }
-    const int tiles = pa_key_tiles(s, BN), row_tiles = pa_row_tiles(p, s, RT);
-    const int unit = static_cast<int>(off / tiles), t0 = static_cast<int>(off - static_cast<int64_t>(unit) * tiles);
-    const int t1 = static_cast<int>(end - pos < tiles - t0 ? t0 + (end - pos) : tiles);
-    const int head = unit / row_tiles, rtile = unit - head * row_tiles;
-    const int row0 = rtile * RT, rows_all = s.nodes * p.groups, rows = min(RT, rows_all - row0);
-    const int64_t mine = 16 * warp;
+    const PaPart w = pa_part<RT, BN>(p, pos, end, &slot, &off);
+    const uint32_t mine = 16 * warp;
     // (a lane looks up the page of key lane % 16 of a step, one step before the copies need it)
-    const auto lookup = [&](int tile) { return tile < t1 ? pa_lookup(p, slot, s, static_cast<int64_t>(tile) * BN + mine + (lane & 15)) : -1; };
-    const auto fetch = [&](int tile, int pg) {
-      if (tile < t1) {
-        const PaRow r = pa_row(p, s, head, static_cast<int64_t>(tile) * BN + mine + (lane & 15), pg);
-        const uint32_t kt = ring + (tile - t0) % ST * (2 * S::SLOT);
+    const auto lookup = [&](uint32_t tile) { return tile < w.t1 ? pa_lookup(p, w, tile * BN + mine + (lane & 15)) : -1; };
+    uint32_t into = 0;  // ring slot of the next copies
+    const auto fetch = [&](uint32_t tile, int pg) {
+      if (tile < w.t1) {
+        const PaRow r = pa_row(p, w, tile * BN + mine + (lane & 15), pg);
+        const uint32_t kt = ring + into * (2 * S::SLOT);
         const unsigned long long kp = reinterpret_cast<unsigned long long>(r.k), vp = reinterpret_cast<unsigned long long>(r.v);
 #pragma unroll
         for (int i = 0; i < 16 / PER; ++i) {
@@ -713,80 +778,76 @@ __global__ void __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) paged_attn_narr
           pa_copy16(to + S::SLOT, there ? reinterpret_cast<const char*>(b) + word * 16 : c.v.p, there);
         }
       }
+      into = into == ST - 1 ? 0 : into + 1;
       pa_copy_commit();
     };
-    __syncthreads();  // (the unit before is done with the shared memory)
-    int pg = lookup(t0);
-#pragma unroll
-    for (int i = 0; i < ST - 1; ++i) {
-      const int next = lookup(t0 + i + 1);
-      fetch(t0 + i, pg);
-      pg = next;
-    }
-    PaWarp<T, DP> w;
-    w.clear();
+    __syncthreads();  // (the part before is done with the shared memory)
+    PaWarp<T, DP> x;
     uint32_t q_at = 0;
-    if constexpr (DP <= 128) {
-#pragma unroll
-      for (int d = 0; d < DP / 16; ++d)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) w.q[d][j] = pa_q2(p, s, head, row0 + g + 8 * (j & 1), rows_all, 16 * d + 2 * c4 + 8 * (j >> 1));
-    } else {
-      q_at = static_cast<uint32_t>(__cvta_generic_to_shared(sm.q));
-      for (int i = t; i < 16 * DP / 2; i += PA_THREADS) {
-        const int r = i / (DP / 2), d = i % (DP / 2) * 2;
-        reinterpret_cast<uint32_t*>(sm.q)[r * (DP / 2) + (((d / 8) ^ (r & 7)) * 4) + d % 8 / 2] = pa_q2(p, s, head, row0 + r, rows_all, d);
-      }
-      __syncthreads();
-    }
-    const int node0 = row0 / p.groups;
-    const int node[2] = {(row0 + min(g, rows - 1)) / p.groups, (row0 + min(g + 8, rows - 1)) / p.groups};
-    if (p.parents && t1 * static_cast<int64_t>(BN) > s.len) pa_ancestors(p, s, node0, min(RT, s.nodes - node0), sm.seen, sm.up);
-    for (int tile = t0; tile < t1; ++tile) {
-      const int next = lookup(tile + ST);
-      fetch(tile + ST - 1, pg);  // (into the slot that the step before has read)
+    int pg = lookup(w.t0), node[2];
+    const int words_seen = (w.s.nodes + 31) / 32, node0 = static_cast<int>(p.by_group.of(w.row0));
+    // The first ST - 1 tiles are fetched by the loop itself, before there is one to work on.
+#pragma unroll 1
+    for (uint32_t tile = w.t0, out = 0; tile < w.t1 + ST - 1; ++tile) {
+      const int next = lookup(tile + 1);
+      fetch(tile, pg);
       pg = next;
+      if (tile == w.t0) {  // (behind the first copies)
+        x.clear();
+        if constexpr (DP <= 128) {
+          x.load_q(p, w, w.row0);
+        } else {
+          q_at = static_cast<uint32_t>(__cvta_generic_to_shared(sm.q));
+          x.stage_q(p, w, sm.q, RT);
+          __syncthreads();
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) node[h] = static_cast<int>(p.by_group.of(w.row0 + min(g + 8 * h, w.rows - 1)));
+        if (p.parents && static_cast<uint64_t>(w.t1) * BN > static_cast<uint32_t>(w.s.len))
+          pa_ancestors(p, w.s, node0, min(RT, w.s.nodes - node0), sm.seen, sm.up);
+      }
+      if (tile < w.t0 + ST - 1) continue;
       pa_copy_wait<ST - 1>();
       __syncwarp();
-      const uint32_t kt = ring + (tile - t0) % ST * (2 * S::SLOT), vt = kt + S::SLOT;
-      const int64_t first = static_cast<int64_t>(tile) * BN + mine;
-      if (first + 16 <= s.len) {
-        w.template step<16, false>(kt, vt, 0, p.scale, q_at, [](int, int) { return true; }, nullptr);
-      } else if (first < s.len + static_cast<int64_t>(s.nodes)) {
-        const int before = static_cast<int>(s.len - first);
-        w.template step<16, true>(
-            kt, vt, 0, p.scale, q_at,
-            [&](int h, int key) {
-              const int n = key - before;
-              if (n < 0) return true;
-              if (n >= s.nodes) return false;
-              return p.parents ? ((sm.seen[node[h] - node0][n >> 5] >> (n & 31)) & 1) != 0 : n <= node[h];
-            },
-            sm.spare[warp]);
-        if (p.fresh && rtile == 0) pa_store_new<DP>(p, s, slot, head, first, 16, kt, vt, 0, lane, 32);
+      const uint32_t kt = ring + out * (2 * S::SLOT);
+      out = out == ST - 1 ? 0 : out + 1;
+      const int n0 = static_cast<int>((tile - (ST - 1)) * BN + mine) - w.s.len;  // the node at the first key
+      if (n0 < w.s.nodes) {
+        const bool hides = n0 + 16 > 0;
+        uint64_t sees[2] = {0, 0};
+        if (hides) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) sees[h] = pa_sees(p.parents ? sm.seen[node[h] - node0] : nullptr, words_seen, node[h], n0);
+        }
+        x.template step<16>(kt, kt + S::SLOT, p.scale, q_at, hides, sees, sm.spare[warp]);
       }
-      __syncwarp();
+      __syncwarp();  // (the next copies go into the slot that has just been read)
     }
     pa_copy_wait<0>();
-    w.finish_sums();
+    if (p.fresh && w.rtile == 0) {
+      const int64_t n0 = static_cast<int64_t>(w.t0) * BN - w.s.len, n1 = static_cast<int64_t>(w.t1) * BN - w.s.len;
+      if (n1 > 0) pa_store_new<uint4>(p, w, n0 < 0 ? 0 : static_cast<int>(n0), static_cast<int>(n1 < w.s.nodes ? n1 : w.s.nodes), words, t, PA_THREADS);
+    }
+    x.finish_sums();
     // the warps' sums: O of each in its own ring
     __syncwarp();
     float* mine_o = reinterpret_cast<float*>(sm.ring[warp]);
 #pragma unroll
     for (int d = 0; d < DP / 8; ++d)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) *reinterpret_cast<float2*>(mine_o + (g + 8 * h) * DP + 8 * d + 2 * c4) = make_float2(w.o[d][2 * h], w.o[d][2 * h + 1]);
+      for (int h = 0; h < 2; ++h) *reinterpret_cast<float2*>(mine_o + (g + 8 * h) * DP + 8 * d + 2 * c4) = make_float2(x.o[d][2 * h], x.o[d][2 * h + 1]);
     if (c4 == 0) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        sm.m[warp][g + 8 * h] = w.m[h];
-        sm.l[warp][g + 8 * h] = w.l[h];
+        sm.m[warp][g + 8 * h] = x.m[h];
+        sm.l[warp][g + 8 * h] = x.l[h];
       }
     }
     __syncthreads();
-    const bool whole = t0 == 0 && t1 == tiles;
-    float* piece = p.work + (2 * static_cast<int64_t>(blockIdx.x) + (t0 == 0)) * pa_piece(RT, DP);
-    for (int i = t; i < rows * (DP / 4); i += PA_THREADS) {
+    const bool whole = w.t0 == 0 && w.t1 == w.tiles;
+    float* piece = pa_piece_of<RT, DP>(p, w);
+#pragma unroll 1
+    for (int i = t; i < w.rows * (DP / 4); i += PA_THREADS) {
       const int r = i / (DP / 4), d = i % (DP / 4) * 4;
       float m = -CUDART_INF_F;
 #pragma unroll
@@ -796,19 +857,17 @@ __global__ void __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) paged_attn_narr
 #pragma unroll
       for (int k = 0; k < S::WARPS; ++k) {
         const float mk = sm.m[k][r], f = mk == -CUDART_INF_F ? 0.f : pa_exp2(mk - m);
-        const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sm.ring[k]) + r * DP + d);
+        const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sm.ring[k]) + r * DP + d);
         l = fmaf(f, sm.l[k][r], l);
-        o.x = fmaf(f, x.x, o.x);
-        o.y = fmaf(f, x.y, o.y);
-        o.z = fmaf(f, x.z, o.z);
-        o.w = fmaf(f, x.w, o.w);
+        o.x = fmaf(f, y.x, o.x);
+        o.y = fmaf(f, y.y, o.y);
+        o.z = fmaf(f, y.z, o.z);
+        o.w = fmaf(f, y.w, o.w);
       }
       if (whole) {
-        if (d >= c.dim) continue;
-        const int nd = (row0 + r) / p.groups, gg = (row0 + r) % p.groups;
         const float f = 1.f / l;
-        *reinterpret_cast<uint2*>(p.o.p + (s.start + static_cast<int64_t>(nd)) * p.o.row + (head * p.groups + gg) * p.o.head + 2 * d) =
-            make_uint2(pa_pack<T>(o.x * f, o.y * f), pa_pack<T>(o.z * f, o.w * f));
+        if (d < c.dim)
+          *reinterpret_cast<uint2*>(pa_out(p, w.s.start, w.head, w.row0 + r) + 2 * d) = make_uint2(pa_pack<T>(o.x * f, o.y * f), pa_pack<T>(o.z * f, o.w * f));
       } else {
         *reinterpret_cast<float4*>(piece + r * DP + d) = o;
         if (d == 0) {
@@ -817,9 +876,11 @@ __global__ void __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) paged_attn_narr
         }
       }
     }
-    pos += t1 - t0;
-    off += t1 - t0;
+    cut.note(sm.share, w, pos);
+    pos += w.t1 - w.t0;
+    off += w.t1 - w.t0;
   }
+  if (t == 0) cut.store(p);
 }
 
 // Up to 64 rows of a tile: a warp for 16 of them (warps without rows only copy), all over the same tiles of 64 keys.
@@ -830,66 +891,45 @@ struct PaWide {
   uint4 q[DP > 128 ? RT * DP * 2 / 16 : 1];
   const char* row[2][2][BN];  // (where the next tile's rows lie)
   float spare[4][16 * 8];
-  uint32_t seen[RT][PA_TREE / 32];
+  uint32_t seen[RT][PA_TREE / 32 + 1];
   int16_t up[PA_TREE];
-  int64_t from, to, before;
-  int slot;
+  PaShare share;
 };
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) paged_attn_wide_kernel(const PaParams p) {
   using S = PaWide<T, DP>;
   constexpr int RT = S::RT, BN = S::BN, ST = S::STAGES, WORDS = DP / 8, PER = PA_THREADS / WORDS;
+  static_assert(ST == 3, "two tiles on their way, one worked on");
   extern __shared__ __align__(128) unsigned char raw[];
   S& sm = *reinterpret_cast<S*>(raw);
   dependent_trigger();
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, g = lane >> 2, c4 = lane & 3;
   const PgCache& c = p.c;
-  if (warp == 0) {
-    bool bad = false;
-    const PaPlace at = pa_place(p, RT, BN, blockIdx.x, gridDim.x, &bad);
-    if (__any_sync(0xffffffffu, bad) && lane == 0 && blockIdx.x == 0) atomicOr(c.status, YTC_PAGES_INVALID);
-    if (lane == 0) {
-      sm.from = at.at;
-      sm.to = at.total * (blockIdx.x + 1) / gridDim.x;
-      sm.before = at.before;
-      sm.slot = at.slot;
-    }
-  }
-  __syncthreads();
-  int64_t pos = sm.from;
-  const int64_t end = sm.to;
-  int slot = sm.slot;
-  int64_t off = pos - sm.before;
+  pa_share<RT, BN>(p, &sm.share);
+  PaCut cut;
+  uint32_t pos = sm.share.from, off = sm.share.off;
+  const uint32_t end = sm.share.to;
+  int slot = sm.share.slot;
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(sm.ring));
   const int word = t % WORDS, words = c.dim / 8;
   while (pos < end) {
-    bool bad = false;
-    const PaSlot s = pa_slot(p, slot, &bad);
-    const int64_t work = pa_work(p, s, RT, BN);
-    if (off >= work) {
-      off -= work;
-      ++slot;
-      continue;
-    }
-    const int tiles = pa_key_tiles(s, BN), row_tiles = pa_row_tiles(p, s, RT);
-    const int unit = static_cast<int>(off / tiles), t0 = static_cast<int>(off - static_cast<int64_t>(unit) * tiles);
-    const int t1 = static_cast<int>(end - pos < tiles - t0 ? t0 + (end - pos) : tiles);
-    const int head = unit / row_tiles, rtile = unit - head * row_tiles;
-    const int row0 = rtile * RT, rows_all = s.nodes * p.groups, rows = min(RT, rows_all - row0);
-    const int node_last = (row0 + rows - 1) / p.groups;
+    const PaPart w = pa_part<RT, BN>(p, pos, end, &slot, &off);
+    const int words_seen = (w.s.nodes + 31) / 32;
+    const int node0 = static_cast<int>(p.by_group.of(w.row0)), node1 = static_cast<int>(p.by_group.of(w.row0 + w.rows - 1));
     // Thread t < 64 finds row t of a tile, one tile before the copies of it.
-    const auto find = [&](int tile) {
-      if (t < BN && tile < t1) {
-        const int64_t at = static_cast<int64_t>(tile) * BN + t;
-        const PaRow r = pa_row(p, s, head, at, pa_lookup(p, slot, s, at));
+    const auto find = [&](uint32_t tile) {
+      if (t < BN && tile < w.t1) {
+        const uint32_t at = tile * BN + t;
+        const PaRow r = pa_row(p, w, at, pa_lookup(p, w, at));
         sm.row[tile & 1][0][t] = r.k;
         sm.row[tile & 1][1][t] = r.v;
       }
     };
-    const auto fetch = [&](int tile) {
-      if (tile < t1) {
-        const uint32_t kt = ring + (tile - t0) % ST * (2 * S::SLOT);
+    uint32_t into = 0;
+    const auto fetch = [&](uint32_t tile) {
+      if (tile < w.t1) {
+        const uint32_t kt = ring + into * (2 * S::SLOT);
 #pragma unroll
         for (int i = 0; i < BN / PER; ++i) {
           const int row = i * PER + t / WORDS;
@@ -900,130 +940,99 @@ __global__ void __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) paged_attn_wide
           pa_copy16(to + S::SLOT, there ? b + word * 16 : c.v.p, there);
         }
       }
+      into = into == ST - 1 ? 0 : into + 1;
       pa_copy_commit();
     };
-    __syncthreads();
-    find(t0);
-    find(t0 + 1);
-    __syncthreads();
-    fetch(t0);
-    fetch(t0 + 1);
-    __syncthreads();
-    find(t0 + 2);
-    PaWarp<T, DP> w;
-    w.clear();
-    const int wrow = row0 + 16 * warp;
+    PaWarp<T, DP> x;
     uint32_t q_at = 0;
-    if constexpr (DP <= 128) {
-#pragma unroll
-      for (int d = 0; d < DP / 16; ++d)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) w.q[d][j] = pa_q2(p, s, head, wrow + g + 8 * (j & 1), rows_all, 16 * d + 2 * c4 + 8 * (j >> 1));
-    } else {
-      q_at = static_cast<uint32_t>(__cvta_generic_to_shared(sm.q)) + warp * 16 * (DP * 2);
-      for (int i = t; i < RT * DP / 2; i += PA_THREADS) {
-        const int r = i / (DP / 2), d = i % (DP / 2) * 2;
-        reinterpret_cast<uint32_t*>(sm.q)[r * (DP / 2) + (((d / 8) ^ (r & 7)) * 4) + d % 8 / 2] = pa_q2(p, s, head, row0 + r, rows_all, d);
-      }
-    }
-    const int node0 = row0 / p.groups;
-    const int node[2] = {min(wrow + g, rows_all - 1) / p.groups, min(wrow + g + 8, rows_all - 1) / p.groups};
-    if (p.parents && t1 * static_cast<int64_t>(BN) > s.len) pa_ancestors(p, s, node0, node_last - node0 + 1, sm.seen, sm.up);
-    for (int tile = t0; tile < t1; ++tile) {
+    int node[2];
+    __syncthreads();  // (the part before is done with the shared memory)
+    find(w.t0);
+    // In round i tile i is fetched, the rows of tile i + 1 are found, and tile i - 2 is worked on.
+#pragma unroll 1
+    for (uint32_t tile = w.t0, out = 0; tile < w.t1 + ST - 1; ++tile) {
       pa_copy_wait<ST - 2>();
-      __syncthreads();  // the tile is there, the one before has been read, and where the next rows lie has been written
-      fetch(tile + ST - 1);
-      const uint32_t kt = ring + (tile - t0) % ST * (2 * S::SLOT), vt = kt + S::SLOT;
-      const int64_t first = static_cast<int64_t>(tile) * BN;
-      if (16 * warp < rows) {
-        if (first + BN <= s.len) {
-          w.template step<BN, false>(kt, vt, 0, p.scale, q_at, [](int, int) { return true; }, nullptr);
-        } else if (first <= s.len + static_cast<int64_t>(node_last)) {
-          const int before = static_cast<int>(s.len - first);
-          w.template step<BN, true>(
-              kt, vt, 0, p.scale, q_at,
-              [&](int h, int key) {
-                const int n = key - before;
-                if (n < 0) return true;
-                if (n > node_last) return false;
-                return p.parents ? ((sm.seen[node[h] - node0][n >> 5] >> (n & 31)) & 1) != 0 : n <= node[h];
-              },
-              sm.spare[warp]);
+      __syncthreads();  // tile - 2 is there, tile - 3 has been read, and where the rows of `tile` lie has been written
+      fetch(tile);
+      find(tile + 1);
+      if (tile == w.t0) {
+        const int wrow = w.row0 + 16 * warp;
+        x.clear();
+        if constexpr (DP <= 128) {
+          x.load_q(p, w, wrow);
+        } else {
+          q_at = static_cast<uint32_t>(__cvta_generic_to_shared(sm.q)) + warp * 16 * (DP * 2);
+          x.stage_q(p, w, sm.q, RT);
         }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) node[h] = static_cast<int>(p.by_group.of(min(wrow + g + 8 * h, w.rows_all - 1)));
+        if (p.parents && static_cast<uint64_t>(w.t1) * BN > static_cast<uint32_t>(w.s.len)) pa_ancestors(p, w.s, node0, node1 - node0 + 1, sm.seen, sm.up);
       }
-      if (p.fresh && rtile == 0 && first + BN > s.len) pa_store_new<DP>(p, s, slot, head, first, BN, kt, vt, 0, t, PA_THREADS);
-      find(tile + ST);
+      if (tile < w.t0 + ST - 1) continue;
+      const uint32_t kt = ring + out * (2 * S::SLOT);
+      out = out == ST - 1 ? 0 : out + 1;
+      const int n0 = static_cast<int>((tile - (ST - 1)) * BN) - w.s.len;
+      if (16 * warp < w.rows && n0 <= node1) {
+        const bool hides = n0 + BN > 0;
+        uint64_t sees[2] = {0, 0};
+        if (hides) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) sees[h] = pa_sees(p.parents ? sm.seen[min(node[h], node1) - node0] : nullptr, words_seen, node[h], n0);
+        }
+        x.template step<BN>(kt, kt + S::SLOT, p.scale, q_at, hides, sees, sm.spare[warp]);
+      }
     }
     pa_copy_wait<0>();
-    w.finish_sums();
-    const bool whole = t0 == 0 && t1 == tiles;
-    float* piece = p.work + (2 * static_cast<int64_t>(blockIdx.x) + (t0 == 0)) * pa_piece(RT, DP);
+    if (p.fresh && w.rtile == 0) {
+      const int64_t n0 = static_cast<int64_t>(w.t0) * BN - w.s.len, n1 = static_cast<int64_t>(w.t1) * BN - w.s.len;
+      if (n1 > 0) pa_store_new<uint4>(p, w, n0 < 0 ? 0 : static_cast<int>(n0), static_cast<int>(n1 < w.s.nodes ? n1 : w.s.nodes), words, t, PA_THREADS);
+    }
+    x.finish_sums();
+    const bool whole = w.t0 == 0 && w.t1 == w.tiles;
+    float* piece = pa_piece_of<RT, DP>(p, w);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int r = 16 * warp + g + 8 * h;
-      if (r >= rows) continue;
+      if (r >= w.rows) continue;
       if (whole) {
-        char* out = p.o.p + (s.start + static_cast<int64_t>(node[h])) * p.o.row + (head * p.groups + (row0 + r) % p.groups) * p.o.head;
-        const float f = 1.f / w.l[h];
+        char* out = pa_out(p, w.s.start, w.head, w.row0 + r);
+        const float f = 1.f / x.l[h];
 #pragma unroll
         for (int d = 0; d < DP / 8; ++d)
-          if (8 * d < c.dim) *reinterpret_cast<uint32_t*>(out + 16 * d + 4 * c4) = pa_pack<T>(w.o[d][2 * h] * f, w.o[d][2 * h + 1] * f);
+          if (8 * d < c.dim) *reinterpret_cast<uint32_t*>(out + 16 * d + 4 * c4) = pa_pack<T>(x.o[d][2 * h] * f, x.o[d][2 * h + 1] * f);
       } else {
 #pragma unroll
-        for (int d = 0; d < DP / 8; ++d) *reinterpret_cast<float2*>(piece + r * DP + 8 * d + 2 * c4) = make_float2(w.o[d][2 * h], w.o[d][2 * h + 1]);
+        for (int d = 0; d < DP / 8; ++d) *reinterpret_cast<float2*>(piece + r * DP + 8 * d + 2 * c4) = make_float2(x.o[d][2 * h], x.o[d][2 * h + 1]);
         if (c4 == 0) {
-          piece[RT * DP + r] = w.m[h];
-          piece[RT * DP + RT + r] = w.l[h];
+          piece[RT * DP + r] = x.m[h];
+          piece[RT * DP + RT + r] = x.l[h];
         }
       }
     }
-    pos += t1 - t0;
-    off += t1 - t0;
+    cut.note(sm.share, w, pos);
+    pos += w.t1 - w.t0;
+    off += w.t1 - w.t0;
   }
+  if (t == 0) cut.store(p);
 }
 
 // ---------------------------------------------------------------------------------------------- joining
-// CTA (x, y): the unit that cut number x + 1 runs through, if it is the first one inside it; rows y, y + gridDim.y, ...; the
-// pieces are shared by the warps, and their sums by way of shared memory joined in the order of the warps.
+// CTA (x, y): the unit that starts in share x and goes on behind it, rows y, y + gridDim.y, ... of it. The pieces of a row are
+// shared by the warps, and their sums are joined in the order of the warps.
 template <typename T, int DP>
-__global__ void __launch_bounds__(PA_THREADS) paged_attn_join_kernel(const PaParams p, int rt, int bn, int parts) {
+__global__ void __launch_bounds__(PA_THREADS) paged_attn_join_kernel(const PaParams p, int rt) {
   constexpr int WARPS = PA_THREADS / 32, C4 = DP / 4, PER = (C4 + 31) / 32;
-  __shared__ int64_t shared_at[3];
-  __shared__ int shared_slot;
   __shared__ float sums[WARPS][DP + 1];
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, cut = blockIdx.x + 1;
-  if (t < 32) {
-    bool bad = false;
-    const PaPlace at = pa_place(p, rt, bn, cut, parts, &bad);
-    if (t == 0) {
-      shared_at[0] = at.total;
-      shared_at[1] = at.at;
-      shared_at[2] = at.before;
-      shared_slot = at.slot;
-    }
-  }
-  __syncthreads();
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, first = blockIdx.x;
   dependent_wait();
-  const int64_t total = shared_at[0], at = shared_at[1];
-  const int slot = shared_slot;
-  if (slot >= p.c.slots) return;
-  bool bad = false;
-  const PaSlot s = pa_slot(p, slot, &bad);
-  const int tiles = pa_key_tiles(s, bn), row_tiles = pa_row_tiles(p, s, rt);
-  const int64_t off = at - shared_at[2];
-  const int unit = static_cast<int>(off / tiles), inside = static_cast<int>(off - static_cast<int64_t>(unit) * tiles);
-  if (inside == 0 || total * (cut - 1) / parts > at - inside) return;
-  const int64_t stop = at - inside + tiles;
-  int last = cut;  // the last share that has tiles of the unit
-  while (last + 1 < parts && total * (last + 1) / parts < stop) ++last;
-  const int head = unit / row_tiles, row0 = (unit - head * row_tiles) * rt, rows = min(rt, s.nodes * p.groups - row0);
+  const int4 a = p.cuts[2 * first];
+  const int last = p.cuts[2 * first + 1].x;
   const int64_t size = pa_piece(rt, DP);
-  const auto piece = [&](int i) { return p.work + (2 * static_cast<int64_t>(i) + (i == cut - 1)) * size; };
-  const auto empty = [&](int i) { return total * i / parts == total * (i + 1) / parts; };
-  for (int r = blockIdx.y; r < rows; r += gridDim.y) {
+  // (the unit is the last of its first share and the first of the others)
+  const float* const at = p.work + 2 * static_cast<int64_t>(first) * size;
+  for (int r = blockIdx.y; r < a.x; r += gridDim.y) {
     float m = -CUDART_INF_F;
-    for (int i = cut - 1 + lane; i <= last; i += 32)
-      if (!empty(i)) m = fmaxf(m, piece(i)[rt * DP + r]);
+    for (int i = lane; i <= last - first; i += 32) m = fmaxf(m, at[(2 * i + (i == 0)) * size + rt * DP + r]);
 #pragma unroll
     for (int w = 16; w; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
     float l = 0.f;
@@ -1031,10 +1040,9 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_join_kernel(const PaPar
 #pragma unroll
     for (int j = 0; j < PER; ++j) o[j] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int i = cut - 1 + warp; i <= last; i += WARPS) {
-      if (empty(i)) continue;
-      const float* x = piece(i);
-      const float mi = x[rt * DP + r], w = mi == -CUDART_INF_F ? 0.f : exp2f(mi - m);
+    for (int i = warp; i <= last - first; i += WARPS) {
+      const float* x = at + (2 * i + (i == 0)) * size;
+      const float mi = x[rt * DP + r], w = mi == -CUDART_INF_F ? 0.f : pa_exp2(mi - m);
       l = fmaf(w, x[rt * DP + rt + r], l);
 #pragma unroll
       for (int j = 0; j < PER; ++j)
@@ -1058,8 +1066,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_join_kernel(const PaPar
       }
     if (lane == 0) sums[warp][DP] = l;
     __syncthreads();
-    const int node = (row0 + r) / p.groups, g = (row0 + r) % p.groups;
-    T* out = reinterpret_cast<T*>(p.o.p + (s.start + node) * p.o.row + (head * p.groups + g) * p.o.head);
+    T* out = reinterpret_cast<T*>(pa_out(p, a.w, a.z, a.y + r));
     float all = 0.f;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) all += sums[w][DP];
@@ -1073,70 +1080,55 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_join_kernel(const PaPar
 }
 
 // ---------------------------------------------------------------------------------------------- host
-// How a call is cut: rows of a tile, padded dim, keys of a tile, CTAs.
+// How a call is cut: padded dim, rows and keys of a tile, CTAs.
 struct PaForm {
-  int rpt, dp, bn, rt, ctas, smem;
-  const void* kernel;
+  int dp, rt, bn, ctas, smem;
+  void (*kernel)(PaParams);
 };
 
-template <typename T, int DP, int RPT>
-static void pa_ffma(PaForm* f) {
-  f->dp = DP;
-  f->rpt = RPT;
-  f->rt = 8 * RPT;
-  f->bn = PA_BN_F<DP>;
-  f->smem = static_cast<int>(sizeof(PaSmemF<T, DP, RPT>));
-  f->kernel = reinterpret_cast<const void*>(paged_attn_ffma_kernel<T, DP, RPT>);
-  f->ctas = sm_count() * (f->smem <= 110 * 1024 ? 2 : 1);
+template <typename T, int DP, int RPT, bool WORDS>
+static PaForm pa_ffma() {
+  using S = PaFfma<T, DP, RPT>;
+  const int smem = static_cast<int>(sizeof(S));
+  return PaForm{DP, S::RT, S::BN, sm_count() * (smem <= 112 * 1024 ? 2 : 1), smem, paged_attn_ffma_kernel<T, DP, RPT, WORDS>};
 }
 template <typename T, int DP>
-static void pa_mma_form(PaForm* f, int rows) {
-  f->dp = DP;
-  f->ctas = sm_count() * (DP == 256 ? 1 : 2);
-  if (rows <= 16) {
-    f->rt = PaNarrow<T, DP>::RT;
-    f->bn = PaNarrow<T, DP>::BN;
-    f->smem = static_cast<int>(sizeof(PaNarrow<T, DP>));
-    f->kernel = reinterpret_cast<const void*>(paged_attn_narrow_kernel<T, DP>);
-  } else {
-    f->rt = PaWide<T, DP>::RT;
-    f->bn = PaWide<T, DP>::BN;
-    f->smem = static_cast<int>(sizeof(PaWide<T, DP>));
-    f->kernel = reinterpret_cast<const void*>(paged_attn_wide_kernel<T, DP>);
+static PaForm pa_form(int rows, bool words) {
+  if constexpr (sizeof(T) == 2) {
+    if (words) {
+      using N = PaNarrow<T, DP>;
+      using W = PaWide<T, DP>;
+      const int ctas = sm_count() * (DP == 256 ? 1 : 2);
+      if (rows <= 16) return PaForm{DP, N::RT, N::BN, ctas, static_cast<int>(sizeof(N)), paged_attn_narrow_kernel<T, DP>};
+      return PaForm{DP, W::RT, W::BN, ctas, static_cast<int>(sizeof(W)), paged_attn_wide_kernel<T, DP>};
+    }
+  } else if (words) {
+    return rows <= 8 ? pa_ffma<T, DP, 1, true>() : rows <= 16 ? pa_ffma<T, DP, 2, true>() : pa_ffma<T, DP, 4, true>();
   }
+  return rows <= 8 ? pa_ffma<T, DP, 1, false>() : pa_ffma<T, DP, 4, false>();
 }
 template <typename T>
 static PaForm pa_form(int dim, int rows, bool words) {
-  PaForm f{};
-  if constexpr (sizeof(T) == 2) {
-    if (words) {
-      dim <= 64 ? pa_mma_form<T, 64>(&f, rows) : dim <= 128 ? pa_mma_form<T, 128>(&f, rows) : pa_mma_form<T, 256>(&f, rows);
-      return f;
-    }
-  }
-  if (dim <= 64) rows <= 8 ? pa_ffma<T, 64, 1>(&f) : rows <= 16 ? pa_ffma<T, 64, 2>(&f) : pa_ffma<T, 64, 4>(&f);
-  else if (dim <= 128) rows <= 8 ? pa_ffma<T, 128, 1>(&f) : rows <= 16 ? pa_ffma<T, 128, 2>(&f) : pa_ffma<T, 128, 4>(&f);
-  else rows <= 8 ? pa_ffma<T, 256, 1>(&f) : rows <= 16 ? pa_ffma<T, 256, 2>(&f) : pa_ffma<T, 256, 4>(&f);
-  return f;
+  return dim <= 64 ? pa_form<T, 64>(rows, words) : dim <= 128 ? pa_form<T, 128>(rows, words) : pa_form<T, 256>(rows, words);
 }
-// The form of a call: `rows` rows over `slots` slots. Tiles of as many rows as a slot with an even share of them has. `words`: all
-// rows are whole 16-byte words on their boundaries.
+// The form of a call: `rows` rows over the cache's slots, tiles of as many rows as a slot with an even share of them has. `words`:
+// all rows are whole 16-byte words on their boundaries.
 static PaForm pa_choose(const ytcuda_pages* c, int rows, int heads, bool words) {
-  const int share = c->slots ? (rows + c->slots - 1) / c->slots : 1;
-  const int64_t tile = static_cast<int64_t>(share) * (heads / c->kv_heads);
-  const int r = static_cast<int>(tile < 4096 ? tile : 4096);
+  const int64_t share = (static_cast<int64_t>(rows) + c->slots - 1) / c->slots * (heads / c->kv_heads);
+  const int r = static_cast<int>(share < 4096 ? share : 4096);
   return c->dtype == YTC_F32    ? pa_form<float>(c->dim, r, words)
          : c->dtype == YTC_BF16 ? pa_form<__nv_bfloat16>(c->dim, r, words)
                                 : pa_form<__half>(c->dim, r, words);
 }
-static uint64_t pa_space(const PaForm& f) { return 4ull * 2 * static_cast<uint64_t>(f.ctas) * static_cast<uint64_t>(pa_piece(f.rt, f.dp)); }
+static uint64_t pa_pieces(const PaForm& f) { return 4ull * 2 * static_cast<uint64_t>(f.ctas) * static_cast<uint64_t>(pa_piece(f.rt, f.dp)); }
+static uint64_t pa_space(const PaForm& f) { return pa_pieces(f) + 2ull * sizeof(int4) * static_cast<uint64_t>(f.ctas); }
 
 template <typename T>
 static cudaError_t pa_join(const PaForm& f, const PaParams& p, cudaStream_t st) {
-  const dim3 grid(f.ctas - 1, f.rt < 16 ? f.rt : 16), block(PA_THREADS);
-  if (f.dp == 64) return pg_launch_behind(paged_attn_join_kernel<T, 64>, grid, block, 0, st, p, f.rt, f.bn, f.ctas);
-  if (f.dp == 128) return pg_launch_behind(paged_attn_join_kernel<T, 128>, grid, block, 0, st, p, f.rt, f.bn, f.ctas);
-  return pg_launch_behind(paged_attn_join_kernel<T, 256>, grid, block, 0, st, p, f.rt, f.bn, f.ctas);
+  const dim3 grid(f.ctas, f.rt <= 16 ? 4 : 8), block(PA_THREADS);
+  if (f.dp == 64) return pg_launch_behind(paged_attn_join_kernel<T, 64>, grid, block, 0, st, p, f.rt);
+  if (f.dp == 128) return pg_launch_behind(paged_attn_join_kernel<T, 128>, grid, block, 0, st, p, f.rt);
+  return pg_launch_behind(paged_attn_join_kernel<T, 256>, grid, block, 0, st, p, f.rt);
 }
 
 }  // namespace ytk
@@ -1180,24 +1172,31 @@ int ytcuda_pages_attend(const ytcuda_pages* cache, int layer, const void* q, con
   const bool words = pg_width(pg_bits(p.c.k) | pg_bits(p.c.v) | pg_bits(p.q) | pg_bits(p.o) | pg_bits(p.k) | pg_bits(p.v) |
                               static_cast<uint64_t>(p.c.dim * size)) == 16;
   const PaForm f = pa_choose(cache, rows, heads, words);
-  YTC_REQUIRE(workspace && workspace_bytes >= ytcuda_pages_attend_workspace(cache, rows, heads) && reinterpret_cast<uint64_t>(workspace) % 16 == 0,
-              "%s: a workspace of %llu bytes on a 16-byte boundary is needed", who,
-              static_cast<unsigned long long>(ytcuda_pages_attend_workspace(cache, rows, heads)));
+  YTC_REQUIRE(workspace && workspace_bytes >= pa_space(f) && reinterpret_cast<uint64_t>(workspace) % 16 == 0,
+              "%s: a workspace of %llu bytes on a 16-byte boundary is needed", who, static_cast<unsigned long long>(pa_space(f)));
+  p.groups = heads / p.c.heads;
+  // the most tiles that the slots can have: row tiles of all slots, each over a full row of the table and its own nodes
+  const int64_t row_tiles = static_cast<int64_t>(rows) * p.groups / f.rt + p.c.slots;
+  const int64_t key_tiles = (static_cast<int64_t>(p.c.max_pages) * p.c.page + rows) / f.bn + 1;
+  if (static_cast<double>(row_tiles) * static_cast<double>(key_tiles) * p.c.heads >= 2147483648.0) {
+    set_last_error("%s: %d rows over tables of %d positions are too much work for one call", who, rows, p.c.max_pages * p.c.page);
+    return YTC_UNSUPPORTED;
+  }
   p.c.k.p += layer * p.c.k.layer;
   p.c.v.p += layer * p.c.v.layer;
+  p.by_group = pg_div(static_cast<uint32_t>(p.groups));
   p.starts = starts;
   p.parents = parents;
   p.rows = rows;
-  p.heads = heads;
-  p.groups = heads / p.c.heads;
   p.fresh = k != nullptr;
   p.scale = (scale != 0.f ? scale : 1.f / sqrtf(static_cast<float>(p.c.dim))) * PA_LOG2E;
   p.work = static_cast<float*>(workspace);
+  p.cuts = reinterpret_cast<int4*>(static_cast<char*>(workspace) + pa_pieces(f));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (const int rc = ensure_dynamic_smem(f.kernel, f.smem)) return rc;
-  void* args[] = {&p};
-  YTC_CUDA(cudaLaunchKernel(f.kernel, dim3(f.ctas), dim3(PA_THREADS), args, f.smem, st));
+  if (const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(f.kernel), f.smem)) return rc;
+  f.kernel<<<f.ctas, PA_THREADS, f.smem, st>>>(p);
   count_launch();
+  YTC_CUDA(cudaGetLastError());
   YTC_CUDA(cache->dtype == YTC_F32 ? pa_join<float>(f, p, st) : cache->dtype == YTC_BF16 ? pa_join<__nv_bfloat16>(f, p, st) : pa_join<__half>(f, p, st));
   count_launch();
   return YTC_OK;

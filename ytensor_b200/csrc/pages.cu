@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32) pages_append_kernel(const PgCac
     }
     const PgPool pool = item & 1 ? c.v : c.k;
     const PgRows src = item & 1 ? v : k;
-    pg_copy_rows<W>(pool.p + layer * pool.layer + pg * pool.page + (at % c.page) * pool.row, pool.head, src.p + row * src.row, src.head,
+    pg_copy_rows<W>(pool.p + layer * pool.layer + pg * pool.page + pg_row_of(c, at) * pool.row, pool.head, src.p + row * src.row, src.head,
                     c.heads, row_words);
   }
 }
@@ -291,8 +291,8 @@ __global__ void __launch_bounds__(PG_WARPS * 32) pages_keep_kernel(const PgCache
             const int a = accepted[static_cast<int64_t>(s) * depth + j];
             if (a != j) {
               const int64_t x = b + a, y = b + j, off = (i - r * row_words) * static_cast<int64_t>(sizeof(W));
-              w[u] = *reinterpret_cast<const W*>(p + pg_page_of(c, s, x) * pool.page + x % c.page * pool.row + off);
-              to[u] = p + pg_page_of(c, s, y) * pool.page + y % c.page * pool.row + off;
+              w[u] = *reinterpret_cast<const W*>(p + pg_page_of(c, s, x) * pool.page + pg_row_of(c, x) * pool.row + off);
+              to[u] = p + pg_page_of(c, s, y) * pool.page + pg_row_of(c, y) * pool.row + off;
             }
           }
         }
@@ -491,7 +491,7 @@ int pg_take(const char* who, const ytcuda_pages* c, PgCache* out) {
     return PgPool{static_cast<char*>(p), s[0] * size, s[1] * size, s[2] * size, s[3] * size};
   };
   for (int i = 0; i < 4; ++i) YTC_REQUIRE(c->k_strides[i] >= 0 && c->v_strides[i] >= 0, "%s: negative stride in a pool", who);
-  *out = PgCache{pool(c->k, c->k_strides), pool(c->v, c->v_strides), c->table, c->lens, c->held, c->refs, c->status, c->scratch,
+  *out = PgCache{pool(c->k, c->k_strides), pool(c->v, c->v_strides), pg_div(static_cast<uint32_t>(c->page)), c->table, c->lens, c->held, c->refs, c->status, c->scratch,
                  c->layers, c->pages, c->page, c->kv_heads, c->dim, c->slots, c->max_pages};
   return YTC_OK;
 }

@@ -16,8 +16,21 @@ struct PgPool {
   int64_t layer, page, head, row;
 };
 
+// Division of whole numbers below 2^31 by a divisor d the host knows: with 2^(l - 1) < d <= 2^l and m = floor(2^(31 + l) / d) + 1
+// the error of n m / 2^(31 + l) is below 2^-l <= 1 / d, which the fraction of n / d leaves room for.
+struct PgDiv {
+  uint32_t mul, shift, d;
+  __host__ __device__ __forceinline__ uint32_t of(uint32_t n) const { return static_cast<uint32_t>((static_cast<uint64_t>(n) * mul) >> shift); }
+};
+inline PgDiv pg_div(uint32_t d) {
+  uint32_t l = 0;
+  while ((1ull << l) < d) ++l;
+  return PgDiv{static_cast<uint32_t>((1ull << (31 + l)) / d + 1), 31 + l, d};
+}
+
 struct PgCache {
   PgPool k, v;
+  PgDiv by_page;
   int32_t *table, *lens, *held, *refs, *status, *scratch;
   int layers, pages, page, heads, dim, slots, max_pages;
 };
@@ -62,12 +75,18 @@ inline uint64_t pg_bits(const PgPool& p) {
 inline uint64_t pg_bits(const PgRows& r) { return reinterpret_cast<uint64_t>(r.p) | static_cast<uint64_t>(r.row | r.head); }
 
 #ifdef __CUDACC__
-// Row of position `at` of a slot in one pool (layer and head added by the caller), nullptr where the slot holds no page there.
+// The page that holds position `at` of a slot; -1 where the slot holds none there.
 __device__ __forceinline__ int pg_page_of(const PgCache& c, int slot, int64_t at) {
-  const int64_t i = at / c.page;
-  if (at < 0 || i >= c.held[slot] || i >= c.max_pages) return -1;
+  if (at < 0 || at > 0x7fffffff) return -1;
+  const int i = static_cast<int>(c.by_page.of(static_cast<uint32_t>(at)));
+  if (i >= c.held[slot] || i >= c.max_pages) return -1;
   const int pg = c.table[static_cast<int64_t>(slot) * c.max_pages + i];
   return pg >= 0 && pg < c.pages ? pg : -1;
+}
+// Row of its page that position `at` has (at: not negative, below 2^31).
+__device__ __forceinline__ int pg_row_of(const PgCache& c, int64_t at) {
+  const uint32_t n = static_cast<uint32_t>(at);
+  return static_cast<int>(n - c.by_page.of(n) * c.by_page.d);
 }
 // A launch behind another of the same call, whose set-up may overlap it: the kernel calls dependent_wait() first of all.
 template <typename... KArgs, typename... Args>

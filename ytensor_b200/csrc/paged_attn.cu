@@ -283,9 +283,9 @@ __device__ __forceinline__ float pa_exp2(float x) {
 }
 
 // ---------------------------------------------------------------------------------------------- FFMA form
-// fp32, and 16-bit rows that no matrix instruction takes (dims that are not a multiple of 8, odd alignments). 8 x 16 threads:
-// thread (a, b) holds rows a + 8 i (RPT of them) with keys b + 16 j of S and with columns 4 b + 64 j of O. Two tiles of keys and
-// values as fp32 in shared memory, the next one on its way while one is worked on (WORDS: by cp.async; else element by element).
+// Rows that are not whole 16-byte words on their boundaries (odd dims and strides), element by element. 8 x 16 threads: thread
+// (a, b) holds rows a + 8 i (RPT of them) with keys b + 16 j of S and with columns 4 b + 64 j of O. Two tiles of keys and values as
+// fp32 in shared memory: the next one is read before one is worked on.
 template <typename T, int DP, int RPT>
 struct PaFfma {
   static constexpr int RT = 8 * RPT, BN = DP == 64 ? 64 : 32;
@@ -296,7 +296,8 @@ struct PaFfma {
   PaShare share;
 };
 
-// O += S V of one tile. HIDDEN: weights of zero take nothing along (a hidden position may hold an infinity or NaN).
+// O += S V of one tile. HIDDEN: weights of zero take nothing along (a hidden position holds an infinity or NaN, and 0 x infinity
+// would spoil every row).
 template <int DP, int RPT, int BN, bool HIDDEN>
 __device__ __forceinline__ void pa_ffma_values(const float (*s)[BN + 4], const float (*v)[DP], int a, int b, float (*o)[DP / 16]) {
 #pragma unroll(HIDDEN ? 1 : 2)
@@ -322,10 +323,9 @@ __device__ __forceinline__ void pa_ffma_values(const float (*s)[BN + 4], const f
   }
 }
 
-template <typename T, int DP, int RPT, bool WORDS>
+template <typename T, int DP, int RPT>
 __global__ void __launch_bounds__(PA_THREADS) paged_attn_ffma_kernel(const PaParams p) {
   using S = PaFfma<T, DP, RPT>;
-  static_assert(!WORDS || std::is_same<T, float>::value, "words are copied as they are");
   constexpr int RT = S::RT, BN = S::BN, KPT = BN / 16, CJ = DP / 64;
   extern __shared__ __align__(128) unsigned char raw[];
   S& sm = *reinterpret_cast<S*>(raw);
@@ -341,36 +341,26 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_ffma_kernel(const PaPar
     const PaPart w = pa_part<RT, BN>(p, pos, end, &slot, &off);
     const int nodes = w.s.nodes, words = (nodes + 31) / 32;
     const int node0 = static_cast<int>(p.by_group.of(w.row0)), node1 = static_cast<int>(p.by_group.of(w.row0 + w.rows - 1));
-    const auto find = [&](uint32_t tile) {  // where the tile's rows lie
+    // Thread t < BN finds where row t of a tile lies, with the page that it looked up one tile earlier.
+    int pg = t < BN ? pa_lookup(p, w, w.t0 * BN + t) : -1;
+    const auto find = [&](uint32_t tile) {
       if (t < BN && tile < w.t1) {
-        const uint32_t at = tile * BN + t;
-        const PaRow r = pa_row(p, w, at, pa_lookup(p, w, at));
+        const PaRow r = pa_row(p, w, tile * BN + t, pg);
         sm.row[tile & 1][0][t] = reinterpret_cast<const T*>(r.k);
         sm.row[tile & 1][1][t] = reinterpret_cast<const T*>(r.v);
+        if (tile + 1 < w.t1) pg = pa_lookup(p, w, (tile + 1) * BN + t);
       }
     };
     const auto fetch = [&](uint32_t tile) {
       if (tile >= w.t1) return;
       const int x = tile & 1;
-      if constexpr (WORDS) {
 #pragma unroll 4
-        for (int i = t; i < BN * DP / 4; i += PA_THREADS) {
-          const int r = i / (DP / 4), d = i % (DP / 4) * 4;
-          const T *kp = sm.row[x][0][r], *vp = sm.row[x][1][r];
-          const bool there = kp != nullptr && d < c.dim;
-          pa_copy16(static_cast<uint32_t>(__cvta_generic_to_shared(&sm.k[x][r][d])), there ? reinterpret_cast<const char*>(kp + d) : c.k.p, there);
-          pa_copy16(static_cast<uint32_t>(__cvta_generic_to_shared(&sm.v[x][r][d])), there ? reinterpret_cast<const char*>(vp + d) : c.v.p, there);
-        }
-        pa_copy_commit();
-      } else {
-#pragma unroll 4
-        for (int i = t; i < BN * DP; i += PA_THREADS) {
-          const int r = i / DP, d = i % DP;
-          const T *kp = sm.row[x][0][r], *vp = sm.row[x][1][r];
-          const bool there = kp != nullptr && d < c.dim;
-          sm.k[x][r][d] = there ? pa_load(kp + d) : 0.f;
-          sm.v[x][r][d] = there ? pa_load(vp + d) : 0.f;
-        }
+      for (int i = t; i < BN * DP; i += PA_THREADS) {
+        const int r = i / DP, d = i % DP;
+        const T *kp = sm.row[x][0][r], *vp = sm.row[x][1][r];
+        const bool there = kp != nullptr && d < c.dim;
+        sm.k[x][r][d] = there ? pa_load(kp + d) : 0.f;
+        sm.v[x][r][d] = there ? pa_load(vp + d) : 0.f;
       }
     };
     __syncthreads();  // (the part before is done with the shared memory)
@@ -395,7 +385,6 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_ffma_kernel(const PaPar
     }
 #pragma unroll 1
     for (uint32_t tile = w.t0; tile < w.t1; ++tile) {
-      if constexpr (WORDS) pa_copy_wait<0>();
       __syncthreads();
       fetch(tile + 1);
       find(tile + 2);
@@ -450,11 +439,19 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_ffma_kernel(const PaPar
         for (int j = 0; j < 4 * CJ; ++j) o[i][j] *= shrink;
       }
       __syncwarp();  // (a row of S is written and read by one half of a warp)
-      if (masked) pa_ffma_values<DP, RPT, BN, true>(sm.s, sm.v[cur], a, b, o);
-      else pa_ffma_values<DP, RPT, BN, false>(sm.s, sm.v[cur], a, b, o);
+      bool fine = true;
+      if (masked) {  // (0 x infinity: see below)
+#pragma unroll 1
+        for (int i = t; i < BN * DP / 4; i += PA_THREADS) {
+          const float4 y = *reinterpret_cast<const float4*>(&sm.v[cur][i / (DP / 4)][i % (DP / 4) * 4]);
+          fine = fine && fabsf(y.x) < CUDART_INF_F && fabsf(y.y) < CUDART_INF_F && fabsf(y.z) < CUDART_INF_F && fabsf(y.w) < CUDART_INF_F;
+        }
+        fine = __syncthreads_and(fine);
+      }
+      if (fine) pa_ffma_values<DP, RPT, BN, false>(sm.s, sm.v[cur], a, b, o);
+      else pa_ffma_values<DP, RPT, BN, true>(sm.s, sm.v[cur], a, b, o);
       __syncwarp();
     }
-    if constexpr (WORDS) pa_copy_wait<0>();
     if (p.fresh && w.rtile == 0) {
       const int64_t n0 = static_cast<int64_t>(w.t0) * BN - w.s.len, n1 = static_cast<int64_t>(w.t1) * BN - w.s.len;
       if (n1 > 0) pa_store_new<T>(p, w, n0 < 0 ? 0 : static_cast<int>(n0), static_cast<int>(n1 < nodes ? n1 : nodes), c.dim, t, PA_THREADS);
@@ -492,12 +489,15 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_ffma_kernel(const PaPar
 }
 
 // ---------------------------------------------------------------------------------------------- matrix-instruction forms
-// 16-bit types with dims of whole 16-byte words: rows of a tile in the M of mma m16n8k16, keys in its N (S = Q K^T) and then in
+// Rows of whole 16-byte words. 16-bit types: rows of a tile in the M of mma m16n8k16, keys in its N (S = Q K^T) and then in
 // its K (O += P V). Keys and values stay as they lie in the pages: cp.async brings rows of 2 DP bytes into a ring, 16-byte words
 // at (word ^ row % 8), so that ldmatrix reads eight rows without bank conflicts; what a row of the table does not reach is zero.
 // The softmax reference of a row is its running maximum, moved only when it grows by more than 2^8 (P then stays below 2^8, and
 // a row of O is hardly ever rescaled); P is rounded to the cache's type as the operand of a matrix instruction has to be, its sum
 // l is of the unrounded numbers in fp32.
+// fp32: every number is two of 11 bits, x = hi + lo with hi = x rounded to 11 bits, and a product the three of m16n8k8 (tf32) that
+// lie above 2^-22 of it: hi hi + hi lo + lo hi. That keeps fp32's accuracy and takes a third of the instructions that fused
+// multiply-adds of single lanes would. An infinity has no such halves: what sees one is NaN.
 constexpr float PA_SLACK = 8.f;
 
 __device__ __forceinline__ void pa_ldmatrix(uint32_t at, uint32_t (&r)[4]) {
@@ -509,11 +509,11 @@ __device__ __forceinline__ void pa_ldmatrix_t(uint32_t at, uint32_t (&r)[4]) {
 template <typename T>
 __device__ __forceinline__ void pa_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if constexpr (std::is_same<T, __nv_bfloat16>::value)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -710,8 +710,9 @@ struct PaWarp {
     }
   }
   // The same into shared memory, `rows` rows by all threads of the CTA.
-  static __device__ __forceinline__ void stage_q(const PaParams& p, const PaPart& w, uint4* to, int rows) {
-    for (int i = threadIdx.x; i < rows * (DP / 8); i += PA_THREADS) {
+  static __device__ __forceinline__ void stage_q(const PaParams& p, const PaPart& w, void* into, int rows) {
+    uint4* to = static_cast<uint4*>(into);
+    for (int i = threadIdx.x; i < rows * (DP / 8); i += blockDim.x) {
       const int r = i / (DP / 8), x = i % (DP / 8);
       const bool there = w.row0 + r < w.rows_all && 8 * x < p.c.dim;
       to[r * (DP / 8) + (x ^ (r & 7))] = there ? reinterpret_cast<const uint4*>(pa_query(p, w, w.row0 + r))[x] : make_uint4(0u, 0u, 0u, 0u);
@@ -727,24 +728,206 @@ struct PaWarp {
   }
 };
 
-// Up to 16 rows: every warp has its own keys (16 of each tile of 64), its own ring, and no barrier until the part ends, where the
-// four warps' sums are joined. What bounds it is the copy of keys and values: 512 bytes a key and head at dim 128.
+// The same in fp32, eight keys a step; rows of the ring are 16 bytes longer than they have to be, so that the words of a fragment lie
+// in different banks.
+__device__ __forceinline__ void pa_mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// (the instruction takes the upper 19 bits of an operand: what it leaves of lo is below 2^-22 of x)
+__device__ __forceinline__ void pa_halves(float x, uint32_t* hi, uint32_t* lo) {
+  *hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+  *lo = __float_as_uint(x - __uint_as_float(*hi));
+}
+__device__ __forceinline__ float pa_lds(uint32_t at) {
+  float x;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(at));
+  return x;
+}
+
+template <int DP>
+struct PaWarp<float, DP> {
+  static constexpr int ROW = DP * 4 + 16;  // bytes of a row in the ring
+  float o[DP / 8][4], m[2], l[2];
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+    m[0] = m[1] = -CUDART_INF_F;
+    l[0] = l[1] = 0.f;
+  }
+
+  // Q of 16 rows in the order of the fragments: for each step of 8 dims four words hi of every lane, then four lo.
+  static __device__ __forceinline__ void stage_q(const PaParams& p, const PaPart& w, void* into, int) {
+    uint4* to = static_cast<uint4*>(into);
+    for (int i = threadIdx.x; i < DP / 8 * 32; i += blockDim.x) {
+      const int lane = i & 31, d = i / 32 * 8 + (lane & 3);
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = w.row0 + (lane >> 2) + 8 * (j & 1), dd = d + 4 * (j >> 1);
+        const bool there = r < w.rows_all && dd < p.c.dim;
+        pa_halves(there ? reinterpret_cast<const float*>(pa_query(p, w, r))[dd] : 0.f, &hi[j], &lo[j]);
+      }
+      to[i / 32 * 64 + lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      to[i / 32 * 64 + 32 + lane] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+  }
+
+  template <int NK>
+  __device__ __forceinline__ void step(uint32_t kt, uint32_t vt, float scale, uint32_t q_at, bool hides, const uint64_t (&sees)[2], float* spare) {
+    static_assert(NK == 8, "one fragment of keys");
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    float s[4];
+    {
+      float whole[2][4], cross[2][4];  // (sums of even and odd steps: four chains of instructions)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) whole[i][j] = cross[i][j] = 0.f;
+      const uint32_t at = kt + g * ROW + 4 * t;
+#pragma unroll
+      for (int d0 = 0; d0 < DP / 8; d0 += 4) {  // (four steps' words first: the products wait for none)
+        uint32_t ah[4][4], al[4][4], bh[4][2], bl[4][2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int d = d0 + i;
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(ah[i][0]), "=r"(ah[i][1]), "=r"(ah[i][2]), "=r"(ah[i][3]) : "r"(q_at + (d * 64 + lane) * 16));
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(al[i][0]), "=r"(al[i][1]), "=r"(al[i][2]), "=r"(al[i][3]) : "r"(q_at + (d * 64 + 32 + lane) * 16));
+          pa_halves(pa_lds(at + 32 * d), &bh[i][0], &bl[i][0]);
+          pa_halves(pa_lds(at + 32 * d + 16), &bh[i][1], &bl[i][1]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          pa_mma_tf32(cross[i & 1], ah[i], bl[i][0], bl[i][1]);
+          pa_mma_tf32(whole[i & 1], ah[i], bh[i][0], bh[i][1]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pa_mma_tf32(cross[i & 1], al[i], bh[i][0], bh[i][1]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[j] = ((cross[0][j] + cross[1][j]) + (whole[0][j] + whole[1][j])) * scale;
+    }
+    bool fine = true;
+    if (hides) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (!((sees[j >> 1] >> (2 * t + (j & 1))) & 1)) s[j] = -CUDART_INF_F;
+#pragma unroll 1
+      for (int i = lane; i < NK * DP; i += 32) fine = fine && fabsf(pa_lds(vt + i / DP * ROW + i % DP * 4)) < CUDART_INF_F;
+      fine = __all_sync(0xffffffffu, fine);
+    }
+    float shrink[2];
+    bool moves = false;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float top = fmaxf(s[2 * h], s[2 * h + 1]);
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const bool up = top > m[h] + PA_SLACK || (m[h] == -CUDART_INF_F && top > m[h]);
+      shrink[h] = up ? pa_exp2(m[h] - top) : 1.f;
+      if (up) m[h] = top;
+      moves = moves || up;
+    }
+    if (__any_sync(0xffffffffu, moves)) {
+#pragma unroll
+      for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[i][j] *= shrink[j >> 1];
+      l[0] *= shrink[0];
+      l[1] *= shrink[1];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      s[j] = pa_exp2(s[j] - (m[j >> 1] == -CUDART_INF_F ? 0.f : m[j >> 1]));
+      l[j >> 1] += s[j];
+    }
+    // keys 2 t and 2 t + 1, which this thread has weights of, are places t and t + 4 of the product
+    uint32_t ah[4], al[4];
+    pa_halves(s[0], &ah[0], &al[0]);
+    pa_halves(s[2], &ah[1], &al[1]);
+    pa_halves(s[1], &ah[2], &al[2]);
+    pa_halves(s[3], &ah[3], &al[3]);
+    const uint32_t at = vt + 2 * t * ROW + 4 * g;
+#pragma unroll
+    for (int d0 = 0; d0 < DP / 8; d0 += 4) {
+      uint32_t bh[4][2], bl[4][2];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float y[2] = {pa_lds(at + 32 * (d0 + i)), pa_lds(at + ROW + 32 * (d0 + i))};
+        if (!fine) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            if (!(fabsf(y[j]) < CUDART_INF_F)) y[j] = 0.f;
+        }
+        pa_halves(y[0], &bh[i][0], &bl[i][0]);
+        pa_halves(y[1], &bh[i][1], &bl[i][1]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pa_mma_tf32(o[d0 + i], ah, bl[i][0], bl[i][1]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pa_mma_tf32(o[d0 + i], al, bh[i][0], bh[i][1]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pa_mma_tf32(o[d0 + i], ah, bh[i][0], bh[i][1]);
+    }
+    if (!fine) {  // as add_infinite of the 16-bit form
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < 4; ++j) spare[(g + 8 * (j >> 1)) * 8 + 2 * t + (j & 1)] = s[j];
+      __syncwarp();
+#pragma unroll 1
+      for (int kk = 0; kk < 8; ++kk) {
+        const float w0 = spare[g * 8 + kk], w1 = spare[(g + 8) * 8 + kk];
+#pragma unroll
+        for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float y = pa_lds(vt + kk * ROW + (8 * d + 2 * t + j) * 4);
+            if (fabsf(y) < CUDART_INF_F) continue;
+            if (w0 != 0.f) o[d][j] = fmaf(w0, y, o[d][j]);
+            if (w1 != 0.f) o[d][2 + j] = fmaf(w1, y, o[d][2 + j]);
+          }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void finish_sums() {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+    }
+  }
+};
+
+// Up to 16 rows: every warp has its own keys (a quarter of each tile), its own ring, and no barrier until the part ends, where the
+// four warps' sums are joined. What bounds it is the copy of keys and values: 512 bytes a key and head at dim 128 (fp32: 1024,
+// and the instructions of three products).
 template <typename T, int DP>
 struct PaNarrow {
-  static constexpr int RT = 16, BN = 64, WARPS = 4, STAGES = DP == 64 ? 6 : 3, SLOT = 16 * DP * 2;  // bytes of 16 keys
+  static constexpr bool F32 = std::is_same<T, float>::value;
+  static constexpr int RT = 16, WARPS = F32 && DP <= 128 ? 8 : 4, THREADS = 32 * WARPS, CTAS = F32 || DP == 256 ? 1 : 2;
+  static constexpr int KEYS = F32 ? 8 : 16, BN = WARPS * KEYS;
+  static constexpr int STAGES = F32 ? (DP == 64 ? 5 : DP == 128 ? 3 : 2) : DP == 64 ? 6 : 3, ROW = F32 ? DP * 4 + 16 : DP * 2, SLOT = KEYS * ROW;
+  static constexpr int Q = F32 ? DP / 8 * 32 * 2 : DP > 128 ? 16 * DP / 8 : 1;
   uint4 ring[WARPS][STAGES][2][SLOT / 16];
-  uint4 q[DP > 128 ? 16 * DP * 2 / 16 : 1];
+  uint4 q[Q];
   float spare[WARPS][16 * 8];
   float m[WARPS][16], l[WARPS][16];
   uint32_t seen[RT][PA_TREE / 32 + 1];
   int16_t up[PA_TREE];
   PaShare share;
+  // Where word `w` of row `r` lies in a slot.
+  static __device__ __forceinline__ uint32_t at(int r, int w) { return r * ROW + ((F32 ? w : w ^ (r & 7)) << 4); }
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) paged_attn_narrow_kernel(const PaParams p) {
+__global__ void __launch_bounds__(PaNarrow<T, DP>::THREADS, PaNarrow<T, DP>::CTAS) paged_attn_narrow_kernel(const PaParams p) {
   using S = PaNarrow<T, DP>;
-  constexpr int RT = S::RT, BN = S::BN, ST = S::STAGES, WORDS = DP / 8, PER = 32 / WORDS;  // rows of a copy instruction
+  constexpr int RT = S::RT, BN = S::BN, ST = S::STAGES, KEYS = S::KEYS, WORDS = DP * sizeof(T) / 16;
   extern __shared__ __align__(128) unsigned char raw[];
   S& sm = *reinterpret_cast<S*>(raw);
   dependent_trigger();
@@ -756,24 +939,24 @@ __global__ void __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) paged_attn_narr
   const uint32_t end = sm.share.to;
   int slot = sm.share.slot;
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(sm.ring[warp]));
-  const int word = lane % WORDS, words = c.dim / 8;
+  const int words = c.dim * static_cast<int>(sizeof(T)) / 16;
   while (pos < end) {
     const PaPart w = pa_part<RT, BN>(p, pos, end, &slot, &off);
-    const uint32_t mine = 16 * warp;
-    // (a lane looks up the page of key lane % 16 of a step, one step before the copies need it)
-    const auto lookup = [&](uint32_t tile) { return tile < w.t1 ? pa_lookup(p, w, tile * BN + mine + (lane & 15)) : -1; };
+    const uint32_t mine = KEYS * warp;
+    // (a lane looks up the page of key lane % KEYS of a step, one step before the copies need it)
+    const auto lookup = [&](uint32_t tile) { return tile < w.t1 ? pa_lookup(p, w, tile * BN + mine + lane % KEYS) : -1; };
     uint32_t into = 0;  // ring slot of the next copies
     const auto fetch = [&](uint32_t tile, int pg) {
       if (tile < w.t1) {
-        const PaRow r = pa_row(p, w, tile * BN + mine + (lane & 15), pg);
+        const PaRow r = pa_row(p, w, tile * BN + mine + lane % KEYS, pg);
         const uint32_t kt = ring + into * (2 * S::SLOT);
         const unsigned long long kp = reinterpret_cast<unsigned long long>(r.k), vp = reinterpret_cast<unsigned long long>(r.v);
 #pragma unroll
-        for (int i = 0; i < 16 / PER; ++i) {
-          const int row = i * PER + lane / WORDS;
+        for (int i = 0; i < KEYS * WORDS / 32; ++i) {
+          const int row = (32 * i + lane) / WORDS, word = (32 * i + lane) % WORDS;
           const unsigned long long a = __shfl_sync(0xffffffffu, kp, row), b = __shfl_sync(0xffffffffu, vp, row);
           const bool there = a != 0 && word < words;
-          const uint32_t to = kt + row * (DP * 2) + ((word ^ (row & 7)) << 4);
+          const uint32_t to = kt + S::at(row, word);
           pa_copy16(to, there ? reinterpret_cast<const char*>(a) + word * 16 : c.k.p, there);
           pa_copy16(to + S::SLOT, there ? reinterpret_cast<const char*>(b) + word * 16 : c.v.p, there);
         }
@@ -792,9 +975,9 @@ __global__ void __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) paged_attn_narr
       const int next = lookup(tile + 1);
       fetch(tile, pg);
       pg = next;
-      if (tile == w.t0) {  // (behind the first copies)
+      if (tile == w.t0 + ST - 2) {  // (behind the first copies)
         x.clear();
-        if constexpr (DP <= 128) {
+        if constexpr (S::Q == 1) {
           x.load_q(p, w, w.row0);
         } else {
           q_at = static_cast<uint32_t>(__cvta_generic_to_shared(sm.q));
@@ -813,20 +996,20 @@ __global__ void __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) paged_attn_narr
       out = out == ST - 1 ? 0 : out + 1;
       const int n0 = static_cast<int>((tile - (ST - 1)) * BN + mine) - w.s.len;  // the node at the first key
       if (n0 < w.s.nodes) {
-        const bool hides = n0 + 16 > 0;
+        const bool hides = n0 + KEYS > 0;
         uint64_t sees[2] = {0, 0};
         if (hides) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) sees[h] = pa_sees(p.parents ? sm.seen[node[h] - node0] : nullptr, words_seen, node[h], n0);
         }
-        x.template step<16>(kt, kt + S::SLOT, p.scale, q_at, hides, sees, sm.spare[warp]);
+        x.template step<KEYS>(kt, kt + S::SLOT, p.scale, q_at, hides, sees, sm.spare[warp]);
       }
       __syncwarp();  // (the next copies go into the slot that has just been read)
     }
     pa_copy_wait<0>();
     if (p.fresh && w.rtile == 0) {
       const int64_t n0 = static_cast<int64_t>(w.t0) * BN - w.s.len, n1 = static_cast<int64_t>(w.t1) * BN - w.s.len;
-      if (n1 > 0) pa_store_new<uint4>(p, w, n0 < 0 ? 0 : static_cast<int>(n0), static_cast<int>(n1 < w.s.nodes ? n1 : w.s.nodes), words, t, PA_THREADS);
+      if (n1 > 0) pa_store_new<uint4>(p, w, n0 < 0 ? 0 : static_cast<int>(n0), static_cast<int>(n1 < w.s.nodes ? n1 : w.s.nodes), words, t, S::THREADS);
     }
     x.finish_sums();
     // the warps' sums: O of each in its own ring
@@ -847,7 +1030,7 @@ __global__ void __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) paged_attn_narr
     const bool whole = w.t0 == 0 && w.t1 == w.tiles;
     float* piece = pa_piece_of<RT, DP>(p, w);
 #pragma unroll 1
-    for (int i = t; i < w.rows * (DP / 4); i += PA_THREADS) {
+    for (int i = t; i < w.rows * (DP / 4); i += S::THREADS) {
       const int r = i / (DP / 4), d = i % (DP / 4) * 4;
       float m = -CUDART_INF_F;
 #pragma unroll
@@ -866,8 +1049,10 @@ __global__ void __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) paged_attn_narr
       }
       if (whole) {
         const float f = 1.f / l;
-        if (d < c.dim)
-          *reinterpret_cast<uint2*>(pa_out(p, w.s.start, w.head, w.row0 + r) + 2 * d) = make_uint2(pa_pack<T>(o.x * f, o.y * f), pa_pack<T>(o.z * f, o.w * f));
+        char* out = pa_out(p, w.s.start, w.head, w.row0 + r) + d * sizeof(T);
+        if (d >= c.dim) continue;
+        if constexpr (S::F32) *reinterpret_cast<float4*>(out) = make_float4(o.x / l, o.y / l, o.z / l, o.w / l);
+        else *reinterpret_cast<uint2*>(out) = make_uint2(pa_pack<T>(o.x * f, o.y * f), pa_pack<T>(o.z * f, o.w * f));
       } else {
         *reinterpret_cast<float4*>(piece + r * DP + d) = o;
         if (d == 0) {
@@ -917,13 +1102,15 @@ __global__ void __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) paged_attn_wide
     const PaPart w = pa_part<RT, BN>(p, pos, end, &slot, &off);
     const int words_seen = (w.s.nodes + 31) / 32;
     const int node0 = static_cast<int>(p.by_group.of(w.row0)), node1 = static_cast<int>(p.by_group.of(w.row0 + w.rows - 1));
-    // Thread t < 64 finds row t of a tile, one tile before the copies of it.
+    // Thread t < 64 finds where row t of a tile lies, one tile before the copies of it, with the page that it looked up one tile
+    // earlier still.
+    int pg = t < BN ? pa_lookup(p, w, w.t0 * BN + t) : -1;
     const auto find = [&](uint32_t tile) {
       if (t < BN && tile < w.t1) {
-        const uint32_t at = tile * BN + t;
-        const PaRow r = pa_row(p, w, at, pa_lookup(p, w, at));
+        const PaRow r = pa_row(p, w, tile * BN + t, pg);
         sm.row[tile & 1][0][t] = r.k;
         sm.row[tile & 1][1][t] = r.v;
+        if (tile + 1 < w.t1) pg = pa_lookup(p, w, (tile + 1) * BN + t);
       }
     };
     uint32_t into = 0;
@@ -1082,30 +1269,26 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_join_kernel(const PaPar
 // ---------------------------------------------------------------------------------------------- host
 // How a call is cut: padded dim, rows and keys of a tile, CTAs.
 struct PaForm {
-  int dp, rt, bn, ctas, smem;
+  int dp, rt, bn, ctas, threads, smem;
   void (*kernel)(PaParams);
 };
 
-template <typename T, int DP, int RPT, bool WORDS>
+template <typename T, int DP, int RPT>
 static PaForm pa_ffma() {
   using S = PaFfma<T, DP, RPT>;
   const int smem = static_cast<int>(sizeof(S));
-  return PaForm{DP, S::RT, S::BN, sm_count() * (smem <= 112 * 1024 ? 2 : 1), smem, paged_attn_ffma_kernel<T, DP, RPT, WORDS>};
+  return PaForm{DP, S::RT, S::BN, sm_count() * (smem <= 112 * 1024 ? 2 : 1), PA_THREADS, smem, paged_attn_ffma_kernel<T, DP, RPT>};
 }
 template <typename T, int DP>
 static PaForm pa_form(int rows, bool words) {
+  using N = PaNarrow<T, DP>;
   if constexpr (sizeof(T) == 2) {
-    if (words) {
-      using N = PaNarrow<T, DP>;
-      using W = PaWide<T, DP>;
-      const int ctas = sm_count() * (DP == 256 ? 1 : 2);
-      if (rows <= 16) return PaForm{DP, N::RT, N::BN, ctas, static_cast<int>(sizeof(N)), paged_attn_narrow_kernel<T, DP>};
-      return PaForm{DP, W::RT, W::BN, ctas, static_cast<int>(sizeof(W)), paged_attn_wide_kernel<T, DP>};
-    }
-  } else if (words) {
-    return rows <= 8 ? pa_ffma<T, DP, 1, true>() : rows <= 16 ? pa_ffma<T, DP, 2, true>() : pa_ffma<T, DP, 4, true>();
+    using W = PaWide<T, DP>;
+    if (words && rows > 16)
+      return PaForm{DP, W::RT, W::BN, sm_count() * (DP == 256 ? 1 : 2), PA_THREADS, static_cast<int>(sizeof(W)), paged_attn_wide_kernel<T, DP>};
   }
-  return rows <= 8 ? pa_ffma<T, DP, 1, false>() : pa_ffma<T, DP, 4, false>();
+  if (words) return PaForm{DP, N::RT, N::BN, sm_count() * N::CTAS, N::THREADS, static_cast<int>(sizeof(N)), paged_attn_narrow_kernel<T, DP>};
+  return rows <= 8 ? pa_ffma<T, DP, 1>() : pa_ffma<T, DP, 4>();
 }
 template <typename T>
 static PaForm pa_form(int dim, int rows, bool words) {
@@ -1194,7 +1377,7 @@ int ytcuda_pages_attend(const ytcuda_pages* cache, int layer, const void* q, con
   p.cuts = reinterpret_cast<int4*>(static_cast<char*>(workspace) + pa_pieces(f));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(f.kernel), f.smem)) return rc;
-  f.kernel<<<f.ctas, PA_THREADS, f.smem, st>>>(p);
+  f.kernel<<<f.ctas, f.threads, f.smem, st>>>(p);
   count_launch();
   YTC_CUDA(cudaGetLastError());
   YTC_CUDA(cache->dtype == YTC_F32 ? pa_join<float>(f, p, st) : cache->dtype == YTC_BF16 ? pa_join<__nv_bfloat16>(f, p, st) : pa_join<__half>(f, p, st));

@@ -396,13 +396,13 @@ def test_sharp_scores_and_scales(paged, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("dim", [64, 20])
-def test_numbers_in_hidden_places(paged, dtype, dim):
+@pytest.mark.parametrize("dim,groups", [(64, 2), (20, 2), (64, 8), (64, 40), (128, 40), (128, 2), (128, 7), (80, 33), (256, 2), (256, 9)])
+def test_numbers_in_hidden_places(paged, dtype, dim, groups):
     """What a node does not see may be infinite or no number: siblings, rows behind the end, pages of others."""
     b = Both(paged, layers=1, heads=1, dim=dim, slots=2, page=16, dtype=dtype)
     b.fill([30, 18])
     b.reserve([5, 3])
-    q, k, v = b.randn(8, 2, dim), b.randn(8, 1, dim), b.randn(8, 1, dim)
+    q, k, v = b.randn(8, groups, dim), b.randn(8, 1, dim), b.randn(8, 1, dim)
     parents = [-1, 0, 0, 1, 2, -1, 0, -1]
     starts = [0, 5, 8]
     plain = b.d.attend(0, q, ints(starts), k, v, parents=ints(parents))

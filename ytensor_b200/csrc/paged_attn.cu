@@ -13,10 +13,14 @@
 #include <type_traits>
 
 #include "pages.cuh"
+#include "ptx_sm100.cuh"
 
 namespace ytk {
 
 constexpr int PA_THREADS = 128;
+#ifndef PA_TC_ROWS
+#define PA_TC_ROWS 64
+#endif
 constexpr int PA_TREE = 1024;  // most nodes of a tree
 constexpr float PA_LOG2E = 1.4426950408889634f;
 
@@ -30,6 +34,7 @@ struct PaParams {
   float scale;  // times log2(e)
   float* work;  // pieces of cut units
   int4* cuts;   // two words for each CTA: the unit that starts in its share and goes on behind it
+  int* timeout; // the device's status word
 };
 
 // What a slot brings: its rows in the call, its nodes, its length.
@@ -1068,10 +1073,10 @@ __global__ void __launch_bounds__(PaNarrow<T, DP>::THREADS, PaNarrow<T, DP>::CTA
   if (t == 0) cut.store(p);
 }
 
-// Up to 64 rows of a tile: a warp for 16 of them (warps without rows only copy), all over the same tiles of 64 keys.
+// Up to 64 rows of a tile: a warp for 16 of them (warps without rows only copy), all over the same tiles of keys.
 template <typename T, int DP>
 struct PaWide {
-  static constexpr int RT = 64, BN = 64, STAGES = 3, SLOT = BN * DP * 2;
+  static constexpr int RT = 64, BN = DP == 256 ? 32 : 64, STAGES = 3, SLOT = BN * DP * 2;
   uint4 ring[STAGES][2][SLOT / 16];
   uint4 q[DP > 128 ? RT * DP * 2 / 16 : 1];
   const char* row[2][2][BN];  // (where the next tile's rows lie)
@@ -1102,7 +1107,7 @@ __global__ void __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) paged_attn_wide
     const PaPart w = pa_part<RT, BN>(p, pos, end, &slot, &off);
     const int words_seen = (w.s.nodes + 31) / 32;
     const int node0 = static_cast<int>(p.by_group.of(w.row0)), node1 = static_cast<int>(p.by_group.of(w.row0 + w.rows - 1));
-    // Thread t < 64 finds where row t of a tile lies, one tile before the copies of it, with the page that it looked up one tile
+    // Thread t < BN finds where row t of a tile lies, one tile before the copies of it, with the page that it looked up one tile
     // earlier still.
     int pg = t < BN ? pa_lookup(p, w, w.t0 * BN + t) : -1;
     const auto find = [&](uint32_t tile) {
@@ -1203,6 +1208,453 @@ __global__ void __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) paged_attn_wide
   if (t == 0) cut.store(p);
 }
 
+// Many rows: tcgen05. A part has up to 256 rows as two tiles of 128, whose scores S and sums O live in tensor memory; keys and values
+// come in tiles of 128 into a ring of shared memory. Two warps copy (cp.async, 16-byte words in the 128-byte swizzle that the
+// instructions' descriptors name: pages may have any size and rows any place), one issues S_t = Q_t K^T and O_t += P_t V, and four
+// warps for each row tile turn S into P, a thread a row, while the tensor core works on the other tile. P stays in tensor memory,
+// over its own scores. What bounds it are the exponentials (one result a clock and quarter SM) and the tensor pipe, which take about
+// the same time; a part with rows in one tile only has nothing to hide them behind.
+template <typename T, int DP>
+struct PaTc {
+  static constexpr int RT = 256, BN = 128, THREADS = 384, STAGES = DP == 64 ? 4 : 2, TILE = 128 * DP * 2;
+  static constexpr int KV = 2 * TILE, REST = KV + STAGES * 2 * TILE;  // offsets: Q, the ring, the rest
+  struct Rest {
+    uint64_t q_full, q_free, k_full[STAGES], v_full[STAGES], empty[STAGES], s_full[2], p_full[2], o_ready[2], o_free[2];
+    uint32_t tmem;
+    int stop;  // a wait has run out
+    int odd;   // the part has hidden values that are not finite
+    int16_t up[8][PA_TREE];  // a slot's parents, for each softmax warp
+    PaShare share;
+  };
+  static constexpr int BYTES = REST + static_cast<int>(sizeof(Rest)) + 1024;
+  // Where 16-byte word `w` of row `r` of a tile lies.
+  static __device__ __forceinline__ uint32_t at(int r, int w) { return (w >> 3) * (128 * 128) + r * 128 + (((w & 7) ^ (r & 7)) << 4); }
+};
+
+__device__ __forceinline__ uint64_t pa_pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void pa_unpair(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t pa_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ float pa_max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ void pa_named_barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+
+// The keys among 128 that a node sees, the first of them node n0 (negative: in front of the nodes). up: the slot's parents (nullptr:
+// a chain).
+__device__ __forceinline__ void pa_sees128(const int16_t* up, int node, int n0, uint32_t (&bits)[4]) {
+  const int upto = up ? -n0 : node + 1 - n0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int n = upto - 32 * i;
+    bits[i] = n >= 32 ? 0xffffffffu : n > 0 ? (1u << n) - 1 : 0u;
+  }
+  if (up)
+    for (int j = node; j >= 0 && j >= n0; j = up[j]) {
+      const int b = j - n0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (b >> 5 == i) bits[i] |= 1u << (b & 31);
+    }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1) paged_attn_tc_kernel(const PaParams p) {
+  using S = PaTc<T, DP>;
+  constexpr int RT = S::RT, BN = S::BN, ST = S::STAGES, TILE = S::TILE, WORDS = DP / 8, PER = 32 / WORDS;
+  extern __shared__ __align__(128) unsigned char raw[];
+  unsigned char* const smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+  typename S::Rest& sm = *reinterpret_cast<typename S::Rest*>(smem + S::REST);
+  dependent_trigger();
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const PgCache& c = p.c;
+  if (threadIdx.x == 0) {
+    mbar_init(&sm.q_full, 2);  // (an arrival of each copying warp)
+    mbar_init(&sm.q_free, 1);
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(&sm.k_full[s], 2);
+      mbar_init(&sm.v_full[s], 2);
+      mbar_init(&sm.empty[s], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&sm.s_full[t], 1);
+      mbar_init(&sm.p_full[t], 4);  // (of each softmax warp)
+      mbar_init(&sm.o_ready[t], 1);
+      mbar_init(&sm.o_free[t], 4);
+    }
+    sm.stop = 0;
+    sm.odd = 0;
+    fence_mbar_init();
+    fence_proxy_async_smem();
+  }
+  if (warp == 1) {
+    tmem_alloc(&sm.tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  pa_share<RT, BN>(p, &sm.share);
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
+  // columns of tensor memory: S0 / P0 at 0, S1 / P1 at 128, O0 at 256, O1 at 384
+  volatile int* const stop = &sm.stop;
+  uint32_t pos = sm.share.from, off = sm.share.off;
+  const uint32_t end = sm.share.to;
+  int slot = sm.share.slot, n_part = 0;
+  bool ok = true;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ the issuer of the matrix instructions (all lanes, one leads)
+    const uint32_t lead = lane == 0 ? 1u : 0u, q0 = smem_u32(smem), kv = q0 + S::KV;
+    constexpr uint32_t FORMAT = std::is_same<T, __half>::value ? 0u : 1u;
+    const uint32_t idesc_s = umma_idesc(FORMAT, 0, 0, 128, 128), idesc_o = umma_idesc(FORMAT, 0, 1, 128, DP);
+    uint32_t n_kv = 0, n_p[2] = {0, 0}, n_e[2] = {0, 0};
+    const auto issue_s = [&](int t, uint32_t stage) {
+      const uint32_t qa = q0 + t * TILE, ka = kv + stage * (2 * TILE);
+#pragma unroll
+      for (int k = 0; k < DP / 16; ++k) {
+        const uint32_t o = (k >> 2) * (128 * 128) + (k & 3) * 32;
+        tc_mma_f16_lead(tmem + 128 * t, umma_smem_desc_sw128(qa + o, 16, 1024), umma_smem_desc_sw128(ka + o, 16, 1024), idesc_s, k != 0, lead);
+      }
+      tc_commit_lead(smem_u32(&sm.s_full[t]), lead);
+    };
+    const auto issue_o = [&](int t, uint32_t stage, bool more) {
+      const uint32_t va = kv + stage * (2 * TILE) + TILE;
+#pragma unroll
+      for (int k = 0; k < BN / 16; ++k)
+        tc_mma_f16_ts_lead(tmem + 256 + 128 * t, tmem + 128 * t + 8 * k, umma_smem_desc_sw128(va + k * 2048, 128 * 128, 1024), idesc_o, more || k != 0, lead);
+      tc_commit_lead(smem_u32(&sm.o_ready[t]), lead);
+    };
+    while (ok && pos < end) {
+      const PaPart w = pa_part<RT, BN>(p, pos, end, &slot, &off);
+      const int n = w.t1 - w.t0, tiles = w.rows > 128 ? 2 : 1;
+      ok = mbar_wait_warp(&sm.q_full, n_part & 1, stop) && mbar_wait_warp(&sm.k_full[n_kv % ST], (n_kv / ST) & 1, stop);
+      if (!ok) break;
+      tc_fence_after();
+      for (int t = 0; t < tiles; ++t) issue_s(t, n_kv % ST);
+      if (n == 1) tc_commit_lead(smem_u32(&sm.q_free), lead);
+      for (int j = 0; ok && j < n; ++j, ++n_kv) {
+        const uint32_t s = n_kv % ST, next = (n_kv + 1) % ST;
+        if (!(ok = mbar_wait_warp(&sm.v_full[s], (n_kv / ST) & 1, stop))) break;
+        for (int t = 0; t < tiles; ++t) {
+          ok = mbar_wait_warp(&sm.p_full[t], n_p[t] & 1, stop);
+          if (ok && j == 0 && n_e[t] > 0) ok = mbar_wait_warp(&sm.o_free[t], (n_e[t] - 1) & 1, stop);  // (O is written anew)
+          if (!ok) break;
+          ++n_p[t];
+          tc_fence_after();
+          issue_o(t, s, j > 0);
+          if (j + 1 < n) {
+            if (t == 0 && !(ok = mbar_wait_warp(&sm.k_full[next], ((n_kv + 1) / ST) & 1, stop))) break;
+            tc_fence_after();
+            issue_s(t, next);  // (behind the product that reads P from the same columns)
+          }
+        }
+        if (!ok) break;
+        if (j + 2 == n) tc_commit_lead(smem_u32(&sm.q_free), lead);
+        tc_commit_lead(smem_u32(&sm.empty[s]), lead);
+      }
+      for (int t = 0; t < tiles; ++t) ++n_e[t];
+      ++n_part;
+      pos += n;
+      off += n;
+    }
+  } else if (warp == 2 || warp == 3) {
+    // ------------------------------------------------------------ copies
+    const int half = warp - 2, words = c.dim / 8, word = lane % WORDS;
+    const uint32_t q0 = smem_u32(smem), kv = q0 + S::KV;
+    uint32_t n_kv = 0;
+    PaCut cut;
+    // A group of copies is told to the issuer when the next one is on its way, or before a wait.
+    uint64_t* told = nullptr;
+    uint32_t look_at = 0;  // (values of a tile with nodes)
+    const auto tell = [&]() {
+      if (look_at) {  // a value that is not finite and that not every row sees must not meet a weight of zero: it goes in at the end
+        bool odd = false;
+#pragma unroll 1
+        for (int i = 0; i < 64 / PER; ++i) {
+          const uint32_t at = look_at + S::at(64 * half + i * PER + lane / WORDS, word);
+          uint32_t x[4];
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at) : "memory");
+          bool here = false;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t y = pa_finite_part<T>(x[k]);
+            here = here || y != x[k];
+            x[k] = y;
+          }
+          if (here) asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+          odd = odd || here;
+        }
+        if (__any_sync(0xffffffffu, odd) && lane == 0) atomicExch(&sm.odd, 1);
+        look_at = 0;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(told);
+      told = nullptr;
+    };
+    const auto sent = [&](uint64_t* bar, uint32_t look) {
+      pa_copy_commit();
+      if (told) {
+        pa_copy_wait<1>();
+        tell();
+      }
+      told = bar;
+      look_at = look;
+    };
+    const auto flush = [&]() {
+      if (told) {
+        pa_copy_wait<0>();
+        tell();
+      }
+    };
+    while (ok && pos < end) {
+      const PaPart w = pa_part<RT, BN>(p, pos, end, &slot, &off);
+      int pg[2];
+      const auto lookup = [&](uint32_t tile) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) pg[i] = tile < w.t1 ? pa_lookup(p, w, tile * BN + 64 * half + 32 * i + lane) : -1;
+      };
+      lookup(w.t0);
+      if (n_part > 0 && !(ok = mbar_wait_warp(&sm.q_free, (n_part - 1) & 1, stop))) break;
+      for (int t = 0; t < (w.rows > 128 ? 2 : 1); ++t)
+#pragma unroll 4
+        for (int i = 0; i < 64 / PER; ++i) {
+          const int r = 64 * half + i * PER + lane / WORDS, row = w.row0 + 128 * t + r;
+          const bool there = row < w.rows_all && word < words;
+          pa_copy16(q0 + t * TILE + S::at(r, word), there ? pa_query(p, w, row) + word * 16 : p.q.p, there);
+        }
+      sent(&sm.q_full, 0);
+      for (uint32_t tile = w.t0; tile < w.t1; ++tile, ++n_kv) {
+        const uint32_t s = n_kv % ST, parity = ((n_kv / ST) & 1) ^ 1, kt = kv + s * (2 * TILE);
+        unsigned long long kp[2], vp[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const PaRow r = pa_row(p, w, tile * BN + 64 * half + 32 * i + lane, pg[i]);
+          kp[i] = reinterpret_cast<unsigned long long>(r.k);
+          vp[i] = reinterpret_cast<unsigned long long>(r.v);
+        }
+        lookup(tile + 1);
+        if (!__all_sync(0xffffffffu, mbar_try_wait(&sm.empty[s], parity))) {
+          flush();
+          if (!(ok = mbar_wait_warp(&sm.empty[s], parity, stop))) break;
+        }
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll 4
+            for (int i = 0; i < 32 / PER; ++i) {
+              const int r = i * PER + lane / WORDS;
+              const unsigned long long a = __shfl_sync(0xffffffffu, v ? vp[h] : kp[h], r);
+              const bool there = a != 0 && word < words;
+              pa_copy16(kt + v * TILE + S::at(64 * half + 32 * h + r, word), there ? reinterpret_cast<const char*>(a) + word * 16 : c.k.p, there);
+            }
+          sent(v ? &sm.v_full[s] : &sm.k_full[s], v && static_cast<int64_t>(tile + 1) * BN > w.s.len ? kt + TILE : 0u);
+        }
+      }
+      if (!ok) break;
+      flush();
+      if (p.fresh && w.rtile == 0) {
+        const int64_t n0 = static_cast<int64_t>(w.t0) * BN - w.s.len, n1 = static_cast<int64_t>(w.t1) * BN - w.s.len;
+        if (n1 > 0) pa_store_new<uint4>(p, w, n0 < 0 ? 0 : static_cast<int>(n0), static_cast<int>(n1 < w.s.nodes ? n1 : w.s.nodes), words, 32 * half + lane, 64);
+      }
+      cut.note(sm.share, w, pos);
+      ++n_part;
+      pos += w.t1 - w.t0;
+      off += w.t1 - w.t0;
+    }
+    pa_copy_wait<0>();
+    if (warp == 2 && lane == 0) cut.store(p);
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------ softmax and results: row tile t, a thread a row
+    const int t = (warp - 4) >> 2, in_tile = (warp & 3) * 32 + lane;
+    const uint32_t lane_sel = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + 128 * t + lane_sel, to = tmem + 256 + 128 * t + lane_sel;
+    const bool pos_scale = p.scale >= 0.f;
+    const float none = pos_scale ? -CUDART_INF_F : CUDART_INF_F;  // a hidden score before the scale
+    uint32_t n_s = 0;
+    while (ok && pos < end) {
+      const PaPart w = pa_part<RT, BN>(p, pos, end, &slot, &off);
+      const int n = w.t1 - w.t0;
+      pos += n;
+      off += n;
+      const bool nodes_here = static_cast<int64_t>(w.t1) * BN > w.s.len;
+      const int r = 128 * t + in_tile;
+      if (128 * t >= w.rows) continue;
+      const int node = static_cast<int>(p.by_group.of(w.row0 + min(r, w.rows - 1)));
+      int16_t* const mine = sm.up[warp - 4];
+      if (p.parents && nodes_here) {
+        __syncwarp();
+        for (int i = lane; i < w.s.nodes; i += 32) {
+          int a = p.parents[w.s.start + i];
+          if (a < -1 || a >= i) {
+            atomicOr(c.status, YTC_PAGES_INVALID);
+            a = -1;
+          }
+          mine[i] = static_cast<int16_t>(a);
+        }
+        __syncwarp();
+      }
+      const int16_t* up = p.parents ? mine : nullptr;
+      float m = -CUDART_INF_F, l = 0.f;
+      for (int j = 0; j < n; ++j, ++n_s) {
+        if (!(ok = mbar_wait_warp(&sm.s_full[t], n_s & 1, stop))) break;
+        tc_fence_after();
+        const int n0 = static_cast<int>((w.t0 + j) * BN) - w.s.len;
+        const bool masked = n0 + BN > 0;
+        uint32_t bits[4];
+        if (masked) pa_sees128(up, node, n0, bits);
+        __syncwarp();
+        float top = none;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t x[64];
+          tmem_ld_32x32b_x64(ts + 64 * h, x);
+          tmem_ld_wait();
+          if (masked) {
+#pragma unroll
+            for (int e = 0; e < 64; ++e)
+              if (!((bits[2 * h + (e >> 5)] >> (e & 31)) & 1)) x[e] = __float_as_uint(none);
+          }
+          if (pos_scale) {
+            float a[4] = {top, none, none, none};
+#pragma unroll
+            for (int e = 0; e < 64; e += 8)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) a[k] = pa_max3(a[k], __uint_as_float(x[e + 2 * k]), __uint_as_float(x[e + 2 * k + 1]));
+            top = pa_max3(fmaxf(a[0], a[1]), a[2], a[3]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 64; ++e) top = fminf(top, __uint_as_float(x[e]));
+          }
+        }
+        top = top == none ? -CUDART_INF_F : top * p.scale;
+        if (j == 0) {
+          m = top;
+        } else {
+          const bool moves = top > m + PA_SLACK || (m == -CUDART_INF_F && top > m);
+          if (__any_sync(0xffffffffu, moves)) {  // O *= 2^(m - top): the product before has to be there
+            if (!(ok = mbar_wait_warp(&sm.o_ready[t], (n_s - 1) & 1, stop))) break;
+            tc_fence_after();
+            const float shrink = moves ? pa_exp2(m - top) : 1.f;
+#pragma unroll 1
+            for (int d = 0; d < DP; d += 16) {
+              uint32_t x[16];
+              tmem_ld_32x32b_x16(to + d, x);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * shrink);
+              tmem_st_32x32b_x16(to + d, x);
+            }
+            l *= shrink;
+            if (moves) m = top;
+          }
+        }
+        const float ref = m == -CUDART_INF_F ? 0.f : m;
+        const uint64_t s2 = pa_pair(p.scale, p.scale), r2 = pa_pair(-ref, -ref);
+        float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t x[64], pk[32];
+          tmem_ld_32x32b_x64(ts + 64 * h, x);
+          tmem_ld_wait();
+          if (masked) {
+#pragma unroll
+            for (int e = 0; e < 64; ++e)
+              if (!((bits[2 * h + (e >> 5)] >> (e & 31)) & 1)) x[e] = __float_as_uint(none);
+          }
+#pragma unroll
+          for (int e = 0; e < 64; e += 2) {
+            float a, b;
+            pa_unpair(pa_fma2(pa_pair(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), s2, r2), a, b);
+            a = pa_exp2(a);
+            b = pa_exp2(b);
+            l0 += a;
+            l1 += b;
+            pk[e >> 1] = pa_pack<T>(a, b);
+          }
+          // (P of the first half lies over scores that have been read: columns 0 .. 31)
+          tmem_st_32x32b_x32(ts + 32 * h, pk);
+        }
+        l += l0 + l1;
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.p_full[t]);
+      }
+      if (!ok) break;
+      if (!(ok = mbar_wait_warp(&sm.o_ready[t], (n_s - 1) & 1, stop))) break;
+      tc_fence_after();
+      const bool whole = w.t0 == 0 && w.t1 == w.tiles, here = r < w.rows;
+      const bool odd = nodes_here && *reinterpret_cast<volatile int*>(&sm.odd);
+      float* piece = pa_piece_of<RT, DP>(p, w) + r * DP;
+      char* out = here ? pa_out(p, w.s.start, w.head, w.row0 + r) : nullptr;
+      const float f = 1.f / l;
+#pragma unroll 1
+      for (int d = 0; d < DP; d += 16) {
+        uint32_t x[16];
+        __syncwarp();
+        tmem_ld_32x32b_x16(to + d, x);
+        tmem_ld_wait();
+        if (odd && here) {  // the values that were left out, of the nodes of this part that the row sees
+          for (int j = min(node, static_cast<int>(static_cast<int64_t>(w.t1) * BN - w.s.len) - 1); j >= 0 && static_cast<int64_t>(j) + w.s.len >= static_cast<int64_t>(w.t0) * BN; --j) {
+            uint32_t sees[4];
+            pa_sees128(up, node, j, sees);
+            if (!(sees[0] & 1)) continue;
+            const uint32_t at = static_cast<uint32_t>(w.s.len + j);
+            const T* v = reinterpret_cast<const T*>(pa_row(p, w, at, pa_lookup(p, w, at)).v);
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (v && d + e < c.dim) {
+                const float y = pa_load(v + d + e);
+                if (!(fabsf(y) < CUDART_INF_F)) x[e] = __float_as_uint(__uint_as_float(x[e]) + y);
+              }
+          }
+        }
+        if (here && whole) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            if (d + 8 * k < c.dim) {
+              uint32_t y[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) y[e] = pa_pack<T>(__uint_as_float(x[8 * k + 2 * e]) * f, __uint_as_float(x[8 * k + 2 * e + 1]) * f);
+              *reinterpret_cast<uint4*>(out + 2 * (d + 8 * k)) = make_uint4(y[0], y[1], y[2], y[3]);
+            }
+        } else if (here) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) *reinterpret_cast<uint4*>(piece + d + 4 * k) = make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
+        }
+      }
+      if (here && !whole) {
+        float* sums = pa_piece_of<RT, DP>(p, w) + RT * DP;
+        sums[r] = m;
+        sums[RT + r] = l;
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.o_free[t]);
+    }
+  }
+  if (!ok && lane == 0) {
+    *stop = 1;
+    if (p.timeout) atomicExch(p.timeout, YTC_TIMEOUT);
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, 512);
+}
+
 // ---------------------------------------------------------------------------------------------- joining
 // CTA (x, y): the unit that starts in share x and goes on behind it, rows y, y + gridDim.y, ... of it. The pieces of a row are
 // shared by the warps, and their sums are joined in the order of the warps.
@@ -1273,17 +1725,25 @@ struct PaForm {
   void (*kernel)(PaParams);
 };
 
+constexpr size_t PA_SHARED = 227 * 1024;  // what a CTA may have
 template <typename T, int DP, int RPT>
 static PaForm pa_ffma() {
   using S = PaFfma<T, DP, RPT>;
+  static_assert(sizeof(S) <= PA_SHARED, "shared memory");
   const int smem = static_cast<int>(sizeof(S));
   return PaForm{DP, S::RT, S::BN, sm_count() * (smem <= 112 * 1024 ? 2 : 1), PA_THREADS, smem, paged_attn_ffma_kernel<T, DP, RPT>};
 }
 template <typename T, int DP>
 static PaForm pa_form(int rows, bool words) {
   using N = PaNarrow<T, DP>;
+  static_assert(N::CTAS * (sizeof(N) + 1024) <= PA_SHARED + 1024, "shared memory");
   if constexpr (sizeof(T) == 2) {
     using W = PaWide<T, DP>;
+    static_assert(sizeof(W) <= PA_SHARED, "shared memory");
+    using C = PaTc<T, DP <= 128 ? DP : 128>;
+    static_assert(C::BYTES <= PA_SHARED, "shared memory");
+    if (DP <= 128 && words && rows > PA_TC_ROWS)
+      return PaForm{DP, C::RT, C::BN, sm_count(), C::THREADS, C::BYTES, paged_attn_tc_kernel<T, DP <= 128 ? DP : 128>};
     if (words && rows > 16)
       return PaForm{DP, W::RT, W::BN, sm_count() * (DP == 256 ? 1 : 2), PA_THREADS, static_cast<int>(sizeof(W)), paged_attn_wide_kernel<T, DP>};
   }
@@ -1308,7 +1768,7 @@ static uint64_t pa_space(const PaForm& f) { return pa_pieces(f) + 2ull * sizeof(
 
 template <typename T>
 static cudaError_t pa_join(const PaForm& f, const PaParams& p, cudaStream_t st) {
-  const dim3 grid(f.ctas, f.rt <= 16 ? 4 : 8), block(PA_THREADS);
+  const dim3 grid(f.ctas, f.rt <= 32 ? 4 : f.rt / 8), block(PA_THREADS);
   if (f.dp == 64) return pg_launch_behind(paged_attn_join_kernel<T, 64>, grid, block, 0, st, p, f.rt);
   if (f.dp == 128) return pg_launch_behind(paged_attn_join_kernel<T, 128>, grid, block, 0, st, p, f.rt);
   return pg_launch_behind(paged_attn_join_kernel<T, 256>, grid, block, 0, st, p, f.rt);
@@ -1375,6 +1835,11 @@ int ytcuda_pages_attend(const ytcuda_pages* cache, int layer, const void* q, con
   p.scale = (scale != 0.f ? scale : 1.f / sqrtf(static_cast<float>(p.c.dim))) * PA_LOG2E;
   p.work = static_cast<float*>(workspace);
   p.cuts = reinterpret_cast<int4*>(static_cast<char*>(workspace) + pa_pieces(f));
+  p.timeout = device_status_word();
+  if (!p.timeout) {
+    set_last_error("%s: no device status word", who);
+    return YTC_CUDA_ERROR;
+  }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(f.kernel), f.smem)) return rc;
   f.kernel<<<f.ctas, f.threads, f.smem, st>>>(p);

@@ -18,9 +18,6 @@
 namespace ytk {
 
 constexpr int PA_THREADS = 128;
-#ifndef PA_TC_ROWS
-#define PA_TC_ROWS 64
-#endif
 constexpr int PA_TREE = 1024;  // most nodes of a tree
 constexpr float PA_LOG2E = 1.4426950408889634f;
 
@@ -54,53 +51,55 @@ __device__ __forceinline__ PaSlot pa_slot(const PaParams& p, int s, bool* bad) {
   }
   return r;
 }
-// Key tiles and row tiles of a slot; the units of a slot are its heads' row tiles, the row tiles of a head next to one another (they
-// read the same keys at about the same time). All numbers stay below 2^31: the host sees to that.
+// The units of a slot are its heads' row tiles, the row tiles of a head next to one another (they read the same keys at about the same
+// time). Work is counted in blocks of RW rows by BN keys; a unit has up to RT rows, so RT / RW blocks a key tile at most. All numbers
+// stay below 2^31: the host sees to that.
 template <int BN>
 __device__ __forceinline__ uint32_t pa_key_tiles(const PaSlot& s) {
   return (static_cast<uint32_t>(s.len) + static_cast<uint32_t>(s.nodes) + BN - 1) / BN;
 }
-template <int RT>
-__device__ __forceinline__ uint32_t pa_row_tiles(const PaParams& p, const PaSlot& s) {
-  return (static_cast<uint32_t>(s.nodes) * static_cast<uint32_t>(p.groups) + RT - 1) / RT;
+template <int RW>
+__device__ __forceinline__ uint32_t pa_row_blocks(const PaParams& p, const PaSlot& s) {
+  return (static_cast<uint32_t>(s.nodes) * static_cast<uint32_t>(p.groups) + RW - 1) / RW;
 }
-template <int RT, int BN>
+template <int RW, int BN>
 __device__ __forceinline__ uint32_t pa_work(const PaParams& p, const PaSlot& s) {
-  return s.nodes ? pa_key_tiles<BN>(s) * pa_row_tiles<RT>(p, s) * p.c.heads : 0u;
+  return s.nodes ? pa_key_tiles<BN>(s) * pa_row_blocks<RW>(p, s) * p.c.heads : 0u;
 }
 
-// The share of a CTA: tiles from .. to of all, the first of them tile `off` of slot `slot`. Shares differ by at most one tile, the
-// longer ones first: share i begins at i * each + min(i, more).
+// The share of a CTA: blocks from .. to of all, the first of them block `off` of slot `slot`. Shares differ by at most one block, the
+// longer ones first: share i begins at i * each + min(i, more). No share is shorter than a key tile of a unit.
 struct PaShare {
   uint32_t from, to, off, each, more;
   int slot;
 };
-__device__ __forceinline__ uint32_t pa_share_of(const PaShare& s, uint32_t tile) {
+__device__ __forceinline__ uint32_t pa_share_of(const PaShare& s, uint32_t block) {
   const uint32_t longer = s.more * (s.each + 1);
-  return tile < longer ? tile / (s.each + 1) : s.more + (tile - longer) / s.each;
+  return block < longer ? block / (s.each + 1) : s.more + (block - longer) / s.each;
 }
 // All threads of the CTA call it; one warp works it out.
-template <int RT, int BN>
+template <int RT, int RW, int BN>
 __device__ __forceinline__ void pa_share(const PaParams& p, PaShare* out) {
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
     bool bad = false;
     uint32_t total = 0, w = 0;
     for (int s0 = 0; s0 < p.c.slots; s0 += 32) {
-      w = s0 + lane < p.c.slots ? pa_work<RT, BN>(p, pa_slot(p, s0 + lane, &bad)) : 0;
+      w = s0 + lane < p.c.slots ? pa_work<RW, BN>(p, pa_slot(p, s0 + lane, &bad)) : 0;
       total += __reduce_add_sync(0xffffffffu, w);
     }
     if (blockIdx.x == 0 && __any_sync(0xffffffffu, bad) && lane == 0) atomicOr(p.c.status, YTC_PAGES_INVALID);
     PaShare r;
-    r.each = total / gridDim.x;
-    r.more = total - r.each * gridDim.x;
-    r.from = blockIdx.x * r.each + min(blockIdx.x, r.more);
-    r.to = r.from + r.each + (blockIdx.x < r.more);
+    const uint32_t parts = min(gridDim.x, max(1u, total / (RT / RW)));
+    r.each = total / parts;
+    r.more = total - r.each * parts;
+    r.from = min(total, blockIdx.x * r.each + min(blockIdx.x, r.more));
+    r.to = blockIdx.x < parts ? r.from + r.each + (blockIdx.x < r.more) : r.from;
     r.off = 0;
     r.slot = p.c.slots;
     uint32_t before = 0;
     for (int s0 = 0; s0 < p.c.slots; s0 += 32) {
-      if (p.c.slots > 32) w = s0 + lane < p.c.slots ? pa_work<RT, BN>(p, pa_slot(p, s0 + lane, &bad)) : 0;
+      if (p.c.slots > 32) w = s0 + lane < p.c.slots ? pa_work<RW, BN>(p, pa_slot(p, s0 + lane, &bad)) : 0;
       uint32_t x = w;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -121,35 +120,54 @@ __device__ __forceinline__ void pa_share(const PaParams& p, PaShare* out) {
   __syncthreads();
 }
 
-// A piece of work: tiles t0 .. t1 of a unit that has `tiles`.
+// A piece of work: key tiles t0 .. t1 of a unit that has `tiles`, `weight` blocks each, the first of them block `first` of all.
 struct PaPart {
   PaSlot s;
-  uint32_t tiles, t0, t1;
+  uint32_t tiles, t0, t1, weight, first;
   int slot, head, rtile, row0, rows, rows_all;
 };
-// The next piece at tile `pos` of all (tile `off` of slot `slot`, both moved past slots without rows).
-template <int RT, int BN>
-__device__ __forceinline__ PaPart pa_part(const PaParams& p, uint32_t pos, uint32_t end, int* slot, uint32_t* off) {
-  PaPart r;
-  bool bad = false;
-  while (true) {
-    r.s = pa_slot(p, *slot, &bad);
-    const uint32_t work = pa_work<RT, BN>(p, r.s);
-    if (*off < work) break;
-    *off -= work;
-    ++*slot;
+// Where a CTA is in its share.
+struct PaAt {
+  uint32_t pos, end, off;
+  int slot;
+  __device__ __forceinline__ explicit PaAt(const PaShare& s) : pos(s.from), end(s.to), off(s.off), slot(s.slot) {}
+};
+// The next piece of the share; false behind the last one. A key tile belongs to the share that its first block lies in.
+template <int RT, int RW, int BN>
+__device__ __forceinline__ bool pa_next(const PaParams& p, PaAt* at, PaPart* out) {
+  constexpr uint32_t MOST = RT / RW;
+  static_assert(MOST == 1 || MOST == 2, "blocks a key tile");
+  while (at->pos < at->end) {
+    bool bad = false;
+    PaPart& r = *out;
+    r.s = pa_slot(p, at->slot, &bad);
+    const uint32_t work = pa_work<RW, BN>(p, r.s);
+    if (at->off >= work) {  // (slots without rows too)
+      at->off -= work;
+      ++at->slot;
+      continue;
+    }
+    r.slot = at->slot;
+    r.tiles = pa_key_tiles<BN>(r.s);
+    const uint32_t blocks = pa_row_blocks<RW>(p, r.s), a_head = r.tiles * blocks;
+    const uint32_t head = at->off / a_head, in_head = at->off - head * a_head;
+    const uint32_t unit = in_head / (r.tiles * MOST), in_unit = in_head - unit * (r.tiles * MOST);
+    r.weight = min(MOST, blocks - unit * MOST);
+    const uint32_t n = min(r.tiles * r.weight - in_unit, at->end - at->pos);
+    r.first = at->pos - in_unit;
+    r.t0 = (in_unit + r.weight - 1) / r.weight;
+    r.t1 = (in_unit + n + r.weight - 1) / r.weight;
+    at->pos += n;
+    at->off += n;
+    if (r.t0 == r.t1) continue;
+    r.head = static_cast<int>(head);
+    r.rtile = static_cast<int>(unit);
+    r.row0 = r.rtile * RT;
+    r.rows_all = r.s.nodes * p.groups;
+    r.rows = min(RT, r.rows_all - r.row0);
+    return true;
   }
-  r.slot = *slot;
-  r.tiles = pa_key_tiles<BN>(r.s);
-  const uint32_t row_tiles = pa_row_tiles<RT>(p, r.s), unit = *off / r.tiles;
-  r.t0 = *off - unit * r.tiles;
-  r.t1 = min(r.tiles, r.t0 + (end - pos));
-  r.head = static_cast<int>(unit / row_tiles);
-  r.rtile = static_cast<int>(unit - r.head * row_tiles);
-  r.row0 = r.rtile * RT;
-  r.rows_all = r.s.nodes * p.groups;
-  r.rows = min(RT, r.rows_all - r.row0);
-  return r;
+  return false;
 }
 
 // Floats of a piece in the workspace: O [rt][dp], m [rt], l [rt]. A CTA has two: its first and its last unit may be cut.
@@ -161,10 +179,10 @@ __device__ __forceinline__ float* pa_piece_of(const PaParams& p, const PaPart& w
 // What joining has to know of the unit that starts in this CTA's share and goes on: kept by one thread, stored at the end.
 struct PaCut {
   int4 a{0, 0, 0, 0}, b{0, 0, 0, 0};  // rows (0: no such unit), first row, head, start of the slot's rows; last share
-  __device__ __forceinline__ void note(const PaShare& sh, const PaPart& w, uint32_t pos) {
+  __device__ __forceinline__ void note(const PaShare& sh, const PaPart& w) {
     if (w.t0 == 0 && w.t1 < w.tiles) {
       a = make_int4(w.rows, w.row0, w.head, w.s.start);
-      b.x = static_cast<int>(pa_share_of(sh, pos + w.tiles - 1));
+      b.x = static_cast<int>(pa_share_of(sh, w.first + (w.tiles - 1) * w.weight));
     }
   }
   __device__ __forceinline__ void store(const PaParams& p) const {
@@ -337,13 +355,11 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_ffma_kernel(const PaPar
   dependent_trigger();
   const int t = threadIdx.x, a = t >> 4, b = t & 15;
   const PgCache& c = p.c;
-  pa_share<RT, BN>(p, &sm.share);
+  pa_share<RT, RT, BN>(p, &sm.share);
   PaCut cut;
-  uint32_t pos = sm.share.from, off = sm.share.off;
-  const uint32_t end = sm.share.to;
-  int slot = sm.share.slot;
-  while (pos < end) {
-    const PaPart w = pa_part<RT, BN>(p, pos, end, &slot, &off);
+  PaAt at(sm.share);
+  PaPart w;
+  while (pa_next<RT, RT, BN>(p, &at, &w)) {
     const int nodes = w.s.nodes, words = (nodes + 31) / 32;
     const int node0 = static_cast<int>(p.by_group.of(w.row0)), node1 = static_cast<int>(p.by_group.of(w.row0 + w.rows - 1));
     // Thread t < BN finds where row t of a tile lies, with the page that it looked up one tile earlier.
@@ -486,9 +502,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_ffma_kernel(const PaPar
         }
       }
     }
-    cut.note(sm.share, w, pos);
-    pos += w.t1 - w.t0;
-    off += w.t1 - w.t0;
+    cut.note(sm.share, w);
   }
   if (t == 0) cut.store(p);
 }
@@ -938,15 +952,13 @@ __global__ void __launch_bounds__(PaNarrow<T, DP>::THREADS, PaNarrow<T, DP>::CTA
   dependent_trigger();
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, g = lane >> 2, c4 = lane & 3;
   const PgCache& c = p.c;
-  pa_share<RT, BN>(p, &sm.share);
+  pa_share<RT, RT, BN>(p, &sm.share);
   PaCut cut;
-  uint32_t pos = sm.share.from, off = sm.share.off;
-  const uint32_t end = sm.share.to;
-  int slot = sm.share.slot;
+  PaAt at(sm.share);
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(sm.ring[warp]));
   const int words = c.dim * static_cast<int>(sizeof(T)) / 16;
-  while (pos < end) {
-    const PaPart w = pa_part<RT, BN>(p, pos, end, &slot, &off);
+  PaPart w;
+  while (pa_next<RT, RT, BN>(p, &at, &w)) {
     const uint32_t mine = KEYS * warp;
     // (a lane looks up the page of key lane % KEYS of a step, one step before the copies need it)
     const auto lookup = [&](uint32_t tile) { return tile < w.t1 ? pa_lookup(p, w, tile * BN + mine + lane % KEYS) : -1; };
@@ -1066,9 +1078,7 @@ __global__ void __launch_bounds__(PaNarrow<T, DP>::THREADS, PaNarrow<T, DP>::CTA
         }
       }
     }
-    cut.note(sm.share, w, pos);
-    pos += w.t1 - w.t0;
-    off += w.t1 - w.t0;
+    cut.note(sm.share, w);
   }
   if (t == 0) cut.store(p);
 }
@@ -1096,15 +1106,13 @@ __global__ void __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) paged_attn_wide
   dependent_trigger();
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, g = lane >> 2, c4 = lane & 3;
   const PgCache& c = p.c;
-  pa_share<RT, BN>(p, &sm.share);
+  pa_share<RT, RT, BN>(p, &sm.share);
   PaCut cut;
-  uint32_t pos = sm.share.from, off = sm.share.off;
-  const uint32_t end = sm.share.to;
-  int slot = sm.share.slot;
+  PaAt at(sm.share);
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(sm.ring));
   const int word = t % WORDS, words = c.dim / 8;
-  while (pos < end) {
-    const PaPart w = pa_part<RT, BN>(p, pos, end, &slot, &off);
+  PaPart w;
+  while (pa_next<RT, RT, BN>(p, &at, &w)) {
     const int words_seen = (w.s.nodes + 31) / 32;
     const int node0 = static_cast<int>(p.by_group.of(w.row0)), node1 = static_cast<int>(p.by_group.of(w.row0 + w.rows - 1));
     // Thread t < BN finds where row t of a tile lies, one tile before the copies of it, with the page that it looked up one tile
@@ -1201,29 +1209,30 @@ __global__ void __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) paged_attn_wide
         }
       }
     }
-    cut.note(sm.share, w, pos);
-    pos += w.t1 - w.t0;
-    off += w.t1 - w.t0;
+    cut.note(sm.share, w);
   }
   if (t == 0) cut.store(p);
 }
 
-// Many rows: tcgen05. A part has up to 256 rows as two tiles of 128, whose scores S and sums O live in tensor memory; keys and values
-// come in tiles of 128 into a ring of shared memory. Two warps copy (cp.async, 16-byte words in the 128-byte swizzle that the
-// instructions' descriptors name: pages may have any size and rows any place), one issues S_t = Q_t K^T and O_t += P_t V, and four
-// warps for each row tile turn S into P, a thread a row, while the tensor core works on the other tile. P stays in tensor memory,
-// over its own scores. What bounds it are the exponentials (one result a clock and quarter SM) and the tensor pipe, which take about
-// the same time; a part with rows in one tile only has nothing to hide them behind.
+// More than 16 rows: tcgen05. Two streams of blocks of 128 rows by 128 keys, whose scores S and sums O live in tensor memory: the two
+// halves of up to 256 rows over the same keys or, where a part has no more than 128 rows, the even and the odd key tiles over the
+// same rows, joined at its end. Keys and values come in tiles of 128 into shared memory, two of each: a tile of keys is free when its
+// scores are there, one of values when its sums are. Two warps copy (cp.async, 16-byte words in the 128-byte swizzle that the
+// instructions' descriptors name: pages may have any size and rows any place), one issues S_t = Q K^T and O_t += P_t V, and four warps
+// for each stream turn S into P, a thread a row, while the tensor core works on the other stream. P stays in tensor memory, over its
+// own scores. What bounds it are the exponentials (one result a clock and quarter SM) and the tensor pipe, which take about the same
+// time.
 template <typename T, int DP>
 struct PaTc {
-  static constexpr int RT = 256, BN = 128, THREADS = 384, STAGES = DP == 64 ? 4 : 2, TILE = 128 * DP * 2;
-  static constexpr int KV = 2 * TILE, REST = KV + STAGES * 2 * TILE;  // offsets: Q, the ring, the rest
+  static constexpr int RT = 256, RW = 128, BN = 128, THREADS = 384, STAGES = DP == 64 ? 4 : 2, TILE = 128 * DP * 2;
+  static constexpr int K = 2 * TILE, V = K + STAGES * TILE, REST = V + STAGES * TILE;  // offsets: Q, keys, values, the rest
   struct Rest {
-    uint64_t q_full, q_free, k_full[STAGES], v_full[STAGES], empty[STAGES], s_full[2], p_full[2], o_ready[2], o_free[2];
+    uint64_t q_full, q_free, k_full[STAGES], v_full[STAGES], k_free[STAGES], v_free[STAGES], s_full[2], p_full[2], o_ready[2], o_free[2], met;
     uint32_t tmem;
     int stop;  // a wait has run out
-    int odd;   // the part has hidden values that are not finite
-    int16_t up[8][PA_TREE];  // a slot's parents, for each softmax warp
+    int odd;   // there are hidden values that are not finite
+    float m[2][2][128], l[2][2][128];  // of the two streams over the same rows; by turns
+    int16_t up[8][PA_TREE];            // a slot's parents, for each softmax warp
     PaShare share;
   };
   static constexpr int BYTES = REST + static_cast<int>(sizeof(Rest)) + 1024;
@@ -1270,7 +1279,7 @@ __device__ __forceinline__ void pa_sees128(const int16_t* up, int node, int n0, 
 template <typename T, int DP>
 __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1) paged_attn_tc_kernel(const PaParams p) {
   using S = PaTc<T, DP>;
-  constexpr int RT = S::RT, BN = S::BN, ST = S::STAGES, TILE = S::TILE, WORDS = DP / 8, PER = 32 / WORDS;
+  constexpr int RT = S::RT, RW = S::RW, BN = S::BN, ST = S::STAGES, TILE = S::TILE, WORDS = DP / 8, PER = 32 / WORDS;
   extern __shared__ __align__(128) unsigned char raw[];
   unsigned char* const smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
   typename S::Rest& sm = *reinterpret_cast<typename S::Rest*>(smem + S::REST);
@@ -1283,14 +1292,16 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1) paged_attn_tc_kernel(
     for (int s = 0; s < ST; ++s) {
       mbar_init(&sm.k_full[s], 2);
       mbar_init(&sm.v_full[s], 2);
-      mbar_init(&sm.empty[s], 1);
+      mbar_init(&sm.k_free[s], 1);
+      mbar_init(&sm.v_free[s], 1);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&sm.s_full[t], 1);
-      mbar_init(&sm.p_full[t], 4);  // (of each softmax warp)
+      mbar_init(&sm.p_full[t], 4);  // (of each softmax warp of the stream)
       mbar_init(&sm.o_ready[t], 1);
-      mbar_init(&sm.o_free[t], 4);
+      mbar_init(&sm.o_free[t], 8);  // (of all softmax warps, or twice of the stream's own)
     }
+    mbar_init(&sm.met, 8);
     sm.stop = 0;
     sm.odd = 0;
     fence_mbar_init();
@@ -1301,24 +1312,26 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1) paged_attn_tc_kernel(
     tmem_relinquish();
   }
   tc_fence_before();
-  pa_share<RT, BN>(p, &sm.share);
+  pa_share<RT, RW, BN>(p, &sm.share);
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
   // columns of tensor memory: S0 / P0 at 0, S1 / P1 at 128, O0 at 256, O1 at 384
   volatile int* const stop = &sm.stop;
-  uint32_t pos = sm.share.from, off = sm.share.off;
-  const uint32_t end = sm.share.to;
-  int slot = sm.share.slot, n_part = 0;
+  PaAt at(sm.share);
+  PaPart w;
+  uint32_t n_part = 0;
   bool ok = true;
 
   if (warp == 0) {
     // ------------------------------------------------------------ the issuer of the matrix instructions (all lanes, one leads)
-    const uint32_t lead = lane == 0 ? 1u : 0u, q0 = smem_u32(smem), kv = q0 + S::KV;
+    const uint32_t lead = lane == 0 ? 1u : 0u, q0 = smem_u32(smem), k0 = q0 + S::K, v0 = q0 + S::V;
     constexpr uint32_t FORMAT = std::is_same<T, __half>::value ? 0u : 1u;
     const uint32_t idesc_s = umma_idesc(FORMAT, 0, 0, 128, 128), idesc_o = umma_idesc(FORMAT, 0, 1, 128, DP);
-    uint32_t n_kv = 0, n_p[2] = {0, 0}, n_e[2] = {0, 0};
-    const auto issue_s = [&](int t, uint32_t stage) {
-      const uint32_t qa = q0 + t * TILE, ka = kv + stage * (2 * TILE);
+    uint32_t n_k = 0, n_v = 0;                 // key and value tiles so far
+    uint32_t p_odd = 0, o_odd = 0, o_any = 0;  // bit t: of stream t, whether the P tiles, the results are odd in number; any results
+    const auto keys = [&](uint32_t n) { return mbar_wait_warp(&sm.k_full[n % ST], (n / ST) & 1, stop); };
+    const auto issue_s = [&](int t, uint32_t qa, uint32_t stage) {
+      const uint32_t ka = k0 + stage * TILE;
 #pragma unroll
       for (int k = 0; k < DP / 16; ++k) {
         const uint32_t o = (k >> 2) * (128 * 128) + (k & 3) * 32;
@@ -1327,50 +1340,85 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1) paged_attn_tc_kernel(
       tc_commit_lead(smem_u32(&sm.s_full[t]), lead);
     };
     const auto issue_o = [&](int t, uint32_t stage, bool more) {
-      const uint32_t va = kv + stage * (2 * TILE) + TILE;
+      const uint32_t va = v0 + stage * TILE;
 #pragma unroll
       for (int k = 0; k < BN / 16; ++k)
         tc_mma_f16_ts_lead(tmem + 256 + 128 * t, tmem + 128 * t + 8 * k, umma_smem_desc_sw128(va + k * 2048, 128 * 128, 1024), idesc_o, more || k != 0, lead);
       tc_commit_lead(smem_u32(&sm.o_ready[t]), lead);
     };
-    while (ok && pos < end) {
-      const PaPart w = pa_part<RT, BN>(p, pos, end, &slot, &off);
-      const int n = w.t1 - w.t0, tiles = w.rows > 128 ? 2 : 1;
-      ok = mbar_wait_warp(&sm.q_full, n_part & 1, stop) && mbar_wait_warp(&sm.k_full[n_kv % ST], (n_kv / ST) & 1, stop);
-      if (!ok) break;
+    // P_t is there, and O_t may be written
+    const auto weights = [&](int t, bool first) {
+      if (!mbar_wait_warp(&sm.p_full[t], (p_odd >> t) & 1, stop)) return false;
+      if (first && ((o_any >> t) & 1) && !mbar_wait_warp(&sm.o_free[t], ((o_odd >> t) & 1) ^ 1, stop)) return false;
+      p_odd ^= 1u << t;
       tc_fence_after();
-      for (int t = 0; t < tiles; ++t) issue_s(t, n_kv % ST);
-      if (n == 1) tc_commit_lead(smem_u32(&sm.q_free), lead);
-      for (int j = 0; ok && j < n; ++j, ++n_kv) {
-        const uint32_t s = n_kv % ST, next = (n_kv + 1) % ST;
-        if (!(ok = mbar_wait_warp(&sm.v_full[s], (n_kv / ST) & 1, stop))) break;
-        for (int t = 0; t < tiles; ++t) {
-          ok = mbar_wait_warp(&sm.p_full[t], n_p[t] & 1, stop);
-          if (ok && j == 0 && n_e[t] > 0) ok = mbar_wait_warp(&sm.o_free[t], (n_e[t] - 1) & 1, stop);  // (O is written anew)
+      return true;
+    };
+    while (ok && pa_next<RT, RW, BN>(p, &at, &w)) {
+      const int n = w.t1 - w.t0;
+      if (!(ok = mbar_wait_warp(&sm.q_full, n_part & 1, stop) && keys(n_k))) break;
+      tc_fence_after();
+      if (w.rows > 128) {  // two row tiles, S of the next key tile behind O of this one (it overwrites P)
+        issue_s(0, q0, n_k % ST);
+        issue_s(1, q0 + TILE, n_k % ST);
+        tc_commit_lead(smem_u32(&sm.k_free[n_k % ST]), lead);
+        ++n_k;
+        for (int j = 0; ok && j < n; ++j, ++n_v) {
+          if (j + 1 == n) tc_commit_lead(smem_u32(&sm.q_free), lead);
+          const uint32_t s = n_v % ST;
+          ok = mbar_wait_warp(&sm.v_full[s], (n_v / ST) & 1, stop);
+          for (int t = 0; ok && t < 2; ++t) {
+            if (!(ok = weights(t, j == 0))) break;
+            issue_o(t, s, j > 0);
+            if (j + 1 < n) {
+              if (t == 0 && !(ok = keys(n_k))) break;
+              tc_fence_after();
+              issue_s(t, q0 + t * TILE, n_k % ST);
+            }
+          }
           if (!ok) break;
-          ++n_p[t];
-          tc_fence_after();
-          issue_o(t, s, j > 0);
+          tc_commit_lead(smem_u32(&sm.v_free[s]), lead);
           if (j + 1 < n) {
-            if (t == 0 && !(ok = mbar_wait_warp(&sm.k_full[next], ((n_kv + 1) / ST) & 1, stop))) break;
-            tc_fence_after();
-            issue_s(t, next);  // (behind the product that reads P from the same columns)
+            tc_commit_lead(smem_u32(&sm.k_free[n_k % ST]), lead);
+            ++n_k;
           }
         }
-        if (!ok) break;
-        if (j + 2 == n) tc_commit_lead(smem_u32(&sm.q_free), lead);
-        tc_commit_lead(smem_u32(&sm.empty[s]), lead);
+      } else {  // one row tile: stream t has the key tiles t, t + 2, ...
+        const auto start = [&](int t) {
+          issue_s(t, q0, n_k % ST);
+          tc_commit_lead(smem_u32(&sm.k_free[n_k % ST]), lead);
+          ++n_k;
+        };
+        start(0);
+        if (n > 1) {
+          if (!(ok = keys(n_k))) break;
+          tc_fence_after();
+          start(1);
+        }
+        for (int j = 0; ok && j < n; ++j, ++n_v) {
+          if (j + 2 >= n && (j + 2 == n || n == 1)) tc_commit_lead(smem_u32(&sm.q_free), lead);  // (all of S has been issued)
+          const uint32_t s = n_v % ST;
+          const int t = j & 1;
+          if (!(ok = mbar_wait_warp(&sm.v_full[s], (n_v / ST) & 1, stop) && weights(t, j < 2))) break;
+          issue_o(t, s, j > 1);
+          tc_commit_lead(smem_u32(&sm.v_free[s]), lead);
+          if (j + 2 < n) {
+            if (!(ok = keys(n_k))) break;
+            tc_fence_after();
+            start(t);
+          }
+        }
       }
-      for (int t = 0; t < tiles; ++t) ++n_e[t];
+      const uint32_t wrote = w.rows > 128 || n > 1 ? 3u : 1u;
+      o_odd ^= wrote;
+      o_any |= wrote;
       ++n_part;
-      pos += n;
-      off += n;
     }
   } else if (warp == 2 || warp == 3) {
-    // ------------------------------------------------------------ copies
+    // ------------------------------------------------------------ copies: half of the rows of a tile each
     const int half = warp - 2, words = c.dim / 8, word = lane % WORDS;
-    const uint32_t q0 = smem_u32(smem), kv = q0 + S::KV;
-    uint32_t n_kv = 0;
+    const uint32_t q0 = smem_u32(smem), k0 = q0 + S::K, v0 = q0 + S::V;
+    uint32_t n_k = 0, n_v = 0;
     PaCut cut;
     // A group of copies is told to the issuer when the next one is on its way, or before a wait.
     uint64_t* told = nullptr;
@@ -1380,9 +1428,9 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1) paged_attn_tc_kernel(
         bool odd = false;
 #pragma unroll 1
         for (int i = 0; i < 64 / PER; ++i) {
-          const uint32_t at = look_at + S::at(64 * half + i * PER + lane / WORDS, word);
+          const uint32_t a = look_at + S::at(64 * half + i * PER + lane / WORDS, word);
           uint32_t x[4];
-          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at) : "memory");
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(a) : "memory");
           bool here = false;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -1390,7 +1438,7 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1) paged_attn_tc_kernel(
             here = here || y != x[k];
             x[k] = y;
           }
-          if (here) asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+          if (here) asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
           odd = odd || here;
         }
         if (__any_sync(0xffffffffu, odd) && lane == 0) atomicExch(&sm.odd, 1);
@@ -1416,8 +1464,24 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1) paged_attn_tc_kernel(
         tell();
       }
     };
-    while (ok && pos < end) {
-      const PaPart w = pa_part<RT, BN>(p, pos, end, &slot, &off);
+    const auto room = [&](uint64_t* bar, uint32_t parity) {
+      if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+      flush();
+      return mbar_wait_warp(bar, parity, stop);
+    };
+    // 64 rows of a tile whose places two lanes' registers hold
+    const auto copy = [&](uint32_t to, const unsigned long long (&from)[2]) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll 4
+        for (int i = 0; i < 32 / PER; ++i) {
+          const int r = i * PER + lane / WORDS;
+          const unsigned long long a = __shfl_sync(0xffffffffu, from[h], r);
+          const bool there = a != 0 && word < words;
+          pa_copy16(to + S::at(64 * half + 32 * h + r, word), there ? reinterpret_cast<const char*>(a) + word * 16 : c.k.p, there);
+        }
+    };
+    while (ok && pa_next<RT, RW, BN>(p, &at, &w)) {
       int pg[2];
       const auto lookup = [&](uint32_t tile) {
 #pragma unroll
@@ -1433,32 +1497,31 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1) paged_attn_tc_kernel(
           pa_copy16(q0 + t * TILE + S::at(r, word), there ? pa_query(p, w, row) + word * 16 : p.q.p, there);
         }
       sent(&sm.q_full, 0);
-      for (uint32_t tile = w.t0; tile < w.t1; ++tile, ++n_kv) {
-        const uint32_t s = n_kv % ST, parity = ((n_kv / ST) & 1) ^ 1, kt = kv + s * (2 * TILE);
-        unsigned long long kp[2], vp[2];
+      unsigned long long kp[2] = {0, 0}, vp[2] = {0, 0};
+      // keys one tile ahead of values
+#pragma unroll 1
+      for (uint32_t tile = w.t0; ok && tile <= w.t1; ++tile) {
+        const unsigned long long old[2] = {vp[0], vp[1]};
+        if (tile < w.t1) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const PaRow r = pa_row(p, w, tile * BN + 64 * half + 32 * i + lane, pg[i]);
-          kp[i] = reinterpret_cast<unsigned long long>(r.k);
-          vp[i] = reinterpret_cast<unsigned long long>(r.v);
+          for (int i = 0; i < 2; ++i) {
+            const PaRow r = pa_row(p, w, tile * BN + 64 * half + 32 * i + lane, pg[i]);
+            kp[i] = reinterpret_cast<unsigned long long>(r.k);
+            vp[i] = reinterpret_cast<unsigned long long>(r.v);
+          }
+          lookup(tile + 1);
+          const uint32_t s = n_k % ST;
+          if (!(ok = room(&sm.k_free[s], ((n_k / ST) & 1) ^ 1))) break;
+          copy(k0 + s * TILE, kp);
+          sent(&sm.k_full[s], 0);
+          ++n_k;
         }
-        lookup(tile + 1);
-        if (!__all_sync(0xffffffffu, mbar_try_wait(&sm.empty[s], parity))) {
-          flush();
-          if (!(ok = mbar_wait_warp(&sm.empty[s], parity, stop))) break;
-        }
-#pragma unroll
-        for (int v = 0; v < 2; ++v) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll 4
-            for (int i = 0; i < 32 / PER; ++i) {
-              const int r = i * PER + lane / WORDS;
-              const unsigned long long a = __shfl_sync(0xffffffffu, v ? vp[h] : kp[h], r);
-              const bool there = a != 0 && word < words;
-              pa_copy16(kt + v * TILE + S::at(64 * half + 32 * h + r, word), there ? reinterpret_cast<const char*>(a) + word * 16 : c.k.p, there);
-            }
-          sent(v ? &sm.v_full[s] : &sm.k_full[s], v && static_cast<int64_t>(tile + 1) * BN > w.s.len ? kt + TILE : 0u);
+        if (tile > w.t0) {
+          const uint32_t s = n_v % ST;
+          if (!(ok = room(&sm.v_free[s], ((n_v / ST) & 1) ^ 1))) break;
+          copy(v0 + s * TILE, old);
+          sent(&sm.v_full[s], static_cast<int64_t>(tile) * BN > w.s.len ? v0 + s * TILE : 0u);
+          ++n_v;
         }
       }
       if (!ok) break;
@@ -1467,31 +1530,26 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1) paged_attn_tc_kernel(
         const int64_t n0 = static_cast<int64_t>(w.t0) * BN - w.s.len, n1 = static_cast<int64_t>(w.t1) * BN - w.s.len;
         if (n1 > 0) pa_store_new<uint4>(p, w, n0 < 0 ? 0 : static_cast<int>(n0), static_cast<int>(n1 < w.s.nodes ? n1 : w.s.nodes), words, 32 * half + lane, 64);
       }
-      cut.note(sm.share, w, pos);
+      cut.note(sm.share, w);
       ++n_part;
-      pos += w.t1 - w.t0;
-      off += w.t1 - w.t0;
     }
     pa_copy_wait<0>();
     if (warp == 2 && lane == 0) cut.store(p);
   } else if (warp >= 4) {
-    // ------------------------------------------------------------ softmax and results: row tile t, a thread a row
+    // ------------------------------------------------------------ softmax and results: stream t, a thread a row
     const int t = (warp - 4) >> 2, in_tile = (warp & 3) * 32 + lane;
     const uint32_t lane_sel = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + 128 * t + lane_sel, to = tmem + 256 + 128 * t + lane_sel;
     const bool pos_scale = p.scale >= 0.f;
     const float none = pos_scale ? -CUDART_INF_F : CUDART_INF_F;  // a hidden score before the scale
-    uint32_t n_s = 0;
-    while (ok && pos < end) {
-      const PaPart w = pa_part<RT, BN>(p, pos, end, &slot, &off);
-      const int n = w.t1 - w.t0;
-      pos += n;
-      off += n;
+    uint32_t n_s = 0, n_other = 0, n_met = 0;  // score tiles of this stream and of the other one, parts with both streams over one row tile
+    int16_t* const mine = sm.up[warp - 4];
+    const int16_t* const up = p.parents ? mine : nullptr;
+    while (ok && pa_next<RT, RW, BN>(p, &at, &w)) {
+      const uint32_t all = w.t1 - w.t0;
+      const bool split = w.rows <= 128;
+      const int n = split ? (all - t + 1) / 2 : all;  // key tiles of this stream
       const bool nodes_here = static_cast<int64_t>(w.t1) * BN > w.s.len;
-      const int r = 128 * t + in_tile;
-      if (128 * t >= w.rows) continue;
-      const int node = static_cast<int>(p.by_group.of(w.row0 + min(r, w.rows - 1)));
-      int16_t* const mine = sm.up[warp - 4];
       if (p.parents && nodes_here) {
         __syncwarp();
         for (int i = lane; i < w.s.nodes; i += 32) {
@@ -1504,12 +1562,19 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1) paged_attn_tc_kernel(
         }
         __syncwarp();
       }
-      const int16_t* up = p.parents ? mine : nullptr;
+      const int r = split ? in_tile : 128 * t + in_tile;
+      const int node = static_cast<int>(p.by_group.of(w.row0 + min(r, w.rows - 1)));
+      const bool idle = r - lane >= w.rows;  // no row of the warp is one: nobody reads its P
       float m = -CUDART_INF_F, l = 0.f;
       for (int j = 0; j < n; ++j, ++n_s) {
         if (!(ok = mbar_wait_warp(&sm.s_full[t], n_s & 1, stop))) break;
+        if (idle) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.p_full[t]);
+          continue;
+        }
         tc_fence_after();
-        const int n0 = static_cast<int>((w.t0 + j) * BN) - w.s.len;
+        const int n0 = static_cast<int>((w.t0 + (split ? 2 * j + t : j)) * BN) - w.s.len;
         const bool masked = n0 + BN > 0;
         uint32_t bits[4];
         if (masked) pa_sees128(up, node, n0, bits);
@@ -1592,56 +1657,93 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1) paged_attn_tc_kernel(
         if (lane == 0) mbar_arrive(&sm.p_full[t]);
       }
       if (!ok) break;
-      if (!(ok = mbar_wait_warp(&sm.o_ready[t], (n_s - 1) & 1, stop))) break;
-      tc_fence_after();
-      const bool whole = w.t0 == 0 && w.t1 == w.tiles, here = r < w.rows;
-      const bool odd = nodes_here && *reinterpret_cast<volatile int*>(&sm.odd);
-      float* piece = pa_piece_of<RT, DP>(p, w) + r * DP;
-      char* out = here ? pa_out(p, w.s.start, w.head, w.row0 + r) : nullptr;
-      const float f = 1.f / l;
-#pragma unroll 1
-      for (int d = 0; d < DP; d += 16) {
-        uint32_t x[16];
+      // The sums: of this stream's own rows or, half of the columns each, of both streams over the same rows.
+      float weight[2] = {1.f, 0.f};
+      int d0 = 0, d1 = DP;
+      if (split) {
+        const int turn = n_met & 1;
+        sm.m[turn][t][in_tile] = m;
+        sm.l[turn][t][in_tile] = l;
         __syncwarp();
-        tmem_ld_32x32b_x16(to + d, x);
-        tmem_ld_wait();
-        if (odd && here) {  // the values that were left out, of the nodes of this part that the row sees
-          for (int j = min(node, static_cast<int>(static_cast<int64_t>(w.t1) * BN - w.s.len) - 1); j >= 0 && static_cast<int64_t>(j) + w.s.len >= static_cast<int64_t>(w.t0) * BN; --j) {
-            uint32_t sees[4];
-            pa_sees128(up, node, j, sees);
-            if (!(sees[0] & 1)) continue;
-            const uint32_t at = static_cast<uint32_t>(w.s.len + j);
-            const T* v = reinterpret_cast<const T*>(pa_row(p, w, at, pa_lookup(p, w, at)).v);
+        if (lane == 0) mbar_arrive(&sm.met);
+        if (!(ok = mbar_wait_warp(&sm.met, n_met & 1, stop))) break;
+        ++n_met;
+        const float m0 = sm.m[turn][0][in_tile], m1 = sm.m[turn][1][in_tile];
+        m = fmaxf(m0, m1);
+        weight[0] = m0 == -CUDART_INF_F ? 0.f : pa_exp2(m0 - m);
+        weight[1] = m1 == -CUDART_INF_F ? 0.f : pa_exp2(m1 - m);
+        l = weight[0] * sm.l[turn][0][in_tile] + weight[1] * sm.l[turn][1][in_tile];
+        d0 = t * (DP / 2);
+        d1 = d0 + DP / 2;
+        const int n1 = static_cast<int>(all / 2), n2 = static_cast<int>(all) - n1;  // key tiles of stream 1, of stream 0
+        n_other += t ? n2 : n1;
+        if ((t ? n2 : n1) > 0 && !(ok = mbar_wait_warp(&sm.o_ready[1 - t], (n_other - 1) & 1, stop))) break;
+      } else if (w.rows > 128) {
+        n_other += all;
+      }
+      if (n > 0 && !(ok = mbar_wait_warp(&sm.o_ready[t], (n_s - 1) & 1, stop))) break;
+      tc_fence_after();
+      const bool whole = w.t0 == 0 && w.t1 == w.tiles, here = r < w.rows, both = split && all > 1;
+      const bool odd = nodes_here && *reinterpret_cast<volatile int*>(&sm.odd);
+      float* const piece = pa_piece_of<RT, DP>(p, w);
+      char* const out = here ? pa_out(p, w.s.start, w.head, w.row0 + r) : nullptr;
+      const float f = 1.f / l;
+      const uint32_t o0 = split ? tmem + 256 + lane_sel : to;
+      if (!idle) {
+#pragma unroll 1
+        for (int d = d0; d < d1; d += 16) {
+          uint32_t x[16];
+          __syncwarp();
+          tmem_ld_32x32b_x16(o0 + d, x);
+          tmem_ld_wait();
+          if (both) {
+            uint32_t y[16];
+            tmem_ld_32x32b_x16(o0 + 128 + d, y);
+            tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (v && d + e < c.dim) {
-                const float y = pa_load(v + d + e);
-                if (!(fabsf(y) < CUDART_INF_F)) x[e] = __float_as_uint(__uint_as_float(x[e]) + y);
+            for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(weight[0] * __uint_as_float(x[e]) + weight[1] * __uint_as_float(y[e]));
+          }
+          if (odd && here) {  // the values that were left out, of the nodes of this part that the row sees
+            for (int j = min(node, static_cast<int>(static_cast<int64_t>(w.t1) * BN - w.s.len) - 1); j >= 0 && static_cast<int64_t>(j) + w.s.len >= static_cast<int64_t>(w.t0) * BN; --j) {
+              uint32_t sees[4];
+              pa_sees128(up, node, j, sees);
+              if (!(sees[0] & 1)) continue;
+              const uint32_t pl = static_cast<uint32_t>(w.s.len + j);
+              const T* v = reinterpret_cast<const T*>(pa_row(p, w, pl, pa_lookup(p, w, pl)).v);
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                if (v && d + e < c.dim) {
+                  const float y = pa_load(v + d + e);
+                  if (!(fabsf(y) < CUDART_INF_F)) x[e] = __float_as_uint(__uint_as_float(x[e]) + y);
+                }
+            }
+          }
+          if (here && whole) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              if (d + 8 * k < c.dim) {
+                uint32_t y[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = pa_pack<T>(__uint_as_float(x[8 * k + 2 * e]) * f, __uint_as_float(x[8 * k + 2 * e + 1]) * f);
+                *reinterpret_cast<uint4*>(out + 2 * (d + 8 * k)) = make_uint4(y[0], y[1], y[2], y[3]);
               }
+          } else if (here) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) *reinterpret_cast<uint4*>(piece + r * DP + d + 4 * k) = make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
           }
         }
-        if (here && whole) {
-#pragma unroll
-          for (int k = 0; k < 2; ++k)
-            if (d + 8 * k < c.dim) {
-              uint32_t y[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) y[e] = pa_pack<T>(__uint_as_float(x[8 * k + 2 * e]) * f, __uint_as_float(x[8 * k + 2 * e + 1]) * f);
-              *reinterpret_cast<uint4*>(out + 2 * (d + 8 * k)) = make_uint4(y[0], y[1], y[2], y[3]);
-            }
-        } else if (here) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) *reinterpret_cast<uint4*>(piece + d + 4 * k) = make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
+        if (here && !whole && d0 == 0) {
+          piece[RT * DP + r] = m;
+          piece[RT * DP + RT + r] = l;
         }
-      }
-      if (here && !whole) {
-        float* sums = pa_piece_of<RT, DP>(p, w) + RT * DP;
-        sums[r] = m;
-        sums[RT + r] = l;
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.o_free[t]);
+      if (lane == 0) {
+        // O of a stream without key tiles in the part has not been written, and nobody waits for it to be read
+        mbar_arrive(&sm.o_free[split ? 0 : t]);
+        if (!split || both) mbar_arrive(&sm.o_free[split ? 1 : t]);
+      }
     }
   }
   if (!ok && lane == 0) {
@@ -1738,14 +1840,17 @@ static PaForm pa_form(int rows, bool words) {
   using N = PaNarrow<T, DP>;
   static_assert(N::CTAS * (sizeof(N) + 1024) <= PA_SHARED + 1024, "shared memory");
   if constexpr (sizeof(T) == 2) {
-    using W = PaWide<T, DP>;
-    static_assert(sizeof(W) <= PA_SHARED, "shared memory");
-    using C = PaTc<T, DP <= 128 ? DP : 128>;
-    static_assert(C::BYTES <= PA_SHARED, "shared memory");
-    if (DP <= 128 && words && rows > PA_TC_ROWS)
-      return PaForm{DP, C::RT, C::BN, sm_count(), C::THREADS, C::BYTES, paged_attn_tc_kernel<T, DP <= 128 ? DP : 128>};
-    if (words && rows > 16)
-      return PaForm{DP, W::RT, W::BN, sm_count() * (DP == 256 ? 1 : 2), PA_THREADS, static_cast<int>(sizeof(W)), paged_attn_wide_kernel<T, DP>};
+    if (words && rows > N::RT) {
+      if constexpr (DP <= 128) {
+        using C = PaTc<T, DP>;
+        static_assert(C::BYTES <= PA_SHARED, "shared memory");
+        return PaForm{DP, C::RT, C::BN, sm_count(), C::THREADS, C::BYTES, paged_attn_tc_kernel<T, DP>};
+      } else {
+        using W = PaWide<T, DP>;
+        static_assert(sizeof(W) <= PA_SHARED, "shared memory");
+        return PaForm{DP, W::RT, W::BN, sm_count(), PA_THREADS, static_cast<int>(sizeof(W)), paged_attn_wide_kernel<T, DP>};
+      }
+    }
   }
   if (words) return PaForm{DP, N::RT, N::BN, sm_count() * N::CTAS, N::THREADS, static_cast<int>(sizeof(N)), paged_attn_narrow_kernel<T, DP>};
   return rows <= 8 ? pa_ffma<T, DP, 1>() : pa_ffma<T, DP, 4>();

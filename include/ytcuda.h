@@ -461,7 +461,7 @@ int ytcuda_latent_attn_fwd(int dtype, const void* q, const void* uk_bf16, const 
  * kernels without a host round trip, so that a captured graph serves any lengths. Calls on one cache are ordered by the
  * caller (one stream, or events), as writes of one tensor are.
  * What only the device can see to be wrong is never followed to memory: the call sets a bit of *status and leaves out what
- * it concerns. YTC_PAGES_FULL: a reserve or compact found too few free pages (or entries of the table) and changed
+ * it concerns (attention reads zeros where a page does not exist). YTC_PAGES_FULL: a reserve or compact found too few free pages (or entries of the table) and changed
  * nothing. YTC_PAGES_INVALID: an index outside its range, a position without a page, or a tree that is none.
  * YTC_PAGES_SHARED: rows would have gone to a page that other slots hold too (reserve comes first). */
 #define YTC_PAGES_FULL 1

@@ -32,6 +32,7 @@ struct PaParams {
   float* work;  // pieces of cut units
   int4* cuts;   // two words for each CTA: the unit that starts in its share and goes on behind it
   int* timeout; // the device's status word
+  int box;      // rows of a page that a TMA copy takes (0: none)
 };
 
 // What a slot brings: its rows in the call, its nodes, its length.
@@ -247,7 +248,10 @@ struct PaRow {
   const char *k, *v;
 };
 __device__ __forceinline__ int pa_lookup(const PaParams& p, const PaPart& w, uint32_t at) {
-  return at < static_cast<uint32_t>(w.s.len) + (p.fresh ? 0u : static_cast<uint32_t>(w.s.nodes)) ? pg_page_of(p.c, w.slot, at) : -1;
+  if (at >= static_cast<uint32_t>(w.s.len) + (p.fresh ? 0u : static_cast<uint32_t>(w.s.nodes))) return -1;
+  const int pg = pg_page_of(p.c, w.slot, at);
+  if (pg < 0) atomicOr(p.c.status, YTC_PAGES_INVALID);
+  return pg;
 }
 __device__ __forceinline__ PaRow pa_row(const PaParams& p, const PaPart& w, uint32_t at, int pg) {
   PaRow r{nullptr, nullptr};
@@ -1217,9 +1221,9 @@ __global__ void __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) paged_attn_wide
 // More than 16 rows: tcgen05. Two streams of blocks of 128 rows by 128 keys, whose scores S and sums O live in tensor memory: the two
 // halves of up to 256 rows over the same keys or, where a part has no more than 128 rows, the even and the odd key tiles over the
 // same rows, joined at its end. Keys and values come in tiles of 128 into shared memory, two of each: a tile of keys is free when its
-// scores are there, one of values when its sums are. Two warps copy (cp.async, 16-byte words in the 128-byte swizzle that the
-// instructions' descriptors name: pages may have any size and rows any place), one issues S_t = Q K^T and O_t += P_t V, and four warps
-// for each stream turn S into P, a thread a row, while the tensor core works on the other stream. P stays in tensor memory, over its
+// scores are there, one of values when its sums are. Two warps copy: tiles in front of the nodes by TMA, `box` rows of a page and 64
+// dims an instruction (a box outside the pool reads zeros); tiles with nodes, and pages whose size is no multiple of 8, by cp.async,
+// 16-byte words in the same 128-byte swizzle. One warp issues S_t = Q K^T and O_t += P_t V, and four warps for each stream turn S into P, a thread a row, while the tensor core works on the other stream. P stays in tensor memory, over its
 // own scores. What bounds it are the exponentials (one result a clock and quarter SM) and the tensor pipe, which take about the same
 // time.
 template <typename T, int DP>
@@ -1277,7 +1281,8 @@ __device__ __forceinline__ void pa_sees128(const int16_t* up, int node, int n0, 
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1) paged_attn_tc_kernel(const PaParams p) {
+__global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1)
+    paged_attn_tc_kernel(const PaParams p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
   using S = PaTc<T, DP>;
   constexpr int RT = S::RT, RW = S::RW, BN = S::BN, ST = S::STAGES, TILE = S::TILE, WORDS = DP / 8, PER = 32 / WORDS;
   extern __shared__ __align__(128) unsigned char raw[];
@@ -1481,11 +1486,36 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1) paged_attn_tc_kernel(
           pa_copy16(to + S::at(64 * half + 32 * h + r, word), there ? reinterpret_cast<const char*>(a) + word * 16 : c.k.p, there);
         }
     };
+    // Half of a tile by TMA: the pages of its boxes are in lanes 0, 1, ... of `page`.
+    const uint32_t lead = lane == 0 ? 1u : 0u;
+    const int boxes = p.box ? 64 / p.box : 0;  // (of one of the two warps; 0 where a box is a whole tile, which one warp fetches)
+    const int my_boxes = p.box == 128 ? 1 - half : boxes;
+    const auto fetch = [&](const CUtensorMap* map, uint64_t* bar, uint32_t to, uint32_t tile, int page) {
+      mbar_expect_tx_lead(smem_u32(bar), static_cast<uint32_t>(my_boxes * p.box) * (DP / 64) * 128, lead);
+      for (int i = 0; i < my_boxes; ++i) {
+        const int row = 64 * half + i * p.box, at_page = __shfl_sync(0xffffffffu, page, i);
+#pragma unroll
+        for (int d = 0; d < DP / 64; ++d)
+          tma_load_4d_lead(to + d * (128 * 128) + row * 128, map, smem_u32(bar), 64 * d, pg_row_of(c, tile * BN + row), w.head, at_page, lead);
+      }
+      flush();
+    };
     while (ok && pa_next<RT, RW, BN>(p, &at, &w)) {
+      // tiles in front of `plain` hold no nodes; the pages of the next tile, a lane a box or a lane a row
+      const uint32_t plain = p.box ? min(static_cast<uint32_t>(w.s.len) / BN, w.t1) : 0;
       int pg[2];
       const auto lookup = [&](uint32_t tile) {
+        pg[0] = pg[1] = -1;
+        if (tile < plain) {
+          pg[0] = c.pages;  // (outside the pool)
+          if (lane < my_boxes) {
+            const int x = pa_lookup(p, w, tile * BN + 64 * half + lane * p.box);
+            pg[0] = x < 0 ? c.pages : x;
+          }
+        } else if (tile < w.t1) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) pg[i] = tile < w.t1 ? pa_lookup(p, w, tile * BN + 64 * half + 32 * i + lane) : -1;
+          for (int i = 0; i < 2; ++i) pg[i] = pa_lookup(p, w, tile * BN + 64 * half + 32 * i + lane);
+        }
       };
       lookup(w.t0);
       if (n_part > 0 && !(ok = mbar_wait_warp(&sm.q_free, (n_part - 1) & 1, stop))) break;
@@ -1498,29 +1528,41 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1) paged_attn_tc_kernel(
         }
       sent(&sm.q_full, 0);
       unsigned long long kp[2] = {0, 0}, vp[2] = {0, 0};
+      int page = 0;
       // keys one tile ahead of values
 #pragma unroll 1
       for (uint32_t tile = w.t0; ok && tile <= w.t1; ++tile) {
         const unsigned long long old[2] = {vp[0], vp[1]};
+        const int old_page = page;
         if (tile < w.t1) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const PaRow r = pa_row(p, w, tile * BN + 64 * half + 32 * i + lane, pg[i]);
-            kp[i] = reinterpret_cast<unsigned long long>(r.k);
-            vp[i] = reinterpret_cast<unsigned long long>(r.v);
-          }
-          lookup(tile + 1);
           const uint32_t s = n_k % ST;
           if (!(ok = room(&sm.k_free[s], ((n_k / ST) & 1) ^ 1))) break;
-          copy(k0 + s * TILE, kp);
-          sent(&sm.k_full[s], 0);
+          if (tile < plain) {
+            page = pg[0];
+            lookup(tile + 1);
+            fetch(&map_k, &sm.k_full[s], k0 + s * TILE, tile, page);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const PaRow r = pa_row(p, w, tile * BN + 64 * half + 32 * i + lane, pg[i]);
+              kp[i] = reinterpret_cast<unsigned long long>(r.k);
+              vp[i] = reinterpret_cast<unsigned long long>(r.v);
+            }
+            lookup(tile + 1);
+            copy(k0 + s * TILE, kp);
+            sent(&sm.k_full[s], 0);
+          }
           ++n_k;
         }
         if (tile > w.t0) {
           const uint32_t s = n_v % ST;
           if (!(ok = room(&sm.v_free[s], ((n_v / ST) & 1) ^ 1))) break;
-          copy(v0 + s * TILE, old);
-          sent(&sm.v_full[s], static_cast<int64_t>(tile) * BN > w.s.len ? v0 + s * TILE : 0u);
+          if (tile - 1 < plain) {
+            fetch(&map_v, &sm.v_full[s], v0 + s * TILE, tile - 1, old_page);
+          } else {
+            copy(v0 + s * TILE, old);
+            sent(&sm.v_full[s], static_cast<int64_t>(tile) * BN > w.s.len ? v0 + s * TILE : 0u);
+          }
           ++n_v;
         }
       }
@@ -1534,6 +1576,15 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1) paged_attn_tc_kernel(
       ++n_part;
     }
     pa_copy_wait<0>();
+    if (!ok) {  // copies in flight have to land before the CTA ends (again with a limit)
+      const long long t0 = clock64();
+      for (uint32_t i = n_k > ST ? n_k - ST : 0; i < n_k; ++i)
+        while (!mbar_test_wait(&sm.k_full[i % ST], (i / ST) & 1) && clock64() - t0 < 20000000ll) {
+        }
+      for (uint32_t i = n_v > ST ? n_v - ST : 0; i < n_v; ++i)
+        while (!mbar_test_wait(&sm.v_full[i % ST], (i / ST) & 1) && clock64() - t0 < 20000000ll) {
+        }
+    }
     if (warp == 2 && lane == 0) cut.store(p);
   } else if (warp >= 4) {
     // ------------------------------------------------------------ softmax and results: stream t, a thread a row
@@ -1824,8 +1875,13 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_join_kernel(const PaPar
 // How a call is cut: padded dim, rows and keys of a tile, CTAs.
 struct PaForm {
   int dp, rt, bn, ctas, threads, smem;
-  void (*kernel)(PaParams);
+  const void* kernel;
+  bool boxes;  // the kernel takes tensor maps of keys and values
 };
+template <typename... A>
+static const void* pa_fn(void (*kernel)(A...)) {
+  return reinterpret_cast<const void*>(kernel);
+}
 
 constexpr size_t PA_SHARED = 227 * 1024;  // what a CTA may have
 template <typename T, int DP, int RPT>
@@ -1833,7 +1889,7 @@ static PaForm pa_ffma() {
   using S = PaFfma<T, DP, RPT>;
   static_assert(sizeof(S) <= PA_SHARED, "shared memory");
   const int smem = static_cast<int>(sizeof(S));
-  return PaForm{DP, S::RT, S::BN, sm_count() * (smem <= 112 * 1024 ? 2 : 1), PA_THREADS, smem, paged_attn_ffma_kernel<T, DP, RPT>};
+  return PaForm{DP, S::RT, S::BN, sm_count() * (smem <= 112 * 1024 ? 2 : 1), PA_THREADS, smem, pa_fn(paged_attn_ffma_kernel<T, DP, RPT>), false};
 }
 template <typename T, int DP>
 static PaForm pa_form(int rows, bool words) {
@@ -1844,15 +1900,15 @@ static PaForm pa_form(int rows, bool words) {
       if constexpr (DP <= 128) {
         using C = PaTc<T, DP>;
         static_assert(C::BYTES <= PA_SHARED, "shared memory");
-        return PaForm{DP, C::RT, C::BN, sm_count(), C::THREADS, C::BYTES, paged_attn_tc_kernel<T, DP>};
+        return PaForm{DP, C::RT, C::BN, sm_count(), C::THREADS, C::BYTES, pa_fn(paged_attn_tc_kernel<T, DP>), true};
       } else {
         using W = PaWide<T, DP>;
         static_assert(sizeof(W) <= PA_SHARED, "shared memory");
-        return PaForm{DP, W::RT, W::BN, sm_count(), PA_THREADS, static_cast<int>(sizeof(W)), paged_attn_wide_kernel<T, DP>};
+        return PaForm{DP, W::RT, W::BN, sm_count(), PA_THREADS, static_cast<int>(sizeof(W)), pa_fn(paged_attn_wide_kernel<T, DP>), false};
       }
     }
   }
-  if (words) return PaForm{DP, N::RT, N::BN, sm_count() * N::CTAS, N::THREADS, static_cast<int>(sizeof(N)), paged_attn_narrow_kernel<T, DP>};
+  if (words) return PaForm{DP, N::RT, N::BN, sm_count() * N::CTAS, N::THREADS, static_cast<int>(sizeof(N)), pa_fn(paged_attn_narrow_kernel<T, DP>), false};
   return rows <= 8 ? pa_ffma<T, DP, 1>() : pa_ffma<T, DP, 4>();
 }
 template <typename T>
@@ -1870,6 +1926,24 @@ static PaForm pa_choose(const ytcuda_pages* c, int rows, int heads, bool words) 
 }
 static uint64_t pa_pieces(const PaForm& f) { return 4ull * 2 * static_cast<uint64_t>(f.ctas) * static_cast<uint64_t>(pa_piece(f.rt, f.dp)); }
 static uint64_t pa_space(const PaForm& f) { return pa_pieces(f) + 2ull * sizeof(int4) * static_cast<uint64_t>(f.ctas); }
+
+// Tensor maps of a layer's keys and values, [pages, heads, rows of a page, dims], for boxes of 64 dims and as many rows as divide a
+// page and a tile; 0 where that is no multiple of 8 (a swizzle's rows) or the strides allow no map.
+static int pa_boxes(const PgCache& c, int dtype, CUtensorMap* k, CUtensorMap* v) {
+  int rows = 128;
+  while (c.page % rows) rows /= 2;
+  if (rows < 8) return 0;
+  const CUtensorMapDataType type = dtype == YTC_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const uint64_t dims[4] = {static_cast<uint64_t>(c.dim), static_cast<uint64_t>(c.page), static_cast<uint64_t>(c.heads), static_cast<uint64_t>(c.pages)};
+  const uint32_t box[4] = {64, static_cast<uint32_t>(rows), 1, 1};
+  for (const PgPool* p : {&c.k, &c.v}) {
+    const uint64_t strides[3] = {static_cast<uint64_t>(p->row), static_cast<uint64_t>(p->head), static_cast<uint64_t>(p->page)};
+    for (const uint64_t s : strides)
+      if (s == 0 || s >= (1ull << 40)) return 0;
+    if (encode_tensor_map(p == &c.k ? k : v, type, 4, p->p, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B) != YTC_OK) return 0;
+  }
+  return rows;
+}
 
 template <typename T>
 static cudaError_t pa_join(const PaForm& f, const PaParams& p, cudaStream_t st) {
@@ -1946,10 +2020,12 @@ int ytcuda_pages_attend(const ytcuda_pages* cache, int layer, const void* q, con
     return YTC_CUDA_ERROR;
   }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(f.kernel), f.smem)) return rc;
-  f.kernel<<<f.ctas, f.threads, f.smem, st>>>(p);
+  if (const int rc = ensure_dynamic_smem(f.kernel, f.smem)) return rc;
+  CUtensorMap map_k{}, map_v{};
+  if (f.boxes) p.box = pa_boxes(p.c, cache->dtype, &map_k, &map_v);
+  void* args[] = {&p, &map_k, &map_v};
+  YTC_CUDA(cudaLaunchKernel(f.kernel, dim3(f.ctas), dim3(f.threads), args, f.smem, st));
   count_launch();
-  YTC_CUDA(cudaGetLastError());
   YTC_CUDA(cache->dtype == YTC_F32 ? pa_join<float>(f, p, st) : cache->dtype == YTC_BF16 ? pa_join<__nv_bfloat16>(f, p, st) : pa_join<__half>(f, p, st));
   count_launch();
   return YTC_OK;

@@ -28,6 +28,7 @@ struct PaParams {
   const int32_t *starts, *parents;
   int rows, groups;
   int fresh;    // k and v hold the new rows: they are read from there, and stored
+  int wide, words;  // rows in pieces of 16 bytes (else of an element), their number
   float scale;  // times log2(e)
   float* work;  // pieces of cut units
   int4* cuts;   // two words for each CTA: the unit that starts in its share and goes on behind it
@@ -267,34 +268,6 @@ __device__ __forceinline__ PaRow pa_row(const PaParams& p, const PaPart& w, uint
   }
   return r;
 }
-// The place in the pages that node n's keys and values go to; a node without one is noted.
-__device__ __forceinline__ bool pa_place(const PaParams& p, const PaPart& w, int n, char** k, char** v) {
-  const int64_t at = static_cast<int64_t>(w.s.len) + n;
-  const int pg = pg_page_of(p.c, w.slot, at);
-  if (pg < 0 || p.c.refs[pg] != 1) {
-    atomicOr(p.c.status, pg < 0 ? YTC_PAGES_INVALID : YTC_PAGES_SHARED);
-    return false;
-  }
-  const int row = pg_row_of(p.c, at);
-  *k = p.c.k.p + pg * p.c.k.page + w.head * p.c.k.head + row * p.c.k.row;
-  *v = p.c.v.p + pg * p.c.v.page + w.head * p.c.v.head + row * p.c.v.row;
-  return true;
-}
-// New rows of nodes n0 .. n1 of a slot and head go to their pages, in `words` pieces of type W each, by `nt` threads of which
-// this is number t.
-template <typename W>
-__device__ __forceinline__ void pa_store_new(const PaParams& p, const PaPart& w, int n0, int n1, int words, int t, int nt) {
-#pragma unroll 1
-  for (int i = t; i < (n1 - n0) * words; i += nt) {
-    const int n = n0 + i / words, x = i % words;
-    char *k, *v;
-    if (!pa_place(p, w, n, &k, &v)) continue;
-    const int64_t row = w.s.start + static_cast<int64_t>(n);
-    reinterpret_cast<W*>(k)[x] = reinterpret_cast<const W*>(p.k.p + row * p.k.row + w.head * p.k.head)[x];
-    reinterpret_cast<W*>(v)[x] = reinterpret_cast<const W*>(p.v.p + row * p.v.row + w.head * p.v.head)[x];
-  }
-}
-
 __device__ __forceinline__ void pa_copy16(uint32_t dst, const char* src, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
@@ -476,10 +449,6 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_ffma_kernel(const PaPar
       if (fine) pa_ffma_values<DP, RPT, BN, false>(sm.s, sm.v[cur], a, b, o);
       else pa_ffma_values<DP, RPT, BN, true>(sm.s, sm.v[cur], a, b, o);
       __syncwarp();
-    }
-    if (p.fresh && w.rtile == 0) {
-      const int64_t n0 = static_cast<int64_t>(w.t0) * BN - w.s.len, n1 = static_cast<int64_t>(w.t1) * BN - w.s.len;
-      if (n1 > 0) pa_store_new<T>(p, w, n0 < 0 ? 0 : static_cast<int>(n0), static_cast<int>(n1 < nodes ? n1 : nodes), c.dim, t, PA_THREADS);
     }
     const bool whole = w.t0 == 0 && w.t1 == w.tiles;
     float* piece = pa_piece_of<RT, DP>(p, w);
@@ -1028,10 +997,6 @@ __global__ void __launch_bounds__(PaNarrow<T, DP>::THREADS, PaNarrow<T, DP>::CTA
       __syncwarp();  // (the next copies go into the slot that has just been read)
     }
     pa_copy_wait<0>();
-    if (p.fresh && w.rtile == 0) {
-      const int64_t n0 = static_cast<int64_t>(w.t0) * BN - w.s.len, n1 = static_cast<int64_t>(w.t1) * BN - w.s.len;
-      if (n1 > 0) pa_store_new<uint4>(p, w, n0 < 0 ? 0 : static_cast<int>(n0), static_cast<int>(n1 < w.s.nodes ? n1 : w.s.nodes), words, t, S::THREADS);
-    }
     x.finish_sums();
     // the warps' sums: O of each in its own ring
     __syncwarp();
@@ -1187,10 +1152,6 @@ __global__ void __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) paged_attn_wide
       }
     }
     pa_copy_wait<0>();
-    if (p.fresh && w.rtile == 0) {
-      const int64_t n0 = static_cast<int64_t>(w.t0) * BN - w.s.len, n1 = static_cast<int64_t>(w.t1) * BN - w.s.len;
-      if (n1 > 0) pa_store_new<uint4>(p, w, n0 < 0 ? 0 : static_cast<int>(n0), static_cast<int>(n1 < w.s.nodes ? n1 : w.s.nodes), words, t, PA_THREADS);
-    }
     x.finish_sums();
     const bool whole = w.t0 == 0 && w.t1 == w.tiles;
     float* piece = pa_piece_of<RT, DP>(p, w);
@@ -1568,10 +1529,6 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1)
       }
       if (!ok) break;
       flush();
-      if (p.fresh && w.rtile == 0) {
-        const int64_t n0 = static_cast<int64_t>(w.t0) * BN - w.s.len, n1 = static_cast<int64_t>(w.t1) * BN - w.s.len;
-        if (n1 > 0) pa_store_new<uint4>(p, w, n0 < 0 ? 0 : static_cast<int>(n0), static_cast<int>(n1 < w.s.nodes ? n1 : w.s.nodes), words, 32 * half + lane, 64);
-      }
       cut.note(sm.share, w);
       ++n_part;
     }
@@ -1808,21 +1765,58 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1)
   if (warp == 1) tmem_dealloc(tmem, 512);
 }
 
-// ---------------------------------------------------------------------------------------------- joining
-// CTA (x, y): the unit that starts in share x and goes on behind it, rows y, y + gridDim.y, ... of it. The pieces of a row are
-// shared by the warps, and their sums are joined in the order of the warps.
+// ---------------------------------------------------------------------------------------------- joining, storing
+// New rows go to their pages, in `words` pieces of type W a head: warp number `warp` of `warps` takes every so manieth row and head.
+template <typename W>
+__device__ __forceinline__ void pa_store_new(const PaParams& p, int64_t warp, int64_t warps) {
+  const PgCache& c = p.c;
+  const int lane = threadIdx.x & 31, words = p.words;
+  const int64_t items = static_cast<int64_t>(p.rows) * c.heads;
+  for (int64_t i = warp; i < items; i += warps) {
+    const int row = static_cast<int>(i / c.heads), head = static_cast<int>(i - static_cast<int64_t>(row) * c.heads);
+    int slot = 0;  // slots that end at or before the row
+    for (int s0 = 0; s0 < c.slots; s0 += 32) slot += __popc(__ballot_sync(0xffffffffu, s0 + lane < c.slots && p.starts[s0 + lane + 1] <= row));
+    if (slot >= c.slots) continue;
+    bool bad = false;
+    const PaSlot s = pa_slot(p, slot, &bad);
+    const int n = row - s.start;
+    if (n < 0 || n >= s.nodes) continue;
+    const int64_t at = static_cast<int64_t>(s.len) + n;
+    const int pg = pg_page_of(c, slot, at);
+    if (pg < 0 || c.refs[pg] != 1) {
+      if (lane == 0) atomicOr(c.status, pg < 0 ? YTC_PAGES_INVALID : YTC_PAGES_SHARED);
+      continue;
+    }
+    const int r = pg_row_of(c, at);
+    const W* ks = reinterpret_cast<const W*>(p.k.p + row * p.k.row + head * p.k.head);
+    const W* vs = reinterpret_cast<const W*>(p.v.p + row * p.v.row + head * p.v.head);
+    W* kd = reinterpret_cast<W*>(c.k.p + pg * c.k.page + head * c.k.head + r * c.k.row);
+    W* vd = reinterpret_cast<W*>(c.v.p + pg * c.v.page + head * c.v.head + r * c.v.row);
+    for (int x = lane; x < 2 * words; x += 32) (x < words ? kd[x] : vd[x - words]) = x < words ? ks[x] : vs[x - words];
+  }
+}
+
+// CTA (x, y): the unit that starts in share x and goes on behind it, rows y, y + joiners, ... of it. The pieces of a row are shared by
+// the warps, and their sums are joined in the order of the warps. CTAs (x, joiners) store the call's new rows meanwhile: nothing reads
+// those places before the call is over.
 template <typename T, int DP>
-__global__ void __launch_bounds__(PA_THREADS) paged_attn_join_kernel(const PaParams p, int rt) {
+__global__ void __launch_bounds__(PA_THREADS) paged_attn_join_kernel(const PaParams p, int rt, int joiners) {
   constexpr int WARPS = PA_THREADS / 32, C4 = DP / 4, PER = (C4 + 31) / 32;
   __shared__ float sums[WARPS][DP + 1];
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, first = blockIdx.x;
+  if (static_cast<int>(blockIdx.y) == joiners) {
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * WARPS + warp, all = static_cast<int64_t>(gridDim.x) * WARPS;
+    if (p.wide) pa_store_new<uint4>(p, at, all);
+    else pa_store_new<T>(p, at, all);
+    return;
+  }
   dependent_wait();
   const int4 a = p.cuts[2 * first];
   const int last = p.cuts[2 * first + 1].x;
   const int64_t size = pa_piece(rt, DP);
   // (the unit is the last of its first share and the first of the others)
   const float* const at = p.work + 2 * static_cast<int64_t>(first) * size;
-  for (int r = blockIdx.y; r < a.x; r += gridDim.y) {
+  for (int r = blockIdx.y; r < a.x; r += joiners) {
     float m = -CUDART_INF_F;
     for (int i = lane; i <= last - first; i += 32) m = fmaxf(m, at[(2 * i + (i == 0)) * size + rt * DP + r]);
 #pragma unroll
@@ -1947,10 +1941,11 @@ static int pa_boxes(const PgCache& c, int dtype, CUtensorMap* k, CUtensorMap* v)
 
 template <typename T>
 static cudaError_t pa_join(const PaForm& f, const PaParams& p, cudaStream_t st) {
-  const dim3 grid(f.ctas, f.rt <= 32 ? 4 : f.rt / 8), block(PA_THREADS);
-  if (f.dp == 64) return pg_launch_behind(paged_attn_join_kernel<T, 64>, grid, block, 0, st, p, f.rt);
-  if (f.dp == 128) return pg_launch_behind(paged_attn_join_kernel<T, 128>, grid, block, 0, st, p, f.rt);
-  return pg_launch_behind(paged_attn_join_kernel<T, 256>, grid, block, 0, st, p, f.rt);
+  const int joiners = f.rt <= 32 ? 4 : f.rt / 8;
+  const dim3 grid(f.ctas, joiners + (p.fresh ? 1 : 0)), block(PA_THREADS);
+  if (f.dp == 64) return pg_launch_behind(paged_attn_join_kernel<T, 64>, grid, block, 0, st, p, f.rt, joiners);
+  if (f.dp == 128) return pg_launch_behind(paged_attn_join_kernel<T, 128>, grid, block, 0, st, p, f.rt, joiners);
+  return pg_launch_behind(paged_attn_join_kernel<T, 256>, grid, block, 0, st, p, f.rt, joiners);
 }
 
 }  // namespace ytk
@@ -2011,6 +2006,8 @@ int ytcuda_pages_attend(const ytcuda_pages* cache, int layer, const void* q, con
   p.parents = parents;
   p.rows = rows;
   p.fresh = k != nullptr;
+  p.wide = words;
+  p.words = words ? p.c.dim * size / 16 : p.c.dim;
   p.scale = (scale != 0.f ? scale : 1.f / sqrtf(static_cast<float>(p.c.dim))) * PA_LOG2E;
   p.work = static_cast<float*>(workspace);
   p.cuts = reinterpret_cast<int4*>(static_cast<char*>(workspace) + pa_pieces(f));

@@ -387,12 +387,26 @@ def test_bad_trees(paged):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_sharp_scores_and_scales(paged, dtype):
-    b = Both(paged, heads=2, dim=64, pages=40, slots=2, dtype=dtype)
-    b.fill([150, 77])
+@pytest.mark.parametrize("dim,groups", [(64, 2), (64, 8), (64, 30), (128, 40), (256, 8)])
+def test_sharp_scores_and_scales(paged, dtype, dim, groups):
+    b = Both(paged, heads=2, dim=dim, pages=60, slots=2, dtype=dtype, max_pages=30)
+    b.fill([300, 77])
     b.reserve([7, 2])
     for scale, sharp in ((0.0, 30.0), (1.0, 1.0), (-0.5, 1.0), (1e-6, 1.0)):
-        b.attend(0, [7, 2], 2, scale=scale, sharp=sharp)
+        b.attend(0, [7, 2], groups, scale=scale, sharp=sharp)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("page", [1, 7, 8, 16, 24, 48, 64, 100, 128, 256])
+@pytest.mark.parametrize("dim", [64, 80, 128])
+def test_many_rows_over_every_page(paged, dtype, page, dim):
+    """Whole key tiles by TMA boxes of what divides a page, or row by row; one row tile and two, in one piece and in several."""
+    b = Both(paged, layers=2, heads=2, dim=dim, page=page, pages=3300 // page + 20, slots=4, max_pages=1400 // page + 6, dtype=dtype, seed=page)
+    b.fill([700, 0, 128, 1279])
+    b.reserve([20, 40, 9, 65])
+    b.attend(1, [20, 40, 9, 65], 4)
+    b.attend(1, [20, 0, 9, 65], 4, tree=False)
+    b.same()
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -1292,7 +1292,7 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1)
     // ------------------------------------------------------------ the issuer of the matrix instructions (all lanes, one leads)
     const uint32_t lead = lane == 0 ? 1u : 0u, q0 = smem_u32(smem), k0 = q0 + S::K, v0 = q0 + S::V;
     constexpr uint32_t FORMAT = std::is_same<T, __half>::value ? 0u : 1u;
-    const uint32_t idesc_s = umma_idesc(FORMAT, 0, 0, 128, 128), idesc_o = umma_idesc(FORMAT, 0, 1, 128, DP);
+    const uint32_t idesc_s = umma_idesc(FORMAT, 0, 0, 128, 128) | (p.scale < 0.f ? 1u << 13 : 0u), idesc_o = umma_idesc(FORMAT, 0, 1, 128, DP);
     uint32_t n_k = 0, n_v = 0;                 // key and value tiles so far
     uint32_t p_odd = 0, o_odd = 0, o_any = 0;  // bit t: of stream t, whether the P tiles, the results are odd in number; any results
     const auto keys = [&](uint32_t n) { return mbar_wait_warp(&sm.k_full[n % ST], (n / ST) & 1, stop); };
@@ -1548,8 +1548,7 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1)
     const int t = (warp - 4) >> 2, in_tile = (warp & 3) * 32 + lane;
     const uint32_t lane_sel = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + 128 * t + lane_sel, to = tmem + 256 + 128 * t + lane_sel;
-    const bool pos_scale = p.scale >= 0.f;
-    const float none = pos_scale ? -CUDART_INF_F : CUDART_INF_F;  // a hidden score before the scale
+    const float scale = fabsf(p.scale);  // (a negative one: the instructions negate Q)
     uint32_t n_s = 0, n_other = 0, n_met = 0;  // score tiles of this stream and of the other one, parts with both streams over one row tile
     int16_t* const mine = sm.up[warp - 4];
     const int16_t* const up = p.parents ? mine : nullptr;
@@ -1587,30 +1586,33 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1)
         uint32_t bits[4];
         if (masked) pa_sees128(up, node, n0, bits);
         __syncwarp();
-        float top = none;
+        if (masked) {  // what is hidden is -infinity from here on
+#pragma unroll 1
+          for (int k = 0; k < BN; k += 16) {
+            const uint32_t b = (k < 64 ? k < 32 ? bits[0] : bits[1] : k < 96 ? bits[2] : bits[3]) >> (k & 16);
+            uint32_t x[16];
+            tmem_ld_32x32b_x16(ts + k, x);
+            tmem_ld_wait();
 #pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] = (b >> e) & 1 ? x[e] : __float_as_uint(-CUDART_INF_F);
+            tmem_st_32x32b_x16(ts + k, x);
+          }
+          tmem_st_wait();
+        }
+        float top = -CUDART_INF_F;
+#pragma unroll 1
         for (int h = 0; h < 2; ++h) {
           uint32_t x[64];
           tmem_ld_32x32b_x64(ts + 64 * h, x);
           tmem_ld_wait();
-          if (masked) {
+          float a[4] = {top, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
-            for (int e = 0; e < 64; ++e)
-              if (!((bits[2 * h + (e >> 5)] >> (e & 31)) & 1)) x[e] = __float_as_uint(none);
-          }
-          if (pos_scale) {
-            float a[4] = {top, none, none, none};
+          for (int e = 0; e < 64; e += 8)
 #pragma unroll
-            for (int e = 0; e < 64; e += 8)
-#pragma unroll
-              for (int k = 0; k < 4; ++k) a[k] = pa_max3(a[k], __uint_as_float(x[e + 2 * k]), __uint_as_float(x[e + 2 * k + 1]));
-            top = pa_max3(fmaxf(a[0], a[1]), a[2], a[3]);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 64; ++e) top = fminf(top, __uint_as_float(x[e]));
-          }
+            for (int k = 0; k < 4; ++k) a[k] = pa_max3(a[k], __uint_as_float(x[e + 2 * k]), __uint_as_float(x[e + 2 * k + 1]));
+          top = pa_max3(fmaxf(a[0], a[1]), a[2], a[3]);
         }
-        top = top == none ? -CUDART_INF_F : top * p.scale;
+        top *= scale;
         if (j == 0) {
           m = top;
         } else {
@@ -1633,18 +1635,13 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1)
           }
         }
         const float ref = m == -CUDART_INF_F ? 0.f : m;
-        const uint64_t s2 = pa_pair(p.scale, p.scale), r2 = pa_pair(-ref, -ref);
+        const uint64_t s2 = pa_pair(scale, scale), r2 = pa_pair(-ref, -ref);
         float l0 = 0.f, l1 = 0.f;
-#pragma unroll
+#pragma unroll 1
         for (int h = 0; h < 2; ++h) {
           uint32_t x[64], pk[32];
           tmem_ld_32x32b_x64(ts + 64 * h, x);
           tmem_ld_wait();
-          if (masked) {
-#pragma unroll
-            for (int e = 0; e < 64; ++e)
-              if (!((bits[2 * h + (e >> 5)] >> (e & 31)) & 1)) x[e] = __float_as_uint(none);
-          }
 #pragma unroll
           for (int e = 0; e < 64; e += 2) {
             float a, b;

@@ -489,9 +489,9 @@ uint64_t ytcuda_pages_scratch(const ytcuda_pages* cache);
 int ytcuda_pages_reserve(const ytcuda_pages* cache, const int32_t* counts, void* stream);
 
 /* Row starts[s] + i of k and v [rows, kv_heads, dim] (i < starts[s + 1] - starts[s], starts [slots + 1] on the device, not
- * decreasing) goes to position lens[s] + i of slot s in one layer. Strides {row, head}. lens stays. */
-int ytcuda_pages_append(const ytcuda_pages* cache, int layer, const void* k, const int64_t* k_strides, const void* v,
-                        const int64_t* v_strides, const int32_t* starts, int rows, void* stream);
+ * decreasing) goes to position lens[s] + i of slot s in one layer. strides: {row, head} of k, then of v. lens stays. */
+int ytcuda_pages_append(const ytcuda_pages* cache, int layer, const void* k, const void* v, const int64_t* strides,
+                        const int32_t* starts, int rows, void* stream);
 
 /* Attention of new rows in one layer. Rows starts[s] .. starts[s + 1] - 1 of q and o [rows, heads, dim] belong to slot s, row
  * starts[s] + i to node i at position lens[s] + i. A node sees the lens[s] positions in front of all nodes, itself, and its
@@ -499,13 +499,12 @@ int ytcuda_pages_append(const ytcuda_pages* cache, int layer, const void* k, con
  * has at most 1024 nodes). heads is a multiple of kv_heads, query head h reads key head h / (heads / kv_heads). With k and v
  * [rows, kv_heads, dim] the nodes' keys and values are stored first, as by ytcuda_pages_append (both NULL: they are in the
  * pages already). scale 0: 1 / sqrt(dim). Scores, softmax and sums in fp32; results rounded to nearest even. Rows behind
- * starts[slots] are left as they were. Strides {row, head}; dim <= 256. workspace: ytcuda_pages_attend_workspace() bytes
+ * starts[slots] are left as they were. dim <= 256; strides: {row, head} of q, of o, of k, of v. workspace: ytcuda_pages_attend_workspace() bytes
  * that no other call uses until this one has run. */
 uint64_t ytcuda_pages_attend_workspace(const ytcuda_pages* cache, int rows, int heads);
-int ytcuda_pages_attend(const ytcuda_pages* cache, int layer, const void* q, const int64_t* q_strides, const void* k,
-                        const int64_t* k_strides, const void* v, const int64_t* v_strides, void* o, const int64_t* o_strides,
-                        const int32_t* starts, const int32_t* parents, int rows, int heads, float scale, void* workspace,
-                        uint64_t workspace_bytes, void* stream);
+int ytcuda_pages_attend(const ytcuda_pages* cache, int layer, const void* q, void* o, const void* k, const void* v,
+                        const int64_t* strides, const int32_t* starts, const int32_t* parents, int rows, int heads, float scale,
+                        void* workspace, uint64_t workspace_bytes, void* stream);
 
 /* Of the rows behind position base[s] (NULL: lens[s]) the first kept[s] of accepted[s][0 .. depth - 1] stay, in every layer:
  * row base + accepted[s][j] moves to base + j, and lens[s] = base + kept[s]. accepted [slots, depth] is strictly increasing

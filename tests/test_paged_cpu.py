@@ -20,10 +20,10 @@ def cache(**change):
 
 
 def calls(c, at):
-    L, two = _lib.lib(), (C.c_int64 * 2)(128, 64)
+    L, st = _lib.lib(), (C.c_int64 * 8)(*[128, 64] * 4)
     yield L.ytcuda_pages_reserve(c, at, None)
-    yield L.ytcuda_pages_append(c, 0, at, two, at, two, at, 1, None)
-    yield L.ytcuda_pages_attend(c, 0, at, two, None, None, None, None, at + 16, two, at, None, 1, 2, 0.0, at, 1 << 40, None)
+    yield L.ytcuda_pages_append(c, 0, at, at, st, at, 1, None)
+    yield L.ytcuda_pages_attend(c, 0, at, at + 16, None, None, st, at, None, 1, 2, 0.0, at, 1 << 40, None)
     yield L.ytcuda_pages_keep(c, at, None, 0, None, None)
     yield L.ytcuda_pages_fork(c, at, None, None)
     yield L.ytcuda_pages_compact(c, c, None)
@@ -41,19 +41,19 @@ def test_bad_caches(change):
 
 
 def test_bad_arguments():
-    L, two = _lib.lib(), (C.c_int64 * 2)(128, 64)
+    L, st = _lib.lib(), (C.c_int64 * 8)(*[128, 64] * 4)
     at = (C.addressof(HERE) + 15) // 16 * 16
     c = cache()
     p = C.addressof(c)
-    attend = lambda layer=0, q=at, k=None, v=None, o=at + 16, starts=at, rows=1, heads=2, work=at, size=1 << 40: (  # noqa: E731
-        L.ytcuda_pages_attend(p, layer, q, two, k, two, v, two, o, two, starts, None, rows, heads, 0.0, work, size, None))
-    for change in (dict(layer=2), dict(layer=-1), dict(q=None), dict(k=at), dict(v=at), dict(o=None), dict(o=at), dict(starts=None),
+    attend = lambda layer=0, q=at, k=None, v=None, o=at + 16, strides=st, starts=at, rows=1, heads=2, work=at, size=1 << 40: (  # noqa: E731
+        L.ytcuda_pages_attend(p, layer, q, o, k, v, strides, starts, None, rows, heads, 0.0, work, size, None))
+    for change in (dict(layer=2), dict(layer=-1), dict(q=None), dict(k=at), dict(v=at), dict(o=None), dict(o=at), dict(starts=None), dict(strides=None),
                    dict(rows=-1), dict(heads=3), dict(heads=0), dict(work=None), dict(size=16), dict(work=at + 4), dict(q=at + 1)):
         assert attend(**change) == _lib.INVALID_ARG, change
     assert attend(rows=0) == _lib.OK
-    for rc in (L.ytcuda_pages_reserve(p, None, None), L.ytcuda_pages_append(p, 2, at, two, at, two, at, 1, None),
-               L.ytcuda_pages_append(p, 0, None, two, at, two, at, 1, None), L.ytcuda_pages_append(p, 0, at, two, at, two, None, 1, None),
-               L.ytcuda_pages_append(p, 0, at, two, at, two, at, -1, None), L.ytcuda_pages_keep(p, None, None, 0, None, None),
+    for rc in (L.ytcuda_pages_reserve(p, None, None), L.ytcuda_pages_append(p, 2, at, at, st, at, 1, None),
+               L.ytcuda_pages_append(p, 0, None, at, st, at, 1, None), L.ytcuda_pages_append(p, 0, at, at, st, None, 1, None),
+               L.ytcuda_pages_append(p, 0, at, at, None, at, 1, None), L.ytcuda_pages_append(p, 0, at, at, st, at, -1, None), L.ytcuda_pages_keep(p, None, None, 0, None, None),
                L.ytcuda_pages_keep(p, at, at, -1, None, None), L.ytcuda_pages_fork(p, at, at, None),
                L.ytcuda_pages_fork(p, None, None, None), L.ytcuda_pages_compact(p, None, None), L.ytcuda_pages_compact(p, p, None)):
         assert rc == _lib.INVALID_ARG
@@ -62,8 +62,7 @@ def test_bad_arguments():
     empty = cache(slots=0)
     assert L.ytcuda_pages_reserve(C.addressof(empty), at, None) == _lib.OK
     big = cache(dim=264)
-    assert L.ytcuda_pages_attend(C.addressof(big), 0, at, two, None, None, None, None, at + 16, two, at, None, 1, 2, 0.0, at, 1 << 40,
-                                 None) == _lib.UNSUPPORTED
+    assert L.ytcuda_pages_attend(C.addressof(big), 0, at, at + 16, None, None, st, at, None, 1, 2, 0.0, at, 1 << 40, None) == _lib.UNSUPPORTED
 
 
 def test_sizes():

@@ -84,9 +84,9 @@ SIGNATURES = {
     "ytcuda_latent_attn_fwd": (_i, [_i, _vp, _vp, _vp, _vp, _i64, _vp, _i, _i, _i64] + [_i] * 5 + [_vp, _f, _vp]),
     "ytcuda_pages_scratch": (_u64, [_vp]),
     "ytcuda_pages_reserve": (_i, [_vp, _vp, _vp]),
-    "ytcuda_pages_append": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _vp]),
+    "ytcuda_pages_append": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _i, _vp]),
     "ytcuda_pages_attend_workspace": (_u64, [_vp, _i, _i]),
-    "ytcuda_pages_attend": (_i, [_vp, _i] + [_vp] * 10 + [_i, _i, _f, _vp, _u64, _vp]),
+    "ytcuda_pages_attend": (_i, [_vp, _i] + [_vp] * 7 + [_i, _i, _f, _vp, _u64, _vp]),
     "ytcuda_pages_keep": (_i, [_vp, _vp, _vp, _i, _vp, _vp]),
     "ytcuda_pages_fork": (_i, [_vp, _vp, _vp, _vp]),
     "ytcuda_pages_compact": (_i, [_vp, _vp, _vp]),

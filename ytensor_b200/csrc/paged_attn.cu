@@ -1957,10 +1957,9 @@ uint64_t ytcuda_pages_attend_workspace(const ytcuda_pages* cache, int rows, int 
   return a > b ? a : b;
 }
 
-int ytcuda_pages_attend(const ytcuda_pages* cache, int layer, const void* q, const int64_t* q_strides, const void* k,
-                        const int64_t* k_strides, const void* v, const int64_t* v_strides, void* o, const int64_t* o_strides,
-                        const int32_t* starts, const int32_t* parents, int rows, int heads, float scale, void* workspace,
-                        uint64_t workspace_bytes, void* stream) {
+int ytcuda_pages_attend(const ytcuda_pages* cache, int layer, const void* q, void* o, const void* k, const void* v,
+                        const int64_t* strides, const int32_t* starts, const int32_t* parents, int rows, int heads, float scale,
+                        void* workspace, uint64_t workspace_bytes, void* stream) {
   const char* who = "ytcuda_pages_attend";
   PaParams p{};
   if (const int rc = pg_take(who, cache, &p.c)) return rc;
@@ -1973,15 +1972,15 @@ int ytcuda_pages_attend(const ytcuda_pages* cache, int layer, const void* q, con
   }
   YTC_REQUIRE((k != nullptr) == (v != nullptr), "%s: k and v come together", who);
   if (rows == 0 || p.c.slots == 0) return YTC_OK;
-  YTC_REQUIRE(starts != nullptr, "%s: null starts", who);
+  YTC_REQUIRE(starts && strides, "%s: null starts or strides", who);
   YTC_REQUIRE(p.c.pages > 0, "%s: a pool without pages", who);
   YTC_REQUIRE(q != o, "%s: q and o are the same memory", who);
   const int size = dtype_size(cache->dtype);
-  if (const int rc = pg_rows(who, "q", q, q_strides, size, &p.q)) return rc;
-  if (const int rc = pg_rows(who, "o", o, o_strides, size, &p.o)) return rc;
+  if (const int rc = pg_rows(who, "q", q, strides, size, &p.q)) return rc;
+  if (const int rc = pg_rows(who, "o", o, strides + 2, size, &p.o)) return rc;
   if (k) {
-    if (const int rc = pg_rows(who, "k", k, k_strides, size, &p.k)) return rc;
-    if (const int rc = pg_rows(who, "v", v, v_strides, size, &p.v)) return rc;
+    if (const int rc = pg_rows(who, "k", k, strides + 4, size, &p.k)) return rc;
+    if (const int rc = pg_rows(who, "v", v, strides + 6, size, &p.v)) return rc;
   }
   const bool words = pg_width(pg_bits(p.c.k) | pg_bits(p.c.v) | pg_bits(p.q) | pg_bits(p.o) | pg_bits(p.k) | pg_bits(p.v) |
                               static_cast<uint64_t>(p.c.dim * size)) == 16;

@@ -5,6 +5,7 @@
 // piece of at most 4 KB with eight 16-byte loads of a lane in flight before the first store. A call that counts and copies is
 // two kernels, the second launched while the first one runs (programmatic dependent launch).
 #include "pages.cuh"
+#include "ptx_sm100.cuh"
 
 namespace ytk {
 
@@ -80,17 +81,28 @@ __device__ __forceinline__ void pg_copy_rows(char* dst, int64_t dst_row, const c
 }
 
 // ---------------------------------------------------------------------------------------------- append
-// A warp stores the keys or the values of one new row. The row's slot: the last one that starts at or before it.
+// A warp stores what `run` new rows hold of one head in keys or values: in the pages that is one stretch of up to 4 KB, and the warps
+// beside it take the other heads of the same rows. A lane finds where each row goes (five reads that depend on one another), for
+// the next item while this one's words are on their way. The row's slot: the last one that starts at or before it.
 template <int BYTES>
-__global__ void __launch_bounds__(PG_WARPS * 32) pages_append_kernel(const PgCache c, const PgRows k, const PgRows v, const int32_t* starts,
-                                                                     int rows, int layer, int row_words) {
+__global__ void __launch_bounds__(PG_WARPS * 32, 4) pages_append_kernel(const PgCache c, const PgRows k, const PgRows v, const int32_t* starts,
+                                                                     int rows, int layer, PgDiv by_words, int run) {
   using W = typename PgWord<BYTES>::type;
-  const int lane = threadIdx.x & 31;
-  const int64_t warps = static_cast<int64_t>(gridDim.x) * PG_WARPS;
-  const int last = min(rows, starts[c.slots]);
-  for (int64_t item = static_cast<int64_t>(blockIdx.x) * PG_WARPS + (threadIdx.x >> 5); item < 2ll * rows; item += warps) {
-    const int row = static_cast<int>(item >> 1);
-    if (row >= last || row < starts[0]) continue;
+  const int lane = threadIdx.x & 31, warps = gridDim.x * PG_WARPS, row_words = by_words.d;
+  const int first = max(0, starts[0]), last = min(rows, starts[c.slots]);
+  const int items = (rows + run - 1) / run * 2 * c.heads;
+  const auto part = [&](int item, int* row0, int* head) {  // and whether it is of values
+    const int x = static_cast<int>(c.by_head.of(item));
+    *head = item - x * c.heads;
+    *row0 = (x >> 1) * run;
+    return (x & 1) != 0;
+  };
+  const auto find = [&](int item) -> unsigned long long {
+    int row0, head;
+    if (item >= items) return 0;
+    const PgPool& pool = part(item, &row0, &head) ? c.v : c.k;
+    const int row = row0 + lane;
+    if (lane >= run || row < first || row >= last) return 0;
     int lo = 0, hi = c.slots;  // starts[lo] <= row < starts[hi]
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -99,13 +111,37 @@ __global__ void __launch_bounds__(PG_WARPS * 32) pages_append_kernel(const PgCac
     const int64_t at = static_cast<int64_t>(c.lens[lo]) + (row - starts[lo]);
     const int pg = pg_page_of(c, lo, at);
     if (pg < 0 || c.refs[pg] != 1) {
-      if (lane == 0) pg_flag(c, pg < 0 ? YTC_PAGES_INVALID : YTC_PAGES_SHARED);
-      continue;
+      pg_flag(c, pg < 0 ? YTC_PAGES_INVALID : YTC_PAGES_SHARED);
+      return 0;
     }
-    const PgPool pool = item & 1 ? c.v : c.k;
-    const PgRows src = item & 1 ? v : k;
-    pg_copy_rows<W>(pool.p + layer * pool.layer + pg * pool.page + pg_row_of(c, at) * pool.row, pool.head, src.p + row * src.row, src.head,
-                    c.heads, row_words);
+    return reinterpret_cast<unsigned long long>(pool.p + layer * pool.layer + pg * pool.page + head * pool.head + pg_row_of(c, at) * pool.row);
+  };
+  int item = blockIdx.x * PG_WARPS + (threadIdx.x >> 5);
+  unsigned long long to = find(item);
+  for (; item < items; item += warps) {
+    int row0, head;
+    const PgRows& src = part(item, &row0, &head) ? v : k;
+    const char* const from = src.p + row0 * src.row + head * src.head;
+    unsigned long long next = 0;
+    for (int w0 = 0; w0 < run * row_words; w0 += 32 * PG_UNROLL) {  // (more than one round only where one row takes it)
+      W w[PG_UNROLL];
+      char* dst[PG_UNROLL];
+#pragma unroll
+      for (int u = 0; u < PG_UNROLL; ++u) {
+        const int i = w0 + lane + 32 * u, r = static_cast<int>(by_words.of(i)), x = i - r * row_words;
+        dst[u] = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, to, r & 31));
+        if (r >= run) dst[u] = nullptr;
+        if (dst[u]) {
+          w[u] = *reinterpret_cast<const W*>(from + r * src.row + x * static_cast<int64_t>(sizeof(W)));
+          dst[u] += x * static_cast<int64_t>(sizeof(W));
+        }
+      }
+      if (w0 == 0) next = find(item + warps);
+#pragma unroll
+      for (int u = 0; u < PG_UNROLL; ++u)
+        if (dst[u]) *reinterpret_cast<W*>(dst[u]) = w[u];
+    }
+    to = next;
   }
 }
 
@@ -131,11 +167,12 @@ __global__ void __launch_bounds__(PG_COUNT) pages_reserve_kernel(const PgCache c
       const int len = c.lens[s], held = c.held[s], count = counts[s];
       mark[s] = -1;
       if (count) {
-        const int64_t need = (static_cast<int64_t>(len) + count + c.page - 1) / c.page;
-        const int first = len / c.page;
         bool ok = count > 0 && len >= 0 && held >= 0 && held <= c.max_pages;
+        const uint32_t end = static_cast<uint32_t>(ok ? len : 0) + static_cast<uint32_t>(ok ? count : 0) - 1;  // the last new position
+        const int64_t need = !ok ? 0 : end > 0x7fffffffu ? (1ll << 31) : static_cast<int64_t>(c.by_page.of(end)) + 1;
+        const int first = static_cast<int>(c.by_page.of(ok ? len : 0));
         int copy = -1;
-        if (ok && len % c.page) {
+        if (ok && pg_row_of(c, len)) {
           const int pg = pg_page_of(c, s, len);
           ok = pg >= 0;
           if (ok && c.refs[pg] > 1) copy = pg;
@@ -193,31 +230,26 @@ __global__ void __launch_bounds__(PG_COUNT) pages_reserve_kernel(const PgCache c
     }
     return;
   }
-  for (int r = t; r < want_all; r += PG_COUNT) {
-    int lo = 0, hi = c.slots;  // base[lo] <= r < base[hi]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      (base[mid] <= r ? lo : hi) = mid;
-    }
-    const int k = r - base[lo], old = mark[lo], len = c.lens[lo], id = ids[r];
+  for (int s = t >> 5; s < c.slots; s += PG_COUNT / 32) {  // a warp a slot
+    const int from = base[s], want = base[s + 1] - from, old = mark[s], len = c.lens[s], held = c.held[s], count = counts[s];
+    if (count <= 0 || old == -2) continue;
     const bool copy = old >= 0;
-    const int i = copy && k == 0 ? len / c.page : c.held[lo] + k - copy;
-    c.table[static_cast<int64_t>(lo) * c.max_pages + i] = id;
-    c.refs[id] = 1;
-    if (copy && k == 0) {
-      const int n = atomicAdd(&n_copies, 1);
-      c.scratch[at.src + n] = old;
-      c.scratch[at.dst + n] = id;
-      c.scratch[at.rows + n] = len % c.page;
-      atomicSub(c.refs + old, 1);
+    for (int k = t & 31; k < want; k += 32) {
+      const int id = ids[from + k], i = copy && k == 0 ? static_cast<int>(c.by_page.of(len)) : held + k - copy;
+      c.table[static_cast<int64_t>(s) * c.max_pages + i] = id;
+      c.refs[id] = 1;
+      if (copy && k == 0) {
+        const int n = atomicAdd(&n_copies, 1);
+        c.scratch[at.src + n] = old;
+        c.scratch[at.dst + n] = id;
+        c.scratch[at.rows + n] = pg_row_of(c, len);
+        atomicSub(c.refs + old, 1);
+      }
     }
+    __syncwarp();
+    if ((t & 31) == 0 && want > copy) c.held[s] = held + want - copy;
   }
   __syncthreads();
-  for (int s = t; s < c.slots; s += PG_COUNT)
-    if (counts[s] > 0 && mark[s] != -2) {
-      const int need = static_cast<int>((static_cast<int64_t>(c.lens[s]) + counts[s] + c.page - 1) / c.page);
-      if (need > c.held[s]) c.held[s] = need;
-    }
   if (t == 0) c.scratch[at.copies] = n_copies;
 }
 
@@ -257,42 +289,54 @@ __device__ __forceinline__ int pg_keep_bad(const PgCache& c, int s, int64_t base
   return __reduce_or_sync(0xffffffffu, bad);
 }
 
-// A warp moves the accepted rows of one slot, layer, head and pool. Rows only move down and in ascending order, so a batch that
-// has been read before it is written never hides a row of a later batch. The CTA that finishes last writes the lengths: every
-// other one has read them by then.
+// A CTA moves the accepted rows of one slot in some of its layers, heads and pools, a warp each: where the rows lie is worked out
+// once for up to PG_MOVES of them. Rows only move down and in ascending order, so a batch that has been read before it is written
+// never hides a row of a later batch. The CTA that finishes last writes the lengths: every other one has read them by then.
+constexpr int PG_MOVES = 128;
 template <int BYTES>
-__global__ void __launch_bounds__(PG_WARPS * 32) pages_keep_kernel(const PgCache c, const int32_t* kept, const int32_t* accepted,
-                                                                   int depth, const int32_t* base, int row_words) {
+__global__ void __launch_bounds__(PG_WARPS * 32, 3) pages_keep_kernel(const PgCache c, const int32_t* kept, const int32_t* accepted,
+                                                                   int depth, const int32_t* base, PgDiv by_words) {
   using W = typename PgWord<BYTES>::type;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int per_slot = 2 * c.layers * c.heads;
-  const int64_t items = accepted ? static_cast<int64_t>(c.slots) * per_slot : 0, warps = static_cast<int64_t>(gridDim.x) * PG_WARPS;
-  for (int64_t item = static_cast<int64_t>(blockIdx.x) * PG_WARPS + warp; item < items; item += warps) {
-    const int s = static_cast<int>(item / per_slot);
-    int rest = static_cast<int>(item - static_cast<int64_t>(s) * per_slot);
-    const PgPool& pool = rest & 1 ? c.v : c.k;
-    rest >>= 1;
-    const int n = kept[s];
-    const int64_t b = base ? base[s] : c.lens[s];
-    if (n <= 0 || pg_keep_bad(c, s, b, n, accepted, depth)) continue;
-    char* const p = pool.p + rest / c.heads * pool.layer + rest % c.heads * pool.head;
-    const int batch = max(1, 32 * PG_UNROLL / row_words);  // rows that fit the lanes' registers (row_words <= 128 * PG_UNROLL)
-    for (int j0 = 0; j0 < n; j0 += batch) {
-      const int m = min(batch, n - j0) * row_words;
-      for (int w0 = 0; w0 < m; w0 += 32 * PG_UNROLL) {  // (more than one round only where one row takes it)
+  __shared__ int page[2][PG_MOVES], row[2][PG_MOVES];  // from, to
+  __shared__ PgDiv by_moves;
+  __shared__ int last;
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const int items = 2 * c.layers * c.heads, s = blockIdx.y;
+  const int n = kept[s];
+  const int64_t b = base ? base[s] : c.lens[s];
+  if (accepted && n > 0 && !pg_keep_bad(c, s, b, n, accepted, depth)) {  // (the same answer in every warp)
+    const int32_t* const mine = accepted + static_cast<int64_t>(s) * depth;
+    for (int j0 = 0; j0 < n; j0 += PG_MOVES) {
+      const int moves = min(PG_MOVES, n - j0);
+      __syncthreads();
+      for (int i = t; i < 2 * moves; i += PG_WARPS * 32) {
+        const int j = i >> 1, to = i & 1;
+        const int64_t at = b + (to ? j0 + j : mine[j0 + j]);
+        page[to][j] = pg_page_of(c, s, at);
+        row[to][j] = pg_row_of(c, at);
+      }
+      if (t == 0) by_moves = pg_div(static_cast<uint32_t>(moves));
+      __syncthreads();
+      // A warp's items in one line of words, PG_UNROLL x 32 of them in flight: rows of an item in ascending order, items in any.
+      const int stride = gridDim.x * PG_WARPS, first = blockIdx.x * PG_WARPS + warp;
+      const int row_words = by_words.d, all = first < items ? ((items - first - 1) / stride + 1) * moves * row_words : 0;
+      const PgDiv of_moves = by_moves;
+      for (int w0 = 0; w0 < all; w0 += 32 * PG_UNROLL) {
         W w[PG_UNROLL];
         char* to[PG_UNROLL];
 #pragma unroll
         for (int u = 0; u < PG_UNROLL; ++u) {
           const int i = w0 + lane + 32 * u;
           to[u] = nullptr;
-          if (i < m) {
-            const int r = i / row_words, j = j0 + r;
-            const int a = accepted[static_cast<int64_t>(s) * depth + j];
-            if (a != j) {
-              const int64_t x = b + a, y = b + j, off = (i - r * row_words) * static_cast<int64_t>(sizeof(W));
-              w[u] = *reinterpret_cast<const W*>(p + pg_page_of(c, s, x) * pool.page + pg_row_of(c, x) * pool.row + off);
-              to[u] = p + pg_page_of(c, s, y) * pool.page + pg_row_of(c, y) * pool.row + off;
+          if (i < all) {
+            const int line = static_cast<int>(by_words.of(i)), x = i - line * row_words, turn = static_cast<int>(of_moves.of(line)), j = line - turn * moves;
+            const int item = first + turn * stride, rest = item >> 1, layer = static_cast<int>(c.by_head.of(rest)), head = rest - layer * c.heads;
+            const PgPool& pool = item & 1 ? c.v : c.k;
+            const int p0 = page[0][j], p1 = page[1][j], r0 = row[0][j], r1 = row[1][j];
+            char* const p = pool.p + layer * pool.layer + head * pool.head + x * static_cast<int64_t>(sizeof(W));
+            if (p0 != p1 || r0 != r1) {
+              w[u] = *reinterpret_cast<const W*>(p + p0 * pool.page + r0 * pool.row);
+              to[u] = p + p1 * pool.page + r1 * pool.row;
             }
           }
         }
@@ -304,81 +348,80 @@ __global__ void __launch_bounds__(PG_WARPS * 32) pages_keep_kernel(const PgCache
       }
     }
   }
-  __shared__ int last;
   int32_t* const ticket = c.scratch + pg_scratch(c.slots, c.max_pages, c.pages).ticket;
   __syncthreads();
-  if (threadIdx.x == 0) {
+  if (t == 0) {
     __threadfence();
-    last = atomicAdd(ticket, 1) == static_cast<int>(gridDim.x) - 1;
+    last = atomicAdd(ticket, 1) == static_cast<int>(gridDim.x * gridDim.y) - 1;
   }
   __syncthreads();
   if (!last) return;
-  if (threadIdx.x == 0) *ticket = 0;
-  for (int s = warp; s < c.slots; s += PG_WARPS) {
-    const int n = kept[s];
-    const int64_t b = base ? base[s] : c.lens[s];
-    const int bad = pg_keep_bad(c, s, b, n, accepted, depth);
+  if (t == 0) *ticket = 0;
+  for (int x = warp; x < c.slots; x += PG_WARPS) {
+    const int m = kept[x];
+    const int64_t from = base ? base[x] : c.lens[x];
+    const int bad = pg_keep_bad(c, x, from, m, accepted, depth);
     if (lane == 0) {
       if (bad) pg_flag(c, bad);
-      else c.lens[s] = static_cast<int>(b + n);
+      else c.lens[x] = static_cast<int>(from + m);
     }
   }
 }
 
 // ---------------------------------------------------------------------------------------------- fork
-// A CTA per slot: the new row of the table goes to the scratch (another slot may still have to read the old one), the counts
-// are whole numbers and may be changed in any order.
-__global__ void __launch_bounds__(256) pages_fork_kernel(const PgCache c, const int32_t* source, const int32_t* gone) {
-  dependent_trigger();
+// One cluster of CTAs: new rows of the table go to the scratch first (another slot may still have to read the old ones) and, behind
+// the cluster's barrier, into the table; nothing else is waited for. The counts are whole numbers and may change in any order. It is
+// as long as four reads that depend on one another.
+constexpr int PG_CLUSTER = 8;
+__global__ void __cluster_dims__(PG_CLUSTER, 1, 1) __launch_bounds__(PG_COUNT) pages_fork_kernel(const PgCache c, const int32_t* source, const int32_t* gone) {
   const PgScratch at = pg_scratch(c.slots, c.max_pages, c.pages);
-  const int s = blockIdx.x, t = threadIdx.x;
-  const int from = source ? source[s] : gone[s] ? -1 : s;
-  int len = 0, held = -1;  // (-1: the slot stays as it is)
-  const int old = c.held[s];
-  if (from != s) {
-    bool ok = from >= -1 && from < c.slots && old >= 0 && old <= c.max_pages;
-    held = 0;
-    if (ok && from >= 0) {
-      len = c.lens[from];
-      held = len / c.page + (len % c.page != 0);
-      ok = len >= 0 && held <= c.held[from] && held <= c.max_pages;
+  constexpr int WARPS = PG_CLUSTER * PG_COUNT / 32;
+  const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) * PG_CLUSTER + blockIdx.x;
+  int32_t *const new_held = c.scratch + at.held, *const new_lens = c.scratch + at.lens, *const rows = c.scratch + at.table;
+  // a warp a stretch of 32 entries of a slot's row
+  const int stretches = c.max_pages ? (c.max_pages + 31) / 32 : 1;
+  const PgDiv by_stretch = pg_div(static_cast<uint32_t>(stretches));
+  const int items = c.slots * stretches;  // (fewer than the table's entries and the slots together)
+  for (int i = warp; i < items; i += WARPS) {
+    const int s = static_cast<int>(by_stretch.of(i)), x = (i - s * stretches) * 32 + lane;
+    const int from = source ? source[s] : gone[s] ? -1 : s, old = c.held[s];
+    const int64_t mine = static_cast<int64_t>(s) * c.max_pages + x;
+    int len = 0, held = -1;  // (-1: the slot stays as it is)
+    if (from != s) {
+      bool ok = from >= -1 && from < c.slots && old >= 0 && old <= c.max_pages;
+      held = 0;
+      if (ok && from >= 0) {
+        len = c.lens[from];
+        held = static_cast<int>(c.by_page.of(static_cast<uint32_t>(max(len, 0))));
+        held += held * c.page != len;
+        ok = len >= 0 && held <= c.held[from] && held <= c.max_pages;
+      }
+      if (!ok) {
+        if (lane == 0) pg_flag(c, YTC_PAGES_INVALID);
+        held = -1;
+      } else {
+        const int gives = x < old ? c.table[mine] : 0, takes = x < held ? c.table[static_cast<int64_t>(from) * c.max_pages + x] : 0;
+        if (x < held) rows[mine] = takes;
+        if (x < old && gives >= 0 && gives < c.pages) atomicSub(c.refs + gives, 1);
+        if (x < held && takes >= 0 && takes < c.pages) atomicAdd(c.refs + takes, 1);
+        if ((x < old && (gives < 0 || gives >= c.pages)) || (x < held && (takes < 0 || takes >= c.pages))) pg_flag(c, YTC_PAGES_INVALID);
+      }
     }
-    if (!ok) {
-      if (t == 0) pg_flag(c, YTC_PAGES_INVALID);
-      held = -1;
+    if (x == 0) {
+      new_held[s] = held;
+      new_lens[s] = len;
     }
   }
-  if (t == 0) {
-    c.scratch[at.held + s] = held;
-    c.scratch[at.lens + s] = len;
-  }
-  if (held < 0) return;
-  const int32_t* mine = c.table + static_cast<int64_t>(s) * c.max_pages;
-  for (int i = t; i < old; i += 256) {
-    const int pg = mine[i];
-    if (pg >= 0 && pg < c.pages) atomicSub(c.refs + pg, 1);
-    else pg_flag(c, YTC_PAGES_INVALID);
-  }
-  if (!held) return;
-  const int32_t* theirs = c.table + static_cast<int64_t>(from) * c.max_pages;
-  for (int i = t; i < held; i += 256) {
-    const int pg = theirs[i];
-    c.scratch[at.table + static_cast<int64_t>(s) * c.max_pages + i] = pg;
-    if (pg >= 0 && pg < c.pages) atomicAdd(c.refs + pg, 1);
-    else pg_flag(c, YTC_PAGES_INVALID);
-  }
-}
-__global__ void __launch_bounds__(256) pages_fork_store_kernel(const PgCache c) {
-  const PgScratch at = pg_scratch(c.slots, c.max_pages, c.pages);
-  const int s = blockIdx.x, t = threadIdx.x;
-  dependent_wait();
-  const int held = c.scratch[at.held + s];
-  if (held < 0) return;
-  const int64_t row = static_cast<int64_t>(s) * c.max_pages;
-  for (int i = t; i < held; i += 256) c.table[row + i] = c.scratch[at.table + row + i];
-  if (t == 0) {
-    c.held[s] = held;
-    c.lens[s] = c.scratch[at.lens + s];
+  cluster_sync_all();
+  for (int i = warp; i < items; i += WARPS) {
+    const int s = static_cast<int>(by_stretch.of(i)), x = (i - s * stretches) * 32 + lane;
+    const int64_t mine = static_cast<int64_t>(s) * c.max_pages + x;
+    const int held = new_held[s], takes = x < c.max_pages ? rows[mine] : 0;
+    if (x < held) c.table[mine] = takes;
+    if (x == 0 && held >= 0) {
+      c.held[s] = held;
+      c.lens[s] = new_lens[s];
+    }
   }
 }
 
@@ -491,7 +534,8 @@ int pg_take(const char* who, const ytcuda_pages* c, PgCache* out) {
     return PgPool{static_cast<char*>(p), s[0] * size, s[1] * size, s[2] * size, s[3] * size};
   };
   for (int i = 0; i < 4; ++i) YTC_REQUIRE(c->k_strides[i] >= 0 && c->v_strides[i] >= 0, "%s: negative stride in a pool", who);
-  *out = PgCache{pool(c->k, c->k_strides), pool(c->v, c->v_strides), pg_div(static_cast<uint32_t>(c->page)), c->table, c->lens, c->held, c->refs, c->status, c->scratch,
+  *out = PgCache{pool(c->k, c->k_strides), pool(c->v, c->v_strides), pg_div(static_cast<uint32_t>(c->page)),
+                 pg_div(static_cast<uint32_t>(c->kv_heads)), c->table, c->lens, c->held, c->refs, c->status, c->scratch,
                  c->layers, c->pages, c->page, c->kv_heads, c->dim, c->slots, c->max_pages};
   return YTC_OK;
 }
@@ -534,23 +578,27 @@ uint64_t ytcuda_pages_scratch(const ytcuda_pages* cache) {
   return 4ull * static_cast<uint64_t>(pg_scratch(cache->slots, cache->max_pages, cache->pages).words);
 }
 
-int ytcuda_pages_append(const ytcuda_pages* cache, int layer, const void* k, const int64_t* k_strides, const void* v,
-                        const int64_t* v_strides, const int32_t* starts, int rows, void* stream) {
+int ytcuda_pages_append(const ytcuda_pages* cache, int layer, const void* k, const void* v, const int64_t* strides,
+                        const int32_t* starts, int rows, void* stream) {
   const char* who = "ytcuda_pages_append";
   PgCache c;
   if (const int rc = pg_take(who, cache, &c)) return rc;
   YTC_REQUIRE(layer >= 0 && layer < c.layers, "%s: layer %d of %d", who, layer, c.layers);
   YTC_REQUIRE(rows >= 0, "%s: negative number of rows", who);
   if (rows == 0 || c.slots == 0) return YTC_OK;
-  YTC_REQUIRE(starts != nullptr, "%s: null starts", who);
+  YTC_REQUIRE(starts && strides, "%s: null starts or strides", who);
   YTC_REQUIRE(c.pages > 0, "%s: a pool without pages", who);
   const int size = dtype_size(cache->dtype);
   PgRows kr, vr;
-  if (const int rc = pg_rows(who, "k", k, k_strides, size, &kr)) return rc;
-  if (const int rc = pg_rows(who, "v", v, v_strides, size, &vr)) return rc;
+  if (const int rc = pg_rows(who, "k", k, strides, size, &kr)) return rc;
+  if (const int rc = pg_rows(who, "v", v, strides + 2, size, &vr)) return rc;
   const int width = pg_width(pg_bits(c.k) | pg_bits(c.v) | pg_bits(kr) | pg_bits(vr) | static_cast<uint64_t>(c.dim * size));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  PG_BY_WIDTH(width, (pages_append_kernel<B><<<copy_grid(2ll * rows), PG_WARPS * 32, 0, st>>>(c, kr, vr, starts, rows, layer, c.dim * size / B)));
+  const int words = c.dim * size / width, a_round = 32 * PG_UNROLL / words, run = a_round < 1 ? 1 : a_round > 32 ? 32 : a_round;
+  const int64_t items = (static_cast<int64_t>(rows) + run - 1) / run * 2 * c.heads;
+  const PgDiv by_words = pg_div(static_cast<uint32_t>(words));
+  YTC_REQUIRE(items < (1ll << 30), "%s: %d rows of %d heads are too many", who, rows, c.heads);
+  PG_BY_WIDTH(width, (pages_append_kernel<B><<<copy_grid(items), PG_WARPS * 32, 0, st>>>(c, kr, vr, starts, rows, layer, by_words, run)));
   count_launch();
   YTC_CUDA(cudaGetLastError());
   return YTC_OK;
@@ -587,9 +635,12 @@ int ytcuda_pages_keep(const ytcuda_pages* cache, const int32_t* kept, const int3
   if (depth == 0) accepted = nullptr;
   const int size = dtype_size(cache->dtype);
   const int width = pg_width(pg_bits(c.k) | pg_bits(c.v) | static_cast<uint64_t>(c.dim * size));
-  const unsigned grid = accepted ? copy_grid(2ll * c.slots * c.layers * c.heads) : 1u;
+  // three CTAs an SM, all that it holds, where there is that much to move: a warp's items one behind another
+  const int64_t a_slot = (2ll * c.layers * c.heads + PG_WARPS - 1) / PG_WARPS, most = (3ll * sm_count() + c.slots - 1) / c.slots;
+  const dim3 grid(accepted ? static_cast<unsigned>(a_slot < most ? a_slot : most) : 1u, static_cast<unsigned>(c.slots));
+  YTC_REQUIRE(c.slots <= 65535, "%s: %d slots (at most 65535)", who, c.slots);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  PG_BY_WIDTH(width, (pages_keep_kernel<B><<<grid, PG_WARPS * 32, 0, st>>>(c, kept, accepted, depth, base, c.dim * size / B)));
+  PG_BY_WIDTH(width, (pages_keep_kernel<B><<<grid, PG_WARPS * 32, 0, st>>>(c, kept, accepted, depth, base, pg_div(static_cast<uint32_t>(c.dim * size / B)))));
   count_launch();
   YTC_CUDA(cudaGetLastError());
   return YTC_OK;
@@ -603,11 +654,9 @@ int ytcuda_pages_fork(const ytcuda_pages* cache, const int32_t* source, const in
   YTC_REQUIRE((source != nullptr) != (gone != nullptr), "%s: source or gone, one of them", who);
   YTC_REQUIRE(c.pages > 0, "%s: a pool without pages", who);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  pages_fork_kernel<<<c.slots, 256, 0, st>>>(c, source, gone);
+  pages_fork_kernel<<<PG_CLUSTER, PG_COUNT, 0, st>>>(c, source, gone);
   count_launch();
   YTC_CUDA(cudaGetLastError());
-  YTC_CUDA(pg_launch_behind(pages_fork_store_kernel, dim3(c.slots), dim3(256), 0, st, c));
-  count_launch();
   return YTC_OK;
 }
 

@@ -22,7 +22,7 @@ struct PgDiv {
   uint32_t mul, shift, d;
   __host__ __device__ __forceinline__ uint32_t of(uint32_t n) const { return static_cast<uint32_t>((static_cast<uint64_t>(n) * mul) >> shift); }
 };
-inline PgDiv pg_div(uint32_t d) {
+__host__ __device__ inline PgDiv pg_div(uint32_t d) {
   uint32_t l = 0;
   while ((1ull << l) < d) ++l;
   return PgDiv{static_cast<uint32_t>((1ull << (31 + l)) / d + 1), 31 + l, d};
@@ -30,7 +30,7 @@ inline PgDiv pg_div(uint32_t d) {
 
 struct PgCache {
   PgPool k, v;
-  PgDiv by_page;
+  PgDiv by_page, by_head;
   int32_t *table, *lens, *held, *refs, *status, *scratch;
   int layers, pages, page, heads, dim, slots, max_pages;
 };

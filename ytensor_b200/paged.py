@@ -25,7 +25,7 @@ import torch
 
 from . import _lib
 from ._lib import check, lib
-from .api import _dt, _i64, _require_cuda, _stream
+from .api import _dt, _i64, _require_cuda
 
 FULL, INVALID, SHARED = 1, 2, 4  # bits of `status`
 _TEXT = {FULL: "too few free pages: nothing was reserved or compacted",
@@ -77,33 +77,36 @@ class PagedCache:
         self.k, self.v, self.table, self.lens, self.held, self.refs = k, v, table, lens, held, refs
         self.layers, self.pages, self.kv_heads, self.page, self.dim = k.shape
         self.slots, self.max_pages, self.dtype, self.device = slots, table.shape[1], k.dtype, k.device
+        self._index, self._per_slot, self._bounds, self._lib = k.get_device(), (slots,), (slots + 1,), lib()
+        self._space = None, 0  # (rows, heads) of the last attend() and the bytes it works in
         self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
         c = _Pages(k.data_ptr(), v.data_ptr(), tuple(k.stride()[:4]), tuple(v.stride()[:4]), table.data_ptr(), lens.data_ptr(),
                    held.data_ptr(), refs.data_ptr(), self.status.data_ptr(), None, self.layers, self.pages, self.page,
                    self.kv_heads, self.dim, self.slots, self.max_pages, _dt(k))
-        self._scratch = torch.zeros(max(4, lib().ytcuda_pages_scratch(C.addressof(c)) // 4), dtype=torch.int32, device=k.device)
+        self._scratch = torch.zeros(max(4, self._lib.ytcuda_pages_scratch(C.addressof(c)) // 4), dtype=torch.int32, device=k.device)
         c.scratch = self._scratch.data_ptr()
         self._c, self._at = c, C.addressof(c)
 
     # ------------------------------------------------------------------ checks of arguments
-    def _here(self):
-        if self.device.index != torch._C._cuda_getDevice():
+    # (What they cost is most of what a small call costs: each attribute is asked for once, and one comparison says that all is well.)
+    def _stream(self) -> int:
+        device = torch._C._cuda_getDevice()
+        if device != self._index:
             raise _bad(f"paged cache: it lies on {self.device}, which is not the current device")
+        return torch._C._cuda_getCurrentRawStream(device)
 
-    def _slots_arg(self, t, name: str, shape=None) -> int:
-        shape = (self.slots,) if shape is None else shape
-        if t.dtype is not torch.int32 or t.shape != shape or t.device != self.device or not t.is_contiguous():
+    def _ints(self, t, name: str, shape: tuple) -> int:
+        if t.dtype is not torch.int32 or t.shape != shape or t.get_device() != self._index or not t.is_contiguous():
             raise _bad(f"paged cache: {name} is a contiguous int32 tensor {list(shape)} on {self.device}")
         return t.data_ptr()
 
-    def _rows_arg(self, t, name: str, rows: int, heads: int) -> tuple:
-        if t.dtype is not self.dtype or t.shape != (rows, heads, self.dim) or t.device != self.device:
-            raise _bad(f"paged cache: {name} is {self.dtype} [{rows}, {heads}, {self.dim}] on {self.device}, "
-                       f"got {t.dtype} {list(t.shape)} on {t.device}")
+    def _rows(self, t, name: str, shape: tuple) -> tuple:
+        """Strides of rows and heads."""
         st = t.stride()
-        if st[2] != 1 and self.dim > 1:
-            raise _bad(f"paged cache: {name} needs a unit stride along dim")
-        return t.data_ptr(), _i64(st[:2])
+        if t.dtype is not self.dtype or t.shape != shape or t.get_device() != self._index or (st[2] != 1 and shape[2] > 1):
+            raise _bad(f"paged cache: {name} is {self.dtype} {list(shape)} with a unit stride along dim, on {self.device}; "
+                       f"got {t.dtype} {list(t.shape)}, strides {list(st)}, on {t.device}")
+        return st
 
     def _layer(self, layer: int) -> int:
         if not 0 <= layer < self.layers:
@@ -115,49 +118,45 @@ class PagedCache:
         """Room for counts[slot] more positions behind lens[slot] (int32 [slots]; 0: the slot stays as it is). Free pages are
         handed out in ascending order, slot by slot; where the next position falls inside a page that other slots hold too,
         the slot first gets a copy of its rows. All slots get their pages or, with FULL in `status`, none."""
-        self._here()
-        check(lib().ytcuda_pages_reserve(self._at, self._slots_arg(counts, "counts"), _stream()))
+        check(self._lib.ytcuda_pages_reserve(self._at, self._ints(counts, "counts", self._per_slot), self._stream()))
 
     def fork(self, source: torch.Tensor) -> None:
         """All slots at once: slot s becomes a copy of slot source[s] as it was before (int32 [slots]; its own number: it stays
         as it is, -1: it is emptied). The copy holds the same pages up to its length; nothing is moved."""
-        self._here()
-        check(lib().ytcuda_pages_fork(self._at, self._slots_arg(source, "source"), None, _stream()))
+        check(self._lib.ytcuda_pages_fork(self._at, self._ints(source, "source", self._per_slot), None, self._stream()))
 
     def free(self, gone: torch.Tensor) -> None:
         """Empties the slots with gone[slot] != 0 (int32 [slots]); pages that nobody else holds are free again."""
-        self._here()
-        check(lib().ytcuda_pages_fork(self._at, None, self._slots_arg(gone, "gone"), _stream()))
+        check(self._lib.ytcuda_pages_fork(self._at, None, self._ints(gone, "gone", self._per_slot), self._stream()))
 
     def keep(self, kept: torch.Tensor, accepted: torch.Tensor | None = None, *, base: torch.Tensor | None = None) -> None:
         """Of the rows behind position base[slot] (int32 [slots], default lens) the first kept[slot] of accepted [slots, depth]
         stay, in every layer: row base + accepted[slot, j] moves to base + j, and lens becomes base + kept. Numbers of
         accepted rows ascend along a row; without `accepted` the first kept[slot] rows stay where they are. The pages behind
         stay with the slot, for the next drafted rows."""
-        self._here()
         depth = accepted.shape[-1] if accepted is not None and accepted.dim() else 0
-        check(lib().ytcuda_pages_keep(self._at, self._slots_arg(kept, "kept"),
-                                      None if accepted is None else self._slots_arg(accepted, "accepted", (self.slots, depth)),
-                                      depth, None if base is None else self._slots_arg(base, "base"), _stream()))
+        check(self._lib.ytcuda_pages_keep(
+            self._at, self._ints(kept, "kept", self._per_slot),
+            None if accepted is None else self._ints(accepted, "accepted", (self.slots, depth)), depth,
+            None if base is None else self._ints(base, "base", self._per_slot), self._stream()))
 
     def compact(self, into: "PagedCache") -> None:
         """The pages in use, in ascending order, become pages 0, 1, .. of another (smaller, larger, differently laid out) cache of
         the same slots, and its table, lens, held and refs those of this one. FULL in its `status`: its pool is too small,
         nothing was written."""
-        self._here()
-        if into.device != self.device:
+        if into._index != self._index:
             raise _bad("paged cache: compact into a cache on another device")
-        check(lib().ytcuda_pages_compact(self._at, into._at, _stream()))
+        check(self._lib.ytcuda_pages_compact(self._at, into._at, self._stream()))
 
     # ------------------------------------------------------------------ one layer
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor) -> None:
         """Stores rows of new tokens: row starts[s] + i of k and v [rows, kv_heads, dim] goes to position lens[s] + i of slot s
         (starts int32 [slots + 1]). lens stays until `keep`, so that every layer of a step writes the same places."""
-        self._here()
         rows = k.shape[0] if k.dim() else 0
-        check(lib().ytcuda_pages_append(self._at, self._layer(layer), *self._rows_arg(k, "k", rows, self.kv_heads),
-                                        *self._rows_arg(v, "v", rows, self.kv_heads),
-                                        self._slots_arg(starts, "starts", (self.slots + 1,)), rows, _stream()))
+        shape = (rows, self.kv_heads, self.dim)
+        ks, vs = self._rows(k, "k", shape), self._rows(v, "v", shape)
+        check(self._lib.ytcuda_pages_append(self._at, self._layer(layer), k.data_ptr(), v.data_ptr(), _i64((*ks[:2], *vs[:2])),
+                                            self._ints(starts, "starts", self._bounds), rows, self._stream()))
 
     def attend(self, layer: int, q: torch.Tensor, starts: torch.Tensor, k: torch.Tensor | None = None,
                v: torch.Tensor | None = None, *, parents: torch.Tensor | None = None, scale: float = 0.0,
@@ -170,23 +169,32 @@ class PagedCache:
         `append`, in the same launch; without them they are in the pages already. scale 0: 1 / sqrt(dim).
 
         Scores, softmax and sums are fp32, results are rounded to nearest even. Rows behind starts[slots] are not written."""
-        self._here()
+        stream = self._stream()
         if q.dim() != 3 or q.shape[1] % self.kv_heads:
             raise _bad(f"paged cache: q is [rows, heads, dim] with heads a multiple of {self.kv_heads}, got {list(q.shape)}")
-        rows, heads = q.shape[0], q.shape[1]
-        if (k is None) != (v is None):
-            raise _bad("paged cache: k and v come together")
+        rows, heads, dim = shape = q.shape
+        if dim != self.dim:
+            raise _bad(f"paged cache: q has dim {dim}, the cache {self.dim}")
         if out is None:
-            out = torch.empty((rows, heads, self.dim), dtype=self.dtype, device=self.device)
-        new = (None,) * 4 if k is None else (*self._rows_arg(k, "k", rows, self.kv_heads), *self._rows_arg(v, "v", rows, self.kv_heads))
-        size = lib().ytcuda_pages_attend_workspace(self._at, rows, heads)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        qs, os = self._rows(q, "q", shape), self._rows(out, "out", shape)
+        if k is not None and v is not None:
+            new = (rows, self.kv_heads, dim)
+            ks, vs = self._rows(k, "k", new), self._rows(v, "v", new)
+            kp, vp, strides = k.data_ptr(), v.data_ptr(), _i64((*qs[:2], *os[:2], *ks[:2], *vs[:2]))
+        elif k is None and v is None:
+            kp, vp, strides = None, None, _i64((*qs[:2], *os[:2], 0, 0, 0, 0))
+        else:
+            raise _bad("paged cache: k and v come together")
+        if self._space[0] != (rows, heads):
+            self._space = (rows, heads), self._lib.ytcuda_pages_attend_workspace(self._at, rows, heads)
+        size = self._space[1]
         # (its own for every call: two streams, or two captured graphs, never share it)
-        space = torch.empty(size, dtype=torch.uint8, device=self.device)
-        check(lib().ytcuda_pages_attend(self._at, self._layer(layer), *self._rows_arg(q, "q", rows, heads), *new,
-                                        *self._rows_arg(out, "out", rows, heads),
-                                        self._slots_arg(starts, "starts", (self.slots + 1,)),
-                                        None if parents is None else self._slots_arg(parents, "parents", (rows,)), rows, heads,
-                                        scale, space.data_ptr(), size, _stream()))
+        space = self.status.new_empty((size + 3) // 4)
+        check(self._lib.ytcuda_pages_attend(self._at, self._layer(layer), q.data_ptr(), out.data_ptr(), kp, vp, strides,
+                                            self._ints(starts, "starts", self._bounds),
+                                            None if parents is None else self._ints(parents, "parents", (rows,)), rows, heads,
+                                            scale, space.data_ptr(), size, stream))
         return out
 
     def check(self) -> None:

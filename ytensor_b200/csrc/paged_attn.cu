@@ -895,15 +895,17 @@ struct PaWarp<float, DP> {
   }
 };
 
-// Up to 16 rows: every warp has its own keys (a quarter of each tile), its own ring, and no barrier until the part ends, where the
-// four warps' sums are joined. What bounds it is the copy of keys and values: 512 bytes a key and head at dim 128 (fp32: 1024,
+// Up to 16 rows: every warp has its own keys (16 of each tile; 8 in fp32), its own ring, and no barrier until the part ends, where the
+// warps' sums are joined. What bounds it is the copy of keys and values: 512 bytes a key and head at dim 128 (fp32: 1024,
 // and the instructions of three products).
 template <typename T, int DP>
 struct PaNarrow {
   static constexpr bool F32 = std::is_same<T, float>::value;
-  static constexpr int RT = 16, WARPS = F32 && DP <= 128 ? 8 : 4, THREADS = 32 * WARPS, CTAS = F32 || DP == 256 ? 1 : 2;
+  static constexpr int RT = 16, WARPS = !F32 || DP == 256 ? 4 : DP == 128 ? 12 : 16, THREADS = 32 * WARPS, CTAS = F32 || DP == 256 ? 1 : 2;
   static constexpr int KEYS = F32 ? 8 : 16, BN = WARPS * KEYS;
-  static constexpr int STAGES = F32 ? (DP == 64 ? 5 : DP == 128 ? 3 : 2) : DP == 64 ? 6 : 3, ROW = F32 ? DP * 4 + 16 : DP * 2, SLOT = KEYS * ROW;
+  // (fp32: as many warps as the shared memory and the registers hold; a step is a chain of instructions that wait for one another, and
+  // 12 warps with two slots are faster than 8 with three: one node behind up to 32000 keys, 4 slots: 227 -> 174 us)
+  static constexpr int STAGES = F32 ? 2 : DP == 64 ? 6 : 3, ROW = F32 ? DP * 4 + 16 : DP * 2, SLOT = KEYS * ROW;
   static constexpr int Q = F32 ? DP / 8 * 32 * 2 : DP > 128 ? 16 * DP / 8 : 1;
   uint4 ring[WARPS][STAGES][2][SLOT / 16];
   uint4 q[Q];

@@ -54,8 +54,14 @@ __device__ __forceinline__ PaSlot pa_slot(const PaParams& p, int s, bool* bad) {
   return r;
 }
 // The units of a slot are its heads' row tiles, the row tiles of a head next to one another (they read the same keys at about the same
-// time). Work is counted in blocks of RW rows by BN keys; a unit has up to RT rows, so RT / RW blocks a key tile at most. All numbers
-// stay below 2^31: the host sees to that.
+// time). Work is counted in costs of key tiles: a unit of up to RW rows costs ONE a key tile, one of two such blocks (RT = 2 RW) costs
+// BOTH, less than twice as much, since it reads the keys once. All numbers stay below 2^31: the host sees to that.
+template <int RT, int RW>
+struct PaCost {
+  static_assert(RT == RW || RT == 2 * RW, "one block of rows or two");
+  static constexpr uint32_t BLOCKS = RT / RW, ONE = BLOCKS == 1 ? 1 : 2, BOTH = BLOCKS == 1 ? 1 : 3;
+  static __device__ __forceinline__ uint32_t of(uint32_t blocks) { return BLOCKS == 1 ? blocks : blocks / 2 * BOTH + blocks % 2 * ONE; }
+};
 template <int BN>
 __device__ __forceinline__ uint32_t pa_key_tiles(const PaSlot& s) {
   return (static_cast<uint32_t>(s.len) + static_cast<uint32_t>(s.nodes) + BN - 1) / BN;
@@ -64,20 +70,20 @@ template <int RW>
 __device__ __forceinline__ uint32_t pa_row_blocks(const PaParams& p, const PaSlot& s) {
   return (static_cast<uint32_t>(s.nodes) * static_cast<uint32_t>(p.groups) + RW - 1) / RW;
 }
-template <int RW, int BN>
+template <int RT, int RW, int BN>
 __device__ __forceinline__ uint32_t pa_work(const PaParams& p, const PaSlot& s) {
-  return s.nodes ? pa_key_tiles<BN>(s) * pa_row_blocks<RW>(p, s) * p.c.heads : 0u;
+  return s.nodes ? pa_key_tiles<BN>(s) * PaCost<RT, RW>::of(pa_row_blocks<RW>(p, s)) * p.c.heads : 0u;
 }
 
-// The share of a CTA: blocks from .. to of all, the first of them block `off` of slot `slot`. Shares differ by at most one block, the
-// longer ones first: share i begins at i * each + min(i, more). No share is shorter than a key tile of a unit.
+// The share of a CTA: from .. to of all costs, the first of them number `off` of slot `slot`. Shares differ by at most one, the longer
+// ones first: share i begins at i * each + min(i, more). No share is shorter than a key tile of a unit.
 struct PaShare {
   uint32_t from, to, off, each, more;
   int slot;
 };
-__device__ __forceinline__ uint32_t pa_share_of(const PaShare& s, uint32_t block) {
+__device__ __forceinline__ uint32_t pa_share_of(const PaShare& s, uint32_t at) {
   const uint32_t longer = s.more * (s.each + 1);
-  return block < longer ? block / (s.each + 1) : s.more + (block - longer) / s.each;
+  return at < longer ? at / (s.each + 1) : s.more + (at - longer) / s.each;
 }
 // All threads of the CTA call it; one warp works it out.
 template <int RT, int RW, int BN>
@@ -87,12 +93,12 @@ __device__ __forceinline__ void pa_share(const PaParams& p, PaShare* out) {
     bool bad = false;
     uint32_t total = 0, w = 0;
     for (int s0 = 0; s0 < p.c.slots; s0 += 32) {
-      w = s0 + lane < p.c.slots ? pa_work<RW, BN>(p, pa_slot(p, s0 + lane, &bad)) : 0;
+      w = s0 + lane < p.c.slots ? pa_work<RT, RW, BN>(p, pa_slot(p, s0 + lane, &bad)) : 0;
       total += __reduce_add_sync(0xffffffffu, w);
     }
     if (blockIdx.x == 0 && __any_sync(0xffffffffu, bad) && lane == 0) atomicOr(p.c.status, YTC_PAGES_INVALID);
     PaShare r;
-    const uint32_t parts = min(gridDim.x, max(1u, total / (RT / RW)));
+    const uint32_t parts = min(gridDim.x, max(1u, total / PaCost<RT, RW>::BOTH));
     r.each = total / parts;
     r.more = total - r.each * parts;
     r.from = min(total, blockIdx.x * r.each + min(blockIdx.x, r.more));
@@ -101,7 +107,7 @@ __device__ __forceinline__ void pa_share(const PaParams& p, PaShare* out) {
     r.slot = p.c.slots;
     uint32_t before = 0;
     for (int s0 = 0; s0 < p.c.slots; s0 += 32) {
-      if (p.c.slots > 32) w = s0 + lane < p.c.slots ? pa_work<RW, BN>(p, pa_slot(p, s0 + lane, &bad)) : 0;
+      if (p.c.slots > 32) w = s0 + lane < p.c.slots ? pa_work<RT, RW, BN>(p, pa_slot(p, s0 + lane, &bad)) : 0;
       uint32_t x = w;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -122,7 +128,7 @@ __device__ __forceinline__ void pa_share(const PaParams& p, PaShare* out) {
   __syncthreads();
 }
 
-// A piece of work: key tiles t0 .. t1 of a unit that has `tiles`, `weight` blocks each, the first of them block `first` of all.
+// A piece of work: key tiles t0 .. t1 of a unit that has `tiles`, each of cost `weight`, the first of them number `first` of all costs.
 struct PaPart {
   PaSlot s;
   uint32_t tiles, t0, t1, weight, first;
@@ -134,16 +140,15 @@ struct PaAt {
   int slot;
   __device__ __forceinline__ explicit PaAt(const PaShare& s) : pos(s.from), end(s.to), off(s.off), slot(s.slot) {}
 };
-// The next piece of the share; false behind the last one. A key tile belongs to the share that its first block lies in.
+// The next piece of the share; false behind the last one. A key tile belongs to the share that its first cost lies in.
 template <int RT, int RW, int BN>
 __device__ __forceinline__ bool pa_next(const PaParams& p, PaAt* at, PaPart* out) {
-  constexpr uint32_t MOST = RT / RW;
-  static_assert(MOST == 1 || MOST == 2, "blocks a key tile");
+  using Cost = PaCost<RT, RW>;
   while (at->pos < at->end) {
     bool bad = false;
     PaPart& r = *out;
     r.s = pa_slot(p, at->slot, &bad);
-    const uint32_t work = pa_work<RW, BN>(p, r.s);
+    const uint32_t work = pa_work<RT, RW, BN>(p, r.s);
     if (at->off >= work) {  // (slots without rows too)
       at->off -= work;
       ++at->slot;
@@ -151,10 +156,10 @@ __device__ __forceinline__ bool pa_next(const PaParams& p, PaAt* at, PaPart* out
     }
     r.slot = at->slot;
     r.tiles = pa_key_tiles<BN>(r.s);
-    const uint32_t blocks = pa_row_blocks<RW>(p, r.s), a_head = r.tiles * blocks;
+    const uint32_t blocks = pa_row_blocks<RW>(p, r.s), a_head = r.tiles * Cost::of(blocks);
     const uint32_t head = at->off / a_head, in_head = at->off - head * a_head;
-    const uint32_t unit = in_head / (r.tiles * MOST), in_unit = in_head - unit * (r.tiles * MOST);
-    r.weight = min(MOST, blocks - unit * MOST);
+    const uint32_t unit = in_head / (r.tiles * Cost::BOTH), in_unit = in_head - unit * (r.tiles * Cost::BOTH);
+    r.weight = blocks - unit * Cost::BLOCKS >= Cost::BLOCKS ? Cost::BOTH : Cost::ONE;
     const uint32_t n = min(r.tiles * r.weight - in_unit, at->end - at->pos);
     r.first = at->pos - in_unit;
     r.t0 = (in_unit + r.weight - 1) / r.weight;
@@ -1795,8 +1800,8 @@ __device__ __forceinline__ void pa_store_new(const PaParams& p, int64_t warp, in
   }
 }
 
-// CTA (x, y): the unit that starts in share x and goes on behind it, rows y, y + joiners, ... of it. The pieces of a row are shared by
-// the warps, and their sums are joined in the order of the warps. CTAs (x, joiners) store the call's new rows meanwhile: nothing reads
+// CTA (x, y): the unit that starts in share x and goes on behind it, rows y, y + joiners, ... of it, or four times as many. Of many
+// pieces the warps take every fourth each, and their sums are joined in the order of the warps; few are one warp's work. CTAs (x, joiners) store the call's new rows meanwhile: nothing reads
 // those places before the call is over.
 template <typename T, int DP>
 __global__ void __launch_bounds__(PA_THREADS) paged_attn_join_kernel(const PaParams p, int rt, int joiners) {
@@ -1815,20 +1820,17 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_join_kernel(const PaPar
   const int64_t size = pa_piece(rt, DP);
   // (the unit is the last of its first share and the first of the others)
   const float* const at = p.work + 2 * static_cast<int64_t>(first) * size;
-  for (int r = blockIdx.y; r < a.x; r += joiners) {
-    float m = -CUDART_INF_F;
-    for (int i = lane; i <= last - first; i += 32) m = fmaxf(m, at[(2 * i + (i == 0)) * size + rt * DP + r]);
-#pragma unroll
-    for (int w = 16; w; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
-    float l = 0.f;
-    float4 o[PER];
+  const int pieces = last - first + 1;
+  // The sums of pieces begin, begin + step, ... of row r, relative to the row's m.
+  const auto gather = [&](int r, float m, int begin, int step, float* l, float4 (&o)[PER]) {
+    *l = 0.f;
 #pragma unroll
     for (int j = 0; j < PER; ++j) o[j] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int i = warp; i <= last - first; i += WARPS) {
+    for (int i = begin; i < pieces; i += step) {
       const float* x = at + (2 * i + (i == 0)) * size;
       const float mi = x[rt * DP + r], w = mi == -CUDART_INF_F ? 0.f : pa_exp2(mi - m);
-      l = fmaf(w, x[rt * DP + rt + r], l);
+      *l = fmaf(w, x[rt * DP + rt + r], *l);
 #pragma unroll
       for (int j = 0; j < PER; ++j)
         if (lane + 32 * j < C4) {
@@ -1839,6 +1841,35 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_join_kernel(const PaPar
           o[j].w = fmaf(w, y.w, o[j].w);
         }
     }
+  };
+  const auto most = [&](int r) {
+    float m = -CUDART_INF_F;
+    for (int i = lane; i < pieces; i += 32) m = fmaxf(m, at[(2 * i + (i == 0)) * size + rt * DP + r]);
+#pragma unroll
+    for (int w = 16; w; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
+    return m;
+  };
+  if (pieces <= 8) {  // a warp a row (the many rows of wide tiles: 148 units of 256 rows in three pieces 17 us with a CTA a row)
+    for (int r = blockIdx.y * WARPS + warp; r < a.x; r += joiners * WARPS) {
+      float l;
+      float4 o[PER];
+      gather(r, most(r), 0, 1, &l, o);
+      T* out = reinterpret_cast<T*>(pa_out(p, a.w, a.z, a.y + r));
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        const int d = 4 * (lane + 32 * j);
+        const float y[4] = {o[j].x, o[j].y, o[j].z, o[j].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (d + e < p.c.dim) pa_store(out + d + e, y[e] / l);
+      }
+    }
+    return;
+  }
+  for (int r = blockIdx.y; r < a.x; r += joiners) {
+    float l;
+    float4 o[PER];
+    gather(r, most(r), warp, WARPS, &l, o);
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < PER; ++j)
@@ -1940,7 +1971,7 @@ static int pa_boxes(const PgCache& c, int dtype, CUtensorMap* k, CUtensorMap* v)
 
 template <typename T>
 static cudaError_t pa_join(const PaForm& f, const PaParams& p, cudaStream_t st) {
-  const int joiners = f.rt <= 32 ? 4 : f.rt / 8;
+  const int joiners = f.rt <= 32 ? 4 : f.rt / 16;
   const dim3 grid(f.ctas, joiners + (p.fresh ? 1 : 0)), block(PA_THREADS);
   if (f.dp == 64) return pg_launch_behind(paged_attn_join_kernel<T, 64>, grid, block, 0, st, p, f.rt, joiners);
   if (f.dp == 128) return pg_launch_behind(paged_attn_join_kernel<T, 128>, grid, block, 0, st, p, f.rt, joiners);
@@ -1990,8 +2021,8 @@ int ytcuda_pages_attend(const ytcuda_pages* cache, int layer, const void* q, voi
   YTC_REQUIRE(workspace && workspace_bytes >= pa_space(f) && reinterpret_cast<uint64_t>(workspace) % 16 == 0,
               "%s: a workspace of %llu bytes on a 16-byte boundary is needed", who, static_cast<unsigned long long>(pa_space(f)));
   p.groups = heads / p.c.heads;
-  // the most tiles that the slots can have: row tiles of all slots, each over a full row of the table and its own nodes
-  const int64_t row_tiles = static_cast<int64_t>(rows) * p.groups / f.rt + p.c.slots;
+  // the most costs that the slots can have: row tiles of all slots, each over a full row of the table and its own nodes
+  const int64_t row_tiles = static_cast<int64_t>(rows) * p.groups / f.rt * 3 + 3ll * p.c.slots;
   const int64_t key_tiles = (static_cast<int64_t>(p.c.max_pages) * p.c.page + rows) / f.bn + 1;
   if (static_cast<double>(row_tiles) * static_cast<double>(key_tiles) * p.c.heads >= 2147483648.0) {
     set_last_error("%s: %d rows over tables of %d positions are too much work for one call", who, rows, p.c.max_pages * p.c.page);

@@ -249,30 +249,42 @@ __device__ __forceinline__ uint64_t pa_sees(const uint32_t* line, int words, int
   return low | (n0 < 0 ? bits << -n0 : bits);
 }
 
-// Where the rows of a position of a slot and head lie; nullptr where there are none. `pg`: its page, looked up before (-1: none).
+// Positions of a slot whose rows are in the pages.
+__device__ __forceinline__ uint32_t pa_paged(const PaParams& p, const PaPart& w) { return static_cast<uint32_t>(w.s.len) + (p.fresh ? 0u : static_cast<uint32_t>(w.s.nodes)); }
+// What the table says of a position, as it stands there: it is asked for ahead of its use, and a warp that looks at a number waits for
+// it. pa_checked: the page, -1 where there is none (which is noted).
+__device__ __forceinline__ int pa_lookup(const PaParams& p, const PaPart& w, uint32_t at) {
+  int pg = -1;
+  const int i = static_cast<int>(p.c.by_page.of(at));
+  if (at < pa_paged(p, w) && i < p.c.held[w.slot] && i < p.c.max_pages) pg = p.c.table[static_cast<int64_t>(w.slot) * p.c.max_pages + i];
+  return pg;
+}
+__device__ __forceinline__ int pa_checked(const PaParams& p, int pg) {
+  if (pg >= 0 && pg < p.c.pages) return pg;
+  atomicOr(p.c.status, YTC_PAGES_INVALID);
+  return -1;
+}
+// Where the rows of a position of a slot and head lie; nullptr where there are none. `pg`: what the table says of it.
 struct PaRow {
   const char *k, *v;
 };
-__device__ __forceinline__ int pa_lookup(const PaParams& p, const PaPart& w, uint32_t at) {
-  if (at >= static_cast<uint32_t>(w.s.len) + (p.fresh ? 0u : static_cast<uint32_t>(w.s.nodes))) return -1;
-  const int pg = pg_page_of(p.c, w.slot, at);
-  if (pg < 0) atomicOr(p.c.status, YTC_PAGES_INVALID);
-  return pg;
-}
 __device__ __forceinline__ PaRow pa_row(const PaParams& p, const PaPart& w, uint32_t at, int pg) {
   PaRow r{nullptr, nullptr};
   const uint32_t len = w.s.len;
-  if (pg >= 0) {
+  if (at < pa_paged(p, w)) {
+    pg = pa_checked(p, pg);
+    if (pg < 0) return r;
     const int row = pg_row_of(p.c, at);
     r.k = p.c.k.p + pg * p.c.k.page + w.head * p.c.k.head + row * p.c.k.row;
     r.v = p.c.v.p + pg * p.c.v.page + w.head * p.c.v.head + row * p.c.v.row;
-  } else if (p.fresh && at >= len && at - len < static_cast<uint32_t>(w.s.nodes)) {
+  } else if (at - len < static_cast<uint32_t>(w.s.nodes)) {
     const int64_t row = w.s.start + static_cast<int64_t>(at - len);
     r.k = p.k.p + row * p.k.row + w.head * p.k.head;
     r.v = p.v.p + row * p.v.row + w.head * p.v.head;
   }
   return r;
 }
+
 __device__ __forceinline__ void pa_copy16(uint32_t dst, const char* src, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
@@ -1248,9 +1260,69 @@ __device__ __forceinline__ void pa_sees128(const int16_t* up, int node, int n0, 
     }
 }
 
+// A CTA of this kernel runs through its code once for a short call, at the speed at which instructions come from the L2 (0.6 us for
+// 128 bytes of straight-line code were measured): what several places need is one loop or one function that is not inlined.
+__device__ __noinline__ bool pa_wait_long(uint64_t* bar, uint32_t parity, volatile int* stop) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, stop)) != 0;
+}
+__device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity, volatile int* stop) {
+  return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || pa_wait_long(bar, parity, stop);
+}
+// Half of a tile has landed: the issuer may have it. look_at: the tile holds values of nodes; one that is not finite and that not every
+// row sees must not meet a weight of zero: it is taken out here, and goes in at the end.
+template <typename T, int DP>
+__device__ __noinline__ void pa_tell(uint64_t* bar, uint32_t look_at, int half, int* odd) {
+  constexpr int WORDS = DP / 8, PER = 32 / WORDS;
+  const int lane = threadIdx.x & 31, word = lane % WORDS;
+  if (look_at) {
+    bool any = false;
+#pragma unroll 1
+    for (int i0 = 0; i0 < 64 / PER; i0 += 4) {
+      uint32_t at[4], x[4][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        at[i] = look_at + PaTc<T, DP>::at(64 * half + (i0 + i) * PER + lane / WORDS, word);
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x[i][0]), "=r"(x[i][1]), "=r"(x[i][2]), "=r"(x[i][3]) : "r"(at[i]) : "memory");
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        bool here = false;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t y = pa_finite_part<T>(x[i][k]);
+          here = here || y != x[i][k];
+          x[i][k] = y;
+        }
+        if (here) asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at[i]), "r"(x[i][0]), "r"(x[i][1]), "r"(x[i][2]), "r"(x[i][3]) : "memory");
+        any = any || here;
+      }
+    }
+    if (__any_sync(0xffffffffu, any) && lane == 0) atomicExch(odd, 1);
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) mbar_arrive(bar);
+}
+// What the values that pa_tell took out of the part's tiles add to column d of a node's row.
+template <typename T, int BN>
+__device__ __noinline__ float pa_odd_values(const PaParams& p, const PaPart& w, const int16_t* up, int node, int d) {
+  float sum = 0.f;
+  const int64_t end = static_cast<int64_t>(w.t1) * BN - w.s.len, begin = static_cast<int64_t>(w.t0) * BN - w.s.len;
+  for (int j = static_cast<int>(end <= node ? end - 1 : node); j >= 0 && j >= begin; --j) {
+    uint32_t sees[4];
+    pa_sees128(up, node, j, sees);
+    if (!(sees[0] & 1)) continue;
+    const uint32_t at = static_cast<uint32_t>(w.s.len + j);
+    const T* v = reinterpret_cast<const T*>(pa_row(p, w, at, pa_lookup(p, w, at)).v);
+    const float y = v ? pa_load(v + d) : 0.f;
+    if (!(fabsf(y) < CUDART_INF_F)) sum += y;
+  }
+  return sum;
+}
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1)
-    paged_attn_tc_kernel(const PaParams p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
+    paged_attn_tc_kernel(const __grid_constant__ PaParams p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
   using S = PaTc<T, DP>;
   constexpr int RT = S::RT, RW = S::RW, BN = S::BN, ST = S::STAGES, TILE = S::TILE, WORDS = DP / 8, PER = 32 / WORDS;
   extern __shared__ __align__(128) unsigned char raw[];
@@ -1302,7 +1374,6 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1)
     const uint32_t idesc_s = umma_idesc(FORMAT, 0, 0, 128, 128) | (p.scale < 0.f ? 1u << 13 : 0u), idesc_o = umma_idesc(FORMAT, 0, 1, 128, DP);
     uint32_t n_k = 0, n_v = 0;                 // key and value tiles so far
     uint32_t p_odd = 0, o_odd = 0, o_any = 0;  // bit t: of stream t, whether the P tiles, the results are odd in number; any results
-    const auto keys = [&](uint32_t n) { return mbar_wait_warp(&sm.k_full[n % ST], (n / ST) & 1, stop); };
     const auto issue_s = [&](int t, uint32_t qa, uint32_t stage) {
       const uint32_t ka = k0 + stage * TILE;
 #pragma unroll
@@ -1321,68 +1392,44 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1)
     };
     // P_t is there, and O_t may be written
     const auto weights = [&](int t, bool first) {
-      if (!mbar_wait_warp(&sm.p_full[t], (p_odd >> t) & 1, stop)) return false;
-      if (first && ((o_any >> t) & 1) && !mbar_wait_warp(&sm.o_free[t], ((o_odd >> t) & 1) ^ 1, stop)) return false;
+      if (!pa_wait(&sm.p_full[t], (p_odd >> t) & 1, stop)) return false;
+      if (first && ((o_any >> t) & 1) && !pa_wait(&sm.o_free[t], ((o_odd >> t) & 1) ^ 1, stop)) return false;
       p_odd ^= 1u << t;
       tc_fence_after();
       return true;
     };
     while (ok && pa_next<RT, RW, BN>(p, &at, &w)) {
-      const int n = w.t1 - w.t0;
-      if (!(ok = mbar_wait_warp(&sm.q_full, n_part & 1, stop) && keys(n_k))) break;
-      tc_fence_after();
-      if (w.rows > 128) {  // two row tiles, S of the next key tile behind O of this one (it overwrites P)
-        issue_s(0, q0, n_k % ST);
-        issue_s(1, q0 + TILE, n_k % ST);
-        tc_commit_lead(smem_u32(&sm.k_free[n_k % ST]), lead);
-        ++n_k;
-        for (int j = 0; ok && j < n; ++j, ++n_v) {
-          if (j + 1 == n) tc_commit_lead(smem_u32(&sm.q_free), lead);
+      // Blocks in the order of the streams 0, 1, 0, 1, ...: two row tiles of a key tile, or one row tile of two key tiles. Behind O of
+      // a block comes S of the stream's next one, which overwrites P. `last`: the block is the last one of its key tile.
+      const bool pair = w.rows > 128;
+      const int n = static_cast<int>(w.t1 - w.t0) << (pair ? 1 : 0);
+      if (!(ok = pa_wait(&sm.q_full, n_part & 1, stop))) break;
+      for (int i = -2; i < n; ++i) {
+        const int t = i & 1;
+        const bool first = !pair || t == 0, last = !pair || t == 1;
+        if (i >= 0) {
           const uint32_t s = n_v % ST;
-          ok = mbar_wait_warp(&sm.v_full[s], (n_v / ST) & 1, stop);
-          for (int t = 0; ok && t < 2; ++t) {
-            if (!(ok = weights(t, j == 0))) break;
-            issue_o(t, s, j > 0);
-            if (j + 1 < n) {
-              if (t == 0 && !(ok = keys(n_k))) break;
-              tc_fence_after();
-              issue_s(t, q0 + t * TILE, n_k % ST);
-            }
+          if (first && !(ok = pa_wait(&sm.v_full[s], (n_v / ST) & 1, stop))) break;
+          if (!(ok = weights(t, i < 2))) break;
+          issue_o(t, s, i > 1);
+          if (last) {
+            tc_commit_lead(smem_u32(&sm.v_free[s]), lead);
+            ++n_v;
           }
-          if (!ok) break;
-          tc_commit_lead(smem_u32(&sm.v_free[s]), lead);
-          if (j + 1 < n) {
-            tc_commit_lead(smem_u32(&sm.k_free[n_k % ST]), lead);
+        }
+        if (i + 2 < n) {
+          const uint32_t s = n_k % ST;
+          if (first && !(ok = pa_wait(&sm.k_full[s], (n_k / ST) & 1, stop))) break;
+          tc_fence_after();
+          issue_s(t, q0 + (pair ? t * TILE : 0), s);
+          if (last) {
+            tc_commit_lead(smem_u32(&sm.k_free[s]), lead);
             ++n_k;
           }
-        }
-      } else {  // one row tile: stream t has the key tiles t, t + 2, ...
-        const auto start = [&](int t) {
-          issue_s(t, q0, n_k % ST);
-          tc_commit_lead(smem_u32(&sm.k_free[n_k % ST]), lead);
-          ++n_k;
-        };
-        start(0);
-        if (n > 1) {
-          if (!(ok = keys(n_k))) break;
-          tc_fence_after();
-          start(1);
-        }
-        for (int j = 0; ok && j < n; ++j, ++n_v) {
-          if (j + 2 >= n && (j + 2 == n || n == 1)) tc_commit_lead(smem_u32(&sm.q_free), lead);  // (all of S has been issued)
-          const uint32_t s = n_v % ST;
-          const int t = j & 1;
-          if (!(ok = mbar_wait_warp(&sm.v_full[s], (n_v / ST) & 1, stop) && weights(t, j < 2))) break;
-          issue_o(t, s, j > 1);
-          tc_commit_lead(smem_u32(&sm.v_free[s]), lead);
-          if (j + 2 < n) {
-            if (!(ok = keys(n_k))) break;
-            tc_fence_after();
-            start(t);
-          }
+          if (i + 3 == n) tc_commit_lead(smem_u32(&sm.q_free), lead);
         }
       }
-      const uint32_t wrote = w.rows > 128 || n > 1 ? 3u : 1u;
+      const uint32_t wrote = n > 1 ? 3u : 1u;
       o_odd ^= wrote;
       o_any |= wrote;
       ++n_part;
@@ -1393,146 +1440,111 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1)
     const uint32_t q0 = smem_u32(smem), k0 = q0 + S::K, v0 = q0 + S::V;
     uint32_t n_k = 0, n_v = 0;
     PaCut cut;
+    const uint32_t lead = lane == 0 ? 1u : 0u;
     // A group of copies is told to the issuer when the next one is on its way, or before a wait.
     uint64_t* told = nullptr;
     uint32_t look_at = 0;  // (values of a tile with nodes)
-    const auto tell = [&]() {
-      if (look_at) {  // a value that is not finite and that not every row sees must not meet a weight of zero: it goes in at the end
-        bool odd = false;
-#pragma unroll 1
-        for (int i = 0; i < 64 / PER; ++i) {
-          const uint32_t a = look_at + S::at(64 * half + i * PER + lane / WORDS, word);
-          uint32_t x[4];
-          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(a) : "memory");
-          bool here = false;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t y = pa_finite_part<T>(x[k]);
-            here = here || y != x[k];
-            x[k] = y;
-          }
-          if (here) asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
-          odd = odd || here;
-        }
-        if (__any_sync(0xffffffffu, odd) && lane == 0) atomicExch(&sm.odd, 1);
-        look_at = 0;
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(told);
-      told = nullptr;
-    };
-    const auto sent = [&](uint64_t* bar, uint32_t look) {
-      pa_copy_commit();
-      if (told) {
-        pa_copy_wait<1>();
-        tell();
-      }
-      told = bar;
-      look_at = look;
-    };
     const auto flush = [&]() {
       if (told) {
         pa_copy_wait<0>();
-        tell();
+        pa_tell<T, DP>(told, look_at, half, &sm.odd);
+        told = nullptr;
       }
     };
-    const auto room = [&](uint64_t* bar, uint32_t parity) {
-      if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-      flush();
-      return mbar_wait_warp(bar, parity, stop);
-    };
-    // 64 rows of a tile whose places two lanes' registers hold
-    const auto copy = [&](uint32_t to, const unsigned long long (&from)[2]) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll 4
-        for (int i = 0; i < 32 / PER; ++i) {
-          const int r = i * PER + lane / WORDS;
-          const unsigned long long a = __shfl_sync(0xffffffffu, from[h], r);
-          const bool there = a != 0 && word < words;
-          pa_copy16(to + S::at(64 * half + 32 * h + r, word), there ? reinterpret_cast<const char*>(a) + word * 16 : c.k.p, there);
-        }
-    };
-    // Half of a tile by TMA: the pages of its boxes are in lanes 0, 1, ... of `page`.
-    const uint32_t lead = lane == 0 ? 1u : 0u;
-    const int boxes = p.box ? 64 / p.box : 0;  // (of one of the two warps; 0 where a box is a whole tile, which one warp fetches)
-    const int my_boxes = p.box == 128 ? 1 - half : boxes;
-    const auto fetch = [&](const CUtensorMap* map, uint64_t* bar, uint32_t to, uint32_t tile, int page) {
-      mbar_expect_tx_lead(smem_u32(bar), static_cast<uint32_t>(my_boxes * p.box) * (DP / 64) * 128, lead);
-      for (int i = 0; i < my_boxes; ++i) {
-        const int row = 64 * half + i * p.box, at_page = __shfl_sync(0xffffffffu, page, i);
-#pragma unroll
-        for (int d = 0; d < DP / 64; ++d)
-          tma_load_4d_lead(to + d * (128 * 128) + row * 128, map, smem_u32(bar), 64 * d, pg_row_of(c, tile * BN + row), w.head, at_page, lead);
-      }
-      flush();
-    };
+    const int my_boxes = p.box == 128 ? 1 - half : p.box ? 64 / p.box : 0;  // (a box that is a whole tile is fetched by one warp)
     while (ok && pa_next<RT, RW, BN>(p, &at, &w)) {
-      // tiles in front of `plain` hold no nodes; the pages of the next tile, a lane a box or a lane a row
+      // tiles in front of `plain` hold no nodes; pages of a tile, a lane a box or a lane two rows
       const uint32_t plain = p.box ? min(static_cast<uint32_t>(w.s.len) / BN, w.t1) : 0;
-      int pg[2];
-      const auto lookup = [&](uint32_t tile) {
-        pg[0] = pg[1] = -1;
-        if (tile < plain) {
-          pg[0] = c.pages;  // (outside the pool)
-          if (lane < my_boxes) {
-            const int x = pa_lookup(p, w, tile * BN + 64 * half + lane * p.box);
-            pg[0] = x < 0 ? c.pages : x;
-          }
-        } else if (tile < w.t1) {
+      const auto lookup = [&](uint32_t tile, int (&pg)[2]) {
+        const bool boxes = tile < plain;
+        const uint32_t x = tile * BN + 64 * half + lane * (boxes ? p.box : 1);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) pg[i] = pa_lookup(p, w, tile * BN + 64 * half + 32 * i + lane);
-        }
+        for (int i = 0; i < 2; ++i) pg[i] = tile < w.t1 && (!boxes || (i == 0 && lane < my_boxes)) ? pa_lookup(p, w, x + 32 * i) : -1;
       };
-      lookup(w.t0);
-      if (n_part > 0 && !(ok = mbar_wait_warp(&sm.q_free, (n_part - 1) & 1, stop))) break;
-      for (int t = 0; t < (w.rows > 128 ? 2 : 1); ++t)
-#pragma unroll 4
-        for (int i = 0; i < 64 / PER; ++i) {
-          const int r = 64 * half + i * PER + lane / WORDS, row = w.row0 + 128 * t + r;
-          const bool there = row < w.rows_all && word < words;
-          pa_copy16(q0 + t * TILE + S::at(r, word), there ? pa_query(p, w, row) + word * 16 : p.q.p, there);
-        }
-      sent(&sm.q_full, 0);
-      unsigned long long kp[2] = {0, 0}, vp[2] = {0, 0};
-      int page = 0;
-      // keys one tile ahead of values
+      const int n = w.t1 - w.t0, q_tiles = w.rows > 128 ? 2 : 1;
+      int pages[2], pages_before[2] = {-1, -1}, pages_next[2] = {-1, -1};  // of key tile i, of the one before, of the next
+      lookup(w.t0, pages);
+      if (n_part > 0 && !(ok = pa_wait(&sm.q_free, (n_part - 1) & 1, stop))) break;
+      // Q, then in round i keys of tile i and values of tile i - 1
 #pragma unroll 1
-      for (uint32_t tile = w.t0; ok && tile <= w.t1; ++tile) {
-        const unsigned long long old[2] = {vp[0], vp[1]};
-        const int old_page = page;
-        if (tile < w.t1) {
-          const uint32_t s = n_k % ST;
-          if (!(ok = room(&sm.k_free[s], ((n_k / ST) & 1) ^ 1))) break;
-          if (tile < plain) {
-            page = pg[0];
-            lookup(tile + 1);
-            fetch(&map_k, &sm.k_full[s], k0 + s * TILE, tile, page);
-          } else {
+      for (int z = -q_tiles; z < 2 * n + 2; ++z) {
+        const bool v = z >= 0 && (z & 1);
+        const int i = z >> 1, mine = v ? i - 1 : i;
+        const uint32_t tile = w.t0 + mine;
+        uint64_t* full = nullptr;
+        uint32_t to, look = 0;
+        unsigned long long from[2];
+        if (z < 0) {
+          const int qt = z + q_tiles;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const PaRow r = pa_row(p, w, tile * BN + 64 * half + 32 * i + lane, pg[i]);
-              kp[i] = reinterpret_cast<unsigned long long>(r.k);
-              vp[i] = reinterpret_cast<unsigned long long>(r.v);
+          for (int x = 0; x < 2; ++x) {
+            const int row = w.row0 + 128 * qt + 64 * half + 32 * x + lane;
+            from[x] = row < w.rows_all ? reinterpret_cast<unsigned long long>(pa_query(p, w, row)) : 0;
+          }
+          to = q0 + qt * TILE;
+          if (z == -1) full = &sm.q_full;
+        } else {
+          if (mine < 0 || mine >= n) {
+            if (v) {
+              pages_before[0] = pages[0], pages_before[1] = pages[1];
+              pages[0] = pages_next[0], pages[1] = pages_next[1];
             }
-            lookup(tile + 1);
-            copy(k0 + s * TILE, kp);
-            sent(&sm.k_full[s], 0);
+            continue;
           }
-          ++n_k;
-        }
-        if (tile > w.t0) {
-          const uint32_t s = n_v % ST;
-          if (!(ok = room(&sm.v_free[s], ((n_v / ST) & 1) ^ 1))) break;
-          if (tile - 1 < plain) {
-            fetch(&map_v, &sm.v_full[s], v0 + s * TILE, tile - 1, old_page);
-          } else {
-            copy(v0 + s * TILE, old);
-            sent(&sm.v_full[s], static_cast<int64_t>(tile) * BN > w.s.len ? v0 + s * TILE : 0u);
+          const uint32_t m = v ? n_v : n_k, s = m % ST;
+          uint64_t* const free = v ? &sm.v_free[s] : &sm.k_free[s];
+          full = v ? &sm.v_full[s] : &sm.k_full[s];
+          to = (v ? v0 : k0) + s * TILE;
+          const int pg[2] = {v ? pages_before[0] : pages[0], v ? pages_before[1] : pages[1]};
+          if (!v) lookup(tile + 1, pages_next);
+          if (!__all_sync(0xffffffffu, mbar_try_wait(free, ((m / ST) & 1) ^ 1))) {
+            flush();
+            if (!(ok = pa_wait(free, ((m / ST) & 1) ^ 1, stop))) break;
           }
-          ++n_v;
+          (v ? n_v : n_k) = m + 1;
+          if (v) {
+            pages_before[0] = pages[0], pages_before[1] = pages[1];
+            pages[0] = pages_next[0], pages[1] = pages_next[1];
+          }
+          if (tile < plain) {
+            const CUtensorMap* const map = v ? &map_v : &map_k;
+            mbar_expect_tx_lead(smem_u32(full), static_cast<uint32_t>(my_boxes * p.box) * (DP / 64) * 128, lead);
+            int mine_page = c.pages;  // (a page outside the pool reads zeros)
+            if (lane < my_boxes && (mine_page = pa_checked(p, pg[0])) < 0) mine_page = c.pages;
+            for (int x = 0; x < my_boxes; ++x) {
+              const int row = 64 * half + x * p.box, page = __shfl_sync(0xffffffffu, mine_page, x);
+#pragma unroll
+              for (int d = 0; d < DP / 64; ++d)
+                tma_load_4d_lead(to + d * (128 * 128) + row * 128, map, smem_u32(full), 64 * d, pg_row_of(c, tile * BN + row), w.head,
+                                 page, lead);
+            }
+            flush();
+            continue;
+          }
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const PaRow r = pa_row(p, w, tile * BN + 64 * half + 32 * x + lane, pg[x]);
+            from[x] = reinterpret_cast<unsigned long long>(v ? r.v : r.k);
+          }
+          if (v && static_cast<int64_t>(tile + 1) * BN > w.s.len) look = to;
         }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll 4
+          for (int x = 0; x < 32 / PER; ++x) {
+            const int r = x * PER + lane / WORDS;
+            const unsigned long long a = __shfl_sync(0xffffffffu, from[h], r);
+            const bool there = a != 0 && word < words;
+            pa_copy16(to + S::at(64 * half + 32 * h + r, word), there ? reinterpret_cast<const char*>(a) + word * 16 : c.k.p, there);
+          }
+        if (!full) continue;  // (the second half of Q goes along)
+        pa_copy_commit();
+        if (told) {
+          pa_copy_wait<1>();
+          pa_tell<T, DP>(told, look_at, half, &sm.odd);
+        }
+        told = full;
+        look_at = look;
       }
       if (!ok) break;
       flush();
@@ -1581,7 +1593,7 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1)
       const bool idle = r - lane >= w.rows;  // no row of the warp is one: nobody reads its P
       float m = -CUDART_INF_F, l = 0.f;
       for (int j = 0; j < n; ++j, ++n_s) {
-        if (!(ok = mbar_wait_warp(&sm.s_full[t], n_s & 1, stop))) break;
+        if (!(ok = pa_wait(&sm.s_full[t], n_s & 1, stop))) break;
         if (idle) {
           __syncwarp();
           if (lane == 0) mbar_arrive(&sm.p_full[t]);
@@ -1625,7 +1637,7 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1)
         } else {
           const bool moves = top > m + PA_SLACK || (m == -CUDART_INF_F && top > m);
           if (__any_sync(0xffffffffu, moves)) {  // O *= 2^(m - top): the product before has to be there
-            if (!(ok = mbar_wait_warp(&sm.o_ready[t], (n_s - 1) & 1, stop))) break;
+            if (!(ok = pa_wait(&sm.o_ready[t], (n_s - 1) & 1, stop))) break;
             tc_fence_after();
             const float shrink = moves ? pa_exp2(m - top) : 1.f;
 #pragma unroll 1
@@ -1678,7 +1690,7 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1)
         sm.l[turn][t][in_tile] = l;
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.met);
-        if (!(ok = mbar_wait_warp(&sm.met, n_met & 1, stop))) break;
+        if (!(ok = pa_wait(&sm.met, n_met & 1, stop))) break;
         ++n_met;
         const float m0 = sm.m[turn][0][in_tile], m1 = sm.m[turn][1][in_tile];
         m = fmaxf(m0, m1);
@@ -1689,11 +1701,11 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1)
         d1 = d0 + DP / 2;
         const int n1 = static_cast<int>(all / 2), n2 = static_cast<int>(all) - n1;  // key tiles of stream 1, of stream 0
         n_other += t ? n2 : n1;
-        if ((t ? n2 : n1) > 0 && !(ok = mbar_wait_warp(&sm.o_ready[1 - t], (n_other - 1) & 1, stop))) break;
+        if ((t ? n2 : n1) > 0 && !(ok = pa_wait(&sm.o_ready[1 - t], (n_other - 1) & 1, stop))) break;
       } else if (w.rows > 128) {
         n_other += all;
       }
-      if (n > 0 && !(ok = mbar_wait_warp(&sm.o_ready[t], (n_s - 1) & 1, stop))) break;
+      if (n > 0 && !(ok = pa_wait(&sm.o_ready[t], (n_s - 1) & 1, stop))) break;
       tc_fence_after();
       const bool whole = w.t0 == 0 && w.t1 == w.tiles, here = r < w.rows, both = split && all > 1;
       const bool odd = nodes_here && *reinterpret_cast<volatile int*>(&sm.odd);
@@ -1715,20 +1727,10 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1)
 #pragma unroll
             for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(weight[0] * __uint_as_float(x[e]) + weight[1] * __uint_as_float(y[e]));
           }
-          if (odd && here) {  // the values that were left out, of the nodes of this part that the row sees
-            for (int j = min(node, static_cast<int>(static_cast<int64_t>(w.t1) * BN - w.s.len) - 1); j >= 0 && static_cast<int64_t>(j) + w.s.len >= static_cast<int64_t>(w.t0) * BN; --j) {
-              uint32_t sees[4];
-              pa_sees128(up, node, j, sees);
-              if (!(sees[0] & 1)) continue;
-              const uint32_t pl = static_cast<uint32_t>(w.s.len + j);
-              const T* v = reinterpret_cast<const T*>(pa_row(p, w, pl, pa_lookup(p, w, pl)).v);
+          if (odd && here) {
 #pragma unroll
-              for (int e = 0; e < 16; ++e)
-                if (v && d + e < c.dim) {
-                  const float y = pa_load(v + d + e);
-                  if (!(fabsf(y) < CUDART_INF_F)) x[e] = __float_as_uint(__uint_as_float(x[e]) + y);
-                }
-            }
+            for (int e = 0; e < 16; ++e)
+              if (d + e < c.dim) x[e] = __float_as_uint(__uint_as_float(x[e]) + pa_odd_values<T, BN>(p, w, up, node, d + e));
           }
           if (here && whole) {
 #pragma unroll

@@ -253,22 +253,25 @@ __global__ void __launch_bounds__(PG_COUNT) pages_reserve_kernel(const PgCache c
   if (t == 0) c.scratch[at.copies] = n_copies;
 }
 
-// A warp copies the rows of one head, layer and pool of a page.
+// A warp copies up to 4 KB of the rows of one head, layer and pool of a page.
 template <int BYTES>
 __global__ void __launch_bounds__(PG_WARPS * 32) pages_copy_kernel(const PgCache c, int row_words) {
   using W = typename PgWord<BYTES>::type;
   const PgScratch at = pg_scratch(c.slots, c.max_pages, c.pages);
   dependent_wait();
-  const int64_t per_copy = 2ll * c.layers * c.heads;
+  const int rows_a_piece = max(1, 32 * PG_UNROLL / row_words), pieces = (c.page + rows_a_piece - 1) / rows_a_piece;
+  const int64_t per_copy = 2ll * c.layers * c.heads * pieces;
   const int64_t items = c.scratch[at.copies] * per_copy, warps = static_cast<int64_t>(gridDim.x) * PG_WARPS;
   for (int64_t item = static_cast<int64_t>(blockIdx.x) * PG_WARPS + (threadIdx.x >> 5); item < items; item += warps) {
     const int n = static_cast<int>(item / per_copy);
     int rest = static_cast<int>(item - n * per_copy);
+    const int first = rest % pieces * rows_a_piece, rows = min(rows_a_piece, c.scratch[at.rows + n] - first);
+    if (rows <= 0) continue;
+    rest /= pieces;
     const PgPool& pool = rest & 1 ? c.v : c.k;
     rest >>= 1;
-    char* const p = pool.p + rest / c.heads * pool.layer + rest % c.heads * pool.head;
-    pg_copy_rows<W>(p + c.scratch[at.dst + n] * pool.page, pool.row, p + c.scratch[at.src + n] * pool.page, pool.row,
-                    c.scratch[at.rows + n], row_words);
+    char* const p = pool.p + rest / c.heads * pool.layer + rest % c.heads * pool.head + first * pool.row;
+    pg_copy_rows<W>(p + c.scratch[at.dst + n] * pool.page, pool.row, p + c.scratch[at.src + n] * pool.page, pool.row, rows, row_words);
   }
 }
 
@@ -302,9 +305,12 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 3) pages_keep_kernel(const PgCa
   __shared__ int last;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int items = 2 * c.layers * c.heads, s = blockIdx.y;
+  const PgScratch at = pg_scratch(c.slots, c.max_pages, c.pages);
   const int n = kept[s];
   const int64_t b = base ? base[s] : c.lens[s];
-  if (accepted && n > 0 && !pg_keep_bad(c, s, b, n, accepted, depth)) {  // (the same answer in every warp)
+  const int bad = pg_keep_bad(c, s, b, n, accepted, depth);  // (the same in every warp)
+  if (blockIdx.x == 0 && t == 0) c.scratch[at.mark + s] = bad;
+  if (accepted && n > 0 && !bad) {
     const int32_t* const mine = accepted + static_cast<int64_t>(s) * depth;
     for (int j0 = 0; j0 < n; j0 += PG_MOVES) {
       const int moves = min(PG_MOVES, n - j0);
@@ -348,23 +354,20 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 3) pages_keep_kernel(const PgCa
       }
     }
   }
-  int32_t* const ticket = c.scratch + pg_scratch(c.slots, c.max_pages, c.pages).ticket;
+  int32_t* const ticket = c.scratch + at.ticket;
   __syncthreads();
   if (t == 0) {
     __threadfence();
     last = atomicAdd(ticket, 1) == static_cast<int>(gridDim.x * gridDim.y) - 1;
+    __threadfence();
   }
   __syncthreads();
   if (!last) return;
   if (t == 0) *ticket = 0;
-  for (int x = warp; x < c.slots; x += PG_WARPS) {
-    const int m = kept[x];
-    const int64_t from = base ? base[x] : c.lens[x];
-    const int bad = pg_keep_bad(c, x, from, m, accepted, depth);
-    if (lane == 0) {
-      if (bad) pg_flag(c, bad);
-      else c.lens[x] = static_cast<int>(from + m);
-    }
+  for (int x = t; x < c.slots; x += PG_WARPS * 32) {
+    const int wrong = __ldcg(c.scratch + at.mark + x);
+    if (wrong) pg_flag(c, wrong);
+    else c.lens[x] = static_cast<int>((base ? base[x] : c.lens[x]) + static_cast<int64_t>(kept[x]));
   }
 }
 
@@ -617,7 +620,8 @@ int ytcuda_pages_reserve(const ytcuda_pages* cache, const int32_t* counts, void*
   pages_reserve_kernel<<<1, PG_COUNT, 0, st>>>(c, counts);
   count_launch();
   YTC_CUDA(cudaGetLastError());
-  const unsigned grid = copy_grid(2ll * c.slots * c.layers * c.heads);
+  const int rows_a_piece = 32 * PG_UNROLL * width / (c.dim * size);
+  const unsigned grid = copy_grid(2ll * c.slots * c.layers * c.heads * (rows_a_piece > 1 ? (c.page + rows_a_piece - 1) / rows_a_piece : c.page));
   PG_BY_WIDTH(width, YTC_CUDA(pg_launch_behind(pages_copy_kernel<B>, dim3(grid), dim3(PG_WARPS * 32), 0, st, c, c.dim * size / B)));
   count_launch();
   return YTC_OK;

@@ -278,6 +278,21 @@ def test_pages_that_do_not_exist(paged):
     assert torch.equal(torch.nan_to_num(b.d.k), torch.nan_to_num(k))
 
 
+@pytest.mark.parametrize("dtype,groups", [(F32, 2), (BF16, 2), (BF16, 40), (F16, 40)])
+def test_attention_reads_zeros_where_a_page_does_not_exist(paged, dtype, groups):
+    b = Both(paged, layers=1, heads=1, dim=64, page=16, pages=40, slots=1, max_pages=40, dtype=dtype)
+    b.fill([400])
+    b.reserve([3])
+    for i, pg in ((3, 40), (9, -2), (17, 1 << 30)):
+        b.p.k[:, b.p.table[0][i]] = b.p.v[:, b.p.table[0][i]] = 0
+        b.d.table[0, i] = pg
+    q, k, v = b.randn(3, groups, 64), b.randn(3, 1, 64), b.randn(3, 1, 64)
+    got = b.d.attend(0, q, ints([0, 3]), k, v)
+    assert int(b.d.status.item()) == INVALID
+    want, size, big = b.p.attend(0, host(q), [0, 3], None, host(k), host(v))
+    b.near(got, want, size, big, 403)
+
+
 def test_base_of_kept_rows(paged):
     b = Both(paged, slots=2, page=4)
     b.fill([10, 5])
@@ -505,6 +520,59 @@ def test_a_captured_step_serves_any_lengths(paged):
         b.same()
 
 
+def test_captured_page_operations(paged):
+    """append, fork, free and compact in one graph, replayed on other states."""
+    b = Both(paged, layers=2, heads=2, dim=64, page=4, pages=60, slots=3, max_pages=12)
+    other = Both(paged, layers=2, heads=2, dim=64, page=4, pages=50, slots=3, max_pages=12)
+    b.fill([9, 5, 0])
+    k, v, starts = b.randn(3, 2, 64), b.randn(3, 2, 64), [0, 2, 3, 3]
+    source, gone, kept, counts, dstarts = ints([0, 0, 1]), ints([0, 1, 0]), ints([2, 1, 0]), ints([2, 1, 1]), ints(starts)
+    g, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(g, stream=stream):
+        b.d.reserve(counts)
+        b.d.append(1, k, v, dstarts)
+        b.d.keep(kept)
+        b.d.fork(source)
+        b.d.free(gone)
+        b.d.compact(other.d)
+    torch.cuda.current_stream().wait_stream(stream)
+    for step in range(4):
+        k.copy_(b.randn(3, 2, 64))
+        source.copy_(ints([[0, 0, 1], [2, 1, 0], [1, 0, 2], [-1, 2, 2]][step]))
+        g.replay()
+        b.p.reserve([2, 1, 1])
+        b.p.append(1, host(k), host(v), starts)
+        b.p.keep([2, 1, 0])
+        b.p.fork([[0, 0, 1], [2, 1, 0], [1, 0, 2], [-1, 2, 2]][step])
+        b.p.fork([0, -1, 2])
+        b.p.compact(other.p)
+        b.same()
+        other.same()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout,dim,heads,groups", [("rows", 128, 3, 20), ("rows", 64, 1, 40), ("odd", 64, 2, 20), ("rows", 256, 2, 10)])
+def test_many_rows_over_other_layouts(paged, dtype, layout, dim, heads, groups):
+    b = Both(paged, heads=heads, dim=dim, page=16, pages=99, slots=3, max_pages=60, dtype=dtype, layout=layout)
+    b.fill([400, 0, 131])
+    b.reserve([6, 3, 9])
+    b.attend(0, [6, 3, 9], groups)
+    b.same()
+
+
+def test_an_axis_of_one_element_has_any_stride(paged):
+    """One head, one layer: their strides say nothing, and the result is that of the plain layout."""
+    b = Both(paged, layers=1, heads=1, dim=64, page=16, pages=20, slots=1)
+    b.fill([100])
+    b.reserve([20])
+    q, kv = b.randn(20, 4, 64), b.randn(20, 1, 64)
+    want = b.d.attend(0, q, ints([0, 20]), kv, kv)
+    odd = paged.PagedCache.over(*(x.as_strided(x.shape, (3, x.stride(1), 5, x.stride(3), 1)) for x in (b.d.k, b.d.v)), b.d.table,
+                                b.d.lens, b.d.held, b.d.refs)
+    assert torch.equal(want, odd.attend(0, q, ints([0, 20]), kv, kv))
+
+
 def test_two_streams_and_two_graphs_at_once(paged):
     """Attention in two layers at the same time."""
     b = Both(paged, layers=2, heads=2, dim=128, page=16, pages=420, slots=2, max_pages=210)
@@ -559,6 +627,8 @@ def test_refusals(paged):
                  lambda: paged.PagedCache.over(*(x.cpu() for x in (c.k, c.v, c.table, c.lens, c.held, c.refs)))):
         with pytest.raises(bad):
             over()
+    with pytest.raises(bad):
+        paged.PagedCache(1, 4, 4, 0, 64, 1, 4)
     wide = paged.PagedCache(1, 4, 4, 1, 264, 1, 4)
     with pytest.raises(bad, match="at most 256"):
         wide.attend(0, torch.zeros(1, 1, 264, dtype=BF16, device="cuda"), ints([0, 1]))

@@ -217,7 +217,8 @@ __device__ __forceinline__ void pa_store(__half* p, float v) { *p = __float2half
 
 // Ancestors of the nodes of a row tile: bit j of seen[i - first] says that node j is node i or one of its ancestors. `up` takes
 // the slot's parents. All threads of the CTA; a parent that is none counts as -1.
-__device__ __forceinline__ void pa_ancestors(const PaParams& p, const PaSlot& s, int first, int count, uint32_t (*seen)[PA_TREE / 32 + 1], int16_t* up) {
+__device__ __forceinline__ void pa_ancestors(const PaParams& p, const PaSlot& s, int first, int count, uint32_t (*seen)[PA_TREE / 32 + 1],
+                                             int16_t* up) {
   const int t = threadIdx.x, nt = blockDim.x;
   for (int i = t; i < s.nodes; i += nt) {
     int a = p.parents[s.start + i];
@@ -245,12 +246,15 @@ __device__ __forceinline__ uint64_t pa_sees(const uint32_t* line, int words, int
   uint32_t w[3];
 #pragma unroll
   for (int i = 0; i < 3; ++i) w[i] = first + i < words ? line[first + i] : 0u;
-  const uint64_t bits = static_cast<uint64_t>(__funnelshift_r(w[0], w[1], shift)) | static_cast<uint64_t>(__funnelshift_r(w[1], w[2], shift)) << 32;
+  const uint64_t bits = static_cast<uint64_t>(__funnelshift_r(w[0], w[1], shift)) |
+                        static_cast<uint64_t>(__funnelshift_r(w[1], w[2], shift)) << 32;
   return low | (n0 < 0 ? bits << -n0 : bits);
 }
 
 // Positions of a slot whose rows are in the pages.
-__device__ __forceinline__ uint32_t pa_paged(const PaParams& p, const PaPart& w) { return static_cast<uint32_t>(w.s.len) + (p.fresh ? 0u : static_cast<uint32_t>(w.s.nodes)); }
+__device__ __forceinline__ uint32_t pa_paged(const PaParams& p, const PaPart& w) {
+  return static_cast<uint32_t>(w.s.len) + (p.fresh ? 0u : static_cast<uint32_t>(w.s.nodes));
+}
 // What the table says of a position, as it stands there: it is asked for ahead of its use, and a warp that looks at a number waits for
 // it. pa_checked: the page, -1 where there is none (which is noted).
 __device__ __forceinline__ int pa_lookup(const PaParams& p, const PaPart& w, uint32_t at) {
@@ -302,7 +306,8 @@ __device__ __forceinline__ float pa_exp2(float x) {
 // ---------------------------------------------------------------------------------------------- FFMA form
 // Rows that are not whole 16-byte words on their boundaries (odd dims and strides), element by element. 8 x 16 threads: thread
 // (a, b) holds rows a + 8 i (RPT of them) with keys b + 16 j of S and with columns 4 b + 64 j of O. Two tiles of keys and values as
-// fp32 in shared memory: the next one is read before one is worked on.
+// fp32 in shared memory: the next one is read before one is worked on. Bound by the loads, an element each: dim 100 in fp16, one token and
+// four heads a group behind 4000 keys, eight slots, 710 us, 0.14 TB/s.
 template <typename T, int DP, int RPT>
 struct PaFfma {
   static constexpr int RT = 8 * RPT, BN = DP == 64 ? 64 : 32;
@@ -485,7 +490,8 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_ffma_kernel(const PaPar
         }
       } else {
 #pragma unroll
-        for (int j = 0; j < CJ; ++j) *reinterpret_cast<float4*>(piece + r * DP + 4 * b + 64 * j) = make_float4(o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]);
+        for (int j = 0; j < CJ; ++j)
+          *reinterpret_cast<float4*>(piece + r * DP + 4 * b + 64 * j) = make_float4(o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]);
         if (b == 0) {
           piece[RT * DP + r] = m[i];
           piece[RT * DP + RT + r] = sum;
@@ -913,8 +919,9 @@ struct PaWarp<float, DP> {
 };
 
 // Up to 16 rows: every warp has its own keys (16 of each tile; 8 in fp32), its own ring, and no barrier until the part ends, where the
-// warps' sums are joined. What bounds it is the copy of keys and values: 512 bytes a key and head at dim 128 (fp32: 1024,
-// and the instructions of three products).
+// warps' sums are joined. What bounds it is the copy of keys and values, 512 bytes a key and head at dim 128: 32 tokens behind up to
+// 16384 keys take 223 us, 6.2 TB/s (dim 256: 4.6). In fp32 (1024 bytes) it is the chain of instructions of a step, 800 for eight keys:
+// 4.5 TB/s.
 template <typename T, int DP>
 struct PaNarrow {
   static constexpr bool F32 = std::is_same<T, float>::value;
@@ -1071,12 +1078,14 @@ __global__ void __launch_bounds__(PaNarrow<T, DP>::THREADS, PaNarrow<T, DP>::CTA
   if (t == 0) cut.store(p);
 }
 
-// Up to 64 rows of a tile: a warp for 16 of them (warps without rows only copy), all over the same tiles of keys.
-template <typename T, int DP>
+// More than 16 rows of 136 to 256 dims (O of two streams would not fit beside S in tensor memory): a warp for 16 of up to 64 rows (warps
+// without rows only copy), all over the same tiles of keys. Bound by mma.sync (8.5 clocks each and scheduler): 64 rows of dim 256 behind
+// 16000 keys, eight slots of eight heads, 700 us, 96 TFLOP/s.
+template <typename T>
 struct PaWide {
-  static constexpr int RT = 64, BN = DP == 256 ? 32 : 64, STAGES = 3, SLOT = BN * DP * 2;
+  static constexpr int DP = 256, RT = 64, BN = 32, STAGES = 3, SLOT = BN * DP * 2;
   uint4 ring[STAGES][2][SLOT / 16];
-  uint4 q[DP > 128 ? RT * DP * 2 / 16 : 1];
+  uint4 q[RT * DP * 2 / 16];
   const char* row[2][2][BN];  // (where the next tile's rows lie)
   float spare[4][16 * 8];
   uint32_t seen[RT][PA_TREE / 32 + 1];
@@ -1084,10 +1093,10 @@ struct PaWide {
   PaShare share;
 };
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) paged_attn_wide_kernel(const PaParams p) {
-  using S = PaWide<T, DP>;
-  constexpr int RT = S::RT, BN = S::BN, ST = S::STAGES, WORDS = DP / 8, PER = PA_THREADS / WORDS;
+template <typename T>
+__global__ void __launch_bounds__(PA_THREADS, 1) paged_attn_wide_kernel(const PaParams p) {
+  using S = PaWide<T>;
+  constexpr int DP = S::DP, RT = S::RT, BN = S::BN, ST = S::STAGES, WORDS = DP / 8, PER = PA_THREADS / WORDS;
   static_assert(ST == 3, "two tiles on their way, one worked on");
   extern __shared__ __align__(128) unsigned char raw[];
   S& sm = *reinterpret_cast<S*>(raw);
@@ -1146,12 +1155,8 @@ __global__ void __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) paged_attn_wide
       if (tile == w.t0) {
         const int wrow = w.row0 + 16 * warp;
         x.clear();
-        if constexpr (DP <= 128) {
-          x.load_q(p, w, wrow);
-        } else {
-          q_at = static_cast<uint32_t>(__cvta_generic_to_shared(sm.q)) + warp * 16 * (DP * 2);
-          x.stage_q(p, w, sm.q, RT);
-        }
+        q_at = static_cast<uint32_t>(__cvta_generic_to_shared(sm.q)) + warp * 16 * (DP * 2);
+        x.stage_q(p, w, sm.q, RT);
 #pragma unroll
         for (int h = 0; h < 2; ++h) node[h] = static_cast<int>(p.by_group.of(min(wrow + g + 8 * h, w.rows_all - 1)));
         if (p.parents && static_cast<uint64_t>(w.t1) * BN > static_cast<uint32_t>(w.s.len)) pa_ancestors(p, w.s, node0, node1 - node0 + 1, sm.seen, sm.up);
@@ -1203,9 +1208,10 @@ __global__ void __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) paged_attn_wide
 // same rows, joined at its end. Keys and values come in tiles of 128 into shared memory, two of each: a tile of keys is free when its
 // scores are there, one of values when its sums are. Two warps copy: tiles in front of the nodes by TMA, `box` rows of a page and 64
 // dims an instruction (a box outside the pool reads zeros); tiles with nodes, and pages whose size is no multiple of 8, by cp.async,
-// 16-byte words in the same 128-byte swizzle. One warp issues S_t = Q K^T and O_t += P_t V, and four warps for each stream turn S into P, a thread a row, while the tensor core works on the other stream. P stays in tensor memory, over its
-// own scores. What bounds it are the exponentials (one result a clock and quarter SM) and the tensor pipe, which take about the same
-// time.
+// 16-byte words in the same 128-byte swizzle. One warp issues S_t = Q K^T and O_t += P_t V, and four warps for each stream turn S into
+// P, a thread a row, while the tensor core works on the other stream. P stays in tensor memory, over its own scores. What bounds it are
+// the exponentials (four results a clock and quarter SM) and the chain S -> P -> O of a block: 128 nodes x 4 heads behind 16000 keys, eight
+// slots, 318 us, 845 TFLOP/s (0.50 of the tensor peak); half a tile of rows, 32 nodes x 4 heads, 117 us, 4.5 TB/s.
 template <typename T, int DP>
 struct PaTc {
   static constexpr int RT = 256, RW = 128, BN = 128, THREADS = 384, STAGES = DP == 64 ? 4 : 2, TILE = 128 * DP * 2;
@@ -1240,7 +1246,6 @@ __device__ __forceinline__ float pa_max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-__device__ __forceinline__ void pa_named_barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
 // The keys among 128 that a node sees, the first of them node n0 (negative: in front of the nodes). up: the slot's parents (nullptr:
 // a chain).
@@ -1803,7 +1808,8 @@ __device__ __forceinline__ void pa_store_new(const PaParams& p, int64_t warp, in
 }
 
 // CTA (x, y): the unit that starts in share x and goes on behind it, rows y, y + joiners, ... of it, or four times as many. Of many
-// pieces the warps take every fourth each, and their sums are joined in the order of the warps; few are one warp's work. CTAs (x, joiners) store the call's new rows meanwhile: nothing reads
+// pieces the warps take every fourth each, and their sums are joined in the order of the warps; few are one warp's work. Three reads
+// that depend on one another: about 3 us behind the attention. CTAs (x, joiners) store the call's new rows meanwhile: nothing reads
 // those places before the call is over.
 template <typename T, int DP>
 __global__ void __launch_bounds__(PA_THREADS) paged_attn_join_kernel(const PaParams p, int rt, int joiners) {
@@ -1851,7 +1857,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_join_kernel(const PaPar
     for (int w = 16; w; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
     return m;
   };
-  if (pieces <= 8) {  // a warp a row (the many rows of wide tiles: 148 units of 256 rows in three pieces 17 us with a CTA a row)
+  if (pieces <= 8) {  // (the many rows of wide tiles: 256 rows in three pieces took 17 us with a CTA a row)
     for (int r = blockIdx.y * WARPS + warp; r < a.x; r += joiners * WARPS) {
       float l;
       float4 o[PER];
@@ -1928,9 +1934,9 @@ static PaForm pa_form(int rows, bool words) {
         static_assert(C::BYTES <= PA_SHARED, "shared memory");
         return PaForm{DP, C::RT, C::BN, sm_count(), C::THREADS, C::BYTES, pa_fn(paged_attn_tc_kernel<T, DP>), true};
       } else {
-        using W = PaWide<T, DP>;
+        using W = PaWide<T>;
         static_assert(sizeof(W) <= PA_SHARED, "shared memory");
-        return PaForm{DP, W::RT, W::BN, sm_count(), PA_THREADS, static_cast<int>(sizeof(W)), pa_fn(paged_attn_wide_kernel<T, DP>), false};
+        return PaForm{DP, W::RT, W::BN, sm_count(), PA_THREADS, static_cast<int>(sizeof(W)), pa_fn(paged_attn_wide_kernel<T>), false};
       }
     }
   }

@@ -83,7 +83,8 @@ __device__ __forceinline__ void pg_copy_rows(char* dst, int64_t dst_row, const c
 // ---------------------------------------------------------------------------------------------- append
 // A warp stores what `run` new rows hold of one head in keys or values: in the pages that is one stretch of up to 4 KB, and the warps
 // beside it take the other heads of the same rows. A lane finds where each row goes (five reads that depend on one another), for
-// the next item while this one's words are on their way. The row's slot: the last one that starts at or before it.
+// the next item while this one's words are on their way. The row's slot: the last one that starts at or before it. Four prompts of up to
+// 8000 rows, fp32, 309 MB in and out: 54 us, 5.7 TB/s (65 us with three CTAs an SM instead of four).
 template <int BYTES>
 __global__ void __launch_bounds__(PG_WARPS * 32, 4) pages_append_kernel(const PgCache c, const PgRows k, const PgRows v, const int32_t* starts,
                                                                      int rows, int layer, PgDiv by_words, int run) {
@@ -146,8 +147,8 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 4) pages_append_kernel(const Pg
 }
 
 // ---------------------------------------------------------------------------------------------- reserve
-// One CTA: what each slot wants, the free pages in ascending order, and who gets which. Reading refs once at 16 bytes a lane is
-// what it costs: 64k pages are 256 KB, which one SM reads in about 4 us.
+// One CTA: what each slot wants, the free pages in ascending order, and who gets which. Seven reads that depend on one another, 6 us; refs
+// are read once, 32 KB a round, until enough free pages are found.
 __global__ void __launch_bounds__(PG_COUNT) pages_reserve_kernel(const PgCache c, const int32_t* counts) {
   dependent_trigger();
   __shared__ int sums[32];
@@ -253,7 +254,7 @@ __global__ void __launch_bounds__(PG_COUNT) pages_reserve_kernel(const PgCache c
   if (t == 0) c.scratch[at.copies] = n_copies;
 }
 
-// A warp copies up to 4 KB of the rows of one head, layer and pool of a page.
+// A warp copies up to 4 KB of the rows of one head, layer and pool of a page. 64 beams of eight searches, 12 layers, 61 MB: 12 us.
 template <int BYTES>
 __global__ void __launch_bounds__(PG_WARPS * 32) pages_copy_kernel(const PgCache c, int row_words) {
   using W = typename PgWord<BYTES>::type;
@@ -294,7 +295,8 @@ __device__ __forceinline__ int pg_keep_bad(const PgCache& c, int s, int64_t base
 
 // A CTA moves the accepted rows of one slot in some of its layers, heads and pools, a warp each: where the rows lie is worked out
 // once for up to PG_MOVES of them. Rows only move down and in ascending order, so a batch that has been read before it is written
-// never hides a row of a later batch. The CTA that finishes last writes the lengths: every other one has read them by then.
+// never hides a row of a later batch. The CTA that finishes last writes the lengths: every other one has read them by then. 64 slots, up
+// to 12 of 48 rows in 28 layers, 72 MB in rows of 256 bytes anywhere in 4 GB: 27 us.
 constexpr int PG_MOVES = 128;
 template <int BYTES>
 __global__ void __launch_bounds__(PG_WARPS * 32, 3) pages_keep_kernel(const PgCache c, const int32_t* kept, const int32_t* accepted,
@@ -374,7 +376,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 3) pages_keep_kernel(const PgCa
 // ---------------------------------------------------------------------------------------------- fork
 // One cluster of CTAs: new rows of the table go to the scratch first (another slot may still have to read the old ones) and, behind
 // the cluster's barrier, into the table; nothing else is waited for. The counts are whole numbers and may change in any order. It is
-// as long as four reads that depend on one another.
+// as long as four reads that depend on one another: 5 us for four slots, 8 for 64 slots of 128 pages.
 constexpr int PG_CLUSTER = 8;
 __global__ void __cluster_dims__(PG_CLUSTER, 1, 1) __launch_bounds__(PG_COUNT) pages_fork_kernel(const PgCache c, const int32_t* source, const int32_t* gone) {
   const PgScratch at = pg_scratch(c.slots, c.max_pages, c.pages);
@@ -474,7 +476,8 @@ __global__ void __launch_bounds__(PG_COUNT) pages_number_kernel(const PgCache c,
     to.held[s] = c.held[s];
   }
 }
-// A warp copies a piece of up to 4 KB of what one page holds of a layer (of a head, where the heads do not lie one behind another).
+// A warp copies a piece of up to 4 KB of what one page holds of a layer (of a head, where the heads do not lie one behind another). 1.2 GB
+// in 384 us, 6.3 TB/s in and out: a plain copy's rate (389 and 402 us with three and four CTAs an SM).
 template <int BYTES>
 __global__ void __launch_bounds__(PG_WARPS * 32) pages_compact_kernel(const PgCache c, const PgCache to, int row_words, int merged) {
   using W = typename PgWord<BYTES>::type;
@@ -533,8 +536,11 @@ int pg_take(const char* who, const ytcuda_pages* c, PgCache* out) {
               "%s: null tensor in the cache", who);
   const int size = dtype_size(c->dtype);
   YTC_REQUIRE((reinterpret_cast<uint64_t>(c->k) | reinterpret_cast<uint64_t>(c->v)) % size == 0, "%s: misaligned pool", who);
+  // (the stride of an axis of one element says nothing: it must not decide how rows are copied)
   auto pool = [&](void* p, const int64_t* s) {
-    return PgPool{static_cast<char*>(p), s[0] * size, s[1] * size, s[2] * size, s[3] * size};
+    const int64_t any = static_cast<int64_t>(c->dim) * size;
+    return PgPool{static_cast<char*>(p), c->layers == 1 ? any : s[0] * size, c->pages == 1 ? any : s[1] * size,
+                  c->kv_heads == 1 ? any : s[2] * size, c->page == 1 ? any : s[3] * size};
   };
   for (int i = 0; i < 4; ++i) YTC_REQUIRE(c->k_strides[i] >= 0 && c->v_strides[i] >= 0, "%s: negative stride in a pool", who);
   *out = PgCache{pool(c->k, c->k_strides), pool(c->v, c->v_strides), pg_div(static_cast<uint32_t>(c->page)),

@@ -63,6 +63,8 @@ class PagedCache:
     def _set(self, k, v, table, lens, held, refs):
         if k.dim() != 5 or k.shape != v.shape or k.dtype != v.dtype:
             raise _bad("paged cache: k and v are [layers, pages, kv_heads, page, dim] of one shape and type")
+        if 0 in (k.shape[0], *k.shape[2:]):
+            raise _bad(f"paged cache: an empty axis in {list(k.shape)}")
         for t in (k, v):
             if t.shape[-1] > 1 and t.stride(-1) != 1:
                 raise _bad("paged cache: k and v need a unit stride along dim")
@@ -168,7 +170,9 @@ class PagedCache:
         multiple of kv_heads; dim is at most 256. k and v [rows, kv_heads, dim] are stored behind the sequences as by
         `append`, in the same launch; without them they are in the pages already. scale 0: 1 / sqrt(dim).
 
-        Scores, softmax and sums are fp32, results are rounded to nearest even. Rows behind starts[slots] are not written."""
+        Scores, softmax and sums are fp32, results are rounded to nearest even. Rows behind starts[slots] are not written. What
+        a node does not see may be infinite or no number; in fp32 a node that sees an infinity gets NaN. `out` shares no
+        memory with q, k or v."""
         stream = self._stream()
         if q.dim() != 3 or q.shape[1] % self.kv_heads:
             raise _bad(f"paged cache: q is [rows, heads, dim] with heads a multiple of {self.kv_heads}, got {list(q.shape)}")

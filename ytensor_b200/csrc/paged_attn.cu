@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_ffma_kernel(const PaPar
   constexpr int RT = S::RT, BN = S::BN, KPT = BN / 16, CJ = DP / 64;
   extern __shared__ __align__(128) unsigned char raw[];
   S& sm = *reinterpret_cast<S*>(raw);
-  dependent_trigger();
+  pg_begin();
   const int t = threadIdx.x, a = t >> 4, b = t & 15;
   const PgCache& c = p.c;
   pa_share<RT, RT, BN>(p, &sm.share);
@@ -948,7 +948,7 @@ __global__ void __launch_bounds__(PaNarrow<T, DP>::THREADS, PaNarrow<T, DP>::CTA
   constexpr int RT = S::RT, BN = S::BN, ST = S::STAGES, KEYS = S::KEYS, WORDS = DP * sizeof(T) / 16;
   extern __shared__ __align__(128) unsigned char raw[];
   S& sm = *reinterpret_cast<S*>(raw);
-  dependent_trigger();
+  pg_begin();
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, g = lane >> 2, c4 = lane & 3;
   const PgCache& c = p.c;
   pa_share<RT, RT, BN>(p, &sm.share);
@@ -1100,7 +1100,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) paged_attn_wide_kernel(const Pa
   static_assert(ST == 3, "two tiles on their way, one worked on");
   extern __shared__ __align__(128) unsigned char raw[];
   S& sm = *reinterpret_cast<S*>(raw);
-  dependent_trigger();
+  pg_begin();
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, g = lane >> 2, c4 = lane & 3;
   const PgCache& c = p.c;
   pa_share<RT, RT, BN>(p, &sm.share);
@@ -1333,7 +1333,6 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1)
   extern __shared__ __align__(128) unsigned char raw[];
   unsigned char* const smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
   typename S::Rest& sm = *reinterpret_cast<typename S::Rest*>(smem + S::REST);
-  dependent_trigger();
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const PgCache& c = p.c;
   if (threadIdx.x == 0) {
@@ -1362,6 +1361,7 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1)
     tmem_relinquish();
   }
   tc_fence_before();
+  pg_begin();
   pa_share<RT, RW, BN>(p, &sm.share);
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
@@ -1809,20 +1809,21 @@ __device__ __forceinline__ void pa_store_new(const PaParams& p, int64_t warp, in
 
 // CTA (x, y): the unit that starts in share x and goes on behind it, rows y, y + joiners, ... of it, or four times as many. Of many
 // pieces the warps take every fourth each, and their sums are joined in the order of the warps; few are one warp's work. Three reads
-// that depend on one another: about 3 us behind the attention. CTAs (x, joiners) store the call's new rows meanwhile: nothing reads
-// those places before the call is over.
+// that depend on one another: about 3 us behind the attention. CTAs (x, joiners ..) store the call's new rows at the same
+// time.
 template <typename T, int DP>
 __global__ void __launch_bounds__(PA_THREADS) paged_attn_join_kernel(const PaParams p, int rt, int joiners) {
   constexpr int WARPS = PA_THREADS / 32, C4 = DP / 4, PER = (C4 + 31) / 32;
   __shared__ float sums[WARPS][DP + 1];
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, first = blockIdx.x;
-  if (static_cast<int>(blockIdx.y) == joiners) {
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * WARPS + warp, all = static_cast<int64_t>(gridDim.x) * WARPS;
+  pg_begin();
+  if (static_cast<int>(blockIdx.y) >= joiners) {
+    const int64_t at = (static_cast<int64_t>(blockIdx.y - joiners) * gridDim.x + blockIdx.x) * WARPS + warp;
+    const int64_t all = static_cast<int64_t>(gridDim.y - joiners) * gridDim.x * WARPS;
     if (p.wide) pa_store_new<uint4>(p, at, all);
     else pa_store_new<T>(p, at, all);
     return;
   }
-  dependent_wait();
   const int4 a = p.cuts[2 * first];
   const int last = p.cuts[2 * first + 1].x;
   const int64_t size = pa_piece(rt, DP);
@@ -1980,10 +1981,12 @@ static int pa_boxes(const PgCache& c, int dtype, CUtensorMap* k, CUtensorMap* v)
 template <typename T>
 static cudaError_t pa_join(const PaForm& f, const PaParams& p, cudaStream_t st) {
   const int joiners = f.rt <= 32 ? 4 : f.rt / 16;
-  const dim3 grid(f.ctas, joiners + (p.fresh ? 1 : 0)), block(PA_THREADS);
-  if (f.dp == 64) return pg_launch_behind(paged_attn_join_kernel<T, 64>, grid, block, 0, st, p, f.rt, joiners);
-  if (f.dp == 128) return pg_launch_behind(paged_attn_join_kernel<T, 128>, grid, block, 0, st, p, f.rt, joiners);
-  return pg_launch_behind(paged_attn_join_kernel<T, 256>, grid, block, 0, st, p, f.rt, joiners);
+  // a warp for each new row and head, up to eight rows of CTAs
+  const int64_t stored = p.fresh ? (static_cast<int64_t>(p.rows) * p.c.heads - 1) / (f.ctas * (PA_THREADS / 32)) + 1 : 0;
+  const dim3 grid(f.ctas, joiners + static_cast<int>(stored < 8 ? stored : 8)), block(PA_THREADS);
+  if (f.dp == 64) return pg_launch(paged_attn_join_kernel<T, 64>, grid, block, 0, st, p, f.rt, joiners);
+  if (f.dp == 128) return pg_launch(paged_attn_join_kernel<T, 128>, grid, block, 0, st, p, f.rt, joiners);
+  return pg_launch(paged_attn_join_kernel<T, 256>, grid, block, 0, st, p, f.rt, joiners);
 }
 
 }  // namespace ytk
@@ -2058,7 +2061,17 @@ int ytcuda_pages_attend(const ytcuda_pages* cache, int layer, const void* q, voi
   CUtensorMap map_k{}, map_v{};
   if (f.boxes) p.box = pa_boxes(p.c, cache->dtype, &map_k, &map_v);
   void* args[] = {&p, &map_k, &map_v};
-  YTC_CUDA(cudaLaunchKernel(f.kernel, dim3(f.ctas), dim3(f.threads), args, f.smem, st));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(f.ctas);
+  cfg.blockDim = dim3(f.threads);
+  cfg.dynamicSmemBytes = f.smem;
+  cfg.stream = st;
+  cudaLaunchAttribute overlapped[1];  // (as pg_launch)
+  overlapped[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  overlapped[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = overlapped;
+  cfg.numAttrs = 1;
+  YTC_CUDA(cudaLaunchKernelExC(&cfg, f.kernel, args));
   count_launch();
   YTC_CUDA(cache->dtype == YTC_F32 ? pa_join<float>(f, p, st) : cache->dtype == YTC_BF16 ? pa_join<__nv_bfloat16>(f, p, st) : pa_join<__half>(f, p, st));
   count_launch();

@@ -89,6 +89,7 @@ template <int BYTES>
 __global__ void __launch_bounds__(PG_WARPS * 32, 4) pages_append_kernel(const PgCache c, const PgRows k, const PgRows v, const int32_t* starts,
                                                                      int rows, int layer, PgDiv by_words, int run) {
   using W = typename PgWord<BYTES>::type;
+  pg_begin();
   const int lane = threadIdx.x & 31, warps = gridDim.x * PG_WARPS, row_words = by_words.d;
   const int first = max(0, starts[0]), last = min(rows, starts[c.slots]);
   const int items = (rows + run - 1) / run * 2 * c.heads;
@@ -150,7 +151,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 4) pages_append_kernel(const Pg
 // One CTA: what each slot wants, the free pages in ascending order, and who gets which. Seven reads that depend on one another, 6 us; refs
 // are read once, 32 KB a round, until enough free pages are found.
 __global__ void __launch_bounds__(PG_COUNT) pages_reserve_kernel(const PgCache c, const int32_t* counts) {
-  dependent_trigger();
+  pg_begin();
   __shared__ int sums[32];
   __shared__ int bad, n_copies;
   const PgScratch at = pg_scratch(c.slots, c.max_pages, c.pages);
@@ -259,7 +260,7 @@ template <int BYTES>
 __global__ void __launch_bounds__(PG_WARPS * 32) pages_copy_kernel(const PgCache c, int row_words) {
   using W = typename PgWord<BYTES>::type;
   const PgScratch at = pg_scratch(c.slots, c.max_pages, c.pages);
-  dependent_wait();
+  pg_begin();
   const int rows_a_piece = max(1, 32 * PG_UNROLL / row_words), pieces = (c.page + rows_a_piece - 1) / rows_a_piece;
   const int64_t per_copy = 2ll * c.layers * c.heads * pieces;
   const int64_t items = c.scratch[at.copies] * per_copy, warps = static_cast<int64_t>(gridDim.x) * PG_WARPS;
@@ -307,6 +308,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 3) pages_keep_kernel(const PgCa
   __shared__ int last;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int items = 2 * c.layers * c.heads, s = blockIdx.y;
+  pg_begin();
   const PgScratch at = pg_scratch(c.slots, c.max_pages, c.pages);
   const int n = kept[s];
   const int64_t b = base ? base[s] : c.lens[s];
@@ -381,6 +383,7 @@ constexpr int PG_CLUSTER = 8;
 __global__ void __cluster_dims__(PG_CLUSTER, 1, 1) __launch_bounds__(PG_COUNT) pages_fork_kernel(const PgCache c, const int32_t* source, const int32_t* gone) {
   const PgScratch at = pg_scratch(c.slots, c.max_pages, c.pages);
   constexpr int WARPS = PG_CLUSTER * PG_COUNT / 32;
+  pg_begin();
   const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) * PG_CLUSTER + blockIdx.x;
   int32_t *const new_held = c.scratch + at.held, *const new_lens = c.scratch + at.lens, *const rows = c.scratch + at.table;
   // a warp a stretch of 32 entries of a slot's row
@@ -433,7 +436,7 @@ __global__ void __cluster_dims__(PG_CLUSTER, 1, 1) __launch_bounds__(PG_COUNT) p
 // ---------------------------------------------------------------------------------------------- compact
 // One CTA: the new numbers of the pages in use, and what the other cache says of its slots.
 __global__ void __launch_bounds__(PG_COUNT) pages_number_kernel(const PgCache c, const PgCache to) {
-  dependent_trigger();
+  pg_begin();
   __shared__ int sums[32];
   const PgScratch at = pg_scratch(c.slots, c.max_pages, c.pages);
   int32_t* const ids = c.scratch + at.ids;
@@ -482,7 +485,7 @@ template <int BYTES>
 __global__ void __launch_bounds__(PG_WARPS * 32) pages_compact_kernel(const PgCache c, const PgCache to, int row_words, int merged) {
   using W = typename PgWord<BYTES>::type;
   const PgScratch at = pg_scratch(c.slots, c.max_pages, c.pages);
-  dependent_wait();
+  pg_begin();
   const int pages = c.scratch[at.copies];
   if (pages < 0) return;
   const int64_t entries = static_cast<int64_t>(c.slots) * c.max_pages, threads = static_cast<int64_t>(gridDim.x) * blockDim.x;
@@ -607,9 +610,9 @@ int ytcuda_pages_append(const ytcuda_pages* cache, int layer, const void* k, con
   const int64_t items = (static_cast<int64_t>(rows) + run - 1) / run * 2 * c.heads;
   const PgDiv by_words = pg_div(static_cast<uint32_t>(words));
   YTC_REQUIRE(items < (1ll << 30), "%s: %d rows of %d heads are too many", who, rows, c.heads);
-  PG_BY_WIDTH(width, (pages_append_kernel<B><<<copy_grid(items), PG_WARPS * 32, 0, st>>>(c, kr, vr, starts, rows, layer, by_words, run)));
+  PG_BY_WIDTH(width, YTC_CUDA(pg_launch(pages_append_kernel<B>, dim3(copy_grid(items)), dim3(PG_WARPS * 32), 0, st, c, kr, vr, starts, rows, layer,
+                                        by_words, run)));
   count_launch();
-  YTC_CUDA(cudaGetLastError());
   return YTC_OK;
 }
 
@@ -623,12 +626,11 @@ int ytcuda_pages_reserve(const ytcuda_pages* cache, const int32_t* counts, void*
   const int size = dtype_size(cache->dtype);
   const int width = pg_width(pg_bits(c.k) | pg_bits(c.v) | static_cast<uint64_t>(c.dim * size));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  pages_reserve_kernel<<<1, PG_COUNT, 0, st>>>(c, counts);
+  YTC_CUDA(pg_launch(pages_reserve_kernel, dim3(1), dim3(PG_COUNT), 0, st, c, counts));
   count_launch();
-  YTC_CUDA(cudaGetLastError());
   const int rows_a_piece = 32 * PG_UNROLL * width / (c.dim * size);
   const unsigned grid = copy_grid(2ll * c.slots * c.layers * c.heads * (rows_a_piece > 1 ? (c.page + rows_a_piece - 1) / rows_a_piece : c.page));
-  PG_BY_WIDTH(width, YTC_CUDA(pg_launch_behind(pages_copy_kernel<B>, dim3(grid), dim3(PG_WARPS * 32), 0, st, c, c.dim * size / B)));
+  PG_BY_WIDTH(width, YTC_CUDA(pg_launch(pages_copy_kernel<B>, dim3(grid), dim3(PG_WARPS * 32), 0, st, c, c.dim * size / B)));
   count_launch();
   return YTC_OK;
 }
@@ -650,9 +652,9 @@ int ytcuda_pages_keep(const ytcuda_pages* cache, const int32_t* kept, const int3
   const dim3 grid(accepted ? static_cast<unsigned>(a_slot < most ? a_slot : most) : 1u, static_cast<unsigned>(c.slots));
   YTC_REQUIRE(c.slots <= 65535, "%s: %d slots (at most 65535)", who, c.slots);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  PG_BY_WIDTH(width, (pages_keep_kernel<B><<<grid, PG_WARPS * 32, 0, st>>>(c, kept, accepted, depth, base, pg_div(static_cast<uint32_t>(c.dim * size / B)))));
+  const PgDiv by_words = pg_div(static_cast<uint32_t>(c.dim * size / width));
+  PG_BY_WIDTH(width, YTC_CUDA(pg_launch(pages_keep_kernel<B>, grid, dim3(PG_WARPS * 32), 0, st, c, kept, accepted, depth, base, by_words)));
   count_launch();
-  YTC_CUDA(cudaGetLastError());
   return YTC_OK;
 }
 
@@ -664,9 +666,8 @@ int ytcuda_pages_fork(const ytcuda_pages* cache, const int32_t* source, const in
   YTC_REQUIRE((source != nullptr) != (gone != nullptr), "%s: source or gone, one of them", who);
   YTC_REQUIRE(c.pages > 0, "%s: a pool without pages", who);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  pages_fork_kernel<<<PG_CLUSTER, PG_COUNT, 0, st>>>(c, source, gone);
+  YTC_CUDA(pg_launch(pages_fork_kernel, dim3(PG_CLUSTER), dim3(PG_COUNT), 0, st, c, source, gone));
   count_launch();
-  YTC_CUDA(cudaGetLastError());
   return YTC_OK;
 }
 
@@ -689,11 +690,10 @@ int ytcuda_pages_compact(const ytcuda_pages* cache, const ytcuda_pages* into, vo
   for (const PgPool* p : {&c.k, &c.v, &to.k, &to.v})
     merged = merged && p->row == c.dim * size && (p->head == c.page * p->row || c.heads == 1);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  pages_number_kernel<<<1, PG_COUNT, 0, st>>>(c, to);
+  YTC_CUDA(pg_launch(pages_number_kernel, dim3(1), dim3(PG_COUNT), 0, st, c, to));
   count_launch();
-  YTC_CUDA(cudaGetLastError());
   const unsigned grid = copy_grid(1ll << 30);
-  PG_BY_WIDTH(width, YTC_CUDA(pg_launch_behind(pages_compact_kernel<B>, dim3(grid), dim3(PG_WARPS * 32), 0, st, c, to, c.dim * size / B, merged)));
+  PG_BY_WIDTH(width, YTC_CUDA(pg_launch(pages_compact_kernel<B>, dim3(grid), dim3(PG_WARPS * 32), 0, st, c, to, c.dim * size / B, merged)));
   count_launch();
   return YTC_OK;
 }

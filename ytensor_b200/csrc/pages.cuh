@@ -88,9 +88,15 @@ __device__ __forceinline__ int pg_row_of(const PgCache& c, int64_t at) {
   const uint32_t n = static_cast<uint32_t>(at);
   return static_cast<int>(n - c.by_page.of(n) * c.by_page.d);
 }
-// A launch behind another of the same call, whose set-up may overlap it: the kernel calls dependent_wait() first of all.
+// Every kernel here is launched so that it may be set up while the one in front of it in the stream still runs (about 1 us a launch),
+// and begins with pg_begin(), before it reads or writes any memory. Only behind its own wait does a kernel let the next one in: what
+// is behind that one in turn may rely on everything in front of this one being over.
+__device__ __forceinline__ void pg_begin() {
+  dependent_wait();
+  dependent_trigger();
+}
 template <typename... KArgs, typename... Args>
-cudaError_t pg_launch_behind(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args&&... args) {
+cudaError_t pg_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args&&... args) {
   const bool was = overlap_scope();
   overlap_scope() = true;
   const cudaError_t e = launch_overlapped(kernel, grid, block, smem, st, static_cast<Args&&>(args)...);

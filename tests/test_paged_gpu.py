@@ -449,15 +449,32 @@ def test_numbers_in_hidden_places(paged, dtype, dim, groups):
                 assert torch.equal(got[row], plain[row]), row
 
 
-def test_results_do_not_depend_on_the_neighbours(paged):
+@pytest.mark.parametrize("dtype,groups", [(F32, 4), (BF16, 4), (BF16, 16), (F16, 16)])
+def test_results_are_the_same_every_time(paged, dtype, groups):
     """The same call twice gives the same bits."""
-    b = Both(paged, heads=2, dim=128, pages=200, slots=3, max_pages=150)
+    b = Both(paged, heads=2, dim=128, pages=200, slots=3, max_pages=150, dtype=dtype)
     b.fill([700, 45, 1300])
     b.reserve([9, 1, 30])
-    q, k, v = b.randn(40, 8, 128), b.randn(40, 2, 128), b.randn(40, 2, 128)
+    q, k, v = b.randn(40, 2 * groups, 128), b.randn(40, 2, 128), b.randn(40, 2, 128)
     first = b.d.attend(0, q, ints([0, 9, 10, 40]), k, v)
-    for _ in range(3):
+    for _ in range(20):
         assert torch.equal(first, b.d.attend(0, q, ints([0, 9, 10, 40]), k, v))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("groups", [2, 12])
+def test_attend_over_many_slots(paged, dtype, groups):
+    """More slots than lanes, idle ones among them, ragged lengths."""
+    slots = 70
+    lens, nodes = [(s * 37) % 90 for s in range(slots)], [s % 4 for s in range(slots)]
+    b = Both(paged, layers=1, heads=2, dim=64, page=16, pages=600, slots=slots, max_pages=8, dtype=dtype)
+    b.reserve(lens)
+    b.append(0, lens)
+    b.keep(lens)
+    b.reserve(nodes)
+    b.attend(0, nodes, groups, tree=True, extra=2)
+    b.attend(0, [0] * 69 + [3], groups, tree=False)
+    b.same()
 
 
 # ---------------------------------------------------------------------------------------------- together

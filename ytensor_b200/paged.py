@@ -20,13 +20,15 @@ and noted in `status`; `check()` reads it. Calls on one cache follow one another
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
 from . import _lib
 from ._lib import check, lib
-from .api import _dt, _i64, _require_cuda
+from .api import _dt, _require_cuda
 
+_FOUR, _EIGHT = struct.Struct("4q").pack, struct.Struct("8q").pack
 FULL, INVALID, SHARED = 1, 2, 4  # bits of `status`
 _TEXT = {FULL: "too few free pages: nothing was reserved or compacted",
          INVALID: "an index out of its range, a position without a page, or a tree that is none",
@@ -103,9 +105,9 @@ class PagedCache:
         return t.data_ptr()
 
     def _rows(self, t, name: str, shape: tuple) -> tuple:
-        """Strides of rows and heads."""
+        """Strides."""
         st = t.stride()
-        if t.dtype is not self.dtype or t.shape != shape or t.get_device() != self._index or (st[2] != 1 and shape[2] > 1):
+        if t.shape != shape or t.dtype is not self.dtype or t.get_device() != self._index or (st[2] != 1 and shape[2] > 1):
             raise _bad(f"paged cache: {name} is {self.dtype} {list(shape)} with a unit stride along dim, on {self.device}; "
                        f"got {t.dtype} {list(t.shape)}, strides {list(st)}, on {t.device}")
         return st
@@ -156,8 +158,9 @@ class PagedCache:
         (starts int32 [slots + 1]). lens stays until `keep`, so that every layer of a step writes the same places."""
         rows = k.shape[0] if k.dim() else 0
         shape = (rows, self.kv_heads, self.dim)
-        ks, vs = self._rows(k, "k", shape), self._rows(v, "v", shape)
-        check(self._lib.ytcuda_pages_append(self._at, self._layer(layer), k.data_ptr(), v.data_ptr(), _i64((*ks[:2], *vs[:2])),
+        kr, kh, _ = self._rows(k, "k", shape)
+        vr, vh, _ = self._rows(v, "v", shape)
+        check(self._lib.ytcuda_pages_append(self._at, self._layer(layer), k.data_ptr(), v.data_ptr(), _FOUR(kr, kh, vr, vh),
                                             self._ints(starts, "starts", self._bounds), rows, self._stream()))
 
     def attend(self, layer: int, q: torch.Tensor, starts: torch.Tensor, k: torch.Tensor | None = None,
@@ -179,15 +182,19 @@ class PagedCache:
         rows, heads, dim = shape = q.shape
         if dim != self.dim:
             raise _bad(f"paged cache: q has dim {dim}, the cache {self.dim}")
+        qr, qh, _ = self._rows(q, "q", shape)
         if out is None:
-            out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        qs, os = self._rows(q, "q", shape), self._rows(out, "out", shape)
+            out = torch.empty_like(q)
+            o_row, o_head, _ = out.stride()
+        else:
+            o_row, o_head, _ = self._rows(out, "out", shape)
         if k is not None and v is not None:
             new = (rows, self.kv_heads, dim)
-            ks, vs = self._rows(k, "k", new), self._rows(v, "v", new)
-            kp, vp, strides = k.data_ptr(), v.data_ptr(), _i64((*qs[:2], *os[:2], *ks[:2], *vs[:2]))
+            kr, kh, _ = self._rows(k, "k", new)
+            vr, vh, _ = self._rows(v, "v", new)
+            kp, vp, strides = k.data_ptr(), v.data_ptr(), _EIGHT(qr, qh, o_row, o_head, kr, kh, vr, vh)
         elif k is None and v is None:
-            kp, vp, strides = None, None, _i64((*qs[:2], *os[:2], 0, 0, 0, 0))
+            kp, vp, strides = None, None, _EIGHT(qr, qh, o_row, o_head, 0, 0, 0, 0)
         else:
             raise _bad("paged cache: k and v come together")
         if self._space[0] != (rows, heads):

@@ -462,6 +462,21 @@ def test_results_are_the_same_every_time(paged, dtype, groups):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nodes,groups", [(1, 1), (1, 7), (5, 3), (16, 1), (33, 2), (64, 5), (200, 3)])
+@pytest.mark.parametrize("dim", [64, 130, 256])
+def test_one_sequence_over_all_processors(paged, dtype, nodes, groups, dim):
+    """One key head: every tile of rows is cut into as many pieces as there are keys for."""
+    b = Both(paged, layers=1, heads=1, dim=dim, page=64, pages=180, slots=1, max_pages=180, dtype=dtype, seed=nodes)
+    b.fill([900])
+    b.reserve([9000])
+    b.append(0, [9000])
+    b.keep([9000])
+    b.reserve([nodes])
+    b.attend(0, [nodes], groups)
+    b.same()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("groups", [2, 12])
 def test_attend_over_many_slots(paged, dtype, groups):
     """More slots than lanes, idle ones among them, ragged lengths."""

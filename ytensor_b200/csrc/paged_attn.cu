@@ -31,7 +31,7 @@ struct PaParams {
   int wide, words;  // rows in pieces of 16 bytes (else of an element), their number
   float scale;  // times log2(e)
   float* work;  // pieces of cut units
-  int4* cuts;   // two words for each CTA: the unit that starts in its share and goes on behind it
+  int4* cuts;   // two words for each CTA: the unit that goes on behind its share
   int* timeout; // the device's status word
   int box;      // rows of a page that a TMA copy takes (0: none)
 };
@@ -183,18 +183,18 @@ template <int RT, int DP>
 __device__ __forceinline__ float* pa_piece_of(const PaParams& p, const PaPart& w) {
   return p.work + (2 * static_cast<int64_t>(blockIdx.x) + (w.t0 == 0)) * pa_piece(RT, DP);
 }
-// What joining has to know of the unit that starts in this CTA's share and goes on: kept by one thread, stored at the end.
+// What joining has to know of the unit that goes on behind this CTA's share: rows (0: no such unit), first row, head, start of the
+// slot's rows; first and last share. Written by one thread.
 struct PaCut {
-  int4 a{0, 0, 0, 0}, b{0, 0, 0, 0};  // rows (0: no such unit), first row, head, start of the slot's rows; last share
-  __device__ __forceinline__ void note(const PaShare& sh, const PaPart& w) {
-    if (w.t0 == 0 && w.t1 < w.tiles) {
-      a = make_int4(w.rows, w.row0, w.head, w.s.start);
-      b.x = static_cast<int>(pa_share_of(sh, w.first + (w.tiles - 1) * w.weight));
-    }
+  int4* at;  // null: not this thread
+  __device__ __forceinline__ PaCut(const PaParams& p, bool mine) : at(mine ? p.cuts + 2 * blockIdx.x : nullptr) {
+    if (mine) at[0] = make_int4(0, 0, 0, 0);
   }
-  __device__ __forceinline__ void store(const PaParams& p) const {
-    p.cuts[2 * blockIdx.x] = a;
-    p.cuts[2 * blockIdx.x + 1] = b;
+  __device__ __forceinline__ void note(const PaShare& sh, const PaPart& w) const {
+    if (at && w.t1 < w.tiles) {
+      at[0] = make_int4(w.rows, w.row0, w.head, w.s.start);
+      at[1] = make_int4(static_cast<int>(pa_share_of(sh, w.first)), static_cast<int>(pa_share_of(sh, w.first + (w.tiles - 1) * w.weight)), 0, 0);
+    }
   }
 };
 // Where the result of a row goes.
@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_ffma_kernel(const PaPar
   const int t = threadIdx.x, a = t >> 4, b = t & 15;
   const PgCache& c = p.c;
   pa_share<RT, RT, BN>(p, &sm.share);
-  PaCut cut;
+  const PaCut cut(p, threadIdx.x == 0);
   PaAt at(sm.share);
   PaPart w;
   while (pa_next<RT, RT, BN>(p, &at, &w)) {
@@ -500,7 +500,6 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_ffma_kernel(const PaPar
     }
     cut.note(sm.share, w);
   }
-  if (t == 0) cut.store(p);
 }
 
 // ---------------------------------------------------------------------------------------------- matrix-instruction forms
@@ -952,7 +951,7 @@ __global__ void __launch_bounds__(PaNarrow<T, DP>::THREADS, PaNarrow<T, DP>::CTA
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, g = lane >> 2, c4 = lane & 3;
   const PgCache& c = p.c;
   pa_share<RT, RT, BN>(p, &sm.share);
-  PaCut cut;
+  const PaCut cut(p, threadIdx.x == 0);
   PaAt at(sm.share);
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(sm.ring[warp]));
   const int words = c.dim * static_cast<int>(sizeof(T)) / 16;
@@ -1075,7 +1074,6 @@ __global__ void __launch_bounds__(PaNarrow<T, DP>::THREADS, PaNarrow<T, DP>::CTA
     }
     cut.note(sm.share, w);
   }
-  if (t == 0) cut.store(p);
 }
 
 // More than 16 rows of 136 to 256 dims (O of two streams would not fit beside S in tensor memory): a warp for 16 of up to 64 rows (warps
@@ -1104,7 +1102,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) paged_attn_wide_kernel(const Pa
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, g = lane >> 2, c4 = lane & 3;
   const PgCache& c = p.c;
   pa_share<RT, RT, BN>(p, &sm.share);
-  PaCut cut;
+  const PaCut cut(p, threadIdx.x == 0);
   PaAt at(sm.share);
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(sm.ring));
   const int word = t % WORDS, words = c.dim / 8;
@@ -1200,7 +1198,6 @@ __global__ void __launch_bounds__(PA_THREADS, 1) paged_attn_wide_kernel(const Pa
     }
     cut.note(sm.share, w);
   }
-  if (t == 0) cut.store(p);
 }
 
 // More than 16 rows: tcgen05. Two streams of blocks of 128 rows by 128 keys, whose scores S and sums O live in tensor memory: the two
@@ -1444,7 +1441,7 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1)
     const int half = warp - 2, words = c.dim / 8, word = lane % WORDS;
     const uint32_t q0 = smem_u32(smem), k0 = q0 + S::K, v0 = q0 + S::V;
     uint32_t n_k = 0, n_v = 0;
-    PaCut cut;
+    const PaCut cut(p, warp == 2 && lane == 0);
     const uint32_t lead = lane == 0 ? 1u : 0u;
     // A group of copies is told to the issuer when the next one is on its way, or before a wait.
     uint64_t* told = nullptr;
@@ -1566,7 +1563,6 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1)
         while (!mbar_test_wait(&sm.v_full[i % ST], (i / ST) & 1) && clock64() - t0 < 20000000ll) {
         }
     }
-    if (warp == 2 && lane == 0) cut.store(p);
   } else if (warp >= 4) {
     // ------------------------------------------------------------ softmax and results: stream t, a thread a row
     const int t = (warp - 4) >> 2, in_tile = (warp & 3) * 32 + lane;
@@ -1807,15 +1803,17 @@ __device__ __forceinline__ void pa_store_new(const PaParams& p, int64_t warp, in
   }
 }
 
-// CTA (x, y): the unit that starts in share x and goes on behind it, rows y, y + joiners, ... of it, or four times as many. Of many
-// pieces the warps take every fourth each, and their sums are joined in the order of the warps; few are one warp's work. Three reads
-// that depend on one another: about 3 us behind the attention. CTAs (x, joiners ..) store the call's new rows at the same
-// time.
+constexpr int PA_JOIN = 256;  // threads of a CTA that joins
+// CTAs (x, 0 .. joiners - 1) take their part of the unit that goes on behind share x: a unit's rows are dealt to the CTAs of all its
+// shares but the last, so that the more pieces there are, the more CTAs join them (one sequence of 60,000 positions, one key head, 64
+// nodes of 8 heads, bf16: 54 us instead of 167 with the CTAs of the first share alone). A row is one warp's work where the pieces are few
+// or the rows many; else its pieces are dealt to the warps of a CTA, whose sums are joined in the order of the warps. Three reads that
+// depend on one another: about 3 us behind the attention. CTAs (x, joiners ..) store the call's new rows at the same time.
 template <typename T, int DP>
-__global__ void __launch_bounds__(PA_THREADS) paged_attn_join_kernel(const PaParams p, int rt, int joiners) {
-  constexpr int WARPS = PA_THREADS / 32, C4 = DP / 4, PER = (C4 + 31) / 32;
+__global__ void __launch_bounds__(PA_JOIN) paged_attn_join_kernel(const PaParams p, int rt, int joiners) {
+  constexpr int WARPS = PA_JOIN / 32, C4 = DP / 4, PER = (C4 + 31) / 32;
   __shared__ float sums[WARPS][DP + 1];
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, first = blockIdx.x;
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   pg_begin();
   if (static_cast<int>(blockIdx.y) >= joiners) {
     const int64_t at = (static_cast<int64_t>(blockIdx.y - joiners) * gridDim.x + blockIdx.x) * WARPS + warp;
@@ -1824,12 +1822,12 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_join_kernel(const PaPar
     else pa_store_new<T>(p, at, all);
     return;
   }
-  const int4 a = p.cuts[2 * first];
-  const int last = p.cuts[2 * first + 1].x;
+  const int4 a = p.cuts[2 * blockIdx.x], shares = p.cuts[2 * blockIdx.x + 1];
+  if (a.x == 0) return;
+  const int first = shares.x, pieces = shares.y - shares.x + 1;
   const int64_t size = pa_piece(rt, DP);
   // (the unit is the last of its first share and the first of the others)
   const float* const at = p.work + 2 * static_cast<int64_t>(first) * size;
-  const int pieces = last - first + 1;
   // The sums of pieces begin, begin + step, ... of row r, relative to the row's m.
   const auto gather = [&](int r, float m, int begin, int step, float* l, float4 (&o)[PER]) {
     *l = 0.f;
@@ -1858,8 +1856,9 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_join_kernel(const PaPar
     for (int w = 16; w; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
     return m;
   };
-  if (pieces <= 8) {  // (the many rows of wide tiles: 256 rows in three pieces took 17 us with a CTA a row)
-    for (int r = blockIdx.y * WARPS + warp; r < a.x; r += joiners * WARPS) {
+  const int ctas = (pieces - 1) * joiners, cta = (static_cast<int>(blockIdx.x) - first) * joiners + blockIdx.y;
+  if (pieces <= 8 || a.x > 2 * ctas) {  // (256 rows in three pieces took 17 us with a CTA a row)
+    for (int r = warp * ctas + cta; r < a.x; r += ctas * WARPS) {
       float l;
       float4 o[PER];
       gather(r, most(r), 0, 1, &l, o);
@@ -1875,7 +1874,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_join_kernel(const PaPar
     }
     return;
   }
-  for (int r = blockIdx.y; r < a.x; r += joiners) {
+  for (int r = cta; r < a.x; r += ctas) {
     float l;
     float4 o[PER];
     gather(r, most(r), warp, WARPS, &l, o);
@@ -1895,7 +1894,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_join_kernel(const PaPar
     float all = 0.f;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) all += sums[w][DP];
-    for (int d = t; d < p.c.dim; d += PA_THREADS) {
+    for (int d = t; d < p.c.dim; d += PA_JOIN) {
       float x = 0.f;
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) x += sums[w][d];
@@ -1909,7 +1908,8 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_join_kernel(const PaPar
 struct PaForm {
   int dp, rt, bn, ctas, threads, smem;
   const void* kernel;
-  bool boxes;  // the kernel takes tensor maps of keys and values
+  bool boxes;      // the kernel takes tensor maps of keys and values
+  int joiners = 1;  // CTAs of a share that join: one for 32 rows
 };
 template <typename... A>
 static const void* pa_fn(void (*kernel)(A...)) {
@@ -1953,9 +1953,11 @@ static PaForm pa_form(int dim, int rows, bool words) {
 static PaForm pa_choose(const ytcuda_pages* c, int rows, int heads, bool words) {
   const int64_t share = (static_cast<int64_t>(rows) + c->slots - 1) / c->slots * (heads / c->kv_heads);
   const int r = static_cast<int>(share < 4096 ? share : 4096);
-  return c->dtype == YTC_F32    ? pa_form<float>(c->dim, r, words)
-         : c->dtype == YTC_BF16 ? pa_form<__nv_bfloat16>(c->dim, r, words)
-                                : pa_form<__half>(c->dim, r, words);
+  PaForm f = c->dtype == YTC_F32    ? pa_form<float>(c->dim, r, words)
+             : c->dtype == YTC_BF16 ? pa_form<__nv_bfloat16>(c->dim, r, words)
+                                    : pa_form<__half>(c->dim, r, words);
+  f.joiners = ((r < f.rt ? r : f.rt) + 31) / 32;
+  return f;
 }
 static uint64_t pa_pieces(const PaForm& f) { return 4ull * 2 * static_cast<uint64_t>(f.ctas) * static_cast<uint64_t>(pa_piece(f.rt, f.dp)); }
 static uint64_t pa_space(const PaForm& f) { return pa_pieces(f) + 2ull * sizeof(int4) * static_cast<uint64_t>(f.ctas); }
@@ -1980,13 +1982,12 @@ static int pa_boxes(const PgCache& c, int dtype, CUtensorMap* k, CUtensorMap* v)
 
 template <typename T>
 static cudaError_t pa_join(const PaForm& f, const PaParams& p, cudaStream_t st) {
-  const int joiners = f.rt <= 32 ? 4 : f.rt / 16;
   // a warp for each new row and head, up to eight rows of CTAs
-  const int64_t stored = p.fresh ? (static_cast<int64_t>(p.rows) * p.c.heads - 1) / (f.ctas * (PA_THREADS / 32)) + 1 : 0;
-  const dim3 grid(f.ctas, joiners + static_cast<int>(stored < 8 ? stored : 8)), block(PA_THREADS);
-  if (f.dp == 64) return pg_launch(paged_attn_join_kernel<T, 64>, grid, block, 0, st, p, f.rt, joiners);
-  if (f.dp == 128) return pg_launch(paged_attn_join_kernel<T, 128>, grid, block, 0, st, p, f.rt, joiners);
-  return pg_launch(paged_attn_join_kernel<T, 256>, grid, block, 0, st, p, f.rt, joiners);
+  const int64_t stored = p.fresh ? (static_cast<int64_t>(p.rows) * p.c.heads - 1) / (f.ctas * (PA_JOIN / 32)) + 1 : 0;
+  const dim3 grid(f.ctas, f.joiners + static_cast<int>(stored < 8 ? stored : 8)), block(PA_JOIN);
+  if (f.dp == 64) return pg_launch(paged_attn_join_kernel<T, 64>, grid, block, 0, st, p, f.rt, f.joiners);
+  if (f.dp == 128) return pg_launch(paged_attn_join_kernel<T, 128>, grid, block, 0, st, p, f.rt, f.joiners);
+  return pg_launch(paged_attn_join_kernel<T, 256>, grid, block, 0, st, p, f.rt, f.joiners);
 }
 
 }  // namespace ytk

@@ -40,6 +40,14 @@ def test_bad_caches(change):
     assert all(rc == _lib.INVALID_ARG for rc in calls(None, at))
 
 
+@pytest.mark.parametrize("change", [dict(layers=1 << 14, kv_heads=1 << 10, dim=4), dict(layers=1 << 16, kv_heads=8, dim=64, page=1 << 15),
+                                    dict(pages=1 << 30), dict(slots=1 << 30, max_pages=1)])
+def test_extents_above_the_limits(change):
+    at = (C.addressof(HERE) + 15) // 16 * 16
+    c = cache(**change)
+    assert all(rc == _lib.INVALID_ARG for rc in calls(C.addressof(c), at))
+
+
 def test_bad_arguments():
     L, st = _lib.lib(), (C.c_int64 * 8)(*[128, 64] * 4)
     at = (C.addressof(HERE) + 15) // 16 * 16

@@ -461,6 +461,35 @@ def test_results_are_the_same_every_time(paged, dtype, groups):
         assert torch.equal(first, b.d.attend(0, q, ints([0, 9, 10, 40]), k, v))
 
 
+def test_accepted_without_columns(paged):
+    """No row can be kept of none: a kept row is refused, as it is of a shorter list."""
+    b = Both(paged, pages=20, page=4, slots=3, max_pages=4)
+    b.fill([3, 5, 2])
+    b.reserve([2, 2, 2])
+    none = torch.zeros(3, 0, dtype=torch.int32, device="cuda")
+    b.d.keep(ints([0, 1, 0]), none)
+    assert b.d.lens.tolist() == [3, 5, 2]
+    with pytest.raises(RuntimeError):
+        b.d.check()
+    b.d.keep(ints([0, 0, 0]), none, base=ints([2, 4, 0]))
+    assert b.d.lens.tolist() == [2, 4, 0]
+    b.d.check()
+
+
+def test_rows_of_q_that_overlap(paged):
+    """Queries are only read: they may lie in one another, and the result is a tensor of its own."""
+    b = Both(paged, layers=1, heads=2, dim=64, page=16, pages=20, slots=1, max_pages=8)
+    b.fill([40])
+    b.reserve([5])
+    flat = b.randn(400)
+    k = b.randn(5, 2, 64)
+    for strides in ((1, 1, 1), (1, 64, 1), (0, 64, 1), (64, 0, 1), (0, 0, 1)):
+        q = flat.as_strided((5, 2, 64), strides)
+        got = b.d.attend(0, q, ints([0, 5]), k, k)
+        assert got.stride(2) == 1
+        b.near(got, *b.p.attend(0, host(q), [0, 5], None, host(k), host(k), 0.0), 45)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("nodes,groups", [(1, 1), (1, 7), (5, 3), (16, 1), (33, 2), (64, 5), (200, 3)])
 @pytest.mark.parametrize("dim", [64, 130, 256])

@@ -530,10 +530,15 @@ int pg_take(const char* who, const ytcuda_pages* c, PgCache* out) {
   YTC_REQUIRE(c->layers >= 1 && c->pages >= 0 && c->page >= 1 && c->kv_heads >= 1 && c->dim >= 1 && c->slots >= 0 && c->max_pages >= 0,
               "%s: bad extents (layers %d, pages %d of %d positions, heads %d, dim %d, slots %d of %d pages)", who, c->layers, c->pages,
               c->page, c->kv_heads, c->dim, c->slots, c->max_pages);
-  YTC_REQUIRE(c->page <= 65536 && c->kv_heads <= 65536 && c->dim <= 65536 && c->layers <= 65536 &&
+  // (below them the numbers that kernels keep in 32 bits do not overflow: pieces of all layers of a page, words that a warp moves)
+  YTC_REQUIRE(c->page <= 65536 && c->kv_heads <= 65536 && c->dim <= 65536 && c->layers <= 65536 && c->slots < (1 << 30) && c->pages < (1 << 30) &&
                   static_cast<int64_t>(c->slots) * c->max_pages < (1ll << 31) &&
-                  static_cast<int64_t>(c->page) * c->kv_heads * c->dim < (1ll << 31),
-              "%s: extents above the limits (pages of 65536 positions and 2^31 elements a layer, tables of 2^31 entries)", who);
+                  static_cast<int64_t>(c->page) * c->kv_heads * c->dim < (1ll << 31) &&
+                  static_cast<int64_t>(c->layers) * c->kv_heads * c->dim <= (1ll << 25) &&
+                  static_cast<int64_t>(c->layers) * c->kv_heads * c->dim * c->page < (1ll << 36),
+              "%s: extents above the limits (pages of 65536 positions and 2^31 elements a layer, 2^25 elements a position and 2^36 a page of all "
+              "layers, 2^30 slots and pages, tables of 2^31 entries)",
+              who);
   YTC_REQUIRE(c->slots == 0 || c->pages == 0 || (c->k && c->v && c->lens && c->held && c->refs && c->status && c->scratch &&
                                                 (c->table || c->max_pages == 0)),
               "%s: null tensor in the cache", who);
@@ -644,7 +649,6 @@ int ytcuda_pages_keep(const ytcuda_pages* cache, const int32_t* kept, const int3
   if (c.slots == 0) return YTC_OK;
   YTC_REQUIRE(kept != nullptr, "%s: null kept", who);
   YTC_REQUIRE(c.pages > 0, "%s: a pool without pages", who);
-  if (depth == 0) accepted = nullptr;
   const int size = dtype_size(cache->dtype);
   const int width = pg_width(pg_bits(c.k) | pg_bits(c.v) | static_cast<uint64_t>(c.dim * size));
   // three CTAs an SM, all that it holds, where there is that much to move: a warp's items one behind another

@@ -139,9 +139,10 @@ class PagedCache:
         accepted rows ascend along a row; without `accepted` the first kept[slot] rows stay where they are. The pages behind
         stay with the slot, for the next drafted rows."""
         depth = accepted.shape[-1] if accepted is not None and accepted.dim() else 0
+        kept_at = self._ints(kept, "kept", self._per_slot)
         check(self._lib.ytcuda_pages_keep(
-            self._at, self._ints(kept, "kept", self._per_slot),
-            None if accepted is None else self._ints(accepted, "accepted", (self.slots, depth)), depth,
+            self._at, kept_at,  # (no columns: nothing of it is read, but it is not "without accepted")
+            None if accepted is None else self._ints(accepted, "accepted", (self.slots, depth)) or kept_at, depth,
             None if base is None else self._ints(base, "base", self._per_slot), self._stream()))
 
     def compact(self, into: "PagedCache") -> None:
@@ -185,6 +186,8 @@ class PagedCache:
         qr, qh, _ = self._rows(q, "q", shape)
         if out is None:
             out = torch.empty_like(q)
+            if out.stride(2) != 1:  # (rows of q that overlap)
+                out = torch.empty(shape, dtype=q.dtype, device=q.device)
             o_row, o_head, _ = out.stride()
         else:
             o_row, o_head, _ = self._rows(out, "out", shape)
@@ -197,9 +200,10 @@ class PagedCache:
             kp, vp, strides = None, None, _EIGHT(qr, qh, o_row, o_head, 0, 0, 0, 0)
         else:
             raise _bad("paged cache: k and v come together")
-        if self._space[0] != (rows, heads):
-            self._space = (rows, heads), self._lib.ytcuda_pages_attend_workspace(self._at, rows, heads)
-        size = self._space[1]
+        known = self._space
+        if known[0] != (rows, heads):
+            known = self._space = (rows, heads), self._lib.ytcuda_pages_attend_workspace(self._at, rows, heads)
+        size = known[1]
         # (its own for every call: two streams, or two captured graphs, never share it)
         space = self.status.new_empty((size + 3) // 4)
         check(self._lib.ytcuda_pages_attend(self._at, self._layer(layer), q.data_ptr(), out.data_ptr(), kp, vp, strides,

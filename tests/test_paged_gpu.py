@@ -50,6 +50,11 @@ class Both:
             make = lambda: torch.full(shape, math.nan, dtype=dtype, device="cuda")  # noqa: E731
         elif layout == "rows":  # [layers, pages, page, heads, dim]
             make = lambda: torch.full((layers, pages, page, heads, dim), math.nan, dtype=dtype, device="cuda").transpose(2, 3)  # noqa: E731
+        elif layout == "far":  # 1.6 GB from page to page: offsets in bytes and in elements pass 32 bits
+            stride = (1600 << 20) // torch.finfo(dtype).bits * 8
+            space = torch.empty(layers * pages * stride, dtype=dtype, device="cuda")
+            make = lambda: space.as_strided(shape, (pages * stride, stride, page * dim, dim, 1), space_at.pop()).fill_(math.nan)  # noqa: E731
+            space_at = [stride // 2, 0]  # (values half way between keys)
         else:  # odd strides: no row starts on more than an element's boundary
             make = lambda: torch.full((*shape[:-1], dim + 3), math.nan, dtype=dtype, device="cuda")[..., 1:dim + 1]  # noqa: E731
         zeros = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")  # noqa: E731
@@ -459,6 +464,29 @@ def test_results_are_the_same_every_time(paged, dtype, groups):
     first = b.d.attend(0, q, ints([0, 9, 10, 40]), k, v)
     for _ in range(20):
         assert torch.equal(first, b.d.attend(0, q, ints([0, 9, 10, 40]), k, v))
+
+
+@pytest.mark.parametrize("dtype,dim,groups", [(BF16, 64, 2), (BF16, 64, 30), (F16, 128, 30), (BF16, 256, 30), (F16, 256, 2), (F32, 128, 2),
+                                              (F32, 30, 3), (BF16, 30, 9)])
+def test_offsets_above_32_bits(paged, dtype, dim, groups):
+    b = Both(paged, layers=2, heads=2, dim=dim, page=32, pages=7, slots=2, max_pages=6, dtype=dtype, layout="far")
+    b.fill([90, 20])
+    b.reserve([5, 8])
+    b.attend(1, [5, 8], groups)
+    b.append(0, [5, 8])
+    b.keep([3, 4], [[0, 2, 4, 0], [1, 2, 5, 7]])
+    b.attend(1, [1, 3], groups)
+    b.fork([0, 0])
+    b.reserve([7, 9])
+    b.append(0, [7, 9])
+    b.attend(1, [7, 9], groups)
+    b.keep([7, 9])
+    b.same()
+    other = Both(paged, layers=2, heads=2, dim=dim, page=32, pages=7, slots=2, max_pages=6, dtype=dtype)
+    b.d.compact(other.d)
+    b.p.compact(other.p)
+    other.same()
+    torch.cuda.empty_cache()
 
 
 def test_accepted_without_columns(paged):

@@ -128,7 +128,7 @@ __device__ __forceinline__ void pa_share(const PaParams& p, PaShare* out) {
   __syncthreads();
 }
 
-// A piece of work: key tiles t0 .. t1 of a unit that has `tiles`, each of cost `weight`, the first of them number `first` of all costs.
+// A piece of work: key tiles t0 .. t1 of a unit that sees `tiles` of them, each of cost `weight`, the first of them number `first` of all costs.
 struct PaPart {
   PaSlot s;
   uint32_t tiles, t0, t1, weight, first;
@@ -140,7 +140,10 @@ struct PaAt {
   int slot;
   __device__ __forceinline__ explicit PaAt(const PaShare& s) : pos(s.from), end(s.to), off(s.off), slot(s.slot) {}
 };
-// The next piece of the share; false behind the last one. A key tile belongs to the share that its first cost lies in.
+// The next piece of the share; false behind the last one. A key tile belongs to the share that its first cost lies in. No node sees a
+// later one: tiles behind the last node of a row tile are passed over. In the line they count all the same, but the row tiles stand
+// there as first, last, second, last but one, ..., so that what is passed over is about the same in every share of many row tiles (four
+// prompts of 8000, fp16, 8 key heads of 4: 9.2 ms with all tiles, 8.6 passed over in order, 5.1 so).
 template <int RT, int RW, int BN>
 __device__ __forceinline__ bool pa_next(const PaParams& p, PaAt* at, PaPart* out) {
   using Cost = PaCost<RT, RW>;
@@ -155,23 +158,26 @@ __device__ __forceinline__ bool pa_next(const PaParams& p, PaAt* at, PaPart* out
       continue;
     }
     r.slot = at->slot;
-    r.tiles = pa_key_tiles<BN>(r.s);
-    const uint32_t blocks = pa_row_blocks<RW>(p, r.s), a_head = r.tiles * Cost::of(blocks);
+    const uint32_t tiles = pa_key_tiles<BN>(r.s), blocks = pa_row_blocks<RW>(p, r.s), a_head = tiles * Cost::of(blocks);
     const uint32_t head = at->off / a_head, in_head = at->off - head * a_head;
-    const uint32_t unit = in_head / (r.tiles * Cost::BOTH), in_unit = in_head - unit * (r.tiles * Cost::BOTH);
-    r.weight = blocks - unit * Cost::BLOCKS >= Cost::BLOCKS ? Cost::BOTH : Cost::ONE;
-    const uint32_t n = min(r.tiles * r.weight - in_unit, at->end - at->pos);
+    const uint32_t unit = in_head / (tiles * Cost::BOTH), in_unit = in_head - unit * (tiles * Cost::BOTH);
+    const uint32_t full = blocks / Cost::BLOCKS;  // units of BOTH
+    r.weight = unit < full ? Cost::BOTH : Cost::ONE;
+    const uint32_t n = min(tiles * r.weight - in_unit, at->end - at->pos);
     r.first = at->pos - in_unit;
     r.t0 = (in_unit + r.weight - 1) / r.weight;
     r.t1 = (in_unit + n + r.weight - 1) / r.weight;
     at->pos += n;
     at->off += n;
-    if (r.t0 == r.t1) continue;
     r.head = static_cast<int>(head);
-    r.rtile = static_cast<int>(unit);
+    r.rtile = static_cast<int>(unit >= full ? unit : unit & 1 ? full - 1 - unit / 2 : unit / 2);
     r.row0 = r.rtile * RT;
     r.rows_all = r.s.nodes * p.groups;
     r.rows = min(RT, r.rows_all - r.row0);
+    const uint32_t last = p.by_group.of(static_cast<uint32_t>(r.row0 + r.rows - 1));  // node of the last row
+    r.tiles = (static_cast<uint32_t>(r.s.len) + last + BN) / BN;
+    r.t1 = min(r.t1, r.tiles);
+    if (r.t0 >= r.t1) continue;
     return true;
   }
   return false;

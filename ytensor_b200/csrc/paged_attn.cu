@@ -257,6 +257,14 @@ __device__ __forceinline__ uint64_t pa_sees(const uint32_t* line, int words, int
   return low | (n0 < 0 ? bits << -n0 : bits);
 }
 
+// Whether any of NK keys is hidden from any row of the warp: in a prompt's tiles few are, and looking for hidden values that are not
+// finite takes as long as the products.
+template <int NK>
+__device__ __forceinline__ bool pa_any_hidden(const uint64_t (&sees)[2]) {
+  constexpr uint64_t all = NK < 64 ? (1ull << (NK % 64)) - 1 : ~0ull;
+  return __any_sync(0xffffffffu, (sees[0] & sees[1] & all) != all);
+}
+
 // Positions of a slot whose rows are in the pages.
 __device__ __forceinline__ uint32_t pa_paged(const PaParams& p, const PaPart& w) {
   return static_cast<uint32_t>(w.s.len) + (p.fresh ? 0u : static_cast<uint32_t>(w.s.nodes));
@@ -1017,11 +1025,12 @@ __global__ void __launch_bounds__(PaNarrow<T, DP>::THREADS, PaNarrow<T, DP>::CTA
       out = out == ST - 1 ? 0 : out + 1;
       const int n0 = static_cast<int>((tile - (ST - 1)) * BN + mine) - w.s.len;  // the node at the first key
       if (n0 < w.s.nodes) {
-        const bool hides = n0 + KEYS > 0;
+        bool hides = n0 + KEYS > 0;
         uint64_t sees[2] = {0, 0};
         if (hides) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) sees[h] = pa_sees(p.parents ? sm.seen[node[h] - node0] : nullptr, words_seen, node[h], n0);
+          hides = pa_any_hidden<KEYS>(sees);
         }
         x.template step<KEYS>(kt, kt + S::SLOT, p.scale, q_at, hides, sees, sm.spare[warp]);
       }
@@ -1082,25 +1091,26 @@ __global__ void __launch_bounds__(PaNarrow<T, DP>::THREADS, PaNarrow<T, DP>::CTA
   }
 }
 
-// More than 16 rows of 136 to 256 dims (O of two streams would not fit beside S in tensor memory): a warp for 16 of up to 64 rows (warps
-// without rows only copy), all over the same tiles of keys. Bound by mma.sync (8.5 clocks each and scheduler): 64 rows of dim 256 behind
-// 16000 keys, eight slots of eight heads, 700 us, 96 TFLOP/s.
+// More than 16 rows of 136 to 256 dims (O of two streams would not fit beside S in tensor memory): a warp for 16 of up to 128 rows (warps
+// without rows only copy), all over the same tiles of keys. Bound by chains of instructions that wait for one another, two warps a
+// scheduler (all that the registers hold): 256 rows of dim 256 behind 16000 keys, eight slots of eight heads, 1.44 ms, 187 TFLOP/s (with
+// four warps 2.66; mma.sync alone would take 0.5).
 template <typename T>
 struct PaWide {
-  static constexpr int DP = 256, RT = 64, BN = 32, STAGES = 3, SLOT = BN * DP * 2;
+  static constexpr int DP = 256, WARPS = 8, THREADS = 32 * WARPS, RT = 16 * WARPS, BN = 32, STAGES = 3, SLOT = BN * DP * 2;
   uint4 ring[STAGES][2][SLOT / 16];
   uint4 q[RT * DP * 2 / 16];
   const char* row[2][2][BN];  // (where the next tile's rows lie)
-  float spare[4][16 * 8];
+  float spare[WARPS][16 * 8];
   uint32_t seen[RT][PA_TREE / 32 + 1];
   int16_t up[PA_TREE];
   PaShare share;
 };
 
 template <typename T>
-__global__ void __launch_bounds__(PA_THREADS, 1) paged_attn_wide_kernel(const PaParams p) {
+__global__ void __launch_bounds__(PaWide<T>::THREADS, 1) paged_attn_wide_kernel(const PaParams p) {
   using S = PaWide<T>;
-  constexpr int DP = S::DP, RT = S::RT, BN = S::BN, ST = S::STAGES, WORDS = DP / 8, PER = PA_THREADS / WORDS;
+  constexpr int DP = S::DP, RT = S::RT, BN = S::BN, ST = S::STAGES, WORDS = DP / 8, PER = S::THREADS / WORDS;
   static_assert(ST == 3, "two tiles on their way, one worked on");
   extern __shared__ __align__(128) unsigned char raw[];
   S& sm = *reinterpret_cast<S*>(raw);
@@ -1170,11 +1180,12 @@ __global__ void __launch_bounds__(PA_THREADS, 1) paged_attn_wide_kernel(const Pa
       out = out == ST - 1 ? 0 : out + 1;
       const int n0 = static_cast<int>((tile - (ST - 1)) * BN) - w.s.len;
       if (16 * warp < w.rows && n0 <= node1) {
-        const bool hides = n0 + BN > 0;
+        bool hides = n0 + BN > 0;
         uint64_t sees[2] = {0, 0};
         if (hides) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) sees[h] = pa_sees(p.parents ? sm.seen[min(node[h], node1) - node0] : nullptr, words_seen, node[h], n0);
+          hides = pa_any_hidden<BN>(sees);
         }
         x.template step<BN>(kt, kt + S::SLOT, p.scale, q_at, hides, sees, sm.spare[warp]);
       }
@@ -1943,7 +1954,7 @@ static PaForm pa_form(int rows, bool words) {
       } else {
         using W = PaWide<T>;
         static_assert(sizeof(W) <= PA_SHARED, "shared memory");
-        return PaForm{DP, W::RT, W::BN, sm_count(), PA_THREADS, static_cast<int>(sizeof(W)), pa_fn(paged_attn_wide_kernel<T>), false};
+        return PaForm{DP, W::RT, W::BN, sm_count(), W::THREADS, static_cast<int>(sizeof(W)), pa_fn(paged_attn_wide_kernel<T>), false};
       }
     }
   }

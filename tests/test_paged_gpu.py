@@ -454,6 +454,27 @@ def test_numbers_in_hidden_places(paged, dtype, dim, groups):
                 assert torch.equal(got[row], plain[row]), row
 
 
+@pytest.mark.parametrize("dtype,dim,groups", [(F32, 64, 1), (F32, 20, 2), (BF16, 64, 1), (BF16, 64, 4), (F16, 128, 3), (BF16, 128, 12), (BF16, 30, 4),
+                                              (BF16, 256, 2), (F16, 200, 5)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_numbers_in_hidden_places_of_a_chain(paged, dtype, dim, groups, bad):
+    """Pieces of prompts: what is no number reaches the rows that see it, whole tiles of keys behind it, and no row in front."""
+    b = Both(paged, layers=1, heads=1, dim=dim, slots=3, page=32, pages=60, max_pages=30, dtype=dtype)
+    b.fill([70, 0, 5])
+    b.reserve([500, 333, 3])
+    q, k, v = b.randn(836, groups, dim), b.randn(836, 1, dim), b.randn(836, 1, dim)
+    starts = ints([0, 500, 833, 836])
+    plain = b.d.attend(0, q, starts, k, v)
+    v2 = v.clone()
+    v2[100, 0, 5] = v2[300, 0, 3] = v2[700, 0, 2] = bad
+    got = b.d.attend(0, q, starts, k, v2)
+    touched = torch.zeros(836, dim, dtype=torch.bool, device="cuda")
+    touched[100:500, 5] = touched[300:500, 3] = touched[700:833, 2] = True
+    touched = touched[:, None].expand_as(got)
+    assert not bool(torch.isfinite(got[touched]).any())
+    assert torch.equal(got[~touched], plain[~touched])
+
+
 @pytest.mark.parametrize("dtype,groups", [(F32, 4), (BF16, 4), (BF16, 16), (F16, 16)])
 def test_results_are_the_same_every_time(paged, dtype, groups):
     """The same call twice gives the same bits."""

@@ -143,7 +143,8 @@ struct PaAt {
 // The next piece of the share; false behind the last one. A key tile belongs to the share that its first cost lies in. No node sees a
 // later one: tiles behind the last node of a row tile are passed over. In the line they count all the same, but the row tiles stand
 // there as first, last, second, last but one, ..., so that what is passed over is about the same in every share of many row tiles (four
-// prompts of 8000, fp16, 8 key heads of 4: 9.2 ms with all tiles, 8.6 passed over in order, 5.1 so).
+// prompts of 8000, fp16, 8 key heads of 4: 9.2 ms with all tiles, 8.6 passed over in order, 5.1 so; 3.2, 655 TFLOP/s, since tiles that
+// all rows see are neither masked nor looked through).
 template <int RT, int RW, int BN>
 __device__ __forceinline__ bool pa_next(const PaParams& p, PaAt* at, PaPart* out) {
   using Cost = PaCost<RT, RW>;
@@ -1287,8 +1288,8 @@ __device__ __noinline__ bool pa_wait_long(uint64_t* bar, uint32_t parity, volati
 __device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity, volatile int* stop) {
   return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || pa_wait_long(bar, parity, stop);
 }
-// Half of a tile has landed: the issuer may have it. look_at: the tile holds values of nodes; one that is not finite and that not every
-// row sees must not meet a weight of zero: it is taken out here, and goes in at the end.
+// Half of a tile has landed: the issuer may have it. look_at: the tile holds values that not every row sees; one that is not finite must
+// not meet a weight of zero: it is taken out here, and goes in at the end.
 template <typename T, int DP>
 __device__ __noinline__ void pa_tell(uint64_t* bar, uint32_t look_at, int half, int* odd) {
   constexpr int WORDS = DP / 8, PER = 32 / WORDS;
@@ -1322,7 +1323,8 @@ __device__ __noinline__ void pa_tell(uint64_t* bar, uint32_t look_at, int half, 
   __syncwarp();
   if (lane == 0) mbar_arrive(bar);
 }
-// What the values that pa_tell took out of the part's tiles add to column d of a node's row.
+// What the values that pa_tell took out of the part's tiles add to column d of a node's row. (One that stayed in, in a tile that all
+// rows see, is added once more: no infinity changes by it.)
 template <typename T, int BN>
 __device__ __noinline__ float pa_odd_values(const PaParams& p, const PaPart& w, const int16_t* up, int node, int d) {
   float sum = 0.f;
@@ -1472,6 +1474,8 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1)
     };
     const int my_boxes = p.box == 128 ? 1 - half : p.box ? 64 / p.box : 0;  // (a box that is a whole tile is fetched by one warp)
     while (ok && pa_next<RT, RW, BN>(p, &at, &w)) {
+      // all rows see the positions in front of `open`
+      const int64_t open = w.s.len + (p.parents ? 0 : static_cast<int64_t>(p.by_group.of(w.row0)) + 1);
       // tiles in front of `plain` hold no nodes; pages of a tile, a lane a box or a lane two rows
       const uint32_t plain = p.box ? min(static_cast<uint32_t>(w.s.len) / BN, w.t1) : 0;
       const auto lookup = [&](uint32_t tile, int (&pg)[2]) {
@@ -1545,7 +1549,7 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1)
             const PaRow r = pa_row(p, w, tile * BN + 64 * half + 32 * x + lane, pg[x]);
             from[x] = reinterpret_cast<unsigned long long>(v ? r.v : r.k);
           }
-          if (v && static_cast<int64_t>(tile + 1) * BN > w.s.len) look = to;
+          if (v && static_cast<int64_t>(tile + 1) * BN > open) look = to;
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -1619,9 +1623,12 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1)
         }
         tc_fence_after();
         const int n0 = static_cast<int>((w.t0 + (split ? 2 * j + t : j)) * BN) - w.s.len;
-        const bool masked = n0 + BN > 0;
+        bool masked = n0 + BN > 0;
         uint32_t bits[4];
-        if (masked) pa_sees128(up, node, n0, bits);
+        if (masked) {
+          pa_sees128(up, node, n0, bits);
+          masked = __any_sync(0xffffffffu, (bits[0] & bits[1] & bits[2] & bits[3]) != 0xffffffffu);
+        }
         __syncwarp();
         if (masked) {  // what is hidden is -infinity from here on
 #pragma unroll 1

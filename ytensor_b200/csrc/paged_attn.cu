@@ -1323,16 +1323,20 @@ __device__ __noinline__ void pa_tell(uint64_t* bar, uint32_t look_at, int half, 
   __syncwarp();
   if (lane == 0) mbar_arrive(bar);
 }
-// What the values that pa_tell took out of the part's tiles add to column d of a node's row. (One that stayed in, in a tile that all
-// rows see, is added once more: no infinity changes by it.)
+// What the values that pa_tell took out of the part's tiles add to column d of a node's row: those of the nodes that it sees and, where the
+// first of the tiles begins in front of the nodes, of the sequence's last positions, which all rows see. (One that stayed in, in a tile
+// that all rows see, is added once more: no infinity changes by it.)
 template <typename T, int BN>
 __device__ __noinline__ float pa_odd_values(const PaParams& p, const PaPart& w, const int16_t* up, int node, int d) {
   float sum = 0.f;
-  const int64_t end = static_cast<int64_t>(w.t1) * BN - w.s.len, begin = static_cast<int64_t>(w.t0) * BN - w.s.len;
-  for (int j = static_cast<int>(end <= node ? end - 1 : node); j >= 0 && j >= begin; --j) {
-    uint32_t sees[4];
-    pa_sees128(up, node, j, sees);
-    if (!(sees[0] & 1)) continue;
+  const uint32_t t0 = max(w.t0, static_cast<uint32_t>(w.s.len) / BN);  // (tiles in front of it hold no nodes)
+  const int64_t end = static_cast<int64_t>(w.t1) * BN - w.s.len, begin = static_cast<int64_t>(t0) * BN - w.s.len;
+  for (int j = static_cast<int>(end <= node ? end - 1 : node); j >= begin; --j) {
+    if (j >= 0) {
+      uint32_t sees[4];
+      pa_sees128(up, node, j, sees);
+      if (!(sees[0] & 1)) continue;
+    }
     const uint32_t at = static_cast<uint32_t>(w.s.len + j);
     const T* v = reinterpret_cast<const T*>(pa_row(p, w, at, pa_lookup(p, w, at)).v);
     const float y = v ? pa_load(v + d) : 0.f;

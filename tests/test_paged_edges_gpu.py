@@ -52,3 +52,50 @@ def test_numbers_in_seen_places(paged, dtype, dim, groups, length, places, tree)
     b.d.k[0, int(b.d.table[0, places[0] // 16]), 0, places[0] % 16, 1] = math.nan
     got = b.d.attend(0, q, starts, k, v, parents=parents)
     assert bool(torch.isnan(got[:6]).all()) and torch.equal(got[6:], plain[6:])
+
+
+@pytest.mark.parametrize("dtype,dim,groups", [(BF16, 64, 1), (F16, 128, 4), (BF16, 128, 12)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_one_number_that_is_none_in_a_deep_tree(paged, dtype, dim, groups, bad):
+    """1024 nodes, most of them in one line, and a value that those behind it see: the rows are right and the call is not given up."""
+    n = 1024
+    b = Both(paged, layers=1, heads=2, dim=dim, slots=2, page=32, pages=160, max_pages=100, dtype=dtype, seed=groups)
+    b.fill([300, 70])
+    b.reserve([n, 40])
+    q, k, v = b.randn(n + 40, 2 * groups, dim), b.randn(n + 40, 2, dim), b.randn(n + 40, 2, dim)
+    parents = [max(-1, i - (2 if i % 50 == 7 else 1)) for i in range(n)] + [i - 1 for i in range(40)]
+    starts, up = ints([0, n, n + 40]), ints(parents)
+    plain = b.d.attend(0, q, starts, k, v, parents=up)
+    for node in (0, 6, 500):
+        v2 = v.clone()
+        v2[node, 1, dim - 3] = bad
+        got = b.d.attend(0, q, starts, k, v2, parents=up)
+        wrong = torch.zeros_like(got, dtype=torch.bool)
+        sees = [False] * n
+        for i in range(n):
+            sees[i] = i == node or (parents[i] >= 0 and sees[parents[i]])
+        wrong[:n, groups:, dim - 3] = torch.tensor(sees, device="cuda")[:, None]
+        assert torch.equal(got[~wrong], plain[~wrong])
+        assert bool(torch.isnan(got[wrong]).all()) if math.isnan(bad) else bool((got[wrong] == bad).all())
+    from ytensor_b200 import _lib
+    assert _lib.lib().ytcuda_device_status(None) == _lib.OK
+
+
+@pytest.mark.parametrize("dtype,dim,groups", [(BF16, 64, 1), (F16, 128, 4), (BF16, 128, 4)])
+def test_one_number_that_is_none_in_a_long_chain(paged, dtype, dim, groups):
+    """A prompt of thousands of tokens: rows from the number on, and no others."""
+    n, node, bad = 6000, 2500, math.nan
+    b = Both(paged, layers=1, heads=1, dim=dim, slots=1, page=128, pages=60, max_pages=60, dtype=dtype)
+    b.fill([200])
+    b.reserve([n])
+    q, k, v = b.randn(n, groups, dim), b.randn(n, 1, dim), b.randn(n, 1, dim)
+    starts = ints([0, n])
+    plain = b.d.attend(0, q, starts, k, v)
+    v2 = v.clone()
+    v2[node, 0, 11] = bad
+    got = b.d.attend(0, q, starts, k, v2)
+    wrong = torch.zeros_like(got, dtype=torch.bool)
+    wrong[node:, :, 11] = True
+    assert bool(torch.isnan(got[wrong]).all()) and torch.equal(got[~wrong], plain[~wrong])
+    from ytensor_b200 import _lib
+    assert _lib.lib().ytcuda_device_status(None) == _lib.OK

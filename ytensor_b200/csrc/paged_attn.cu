@@ -1235,11 +1235,14 @@ struct PaTc {
     uint64_t q_full, q_free, k_full[STAGES], v_full[STAGES], k_free[STAGES], v_free[STAGES], s_full[2], p_full[2], o_ready[2], o_free[2], met;
     uint32_t tmem;
     int stop;  // a wait has run out
-    int odd;   // there are hidden values that are not finite
+    int odd[8];  // number of the part, from 1, in which a tile that was looked through had values that are not finite (by the part's number)
     float m[2][2][128], l[2][2][128];  // of the two streams over the same rows; by turns
     int16_t up[8][PA_TREE];            // a slot's parents, for each softmax warp
     PaShare share;
   };
+  // (of the parts behind the one whose results a warp writes, the other stream may have weighed one, and the values of STAGES tiles, one of a
+  // part at least, may be here)
+  static_assert(STAGES + 2 <= 8, "numbers of parts at hand");
   static constexpr int BYTES = REST + static_cast<int>(sizeof(Rest)) + 1024;
   // Where 16-byte word `w` of row `r` of a tile lies.
   static __device__ __forceinline__ uint32_t at(int r, int w) { return (w >> 3) * (128 * 128) + r * 128 + (((w & 7) ^ (r & 7)) << 4); }
@@ -1291,7 +1294,7 @@ __device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity, volatile
 // Half of a tile has landed: the issuer may have it. look_at: the tile holds values that not every row sees; one that is not finite must
 // not meet a weight of zero: it is taken out here, and goes in at the end.
 template <typename T, int DP>
-__device__ __noinline__ void pa_tell(uint64_t* bar, uint32_t look_at, int half, int* odd) {
+__device__ __noinline__ void pa_tell(uint64_t* bar, uint32_t look_at, int half, int* odd, uint32_t part) {
   constexpr int WORDS = DP / 8, PER = 32 / WORDS;
   const int lane = threadIdx.x & 31, word = lane % WORDS;
   if (look_at) {
@@ -1317,32 +1320,45 @@ __device__ __noinline__ void pa_tell(uint64_t* bar, uint32_t look_at, int half, 
         any = any || here;
       }
     }
-    if (__any_sync(0xffffffffu, any) && lane == 0) atomicExch(odd, 1);
+    if (__any_sync(0xffffffffu, any) && lane == 0) atomicExch(odd + part % 8, static_cast<int>(part + 1));
   }
   fence_proxy_async_smem();
   __syncwarp();
   if (lane == 0) mbar_arrive(bar);
 }
-// What the values that pa_tell took out of the part's tiles add to column d of a node's row: those of the nodes that it sees and, where the
-// first of the tiles begins in front of the nodes, of the sequence's last positions, which all rows see. (One that stayed in, in a tile
-// that all rows see, is added once more: no infinity changes by it.)
+// All rows of a part see the positions in front of this one: pa_tell looks through the key tiles from the one that it lies in on.
+__device__ __forceinline__ int64_t pa_open(const PaParams& p, const PaPart& w) {
+  return w.s.len + (p.parents ? 0 : static_cast<int64_t>(p.by_group.of(w.row0)) + 1);
+}
+// What the values that pa_tell took out of the part's tiles add to columns d .. d + 15 of a node's row: those of the nodes that it sees and,
+// where the first of the tiles begins in front of the nodes, of the sequence's last positions, which all rows see. Up the tree once
+// for 16 columns: at most 1024 nodes, or a chain's nodes from its row tile on, and 127 positions. Some milliseconds for the deepest tree; a
+// walk for each key and column is longer than a wait may be.
 template <typename T, int BN>
-__device__ __noinline__ float pa_odd_values(const PaParams& p, const PaPart& w, const int16_t* up, int node, int d) {
-  float sum = 0.f;
-  const uint32_t t0 = max(w.t0, static_cast<uint32_t>(w.s.len) / BN);  // (tiles in front of it hold no nodes)
-  const int64_t end = static_cast<int64_t>(w.t1) * BN - w.s.len, begin = static_cast<int64_t>(t0) * BN - w.s.len;
-  for (int j = static_cast<int>(end <= node ? end - 1 : node); j >= begin; --j) {
-    if (j >= 0) {
-      uint32_t sees[4];
-      pa_sees128(up, node, j, sees);
-      if (!(sees[0] & 1)) continue;
-    }
+__device__ __noinline__ void pa_odd_values(const PaParams& p, const PaPart& w, const int16_t* up, int node, int d, float* sum) {
+  const uint32_t t0 = max(w.t0, static_cast<uint32_t>(pa_open(p, w) / BN));
+  const int begin = static_cast<int>(static_cast<int64_t>(t0) * BN - w.s.len), end = static_cast<int>(static_cast<int64_t>(w.t1) * BN - w.s.len);
+#pragma unroll
+  for (int e = 0; e < 16; ++e) sum[e] = 0.f;
+  for (int j = up ? node : min(node, end - 1); j >= begin; j = up && j >= 0 ? up[j] : j - 1) {  // (-1 follows a root: the sequence)
+    if (j >= end) continue;
     const uint32_t at = static_cast<uint32_t>(w.s.len + j);
-    const T* v = reinterpret_cast<const T*>(pa_row(p, w, at, pa_lookup(p, w, at)).v);
-    const float y = v ? pa_load(v + d) : 0.f;
-    if (!(fabsf(y) < CUDART_INF_F)) sum += y;
+    const char* const v = pa_row(p, w, at, pa_lookup(p, w, at)).v;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (!v || d + 8 * k >= p.c.dim) continue;
+      const uint4 x = *reinterpret_cast<const uint4*>(v + 2 * (d + 8 * k));
+      const uint32_t y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint16_t bits = static_cast<uint16_t>(y[e >> 1] >> (16 * (e & 1)));
+        T z;
+        memcpy(&z, &bits, 2);
+        const float f = pa_load(&z);
+        if (!(fabsf(f) < CUDART_INF_F)) sum[8 * k + e] += f;
+      }
+    }
   }
-  return sum;
 }
 
 template <typename T, int DP>
@@ -1372,7 +1388,7 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1)
     }
     mbar_init(&sm.met, 8);
     sm.stop = 0;
-    sm.odd = 0;
+    for (int i = 0; i < 8; ++i) sm.odd[i] = 0;
     fence_mbar_init();
     fence_proxy_async_smem();
   }
@@ -1472,14 +1488,13 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1)
     const auto flush = [&]() {
       if (told) {
         pa_copy_wait<0>();
-        pa_tell<T, DP>(told, look_at, half, &sm.odd);
+        pa_tell<T, DP>(told, look_at, half, sm.odd, n_part);
         told = nullptr;
       }
     };
     const int my_boxes = p.box == 128 ? 1 - half : p.box ? 64 / p.box : 0;  // (a box that is a whole tile is fetched by one warp)
     while (ok && pa_next<RT, RW, BN>(p, &at, &w)) {
-      // all rows see the positions in front of `open`
-      const int64_t open = w.s.len + (p.parents ? 0 : static_cast<int64_t>(p.by_group.of(w.row0)) + 1);
+      const int64_t open = pa_open(p, w);
       // tiles in front of `plain` hold no nodes; pages of a tile, a lane a box or a lane two rows
       const uint32_t plain = p.box ? min(static_cast<uint32_t>(w.s.len) / BN, w.t1) : 0;
       const auto lookup = [&](uint32_t tile, int (&pg)[2]) {
@@ -1568,7 +1583,7 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1)
         pa_copy_commit();
         if (told) {
           pa_copy_wait<1>();
-          pa_tell<T, DP>(told, look_at, half, &sm.odd);
+          pa_tell<T, DP>(told, look_at, half, sm.odd, n_part);
         }
         told = full;
         look_at = look;
@@ -1737,7 +1752,7 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1)
       if (n > 0 && !(ok = pa_wait(&sm.o_ready[t], (n_s - 1) & 1, stop))) break;
       tc_fence_after();
       const bool whole = w.t0 == 0 && w.t1 == w.tiles, here = r < w.rows, both = split && all > 1;
-      const bool odd = nodes_here && *reinterpret_cast<volatile int*>(&sm.odd);
+      const bool odd = *reinterpret_cast<volatile int*>(&sm.odd[n_part % 8]) == static_cast<int>(n_part + 1);
       float* const piece = pa_piece_of<RT, DP>(p, w);
       char* const out = here ? pa_out(p, w.s.start, w.head, w.row0 + r) : nullptr;
       const float f = 1.f / l;
@@ -1757,9 +1772,10 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1)
             for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(weight[0] * __uint_as_float(x[e]) + weight[1] * __uint_as_float(y[e]));
           }
           if (odd && here) {
+            float more[16];
+            pa_odd_values<T, BN>(p, w, up, node, d, more);
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (d + e < c.dim) x[e] = __float_as_uint(__uint_as_float(x[e]) + pa_odd_values<T, BN>(p, w, up, node, d + e));
+            for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) + more[e]);
           }
           if (here && whole) {
 #pragma unroll
@@ -1787,6 +1803,7 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1)
         mbar_arrive(&sm.o_free[split ? 0 : t]);
         if (!split || both) mbar_arrive(&sm.o_free[split ? 1 : t]);
       }
+      ++n_part;
     }
   }
   if (!ok && lane == 0) {

@@ -484,8 +484,9 @@ typedef struct {
 uint64_t ytcuda_pages_scratch(const ytcuda_pages* cache);
 
 /* Room for counts[slot] more positions behind lens[slot] (0: the slot is left as it is): free pages are handed out, the lowest
- * numbers first, in the order of the slots; where position lens[slot] falls inside a page that other slots hold too, the slot
- * gets a copy of its rows (its first new page). All slots get theirs or none. */
+ * numbers first, in the order of the slots and, in a slot, of its table: for new entries and for those that the new positions go to
+ * and other slots hold too. Of the page that position lens[slot] falls inside the rows in front of it are copied. Slots that share a
+ * page and ask in one call get one each. All slots get theirs or none. */
 int ytcuda_pages_reserve(const ytcuda_pages* cache, const int32_t* counts, void* stream);
 
 /* Row starts[s] + i of k and v [rows, kv_heads, dim] (i < starts[s + 1] - starts[s], starts [slots + 1] on the device, not

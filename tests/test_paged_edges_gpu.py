@@ -7,6 +7,7 @@ import pytest
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
+from plain_pages import FULL, INVALID, PlainPages  # noqa: E402
 from test_paged_gpu import BF16, F16, F32, Both, ints, paged  # noqa: E402,F401
 
 # every form: narrow, tcgen05 with one row block and two, wide, element by element
@@ -99,3 +100,129 @@ def test_one_number_that_is_none_in_a_long_chain(paged, dtype, dim, groups):
     assert bool(torch.isnan(got[wrong]).all()) and torch.equal(got[~wrong], plain[~wrong])
     from ytensor_b200 import _lib
     assert _lib.lib().ytcuda_device_status(None) == _lib.OK
+
+
+class Shortened(PlainPages):
+    """`reserve` replaces every page that others hold too among those that the new positions go to, not only the first: a sequence that
+    was shortened has such pages behind its length."""
+
+    def reserve(self, counts):
+        free = [p for p, r in enumerate(self.refs) if r == 0]
+        want = []
+        for s, n in enumerate(counts):
+            if n <= 0:
+                if n < 0:
+                    self.status |= INVALID
+                continue
+            need, table = self._pages(self.lens[s] + n), self.table[s]
+            if need > self.max_pages:
+                self.status |= FULL
+                return
+            want += [(s, i) for i in range(self.lens[s] // self.page, need) if i >= len(table) or self.refs[table[i]] > 1]
+        if len(want) > len(free):
+            self.status |= FULL
+            return
+        for (s, i), new in zip(want, free):
+            if i < len(self.table[s]):
+                old, rows = self.table[s][i], max(0, self.lens[s] - i * self.page)
+                for pool in (self.k, self.v):
+                    pool[:, new, :, :rows] = pool[:, old, :, :rows]
+                self.refs[old] -= 1
+                self.table[s][i] = new
+            else:
+                self.table[s].append(new)
+            self.refs[new] = 1
+
+
+def shortened(paged, **how):
+    b = Both(paged, **how)
+    b.p.__class__ = Shortened
+    return b
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("page,base", [(16, 20), (16, 32), (16, 0), (16, 47), (4, 13), (1, 11), (5, 25)])
+def test_a_shortened_copy_goes_on(paged, dtype, page, base):
+    """A fork whose length is taken back by more than a page, into a page or to its end: room for new positions is room that can be
+    written, and what the other slots hold stays as it is."""
+    b = shortened(paged, page=page, slots=3, pages=200, max_pages=80, dtype=dtype)
+    b.fill([50, 7, 0])
+    b.fork([0, 1, 0])
+    b.keep([0, 0, 0], None, [50, 7, base])
+    b.same()
+    b.reserve([0, 0, 40])
+    b.same()
+    for layer in range(2):
+        b.attend(layer, [0, 0, 40], 2)
+    b.same()
+    b.keep([0, 0, 40])
+    b.attend(0, [0, 0, 0], 2)
+    b.same()
+    b.d.check()
+    b.fork([2, 0, 0])  # all copies shortened, two of them go on at once
+    b.keep([0, 0, 0], None, [base, 50, 50 - page])
+    b.reserve([3 * page, 0, 2 * page + 1])
+    b.same()
+    for layer in range(2):
+        b.append(layer, [3 * page, 0, 2 * page + 1])
+    b.keep([3 * page, 0, 2 * page + 1])
+    b.same()
+    b.d.check()
+
+
+def test_a_shortened_copy_without_free_pages(paged):
+    """All pages or none: those that would be replaced count, too."""
+    b = shortened(paged, page=4, slots=2, pages=7, max_pages=8)
+    b.fill([16, 0])
+    b.fork([0, 0])
+    b.keep([0, 0], None, [16, 2])
+    b.reserve([0, 15])  # pages 0 to 3 again and one more: five of three
+    assert b.p.status == FULL
+    b.same()
+    b.d.status.zero_()
+    b.p.status = 0
+    b.reserve([0, 10])  # three of three
+    assert b.same().p.status == 0 and min(b.p.refs) == 1
+
+
+@pytest.mark.parametrize("page,dim", [(16, 64), (4, 7), (1, 16)])
+def test_pages_over_many_steps_with_shortening(paged, page, dim):
+    b = shortened(paged, page=page, dim=dim, pages=60, slots=5, max_pages=14, seed=page)
+    r = b.rng
+    for step in range(60):
+        kind = r.choice(["grow", "grow", "fork", "free", "shorten"])
+        if kind == "grow":
+            counts = [r.choice([0, 1, r.randint(1, 3 * page)]) for _ in range(5)]
+            b.reserve(counts)
+            if b.p.status & FULL:
+                b.same()
+                b.d.status.zero_()
+                b.p.status = 0
+                continue
+            for layer in range(2):
+                b.append(layer, counts)
+            b.keep(counts)
+        elif kind == "fork":
+            b.fork([r.choice([s, r.randrange(-1, 5)]) for s in range(5)])
+        elif kind == "free":
+            gone = [int(r.random() < 0.2) for _ in range(5)]
+            b.d.free(ints(gone))
+            b.p.fork([-1 if x else s for s, x in enumerate(gone)])
+        else:
+            b.keep([0] * 5, None, [r.choice([n, r.randint(0, n)]) for n in b.p.lens])
+        b.same()
+        assert b.p.status == 0
+
+
+def test_many_shared_pages_behind_a_shortened_sequence(paged):
+    """More of them than a warp takes at a time, in more slots than a round."""
+    slots = 1100
+    b = shortened(paged, layers=1, heads=1, dim=2, page=1, slots=slots, pages=40000, max_pages=100)
+    b.reserve([90] + [0] * (slots - 1))
+    b.append(0, [90] + [0] * (slots - 1))
+    b.keep([90] + [0] * (slots - 1))
+    b.fork([0 if s % 3 == 0 else s for s in range(slots)])
+    b.keep([0] * slots, None, [(s * 7) % 90 if s % 3 == 0 else 0 for s in range(slots)])
+    b.reserve([100 - (s * 7) % 90 if s % 3 == 0 else s % 4 for s in range(slots)])
+    b.same()
+    assert b.p.status == 0

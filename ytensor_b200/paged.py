@@ -4,7 +4,7 @@ tokens ahead, or searches with beams.
 A pool holds the keys and values of all layers, [layers, pages, kv_heads, page, dim]. A slot is one sequence: position p lies
 in row p % page of the page that table[slot, p // page] names; the slot holds the first held[slot] entries of its row of the
 table, and lens[slot] positions are written. refs[page] counts the slots that hold a page: a fork shares pages instead of
-copying them, and `reserve` copies the one page that would be written while others hold it too. YTensor has one contiguous
+copying them, and `reserve` replaces those that would be written while others hold them too. YTensor has one contiguous
 cache per model (reference example/qwen3/src/qwen3.cpp:70-126) and no counterpart.
 
 Everything lives on the device and no call waits for it, so that a step can be captured in a CUDA graph and replayed at any
@@ -120,8 +120,9 @@ class PagedCache:
     # ------------------------------------------------------------------ pages
     def reserve(self, counts: torch.Tensor) -> None:
         """Room for counts[slot] more positions behind lens[slot] (int32 [slots]; 0: the slot stays as it is). Free pages are
-        handed out in ascending order, slot by slot; where the next position falls inside a page that other slots hold too,
-        the slot first gets a copy of its rows. All slots get their pages or, with FULL in `status`, none."""
+        handed out in ascending order, slot by slot, for new entries of the table and for those that the new positions go to and
+        other slots hold too; of the page that the next position falls inside the slot's rows are copied. (b slots that share a
+        page and ask in one call get b pages.) All slots get their pages or, with FULL in `status`, none."""
         check(self._lib.ytcuda_pages_reserve(self._at, self._ints(counts, "counts", self._per_slot), self._stream()))
 
     def fork(self, source: torch.Tensor) -> None:

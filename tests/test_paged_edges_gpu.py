@@ -226,3 +226,33 @@ def test_many_shared_pages_behind_a_shortened_sequence(paged):
     b.reserve([100 - (s * 7) % 90 if s % 3 == 0 else s % 4 for s in range(slots)])
     b.same()
     assert b.p.status == 0
+
+
+@pytest.mark.parametrize("dtype,dim,groups", [(F32, 64, 2), (F32, 30, 2), (BF16, 64, 1), (F16, 128, 12), (BF16, 256, 2), (F16, 200, 9)])
+def test_starts_that_descend(paged, dtype, dim, groups):
+    """Slots that claim one another's rows: nothing is computed, the status says so, and the next call is as ever."""
+    b = Both(paged, layers=1, heads=1, dim=dim, slots=3, page=16, pages=80, max_pages=20, dtype=dtype)
+    b.fill([100, 30, 70])
+    b.reserve([8, 8, 8])
+    q, k, v = b.randn(8, groups, dim), b.randn(8, 1, dim), b.randn(8, 1, dim)
+    plain = b.d.attend(0, q, ints([0, 3, 5, 8]), k, v)
+    for starts in ([0, 8, 0, 8], [8, 0, 4, 8], [0, 5, 3, 8], [0, 8, 8, 7]):
+        out = torch.full_like(q, 3.0)
+        b.d.attend(0, q, ints(starts), k, v, out=out)
+        assert int(b.d.status.item()) == INVALID and bool((out == 3).all())
+        b.d.status.zero_()
+    assert torch.equal(plain, b.d.attend(0, q, ints([0, 3, 5, 8]), k, v))
+    b.d.check()
+
+
+def test_starts_that_descend_over_long_sequences(paged):
+    """256 slots of a million positions, every other one with all of 8000 rows: more work than 32 bits count."""
+    slots, rows, length = 256, 8000, 1 << 20
+    z = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")  # noqa: E731
+    k = torch.zeros(1, 2, 8, 1024, 8, dtype=BF16, device="cuda")
+    c = paged.PagedCache.over(k, k.clone(), z(slots, 1040), z(slots) + length, z(slots) + 1040, z(2) + 1)
+    q = torch.zeros(rows, 64, 8, dtype=BF16, device="cuda")
+    new = torch.zeros(rows, 8, 8, dtype=BF16, device="cuda")
+    out = torch.full_like(q, 3.0)
+    c.attend(0, q, ints([0, rows] * (slots // 2) + [rows]), new, new, out=out)
+    assert int(c.status.item()) & INVALID and bool((out == 3).all())

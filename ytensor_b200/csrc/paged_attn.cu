@@ -90,12 +90,15 @@ template <int RT, int RW, int BN>
 __device__ __forceinline__ void pa_share(const PaParams& p, PaShare* out) {
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
-    bool bad = false;
+    bool bad = false, down = false;
     uint32_t total = 0, w = 0;
     for (int s0 = 0; s0 < p.c.slots; s0 += 32) {
       w = s0 + lane < p.c.slots ? pa_work<RT, RW, BN>(p, pa_slot(p, s0 + lane, &bad)) : 0;
+      down = down || (s0 + lane < p.c.slots && p.starts[s0 + lane + 1] < p.starts[s0 + lane]);
       total += __reduce_add_sync(0xffffffffu, w);
     }
+    // (starts that descend: slots would claim the same rows, and the sum of their costs could pass 32 bits. Nothing is computed.)
+    if (__any_sync(0xffffffffu, down)) total = 0;
     if (blockIdx.x == 0 && __any_sync(0xffffffffu, bad) && lane == 0) atomicOr(p.c.status, YTC_PAGES_INVALID);
     PaShare r;
     const uint32_t parts = min(gridDim.x, max(1u, total / PaCost<RT, RW>::BOTH));

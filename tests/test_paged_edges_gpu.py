@@ -256,3 +256,24 @@ def test_starts_that_descend_over_long_sequences(paged):
     out = torch.full_like(q, 3.0)
     c.attend(0, q, ints([0, rows] * (slots // 2) + [rows]), new, new, out=out)
     assert int(c.status.item()) & INVALID and bool((out == 3).all())
+
+
+def test_check_says_that_a_wait_ran_out(paged):
+    """A kernel that gives up a wait leaves it in the device's status word: check() reads that, too, and once."""
+    from ytensor_b200 import _lib
+    L = _lib.lib()
+    b = Both(paged, layers=1, heads=1, slots=1)
+    b.d.check()
+    old, waited = L.ytcuda_get_wait_limit(), torch.zeros(1, dtype=torch.int64, device="cuda")
+    _lib.check(L.ytcuda_set_wait_limit(2_000_000))  # about a millisecond
+    try:
+        for also in (False, True):
+            _lib.check(L.ytcuda_wait_probe(waited.data_ptr(), torch.cuda.current_stream().cuda_stream))
+            if also:
+                b.d.keep(ints([1]))  # a row without a page
+            with pytest.raises(_lib.YtCudaError, match="wait ran out.*tree that is none" if also else "wait ran out") as e:
+                b.d.check()
+            assert e.value.status == _lib.TIMEOUT
+            b.d.check()
+    finally:
+        _lib.check(L.ytcuda_set_wait_limit(old))

@@ -214,8 +214,16 @@ class PagedCache:
         return out
 
     def check(self) -> None:
-        """Raises what the device has noted since the last check (waits for the current stream)."""
+        """Raises what the device has noted since the last check (waits for the current stream): what `status` says of this cache,
+        and a wait of a kernel on this device that ran out (YtCudaError with status TIMEOUT: rows of an attend() may be
+        unwritten)."""
+        with torch.cuda.device(self._index):
+            waits = self._lib.ytcuda_device_status(torch.cuda.current_stream().cuda_stream)
         bits = int(self.status.item())
         if bits:
             self.status.zero_()
-            raise _lib.YtCudaError(_lib.INVALID_ARG, "paged cache: " + "; ".join(t for b, t in _TEXT.items() if bits & b))
+        said = [t for b, t in _TEXT.items() if bits & b]
+        if waits != _lib.OK:
+            raise _lib.YtCudaError(waits, "paged cache: " + "; ".join([_lib.last_error() or "a wait on the device ran out", *said]))
+        if said:
+            raise _lib.YtCudaError(_lib.INVALID_ARG, "paged cache: " + "; ".join(said))

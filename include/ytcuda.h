@@ -521,7 +521,7 @@ int ytcuda_pages_fork(const ytcuda_pages* cache, const int32_t* source, const in
 
 /* The pages in use, in the order of their numbers, become pages 0, 1, .. of another cache with the same slots, layers, heads,
  * type and table, and its table, lens, held and refs those of this one. The other cache's status says YTC_PAGES_FULL where
- * its pool is too small: nothing is written then. */
+ * its pool is too small: nothing is written then. The caches may be views of one pool that have no element in common. */
 int ytcuda_pages_compact(const ytcuda_pages* cache, const ytcuda_pages* into, void* stream);
 
 /* ---------------------------------------------------------------- handles of the models below */

@@ -2,6 +2,7 @@
 share memory, starts that descend. The plain cache and the tolerances are those of test_paged_gpu.py."""
 import math
 
+import numpy as np
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -277,3 +278,83 @@ def test_check_says_that_a_wait_ran_out(paged):
             b.d.check()
     finally:
         _lib.check(L.ytcuda_set_wait_limit(old))
+
+
+def numpy_of(t, base):
+    """The same places of a numpy array that torch's strides give, over the storage of `base`."""
+    size, flat = t.element_size(), np.zeros(base.untyped_storage().nbytes() // t.element_size(), f"u{t.element_size()}")
+    return np.lib.stride_tricks.as_strided(flat[t.storage_offset():], t.shape, [x * size for x in t.stride()]), flat
+
+
+def meet(x, y):
+    """Whether two views of one storage have an element in common."""
+    seen = []
+    for t in (x, y):
+        view, flat = numpy_of(t, x)
+        view[...] = 1
+        seen.append(flat)
+    return bool((seen[0] & seen[1]).any())
+
+
+VIEWS = {  # two views of one tensor, [layers, pages, heads, page, dim] each
+    "pages": ((2, 24, 2, 4, 16), lambda t: (t[:, :12], t[:, 12:])),
+    "pages that overlap": ((2, 24, 2, 4, 16), lambda t: (t[:, :12], t[:, 11:])),
+    "layers": ((4, 12, 2, 4, 16), lambda t: (t[:2], t[2:])),
+    "the same": ((2, 12, 2, 4, 16), lambda t: (t, t)),
+    "layers that overlap": ((3, 12, 2, 4, 16), lambda t: (t[:2], t[1:])),
+    "every other page": ((2, 24, 2, 4, 16), lambda t: (t[:, ::2], t[:, 1::2])),
+    "every other page, and all from one on": ((2, 24, 2, 4, 16), lambda t: (t[:, ::2], t[:, 3:])),
+    "heads": ((2, 12, 4, 4, 16), lambda t: (t[:, :, :2], t[:, :, 2:])),
+    "heads that overlap": ((2, 12, 3, 4, 16), lambda t: (t[:, :, :2], t[:, :, 1:])),
+    "rows of a page": ((2, 12, 2, 8, 16), lambda t: (t[:, :, :, ::2], t[:, :, :, 1::2])),
+    "halves of a row": ((2, 12, 2, 4, 32), lambda t: (t[..., :16], t[..., 16:])),
+    "halves of a row that overlap": ((2, 12, 2, 4, 31), lambda t: (t[..., :16], t[..., 15:])),
+    "heads behind positions": ((2, 24, 4, 2, 16), lambda t: (t[:, :12].transpose(2, 3), t[:, 12:].transpose(2, 3))),
+    "one order in the other": ((2, 12, 4, 4, 16), lambda t: (t[:, :10], t[:, 2:].transpose(2, 3))),
+}
+
+
+@pytest.mark.parametrize("which", VIEWS)
+@pytest.mark.parametrize("pool", ["k", "v", "k and v"])
+def test_caches_that_are_views_of_one_pool(paged, which, pool):
+    """compact() takes two of them that have no element in common, whatever their strides, and refuses them otherwise."""
+    shape, views = VIEWS[which]
+    g = torch.Generator(device="cuda").manual_seed(1)
+    whole = torch.randn(shape, generator=g, device="cuda").to(BF16)
+    mine, theirs = views(whole)
+    if pool == "k":
+        kv, into = (mine, mine.clone()), (theirs, theirs.clone())
+    elif pool == "v":
+        kv, into = (mine.clone(), mine), (theirs.clone(), theirs)
+    else:  # keys of one beside values of the other
+        kv, into = (mine, mine.clone()), (theirs.clone(), theirs)
+    z = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")  # noqa: E731
+    a = paged.PagedCache.over(*kv, z(2, 6), z(2), z(2), z(kv[0].shape[1]))
+    b = paged.PagedCache.over(*into, z(2, 6), z(2), z(2), z(into[0].shape[1]))
+    fresh = paged.PagedCache(*into[0].shape[:2], a.page, a.kv_heads, a.dim, 2, 6)
+    a.reserve(ints([3 * a.page - 1, 2 * a.page]))
+    a.keep(ints([3 * a.page - 1, 2 * a.page]))
+    a.compact(fresh)
+    if meet(mine, theirs):
+        with pytest.raises(ValueError, match="share memory"):
+            a.compact(b)
+        return
+    a.compact(b)
+    for cache in (a, b, fresh):
+        cache.check()
+    assert torch.equal(b.k[:, :5], fresh.k[:, :5]) and torch.equal(b.v[:, :5], fresh.v[:, :5])
+    assert torch.equal(b.refs, fresh.refs) and torch.equal(b.lens, fresh.lens)
+    assert all(torch.equal(b.table[s, :n], fresh.table[s, :n]) for s, n in ((0, 3), (1, 2)))
+
+
+def test_caches_that_share_counts(paged):
+    z = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")  # noqa: E731
+    k = lambda: torch.zeros(1, 8, 1, 4, 16, device="cuda")  # noqa: E731
+    space = z(100)
+    part = lambda at, *s: space[at:at + math.prod(s)].view(s)  # noqa: E731
+    a = paged.PagedCache.over(k(), k(), part(0, 2, 5), part(10, 2), part(12, 2), part(14, 8))
+    for at in ((30, 42, 44, 46), (22, 32, 34, 36)):
+        a.compact(paged.PagedCache.over(k(), k(), part(at[0], 2, 5), part(at[1], 2), part(at[2], 2), part(at[3], 8)))
+    for at in ((21, 42, 44, 46), (30, 9, 44, 46), (30, 42, 13, 46), (30, 42, 44, 7), (30, 12, 44, 46), (0, 42, 44, 46)):
+        with pytest.raises(ValueError, match="share memory"):
+            a.compact(paged.PagedCache.over(k(), k(), part(at[0], 2, 5), part(at[1], 2), part(at[2], 2), part(at[3], 8)))

@@ -617,6 +617,55 @@ int pg_rows(const char* who, const char* what, const void* p, const int64_t* str
   return YTC_OK;
 }
 
+// Two boxes meet where a sum of strides, each times a number of its range (an index of a minus one of b), is the distance of their first
+// elements. The strides are tried from the largest down, those numbers only that the smaller ones can make up for: one or two for strides
+// of axes that lie in one another. Where that takes too long they count as meeting.
+struct PgMeet {
+  int64_t stride[9], lo[9], hi[9], least[10], most[10];  // least, most: of all terms from one on
+  int n, left;
+  bool from(int i, int64_t rest) {
+    if (rest < least[i] || rest > most[i]) return false;
+    if (i == n || (stride[i] == 1 && i == n - 1)) return true;
+    if (--left < 0) return true;
+    // stride x in rest - most .. rest - least of the others
+    const auto down = [](int64_t a, int64_t b) { return a / b - (a % b < 0); };
+    const int64_t first = -down(most[i + 1] - rest, stride[i]), last = down(rest - least[i + 1], stride[i]);
+    for (int64_t x = first > lo[i] ? first : lo[i]; x <= last && x <= hi[i]; ++x)
+      if (from(i + 1, rest - x * stride[i])) return true;
+    return false;
+  }
+};
+bool pg_meet(const PgBox& a, const PgBox& b, int size) {
+  if (!a.p || !b.p) return false;
+  PgMeet m;
+  m.n = 0;
+  m.left = 100000;
+  const auto add = [&](int64_t stride, int64_t lo, int64_t hi) {
+    if (stride < 0) {
+      const int64_t x = lo;
+      stride = -stride, lo = -hi, hi = -x;
+    }
+    if (stride == 0 || lo == hi) return;
+    int i = 0;
+    while (i < m.n && m.stride[i] > stride) ++i;
+    if (i < m.n && m.stride[i] == stride) {
+      m.lo[i] += lo, m.hi[i] += hi;
+      return;
+    }
+    for (int j = m.n++; j > i; --j) m.stride[j] = m.stride[j - 1], m.lo[j] = m.lo[j - 1], m.hi[j] = m.hi[j - 1];
+    m.stride[i] = stride, m.lo[i] = lo, m.hi[i] = hi;
+  };
+  for (int i = 0; i < 4; ++i) {
+    if (a.extent[i] <= 0 || b.extent[i] <= 0) return false;
+    add(a.stride[i] / size, 0, a.extent[i] - 1);
+    add(b.stride[i] / size, -(b.extent[i] - 1), 0);
+  }
+  add(1, -(b.dim - 1), a.dim - 1);
+  m.least[m.n] = m.most[m.n] = 0;
+  for (int i = m.n - 1; i >= 0; --i) m.least[i] = m.least[i + 1] + m.stride[i] * m.lo[i], m.most[i] = m.most[i + 1] + m.stride[i] * m.hi[i];
+  return m.from(0, (b.p - a.p) / size);
+}
+
 static unsigned copy_grid(int64_t items) {
   const int64_t blocks = (items + PG_WARPS - 1) / PG_WARPS, most = 8ll * sm_count();
   return static_cast<unsigned>(blocks < 1 ? 1 : blocks < most ? blocks : most);
@@ -738,10 +787,17 @@ int ytcuda_pages_compact(const ytcuda_pages* cache, const ytcuda_pages* into, vo
               "%s: the caches differ in type, layers, page, heads, dim, slots or table", who);
   if (c.slots == 0) return YTC_OK;
   YTC_REQUIRE(c.pages > 0 && to.pages > 0, "%s: a pool without pages", who);
-  YTC_REQUIRE(c.k.p != to.k.p && c.k.p != to.v.p && c.v.p != to.v.p && c.v.p != to.k.p && c.table != to.table && c.lens != to.lens &&
-                  c.held != to.held && c.refs != to.refs,
-              "%s: the caches share memory", who);
   const int size = dtype_size(cache->dtype);
+  for (const PgPool* x : {&c.k, &c.v})
+    for (const PgPool* y : {&to.k, &to.v})
+      YTC_REQUIRE(!pg_meet(pg_box(*x, c), pg_box(*y, to), size), "%s: the pools of the caches share memory", who);
+  const auto ints = [](const PgCache& x, int i) {
+    const int64_t n[4] = {static_cast<int64_t>(x.slots) * x.max_pages, x.slots, x.slots, x.pages};
+    const int32_t* const p[4] = {x.table, x.lens, x.held, x.refs};
+    return PgBox{reinterpret_cast<const char*>(p[i]), {n[i] > 0, 1, 1, 1}, {0, 0, 0, 0}, n[i]};
+  };
+  for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < 4; ++j) YTC_REQUIRE(!pg_meet(ints(c, i), ints(to, j), 4), "%s: the tables or counts of the caches share memory", who);
   const int width = pg_width(pg_bits(c.k) | pg_bits(c.v) | pg_bits(to.k) | pg_bits(to.v) | static_cast<uint64_t>(c.dim * size));
   int merged = 1;
   for (const PgPool* p : {&c.k, &c.v, &to.k, &to.v})

@@ -67,6 +67,17 @@ __host__ __device__ __forceinline__ PgScratch pg_scratch(int64_t slots, int64_t 
 int pg_take(const char* who, const ytcuda_pages* c, PgCache* out);
 // The rows of new tokens of a call, checked; `heads` of `dim` elements of `size` bytes.
 int pg_rows(const char* who, const char* what, const void* p, const int64_t* strides, int size, PgRows* out);
+// Elements of `size` bytes at p + sum of index * stride (in bytes): up to four axes, and `dim` elements in a row. And whether two of them have
+// a byte in common.
+struct PgBox {
+  const char* p;
+  int64_t extent[4], stride[4];
+  int64_t dim;
+};
+bool pg_meet(const PgBox& a, const PgBox& b, int size);
+inline PgBox pg_box(const PgPool& p, const PgCache& c) {
+  return PgBox{p.p, {c.layers, c.pages, c.heads, c.page}, {p.layer, p.page, p.head, p.row}, c.dim};
+}
 // The widest of 16, 4 and 2 bytes in which rows of dim elements of these places can be copied.
 inline int pg_width(uint64_t all_bits_or) { return all_bits_or % 16 == 0 ? 16 : all_bits_or % 4 == 0 ? 4 : 2; }
 inline uint64_t pg_bits(const PgPool& p) {

@@ -149,7 +149,7 @@ class PagedCache:
     def compact(self, into: "PagedCache") -> None:
         """The pages in use, in ascending order, become pages 0, 1, .. of another (smaller, larger, differently laid out) cache of
         the same slots, and its table, lens, held and refs those of this one. FULL in its `status`: its pool is too small,
-        nothing was written."""
+        nothing was written. The two may be views of one pool without an element in common."""
         if into._index != self._index:
             raise _bad("paged cache: compact into a cache on another device")
         check(self._lib.ytcuda_pages_compact(self._at, into._at, self._stream()))

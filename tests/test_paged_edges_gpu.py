@@ -358,3 +358,34 @@ def test_caches_that_share_counts(paged):
     for at in ((21, 42, 44, 46), (30, 9, 44, 46), (30, 42, 13, 46), (30, 42, 44, 7), (30, 12, 44, 46), (0, 42, 44, 46)):
         with pytest.raises(ValueError, match="share memory"):
             a.compact(paged.PagedCache.over(k(), k(), part(at[0], 2, 5), part(at[1], 2), part(at[2], 2), part(at[3], 8)))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_results_in_the_tensor_of_the_queries(paged, dtype):
+    """`out` may be a slice of the tensor that q, k and v are slices of, but has no element in common with them."""
+    b = Both(paged, layers=1, heads=2, dim=64, slots=1, page=16, pages=40, max_pages=30, dtype=dtype)
+    b.fill([100])
+    b.reserve([6])
+    starts, whole = ints([0, 6]), b.randn(12, 12, 64)
+    want = None
+    for q, k, v, out in (
+            (lambda t: t[:6, :4], lambda t: t[:6, 4:6], lambda t: t[:6, 6:8], lambda t: t[:6, 8:]),           # beside them
+            (lambda t: t[:6, :4], lambda t: t[:6, 4:6], lambda t: t[:6, 6:8], lambda t: t[6:, :4]),           # behind them
+            (lambda t: t[:6, :4], lambda t: t[:6, 4:6], lambda t: t[:6, 6:8], lambda t: t[:6, 7:11]),         # a head of v
+            (lambda t: t[:6, :4], lambda t: t[:6, 4:6], lambda t: t[:6, 6:8], lambda t: t[:6, 3:7]),          # q, k and v
+            (lambda t: t[:6, :4], lambda t: t[:6, 4:6], lambda t: t[:6, 6:8], lambda t: t[5:11, 4:8]),        # a row of k and v
+            (lambda t: t[:6, :4], lambda t: t[:6, 4:6], lambda t: t[:6, 6:8], lambda t: t[5:11, 8:]),
+            (lambda t: t[:6, :4], lambda t: t[:6, 4:6], lambda t: t[:6, 6:8], lambda t: t[:6, :4]),           # q
+            (lambda t: t[:6, :4], lambda t: t[:6, 4:6], lambda t: t[:6, 6:8], lambda t: t[1:7, :4])):
+        t = whole.clone()
+        x, y, z, o = q(t), k(t), v(t), out(t)
+        if any(meet(o, i) for i in (x, y, z)):
+            with pytest.raises(ValueError, match="shares memory"):
+                b.d.attend(0, x, starts, y, z, out=o)
+            assert torch.equal(t, whole)
+        else:
+            want = b.d.attend(0, x.clone(), starts, y.clone(), z.clone()) if want is None else want
+            assert torch.equal(b.d.attend(0, x, starts, y, z, out=o), want)
+    # keys and values that are in the pages already: only q counts
+    t = whole.clone()
+    assert torch.equal(b.d.attend(0, t[:6, :4], starts, out=t[:6, 4:8]), want)

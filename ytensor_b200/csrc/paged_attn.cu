@@ -2067,7 +2067,6 @@ int ytcuda_pages_attend(const ytcuda_pages* cache, int layer, const void* q, voi
   if (rows == 0 || p.c.slots == 0) return YTC_OK;
   YTC_REQUIRE(starts && strides, "%s: null starts or strides", who);
   YTC_REQUIRE(p.c.pages > 0, "%s: a pool without pages", who);
-  YTC_REQUIRE(q != o, "%s: q and o are the same memory", who);
   const int size = dtype_size(cache->dtype);
   if (const int rc = pg_rows(who, "q", q, strides, size, &p.q)) return rc;
   if (const int rc = pg_rows(who, "o", o, strides + 2, size, &p.o)) return rc;
@@ -2075,6 +2074,11 @@ int ytcuda_pages_attend(const ytcuda_pages* cache, int layer, const void* q, voi
     if (const int rc = pg_rows(who, "k", k, strides + 4, size, &p.k)) return rc;
     if (const int rc = pg_rows(who, "v", v, strides + 6, size, &p.v)) return rc;
   }
+  // (the CTAs write rows of o while others still read q, k and v; slices of one tensor that have no element in common are fine)
+  const auto box = [&](const PgRows& r, int n) { return PgBox{r.p, {rows, n, 1, 1}, {r.row, r.head, 0, 0}, p.c.dim}; };
+  YTC_REQUIRE(!pg_meet(box(p.o, heads), box(p.q, heads), size) && !pg_meet(box(p.o, heads), box(p.k, p.c.heads), size) &&
+                  !pg_meet(box(p.o, heads), box(p.v, p.c.heads), size),
+              "%s: o shares memory with q, k or v", who);
   const bool words = pg_width(pg_bits(p.c.k) | pg_bits(p.c.v) | pg_bits(p.q) | pg_bits(p.o) | pg_bits(p.k) | pg_bits(p.v) |
                               static_cast<uint64_t>(p.c.dim * size)) == 16;
   const PaForm f = pa_choose(cache, rows, heads, words);

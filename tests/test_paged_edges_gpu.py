@@ -389,3 +389,22 @@ def test_results_in_the_tensor_of_the_queries(paged, dtype):
     # keys and values that are in the pages already: only q counts
     t = whole.clone()
     assert torch.equal(b.d.attend(0, t[:6, :4], starts, out=t[:6, 4:8]), want)
+
+
+def test_results_that_lie_in_one_another(paged):
+    """Rows and heads of `out` are each written by some CTA: they may stand in any order, but not in one another."""
+    b = Both(paged, layers=1, heads=2, dim=64, slots=1, page=16, pages=20, max_pages=8)
+    b.fill([40])
+    b.reserve([5])
+    q, k, starts = b.randn(5, 4, 64), b.randn(5, 2, 64), ints([0, 5])
+    want = b.d.attend(0, q, starts, k, k)
+    for strides in ((256, 64, 1), (64, 320, 1), (400, 80, 1), (512, 128, 1), (72, 400, 1)):
+        out = torch.zeros(4000, dtype=BF16, device="cuda").as_strided((5, 4, 64), strides)
+        assert torch.equal(b.d.attend(0, q, starts, k, k, out=out), want)
+    for strides in ((0, 64, 1), (256, 0, 1), (192, 64, 1), (256, 63, 1), (64, 64, 1), (32, 320, 1)):
+        out = torch.zeros(4000, dtype=BF16, device="cuda").as_strided((5, 4, 64), strides)
+        with pytest.raises(ValueError, match="lie in one another"):
+            b.d.attend(0, q, starts, k, k, out=out)
+        assert not bool(out.any())
+    one = torch.zeros(4000, dtype=BF16, device="cuda").as_strided((1, 4, 64), (0, 64, 1))  # (a single row's stride says nothing)
+    b.d.attend(0, q[:1], ints([0, 1]), k[:1], k[:1], out=one)

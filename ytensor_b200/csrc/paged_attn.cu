@@ -2079,6 +2079,11 @@ int ytcuda_pages_attend(const ytcuda_pages* cache, int layer, const void* q, voi
   YTC_REQUIRE(!pg_meet(box(p.o, heads), box(p.q, heads), size) && !pg_meet(box(p.o, heads), box(p.k, p.c.heads), size) &&
                   !pg_meet(box(p.o, heads), box(p.v, p.c.heads), size),
               "%s: o shares memory with q, k or v", who);
+  // (a row behind row 0, a head behind head 0 of the same row)
+  const PgBox row0{p.o.p, {1, heads, 1, 1}, {0, p.o.head, 0, 0}, p.c.dim}, head0{p.o.p, {1, 1, 1, 1}, {0, 0, 0, 0}, p.c.dim};
+  const PgBox rows_behind{p.o.p + p.o.row, {rows - 1, heads, 1, 1}, {p.o.row, p.o.head, 0, 0}, p.c.dim};
+  const PgBox heads_behind{p.o.p + p.o.head, {heads - 1, 1, 1, 1}, {p.o.head, 0, 0, 0}, p.c.dim};
+  YTC_REQUIRE(!pg_meet(row0, rows_behind, size) && !pg_meet(head0, heads_behind, size), "%s: rows or heads of o lie in one another", who);
   const bool words = pg_width(pg_bits(p.c.k) | pg_bits(p.c.v) | pg_bits(p.q) | pg_bits(p.o) | pg_bits(p.k) | pg_bits(p.v) |
                               static_cast<uint64_t>(p.c.dim * size)) == 16;
   const PaForm f = pa_choose(cache, rows, heads, words);

@@ -176,8 +176,8 @@ class PagedCache:
         `append`, in the same launch; without them they are in the pages already. scale 0: 1 / sqrt(dim).
 
         Scores, softmax and sums are fp32, results are rounded to nearest even. Rows behind starts[slots] are not written. What
-        a node does not see may be infinite or no number; in fp32 a node that sees an infinity gets NaN. `out` shares no
-        memory with q, k or v."""
+        a node does not see may be infinite or no number; in fp32 a node that sees an infinity gets NaN. `out` has no
+        element in common with q, k or v, and its rows and heads none with one another."""
         stream = self._stream()
         if q.dim() != 3 or q.shape[1] % self.kv_heads:
             raise _bad(f"paged cache: q is [rows, heads, dim] with heads a multiple of {self.kv_heads}, got {list(q.shape)}")

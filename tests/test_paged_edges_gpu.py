@@ -408,3 +408,31 @@ def test_results_that_lie_in_one_another(paged):
         assert not bool(out.any())
     one = torch.zeros(4000, dtype=BF16, device="cuda").as_strided((1, 4, 64), (0, 64, 1))  # (a single row's stride says nothing)
     b.d.attend(0, q[:1], ints([0, 1]), k[:1], k[:1], out=one)
+
+
+def test_more_slots_than_a_grid_is_high(paged):
+    slots = 70001
+    c = paged.PagedCache(1, slots, 4, 1, 8, slots, 1, BF16)
+    two, starts = torch.full((slots,), 2, dtype=torch.int32, device="cuda"), torch.arange(0, 2 * slots + 1, 2, dtype=torch.int32, device="cuda")
+    k = torch.arange(2 * slots * 8, device="cuda").view(2 * slots, 1, 8).remainder(251).to(BF16)
+    v = k + 1
+    c.reserve(two)
+    c.append(0, k, v, starts)
+    take = torch.arange(slots, device="cuda") % 2  # every slot keeps one row, the first or the second
+    c.keep(torch.ones_like(two), take.to(torch.int32).view(slots, 1))
+    c.check()
+    rows = torch.arange(slots, device="cuda") * 2 + take
+    assert torch.equal(c.k[0, :, 0, 0], k[rows, 0]) and torch.equal(c.v[0, :, 0, 0], v[rows, 0]) and bool((c.lens == 1).all())
+    c.keep(two)
+    c.check()
+    assert bool((c.lens == 3).all())
+    c.fork(torch.arange(slots, dtype=torch.int32, device="cuda").flip(0))
+    c.keep(torch.zeros_like(two))
+    c.reserve(torch.ones_like(two))
+    c.check()
+    assert torch.equal(c.k[0, c.table[:, 0].long(), 0, 0], k[rows, 0].flip(0))
+    q = k[:slots, :, :]
+    one = torch.arange(slots + 1, dtype=torch.int32, device="cuda")
+    out = c.attend(0, q, one, k[:slots], v[:slots])
+    c.check()
+    assert bool(torch.isfinite(out).all())

@@ -360,13 +360,13 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 3) pages_keep_kernel(const PgCa
   __shared__ PgDiv by_moves;
   __shared__ int last;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  const int items = 2 * c.layers * c.heads, s = blockIdx.y;
+  const int items = 2 * c.layers * c.heads, s = blockIdx.x;
   pg_begin();
   const PgScratch at = pg_scratch(c.slots, c.max_pages, c.pages);
   const int n = kept[s];
   const int64_t b = base ? base[s] : c.lens[s];
   const int bad = pg_keep_bad(c, s, b, n, accepted, depth);  // (the same in every warp)
-  if (blockIdx.x == 0 && t == 0) c.scratch[at.mark + s] = bad;
+  if (blockIdx.y == 0 && t == 0) c.scratch[at.mark + s] = bad;
   if (accepted && n > 0 && !bad) {
     const int32_t* const mine = accepted + static_cast<int64_t>(s) * depth;
     for (int j0 = 0; j0 < n; j0 += PG_MOVES) {
@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(PG_WARPS * 32, 3) pages_keep_kernel(const PgCa
       if (t == 0) by_moves = pg_div(static_cast<uint32_t>(moves));
       __syncthreads();
       // A warp's items in one line of words, PG_UNROLL x 32 of them in flight: rows of an item in ascending order, items in any.
-      const int stride = gridDim.x * PG_WARPS, first = blockIdx.x * PG_WARPS + warp;
+      const int stride = gridDim.y * PG_WARPS, first = blockIdx.y * PG_WARPS + warp;
       const int row_words = by_words.d, all = first < items ? ((items - first - 1) / stride + 1) * moves * row_words : 0;
       const PgDiv of_moves = by_moves;
       for (int w0 = 0; w0 < all; w0 += 32 * PG_UNROLL) {
@@ -755,8 +755,7 @@ int ytcuda_pages_keep(const ytcuda_pages* cache, const int32_t* kept, const int3
   const int width = pg_width(pg_bits(c.k) | pg_bits(c.v) | static_cast<uint64_t>(c.dim * size));
   // three CTAs an SM, all that it holds, where there is that much to move: a warp's items one behind another
   const int64_t a_slot = (2ll * c.layers * c.heads + PG_WARPS - 1) / PG_WARPS, most = (3ll * sm_count() + c.slots - 1) / c.slots;
-  const dim3 grid(accepted ? static_cast<unsigned>(a_slot < most ? a_slot : most) : 1u, static_cast<unsigned>(c.slots));
-  YTC_REQUIRE(c.slots <= 65535, "%s: %d slots (at most 65535)", who, c.slots);
+  const dim3 grid(static_cast<unsigned>(c.slots), accepted ? static_cast<unsigned>(a_slot < most ? a_slot : most) : 1u);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const PgDiv by_words = pg_div(static_cast<uint32_t>(c.dim * size / width));
   PG_BY_WIDTH(width, YTC_CUDA(pg_launch(pages_keep_kernel<B>, grid, dim3(PG_WARPS * 32), 0, st, c, kept, accepted, depth, base, by_words)));

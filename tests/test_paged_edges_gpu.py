@@ -436,3 +436,36 @@ def test_more_slots_than_a_grid_is_high(paged):
     out = c.attend(0, q, one, k[:slots], v[:slots])
     c.check()
     assert bool(torch.isfinite(out).all())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("dim,groups", [(64, 1), (128, 4), (256, 2), (64, 20), (128, 32), (256, 17), (128, 140), (30, 2), (30, 9)])
+def test_many_small_weights_beside_large_ones(paged, dtype, dim, groups):
+    """Sixteen keys with a weight of one and a value of zero, 8000 with weights of 2^-25.5 and values of one: what is left of the small
+    ones is the whole result. Tolerance: fp16 weights, of which the largest are 2^7 or more, are off by 2^-25 at most where they are
+    below 2^-14, so by 2^-32 of the largest; else as ever."""
+    n, slots, scale = 8000, 200, 1.0
+    page, heads = 32, 1
+    c = paged.PagedCache(1, n // page + slots + 9, page, heads, dim, slots, n // page + 1, dtype)
+    starts = torch.tensor([0] + [n] * slots, dtype=torch.int32, device="cuda")
+    counts = ints([n] + [0] * (slots - 1))
+    k, v = torch.zeros(n, 1, dim, dtype=dtype, device="cuda"), torch.ones(n, 1, dim, dtype=dtype, device="cuda")
+    heavy = torch.arange(0, 256, 16, device="cuda")  # one for every warp, stream and block of keys
+    k[heavy, 0, 0], v[heavy] = 4.421875, 0.0
+    c.reserve(counts)
+    c.append(0, k, v, starts)
+    c.keep(counts)
+    c.fork(torch.zeros(slots, dtype=torch.int32, device="cuda"))
+    one = torch.ones(slots, dtype=torch.int32, device="cuda")
+    c.reserve(one)
+    q = torch.zeros(slots, groups, dim, dtype=dtype, device="cuda")
+    q[..., 0] = 4.0
+    new = torch.zeros(slots, 1, dim, dtype=dtype, device="cuda")
+    got = c.attend(0, q, torch.arange(slots + 1, dtype=torch.int32, device="cuda"), new, new + 1, scale=scale)
+    c.check()
+    w = math.exp(-4.0 * float(torch.tensor(4.421875, dtype=dtype)))
+    small = n + 1 - 16
+    want = small * w / (16 + small * w)
+    tol = (torch.finfo(dtype).eps if dtype != F32 else 0) * want * 1.01 + (n * 2.0 ** -32 if dtype == F16 else 0)
+    tol += 2 * (10 * math.sqrt(dim) * 17.7 + 10 * math.sqrt(n)) * 2.0 ** -24 * want
+    assert float((got.double() - want).abs().max()) <= tol

@@ -525,12 +525,16 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_ffma_kernel(const PaPar
 // its K (O += P V). Keys and values stay as they lie in the pages: cp.async brings rows of 2 DP bytes into a ring, 16-byte words
 // at (word ^ row % 8), so that ldmatrix reads eight rows without bank conflicts; what a row of the table does not reach is zero.
 // The softmax reference of a row is its running maximum, moved only when it grows by more than 2^8 (P then stays below 2^8, and
-// a row of O is hardly ever rescaled); P is rounded to the cache's type as the operand of a matrix instruction has to be, its sum
-// l is of the unrounded numbers in fp32.
+// a row of O is hardly ever rescaled); P is rounded to the cache's type as the operand of a matrix instruction has to be (half a step of
+// bf16 or fp16: 2^-8, 2^-11 of a weight), its sum l is of the unrounded numbers in fp32. In fp16 all of P, l and O is taken 2^7 times, which
+// the quotient does not see: P stays below 2^15, and what is too small for a normal number is off by 2^-32 of the largest weight at
+// most (2^-25 otherwise: thousands of small weights beside a large one would be lost).
 // fp32: every number is two of 11 bits, x = hi + lo with hi = x rounded to 11 bits, and a product the three of m16n8k8 (tf32) that
 // lie above 2^-22 of it: hi hi + hi lo + lo hi. That keeps fp32's accuracy and takes a third of the instructions that fused
 // multiply-adds of single lanes would. An infinity has no such halves: what sees one is NaN.
 constexpr float PA_SLACK = 8.f;
+template <typename T>
+constexpr float PA_UP = std::is_same<T, __half>::value ? 7.f : 0.f;
 
 __device__ __forceinline__ void pa_ldmatrix(uint32_t at, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
@@ -654,7 +658,7 @@ struct PaWarp {
       l[0] *= shrink[0];
       l[1] *= shrink[1];
     }
-    const float ref[2] = {m[0] == -CUDART_INF_F ? 0.f : m[0], m[1] == -CUDART_INF_F ? 0.f : m[1]};
+    const float ref[2] = {m[0] == -CUDART_INF_F ? 0.f : m[0] - PA_UP<T>, m[1] == -CUDART_INF_F ? 0.f : m[1] - PA_UP<T>};
 #pragma unroll
     for (int n = 0; n < NK / 8; ++n)
 #pragma unroll
@@ -1700,7 +1704,7 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1)
             if (moves) m = top;
           }
         }
-        const float ref = m == -CUDART_INF_F ? 0.f : m;
+        const float ref = m == -CUDART_INF_F ? 0.f : m - PA_UP<T>;
         const uint64_t s2 = pa_pair(scale, scale), r2 = pa_pair(-ref, -ref);
         float l0 = 0.f, l1 = 0.f;
 #pragma unroll 1

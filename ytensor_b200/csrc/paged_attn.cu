@@ -2098,7 +2098,8 @@ int ytcuda_pages_attend(const ytcuda_pages* cache, int layer, const void* q, voi
   const int64_t row_tiles = static_cast<int64_t>(rows) * p.groups / f.rt * 3 + 3ll * p.c.slots;
   const int64_t key_tiles = (static_cast<int64_t>(p.c.max_pages) * p.c.page + rows) / f.bn + 1;
   if (static_cast<double>(row_tiles) * static_cast<double>(key_tiles) * p.c.heads >= 2147483648.0) {
-    set_last_error("%s: %d rows over tables of %d positions are too much work for one call", who, rows, p.c.max_pages * p.c.page);
+    set_last_error("%s: %d rows over tables of %lld positions are too much work for one call", who, rows,
+                   static_cast<long long>(p.c.max_pages) * p.c.page);
     return YTC_UNSUPPORTED;
   }
   p.c.k.p += layer * p.c.k.layer;

@@ -427,7 +427,6 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_ffma_kernel(const PaPar
       fetch(tile + 1);
       find(tile + 2);
       const int cur = tile & 1, n0 = static_cast<int>(tile * BN) - w.s.len;  // the node at the tile's first key
-      if (n0 > node1) continue;                                              // (no row of the tile sees any of it)
       float x[RPT][KPT];
 #pragma unroll
       for (int i = 0; i < RPT; ++i)
@@ -1187,7 +1186,7 @@ __global__ void __launch_bounds__(PaWide<T>::THREADS, 1) paged_attn_wide_kernel(
       const uint32_t kt = ring + out * (2 * S::SLOT);
       out = out == ST - 1 ? 0 : out + 1;
       const int n0 = static_cast<int>((tile - (ST - 1)) * BN) - w.s.len;
-      if (16 * warp < w.rows && n0 <= node1) {
+      if (16 * warp < w.rows) {
         bool hides = n0 + BN > 0;
         uint64_t sees[2] = {0, 0};
         if (hides) {
@@ -1753,7 +1752,7 @@ __global__ void __launch_bounds__(PaTc<T, DP>::THREADS, 1)
         const int n1 = static_cast<int>(all / 2), n2 = static_cast<int>(all) - n1;  // key tiles of stream 1, of stream 0
         n_other += t ? n2 : n1;
         if ((t ? n2 : n1) > 0 && !(ok = pa_wait(&sm.o_ready[1 - t], (n_other - 1) & 1, stop))) break;
-      } else if (w.rows > 128) {
+      } else {
         n_other += all;
       }
       if (n > 0 && !(ok = pa_wait(&sm.o_ready[t], (n_s - 1) & 1, stop))) break;

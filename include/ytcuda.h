@@ -501,9 +501,10 @@ int ytcuda_pages_append(const ytcuda_pages* cache, int layer, const void* k, con
  * head h reads key head h / (heads / kv_heads). With k and v [rows, kv_heads, dim] the nodes' keys and values are stored
  * first, as by ytcuda_pages_append (both NULL: they are in the pages already). scale 0: 1 / sqrt(dim). Scores, softmax and
  * sums in fp32; results rounded to nearest even. What a node does not see may be infinite or no number; in fp32 (a number is
- * two of 11 bits there) a node that sees an infinity gets NaN. o has no element in common with q, k or v, and its rows and
- * heads none with one another. Rows behind starts[slots] are left as they were. dim <= 256; strides: {row, head} of q, of o,
- * of k, of v. workspace: ytcuda_pages_attend_workspace() bytes that no other call uses until this one has run. */
+ * two of 11 bits there) a node that sees an infinity or a number of 0x1.ffep127 or more may get NaN. o has no element in
+ * common with q, k or v, and its rows and heads none with one another. Rows behind starts[slots] are left as they were. dim <=
+ * 256; strides: {row, head} of q, of o, of k, of v. workspace: ytcuda_pages_attend_workspace() bytes that no other call uses
+ * until this one has run. */
 uint64_t ytcuda_pages_attend_workspace(const ytcuda_pages* cache, int rows, int heads);
 int ytcuda_pages_attend(const ytcuda_pages* cache, int layer, const void* q, void* o, const void* k, const void* v,
                         const int64_t* strides, const int32_t* starts, const int32_t* parents, int rows, int heads, float scale,

@@ -469,3 +469,23 @@ def test_many_small_weights_beside_large_ones(paged, dtype, dim, groups):
     tol = (torch.finfo(dtype).eps if dtype != F32 else 0) * want * 1.01 + (n * 2.0 ** -32 if dtype == F16 else 0)
     tol += 2 * (10 * math.sqrt(dim) * 17.7 + 10 * math.sqrt(n)) * 2.0 ** -24 * want
     assert float((got.double() - want).abs().max()) <= tol
+
+
+@pytest.mark.parametrize("dtype,dim,groups", FORMS)
+@pytest.mark.parametrize("tree", [True, False])
+def test_the_largest_numbers_in_hidden_places(paged, dtype, dim, groups, tree):
+    """A hidden value may be the largest or lowest finite number: it has no part in the rows that do not see it."""
+    b = Both(paged, layers=1, heads=1, dim=dim, slots=2, page=16, pages=60, max_pages=30, dtype=dtype)
+    b.fill([200, 18])
+    b.reserve([6, 3])
+    q, k, v = b.randn(9, groups, dim), b.randn(9, 1, dim), b.randn(9, 1, dim)
+    starts, parents = ints([0, 6, 9]), ints([-1, 0, 0, 1, 2, -1, -1, 0, -1]) if tree else None
+    plain = b.d.attend(0, q, starts, k, v, parents=parents)
+    for huge in (torch.finfo(dtype).max, torch.finfo(dtype).min):
+        k2, v2 = k.clone(), v.clone()
+        v2[5], k2[5], v2[8, 0, 3] = huge, 0, huge  # only the last nodes of the slots see them
+        got = b.d.attend(0, q, starts, k2, v2, parents=parents)
+        rest = [0, 1, 2, 3, 4, 6, 7]
+        assert torch.equal(got[rest], plain[rest])
+        if dtype != F32:  # a weight of the node's own of 1 / 206 or so: the result is as large, and finite
+            assert bool((got[5] * math.copysign(1, huge) > torch.finfo(dtype).max / 1e7).all()) and bool(torch.isfinite(got[[5, 8]]).all())

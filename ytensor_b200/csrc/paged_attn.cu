@@ -530,7 +530,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attn_ffma_kernel(const PaPar
 // most (2^-25 otherwise: thousands of small weights beside a large one would be lost).
 // fp32: every number is two of 11 bits, x = hi + lo with hi = x rounded to 11 bits, and a product the three of m16n8k8 (tf32) that
 // lie above 2^-22 of it: hi hi + hi lo + lo hi. That keeps fp32's accuracy and takes a third of the instructions that fused
-// multiply-adds of single lanes would. An infinity has no such halves: what sees one is NaN.
+// multiply-adds of single lanes would. An infinity has no such halves, nor have the largest numbers: what sees one is NaN.
 constexpr float PA_SLACK = 8.f;
 template <typename T>
 constexpr float PA_UP = std::is_same<T, __half>::value ? 7.f : 0.f;
@@ -775,6 +775,8 @@ __device__ __forceinline__ void pa_halves(float x, uint32_t* hi, uint32_t* lo) {
   *hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
   *lo = __float_as_uint(x - __uint_as_float(*hi));
 }
+// Whether x has two halves: an infinity or NaN has none, nor has a number so near the largest one that hi would be an infinity.
+__device__ __forceinline__ bool pa_halved(float x) { return fabsf(x) < 0x1.ffep127f; }
 __device__ __forceinline__ float pa_lds(uint32_t at) {
   float x;
   asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(at));
@@ -852,7 +854,7 @@ struct PaWarp<float, DP> {
       for (int j = 0; j < 4; ++j)
         if (!((sees[j >> 1] >> (2 * t + (j & 1))) & 1)) s[j] = -CUDART_INF_F;
 #pragma unroll 1
-      for (int i = lane; i < NK * DP; i += 32) fine = fine && fabsf(pa_lds(vt + i / DP * ROW + i % DP * 4)) < CUDART_INF_F;
+      for (int i = lane; i < NK * DP; i += 32) fine = fine && pa_halved(pa_lds(vt + i / DP * ROW + i % DP * 4));
       fine = __all_sync(0xffffffffu, fine);
     }
     float shrink[2];
@@ -896,7 +898,7 @@ struct PaWarp<float, DP> {
         if (!fine) {
 #pragma unroll
           for (int j = 0; j < 2; ++j)
-            if (!(fabsf(y[j]) < CUDART_INF_F)) y[j] = 0.f;
+            if (!pa_halved(y[j])) y[j] = 0.f;
         }
         pa_halves(y[0], &bh[i][0], &bl[i][0]);
         pa_halves(y[1], &bh[i][1], &bl[i][1]);
@@ -921,7 +923,7 @@ struct PaWarp<float, DP> {
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const float y = pa_lds(vt + kk * ROW + (8 * d + 2 * t + j) * 4);
-            if (fabsf(y) < CUDART_INF_F) continue;
+            if (pa_halved(y)) continue;
             if (w0 != 0.f) o[d][j] = fmaf(w0, y, o[d][j]);
             if (w1 != 0.f) o[d][2 + j] = fmaf(w1, y, o[d][2 + j]);
           }

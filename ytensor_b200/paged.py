@@ -173,11 +173,11 @@ class PagedCache:
         [rows]) names for each row a smaller node of its slot, or -1 where it follows the sequence itself; at most 1024 nodes
         a slot. Without parents the nodes are a chain (the next token, or a piece of a prompt), of any length. heads is a
         multiple of kv_heads; dim is at most 256. k and v [rows, kv_heads, dim] are stored behind the sequences as by
-        `append`, in the same launch; without them they are in the pages already. scale 0: 1 / sqrt(dim).
+        `append`, in the same call; without them they are in the pages already. scale 0: 1 / sqrt(dim).
 
         Scores, softmax and sums are fp32, results are rounded to nearest even. Rows behind starts[slots] are not written. What
-        a node does not see may be infinite or no number; in fp32 a node that sees an infinity gets NaN. `out` has no
-        element in common with q, k or v, and its rows and heads none with one another."""
+        a node does not see may be infinite or no number; in fp32 a node that sees an infinity, or a number within 2^-12 of the
+        largest, may get NaN. `out` has no element in common with q, k or v, and its rows and heads none with one another."""
         stream = self._stream()
         if q.dim() != 3 or q.shape[1] % self.kv_heads:
             raise _bad(f"paged cache: q is [rows, heads, dim] with heads a multiple of {self.kv_heads}, got {list(q.shape)}")

@@ -500,11 +500,15 @@ int ytcuda_pages_append(const ytcuda_pages* cache, int layer, const void* k, con
  * slot or -1 (NULL: node i - 1, a chain; with parents a slot has at most 1024 nodes). heads is a multiple of kv_heads, query
  * head h reads key head h / (heads / kv_heads). With k and v [rows, kv_heads, dim] the nodes' keys and values are stored
  * first, as by ytcuda_pages_append (both NULL: they are in the pages already). scale 0: 1 / sqrt(dim). Scores, softmax and
- * sums in fp32; results rounded to nearest even. What a node does not see may be infinite or no number; in fp32 (a number is
- * two of 11 bits there) a node that sees an infinity or a number of 0x1.ffep127 or more may get NaN. o has no element in
- * common with q, k or v, and its rows and heads none with one another. Rows behind starts[slots] are left as they were. dim <=
- * 256; strides: {row, head} of q, of o, of k, of v. workspace: ytcuda_pages_attend_workspace() bytes that no other call uses
- * until this one has run. */
+ * sums in fp32; in the 16-bit types the weights are rounded to the type as operands of the product with the values (half a
+ * step of each; in fp16 one below 2^-32 of a row's largest may be zero, and times an infinity NaN). Results rounded to nearest
+ * even. What a node does not see may be infinite or no number; in fp32 (a number is two of 11 bits there) a node that sees an
+ * infinity or a number of 0x1.ffep127 or more may get NaN. o has no element in common with q, k or v, and its rows and heads
+ * none with one another. Rows behind starts[slots] are left as they were. dim <= 256. The work is counted in 32 bits, and over
+ * full rows of the table, since the host knows no lengths: YTC_UNSUPPORTED where row tiles x key tiles x kv_heads could pass
+ * 2^31 (with 8 kv_heads of 4 heads each, 256 single tokens may have rows of up to 17 million positions, one prompt of 32768
+ * rows up to 20 million in the 16-bit types and one million in fp32). strides: {row, head} of q, of o, of k, of v. workspace:
+ * ytcuda_pages_attend_workspace() bytes that no other call uses until this one has run. */
 uint64_t ytcuda_pages_attend_workspace(const ytcuda_pages* cache, int rows, int heads);
 int ytcuda_pages_attend(const ytcuda_pages* cache, int layer, const void* q, void* o, const void* k, const void* v,
                         const int64_t* strides, const int32_t* starts, const int32_t* parents, int rows, int heads, float scale,

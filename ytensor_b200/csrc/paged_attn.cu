@@ -942,7 +942,7 @@ struct PaWarp<float, DP> {
 
 // Up to 16 rows: every warp has its own keys (16 of each tile; 8 in fp32), its own ring, and no barrier until the part ends, where the
 // warps' sums are joined. What bounds it is the copy of keys and values, 512 bytes a key and head at dim 128: 32 tokens behind up to
-// 16384 keys take 223 us, 6.2 TB/s (dim 256: 4.6). In fp32 (1024 bytes) it is the chain of instructions of a step, 800 for eight keys:
+// 16384 keys take 223 us, 6.2 TB/s, in a burst of 60 calls from a graph, and 229 to 246 call by call (dim 256: 4.6 TB/s). In fp32 (1024 bytes) it is the chain of instructions of a step, 800 for eight keys:
 // 4.5 TB/s.
 template <typename T, int DP>
 struct PaNarrow {
@@ -1100,7 +1100,7 @@ __global__ void __launch_bounds__(PaNarrow<T, DP>::THREADS, PaNarrow<T, DP>::CTA
   }
 }
 
-// More than 16 rows of 136 to 256 dims (O of two streams would not fit beside S in tensor memory): a warp for 16 of up to 128 rows (warps
+// More than 16 rows of 136 to 256 dims (two streams as below would take 768 columns of tensor memory, which has 512): a warp for 16 of up to 128 rows (warps
 // without rows only copy), all over the same tiles of keys. Bound by chains of instructions that wait for one another, two warps a
 // scheduler (all that the registers hold): 256 rows of dim 256 behind 16000 keys, eight slots of eight heads, 1.44 ms, 187 TFLOP/s (with
 // four warps 2.66; mma.sync alone would take 0.5).
@@ -1232,9 +1232,10 @@ __global__ void __launch_bounds__(PaWide<T>::THREADS, 1) paged_attn_wide_kernel(
 // scores are there, one of values when its sums are. Two warps copy: tiles in front of the nodes by TMA, `box` rows of a page and 64
 // dims an instruction (a box outside the pool reads zeros); tiles with nodes, and pages whose size is no multiple of 8, by cp.async,
 // 16-byte words in the same 128-byte swizzle. One warp issues S_t = Q K^T and O_t += P_t V, and four warps for each stream turn S into
-// P, a thread a row, while the tensor core works on the other stream. P stays in tensor memory, over its own scores. What bounds it are
-// the exponentials (four results a clock and quarter SM) and the chain S -> P -> O of a block: 128 nodes x 4 heads behind 16000 keys, eight
-// slots, 318 us, 845 TFLOP/s (0.50 of the tensor peak); half a tile of rows, 32 nodes x 4 heads, 117 us, 4.5 TB/s.
+// P, a thread a row, while the tensor core works on the other stream. P stays in tensor memory, over its own scores. What bounds it is
+// the chain S -> P -> O of a block, which two streams do not cover: 128 nodes x 4 heads behind 16000 keys, eight slots, take 318 us, 845
+// TFLOP/s (0.50 of the tensor peak), where the products alone would take 160 us and the exponentials (four results a clock and quarter
+// SM) 113; half a tile of rows, 32 nodes x 4 heads, 117 us, 4.5 TB/s.
 template <typename T, int DP>
 struct PaTc {
   static constexpr int RT = 256, RW = 128, BN = 128, THREADS = 384, STAGES = DP == 64 ? 4 : 2, TILE = 128 * DP * 2;
@@ -2001,8 +2002,10 @@ template <typename T>
 static PaForm pa_form(int dim, int rows, bool words) {
   return dim <= 64 ? pa_form<T, 64>(rows, words) : dim <= 128 ? pa_form<T, 128>(rows, words) : pa_form<T, 256>(rows, words);
 }
-// The form of a call: `rows` rows over the cache's slots, tiles of as many rows as a slot with an even share of them has. `words`:
-// all rows are whole 16-byte words on their boundaries.
+// The form of a call: `rows` rows over the cache's slots, tiles of as many rows as a slot with an even share of them has. The host knows no
+// more than that. One slot's tree in a cache of many idle ones is taken for few rows a slot: 32 nodes x 4 heads behind 16000 keys, 8 key
+// heads, bf16, take 35 us on tcgen05 (a cache of one slot) and 94 in the narrow form (of 64 slots); behind 50 keys 25 and 15. `words`: all rows
+// are whole 16-byte words on their boundaries.
 static PaForm pa_choose(const ytcuda_pages* c, int rows, int heads, bool words) {
   const int64_t share = (static_cast<int64_t>(rows) + c->slots - 1) / c->slots * (heads / c->kv_heads);
   const int r = static_cast<int>(share < 4096 ? share : 4096);

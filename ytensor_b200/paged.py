@@ -175,9 +175,13 @@ class PagedCache:
         multiple of kv_heads; dim is at most 256. k and v [rows, kv_heads, dim] are stored behind the sequences as by
         `append`, in the same call; without them they are in the pages already. scale 0: 1 / sqrt(dim).
 
-        Scores, softmax and sums are fp32, results are rounded to nearest even. Rows behind starts[slots] are not written. What
-        a node does not see may be infinite or no number; in fp32 a node that sees an infinity, or a number within 2^-12 of the
-        largest, may get NaN. `out` has no element in common with q, k or v, and its rows and heads none with one another."""
+        Scores, softmax and sums are fp32; in the 16-bit types the weights are rounded to the type where they meet the values
+        (half a step of each: 2^-8 in bf16, 2^-11 in fp16, where one below 2^-32 of a row's largest may count as zero and take
+        an infinity along as NaN). Results are rounded to nearest even. A call whose rows, over full rows of the table, are
+        more work than it can count is refused (include/ytcuda.h says from where on). Rows behind starts[slots] are not
+        written. What a node does not see may be infinite or no number; in fp32 a node that sees an infinity, or a number
+        within 2^-12 of the largest, may get NaN. `out` has no element in common with q, k or v, and its rows and heads none
+        with one another."""
         stream = self._stream()
         if q.dim() != 3 or q.shape[1] % self.kv_heads:
             raise _bad(f"paged cache: q is [rows, heads, dim] with heads a multiple of {self.kv_heads}, got {list(q.shape)}")

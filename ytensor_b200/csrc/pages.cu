@@ -194,21 +194,47 @@ __device__ __noinline__ void pg_hand_out(const PgCache& c, const int32_t* counts
   __syncthreads();
   for (int i = t; i < *n_left; i += PG_COUNT) atomicSub(c.refs + left[i], 1);
 }
+// How many of the entries from .. to - 1 of this thread's slot others hold too, for sequences that are written anew: in pieces of 128, dealt to
+// the warps (64 slots of 500 pages each 23 us, with a thread a slot 121).
+__device__ __noinline__ int pg_count_shared(const PgCache& c, int s0, int from, int to, int (*behind)[PG_COUNT]) {
+  const int t = threadIdx.x, lane = t & 31;
+  behind[0][t] = from;
+  behind[1][t] = to;
+  behind[2][t] = 0;
+  __syncthreads();
+  for (int l = 0, turn = t >> 5; l < min(PG_COUNT, c.slots - s0); ++l) {
+    const int begin = behind[0][l], end = behind[1][l], pieces = max(0, end - begin + 127) / 128;
+    for (; turn < pieces; turn += PG_COUNT / 32) {
+      int n = 0;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = begin + 128 * turn + 32 * u + lane;
+        if (i < end) n += pg_shared(c, s0 + l, i);
+      }
+      n = __reduce_add_sync(0xffffffffu, n);
+      if (n && lane == 0) atomicAdd(&behind[2][l], n);
+    }
+    turn -= pieces;
+  }
+  __syncthreads();
+  return behind[2][t];
+}
 __global__ void __launch_bounds__(PG_COUNT) pages_reserve_kernel(const __grid_constant__ PgCache c, const int32_t* counts) {
   pg_begin();
   __shared__ int sums[32];
+  __shared__ int behind[3][PG_COUNT], many[2];  // many: some slot of a round has more such pages than a thread counts by itself
   __shared__ int bad, n_copies, n_left, deep;  // deep: some slot replaces more pages than its first one
   const PgScratch at = pg_scratch(c.slots, c.max_pages, c.pages);
   int32_t* const base = c.scratch + at.base;
   int32_t* const mark = c.scratch + at.mark;
   int32_t* const ids = c.scratch + at.ids;
   const int t = threadIdx.x;
-  if (t == 0) bad = n_copies = n_left = deep = 0;
+  if (t == 0) bad = n_copies = n_left = deep = many[0] = many[1] = 0;
   __syncthreads();
   int want_all = 0;
   for (int s0 = 0; s0 < c.slots; s0 += PG_COUNT) {
     const int s = s0 + t;
-    int want = 0;
+    int want = 0, from = 0, to = 0;  // from, to: entries behind the first that are held already and written now
     if (s < c.slots) {
       const int len = c.lens[s], held = c.held[s], count = counts[s];
       mark[s] = -1;
@@ -230,17 +256,24 @@ __global__ void __launch_bounds__(PG_COUNT) pages_reserve_kernel(const __grid_co
         } else {
           mark[s] = copy;
           want = (need > held ? static_cast<int>(need) - held : 0) + (copy >= 0);
+          from = first + 1;
+          to = min(static_cast<int>(need), held);
 #pragma unroll 1
-          for (int i = first + 1; i < min(static_cast<int>(need), held); ++i)
-            if (pg_shared(c, s, i)) {
+          for (; from < to && to - from <= 4; ++from)
+            if (pg_shared(c, s, from)) {
               ++want;
               deep = 1;
             }
         }
       }
     }
-    int total;
-    const int before = pg_scan(want, sums, &total);
+    if (from < to) many[s0 / PG_COUNT % 2] = 1;
+    int total, before = pg_scan(want, sums, &total);
+    if (many[s0 / PG_COUNT % 2]) {  // (behind the barriers of the sum; a round later the other one is set)
+      const int more = pg_count_shared(c, s0, from, to, behind);
+      if (more) deep = 1;
+      before = pg_scan(want += more, sums, &total);
+    }
     if (s < c.slots) base[s] = want_all + before;
     want_all += total;
   }

@@ -941,9 +941,9 @@ struct PaWarp<float, DP> {
 };
 
 // Up to 16 rows: every warp has its own keys (16 of each tile; 8 in fp32), its own ring, and no barrier until the part ends, where the
-// warps' sums are joined. What bounds it is the copy of keys and values, 512 bytes a key and head at dim 128: 32 tokens behind up to
-// 16384 keys take 223 us, 6.2 TB/s, in a burst of 60 calls from a graph, and 229 to 246 call by call (dim 256: 4.6 TB/s). In fp32 (1024 bytes) it is the chain of instructions of a step, 800 for eight keys:
-// 4.5 TB/s.
+// warps' sums are joined. What bounds it is the copy of keys and values, 512 bytes a key and head at dim 128: 32 tokens behind up to 16384
+// keys take 223 us, 6.2 TB/s, in a burst of 60 calls from a graph, and 229 to 246 call by call (dim 256: 4.6 TB/s). In fp32 (1024 bytes) it
+// is the chain of instructions of a step, 800 for eight keys: 4.5 TB/s.
 template <typename T, int DP>
 struct PaNarrow {
   static constexpr bool F32 = std::is_same<T, float>::value;
@@ -1100,10 +1100,10 @@ __global__ void __launch_bounds__(PaNarrow<T, DP>::THREADS, PaNarrow<T, DP>::CTA
   }
 }
 
-// More than 16 rows of 136 to 256 dims (two streams as below would take 768 columns of tensor memory, which has 512): a warp for 16 of up to 128 rows (warps
-// without rows only copy), all over the same tiles of keys. Bound by chains of instructions that wait for one another, two warps a
-// scheduler (all that the registers hold): 256 rows of dim 256 behind 16000 keys, eight slots of eight heads, 1.44 ms, 187 TFLOP/s (with
-// four warps 2.66; mma.sync alone would take 0.5).
+// More than 16 rows of 136 to 256 dims (two streams as below would take 768 columns of tensor memory, which has 512): a warp for 16 of up
+// to 128 rows (warps without rows only copy), all over the same tiles of keys. Bound by chains of instructions that wait for one another,
+// two warps a scheduler (all that the registers hold): 256 rows of dim 256 behind 16000 keys, eight slots of eight heads, 1.44 ms, 187
+// TFLOP/s (with four warps 2.66; mma.sync alone would take 0.5).
 template <typename T>
 struct PaWide {
   static constexpr int DP = 256, WARPS = 8, THREADS = 32 * WARPS, RT = 16 * WARPS, BN = 32, STAGES = 3, SLOT = BN * DP * 2;
